@@ -22,6 +22,7 @@
 #include <tuple>
 
 #include "../../include/phi_qlinear.h"
+#include "capi.hpp"
 #include "device_common.hpp"
 #include "gemv.hpp"
 #include "lora.hpp"
@@ -441,6 +442,10 @@ phi_status fail(phi_status st, const char* fmt, ...) {
     va_end(ap);
     return st;
 }
+
+phi_status ok() { return ::ok(); }
+
+phi_status check_hip(hipError_t e, const char* what) { return ::check_hip(e, what); }
 
 bool device_lost() { return g_lost; }
 

@@ -23,11 +23,7 @@
 #include <mutex>
 
 #include "../../include/phi_qlinear.h"
-
-namespace phi_capi {
-phi_status fail(phi_status st, const char* fmt, ...);
-bool device_lost();
-}  // namespace phi_capi
+#include "capi.hpp"
 
 namespace phi_noalloc {
 

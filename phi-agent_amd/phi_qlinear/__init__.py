@@ -1,7 +1,8 @@
 """Python front end of the gfx950 quantized-linear library.
 
-Thin ctypes bindings over the C ABI in ``include/phi_qlinear.h``
-(``lib/libphi_qlinear.so``).  PyTorch provides device memory and the stream;
+Thin ctypes bindings over the C ABI in ``include/phi_qlinear.h`` and
+``include/phi_decoder.h`` (``lib/libphi_qlinear.so``; the second header's
+operators are in ``decoder.py``).  PyTorch provides device memory and the stream;
 every computation runs in the HIP kernels.  There is no fallback: if the
 library is missing or the device is absent the calls raise.
 
@@ -63,6 +64,14 @@ class GemmPlan(ctypes.Structure):
                 ("tile", ctypes.c_int32), ("reserved", ctypes.c_int32)]
 
 
+class KvCacheDesc(ctypes.Structure):
+    """phi_kv_cache (include/phi_decoder.h)."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p)] + [(n, ctypes.c_int64) for n in (
+                    "blocks", "heads", "page", "dim", "block_stride", "head_stride", "token_stride",
+                    "s_block_stride", "s_head_stride", "s_token_stride")]
+
+
 class GemvItem(ctypes.Structure):
     _fields_ = [("W", ctypes.c_void_p), ("sW", ctypes.c_void_p), ("sw_scalar", ctypes.c_int),
                 ("bias", ctypes.c_void_p), ("C", ctypes.c_void_p), ("ldc", ctypes.c_int64)]
@@ -81,7 +90,8 @@ EXPORTS = ["phi_hip_last_error", "phi_hip_abi_version", "phi_hip_quant_rotate", 
            "phi_hip_quant_rotate_mod_kt", "phi_hip_quant_rotate_act_kt", "phi_hip_i8_gemm_residual_kt",
            "phi_hip_dequant_fp4_rows", "phi_hip_gemm_plan_set", "phi_hip_gemm_plan_get", "phi_hip_gemm_plan_count",
            "phi_hip_gemm_plan_clear", "phi_hip_gemm_is_small", "phi_hip_w4a8_banded_bytes", "phi_hip_w4a8_pack_banded",
-           "phi_hip_w4a8_linear_banded"]
+           "phi_hip_w4a8_linear_banded", "phi_hip_rms_norm_quant", "phi_hip_kv_cache_write", "phi_hip_kv_cache_read",
+           "phi_hip_paged_attention", "phi_hip_paged_attention_workspace_bytes"]
 
 _lib = None
 
@@ -151,6 +161,13 @@ def load() -> ctypes.CDLL:
     L.phi_hip_w4a8_banded_bytes.restype = SZ
     L.phi_hip_w4a8_pack_banded.argtypes = [P, P, I64, P, I64, I64, I64, P]
     L.phi_hip_w4a8_linear_banded.argtypes = [P, P, I, I64, I64, I64, P, I64, P, P, I, I64, P, I, I64, P, P, I]
+    L.phi_hip_rms_norm_quant.argtypes = [P, P, I, I64, P, P, I, I64, P, P, I, F, I64, I64, P, I, I64, P, I64, P, F, I, I]
+    L.phi_hip_kv_cache_write.argtypes = [P, ctypes.POINTER(KvCacheDesc), P, I64, I64, P, I64, I64, I, P, I64]
+    L.phi_hip_kv_cache_read.argtypes = [P, ctypes.POINTER(KvCacheDesc), P, I64, P, I64, I64, P, I64, I64, I]
+    L.phi_hip_paged_attention.argtypes = [P, P, I, I64, I64, I64, I64, ctypes.POINTER(KvCacheDesc), P, I64, I64, P, P, I64,
+                                          I64, I64, F, I, I64, P, I64, I64, P, SZ]
+    L.phi_hip_paged_attention_workspace_bytes.argtypes = [I64, I64, I64, I64, I64, I64, I64, I]
+    L.phi_hip_paged_attention_workspace_bytes.restype = SZ
     for name in EXPORTS:
         f = getattr(L, name)
         if f.restype is None:
@@ -735,3 +752,7 @@ def q8_linear_kt(x: torch.Tensor, Wkt: torch.Tensor, N: int, sW: torch.Tensor,
                                        _dt(bias) if bias is not None else F32, N, _ptr(C), _dt(C),
                                        C.stride(0), _ptr(q8), _ptr(s8), round_mode))
     return C
+
+
+from .decoder import (KvCache, kv_cache_empty, kv_cache_read, kv_cache_write, paged_attention,  # noqa: E402,F401
+                      paged_attention_workspace, rms_norm_quant)
