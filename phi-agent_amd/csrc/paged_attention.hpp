@@ -1,0 +1,160 @@
+// What the attention kernels share: a batch's geometry on the device, the
+// query's integer form, and how partial softmaxes are kept and joined.
+//
+// A row's logits are kept in base 2, x_t = log2(e) scale q.k_t, as
+//   x_t = rq * (sk_t * c_t),   c_t = sum_d Q_d K_td  (exact integers)
+// with K the cache's codes, sk_t their scale, and Q = round(q' / rq) the
+// integer form of q' = log2(e) scale q at 16 bits (bf16 q) or 24 bits (fp32 q)
+// relative to the row's largest |q'|.  Q is split into signed bytes, Q = 256 Q1
+// + Q0 (or 65536 Q2 + 256 Q1 + Q0), so that q.k runs on the int8 matrix
+// instructions, which read K as it lies in the cache at twice the rate of the
+// 16-bit ones: two products of half the cost, no conversion of K, and less
+// error than q itself has (2^-16 of the row's largest element).
+//
+// p.v takes V's codes, exact in fp16, against p_t sv_t in fp16 (11 bits; fp32 q:
+// a second fp16 holds the next 11).  fp16 rather than bf16 for its three more
+// bits; its range is enough because both factors are kept in range: p by the
+// running maximum m, sv by a running power of two (V_SCALE below), with
+// kHead bits above for p to grow before m has to move.
+#pragma once
+
+#include "decoder.hpp"
+#include "device_common.hpp"
+
+namespace phi_dev {
+
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef float v16f __attribute__((ext_vector_type(16)));
+
+// m of a row that has seen nothing: finite, so that exp2(-inf - m) is 0 and
+// exp2(m - m) is 1, and below every logit that matters.
+constexpr float kNoMax = -1e30f;
+
+// One sequence's new tokens and range, as the device arrays give them, within
+// the bounds that the host checked.
+struct SeqInfo {
+    int first, n;  // its rows of q
+    int kv;        // tokens that can be seen
+    int pos0;      // position of its first new token (below 0: rows before any token)
+};
+
+__device__ __forceinline__ SeqInfo seq_info(const PagedAttn& p, int page, int b) {
+    SeqInfo s;
+    const int64_t a = p.q_start[b], e = p.q_start[b + 1], T = p.tokens;
+    s.first = (int)(a < 0 ? 0 : a > T ? T : a);
+    s.n = max(0, (int)(e < 0 ? 0 : e > T ? T : e) - s.first);
+    const int kv = max(0, p.kv_len[b]);
+    s.kv = (int)min((int64_t)min(kv, p.max_kv), (int64_t)p.table_width * page);
+    s.pos0 = kv - s.n;
+    return s;
+}
+
+// Where a call's tokens are split over blocks, split z has the tokens
+// [z * len, (z + 1) * len) of each sequence; each leaves, for every row and head
+// (row * q_heads + head), the undivided sum of p v, m and l = sum of p in
+//   o [splits][tokens * q_heads][dim], ml [splits][tokens * q_heads][2]
+// and attn_join_kernel joins them.  One split: no workspace, out is written.
+struct AttnSplit {
+    int len, count;
+    float* o;
+    float* ml;
+};
+
+hipError_t launch_paged_decode(hipStream_t stream, const KvCache& c, const PagedAttn& p, const AttnSplit& s);
+// Rows (query heads of a key/value head x new tokens) that a block's tile holds.
+constexpr int kDecodeRows = 16;
+
+// The maximum over lanes l, l ^ 16, l ^ 32, l ^ 48, and over l, l ^ 32.
+__device__ __forceinline__ float max_x32(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float max_x16(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float add_x32(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float add_x16(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// Sixteen elements of a query vector at element offset off, as fp32.
+template <bool F32>
+__device__ __forceinline__ void load_q16(const void* __restrict__ q, int64_t off, float (&x)[16]) {
+    if (F32) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float4 t = *(const float4*)((const float*)q + off + 4 * i);
+            x[4 * i] = t.x, x[4 * i + 1] = t.y, x[4 * i + 2] = t.z, x[4 * i + 3] = t.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const uint4 t = *(const uint4*)((const uint16_t*)q + off + 8 * i);
+            const uint32_t w[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+            for (int j = 0; j < 4; j++) x[8 * i + 2 * j] = bf16_to_f32(w[j] & 0xffffu), x[8 * i + 2 * j + 1] = bf16_to_f32(w[j] >> 16);
+        }
+    }
+}
+
+// The integer form's terms (2 or 3 signed bytes an element) and its largest
+// value: 127 (256 + 1) and, a little below 127 (65536 + 256 + 1), 0x7f7f00,
+// because the product with the row's largest element may round one up there.
+template <bool F32> constexpr int q_terms = F32 ? 3 : 2;
+template <bool F32> constexpr float q_steps = F32 ? 8355584.0f : 32639.0f;
+
+// Sixteen elements x * inv as integers, byte-split, term 0 the low one.
+template <bool F32>
+__device__ __forceinline__ void split_q16(const float (&x)[16], float inv, v4i (&out)[q_terms<F32>]) {
+#pragma unroll
+    for (int w = 0; w < 4; w++) {
+        int b[q_terms<F32>][4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            int r = (int)rintf(x[4 * w + j] * inv);
+#pragma unroll
+            for (int t = 0; t < q_terms<F32>; t++) {
+                b[t][j] = (int)(int8_t)r;
+                r = (r - b[t][j]) >> 8;
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < q_terms<F32>; t++) out[t][w] = (int)pack4(b[t][0], b[t][1], b[t][2], b[t][3]);
+    }
+}
+
+// c_t in fp32 (exactly, for bf16 q's two terms at dim <= 256: below 2^31) from
+// the terms' products.
+template <bool F32>
+__device__ __forceinline__ float join_terms(const int (&c)[q_terms<F32>]) {
+    if (F32) return fmaf((float)c[q_terms<F32> - 1], 65536.0f, fmaf((float)c[1], 256.0f, (float)c[0]));
+    return (float)(c[1] * 256 + c[0]);
+}
+
+// p sv enters fp16 as p * sv * 2^(kPre - E), 2^E <= the largest |sv| so far <
+// 2^(E+1), so it is below 2^(kHead + kPre + 1) <= 2^15.  For fp32 q, p never
+// exceeds 1 and the bits above go to the second half's range.
+template <bool F32> constexpr int kHead = F32 ? 0 : 7;
+template <bool F32> constexpr int kPre = F32 ? 14 : 7;
+constexpr int kMinExp = -100;  // E's floor: the factor stays finite
+
+// V's codes as fp16 enter p.v as code * 2^-9 (cvt_pair).
+constexpr float kVUnit = 0x1p9f;
+
+// Byte b of two words of codes biased by 128 as two fp16 values code * 2^-9:
+// the byte alone in 16 bits is the subnormal (code + 128) 2^-24, and one
+// packed fma, exact, takes off the bias.
+template <int B>
+__device__ __forceinline__ h2 cvt_pair(uint32_t lo, uint32_t hi) {
+    const uint32_t u = __builtin_amdgcn_perm(hi, lo, 0x0c000c00u | (uint32_t)((4 + B) << 16) | (uint32_t)B);
+    const h2 x = __builtin_bit_cast(h2, u), mul = {(_Float16)32768.0f, (_Float16)32768.0f}, off = {(_Float16)-0.25f, (_Float16)-0.25f};
+    return __builtin_elementwise_fma(x, mul, off);
+}
+
+}  // namespace phi_dev

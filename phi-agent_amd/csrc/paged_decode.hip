@@ -1,0 +1,351 @@
+// Attention of a few rows over the paged int8 cache: single new tokens, or a
+// handful, with the query heads that share a key/value head.
+//
+// Bound by the cache's one read.  A wave takes 32 tokens a step straight from
+// memory in the order that the matrix instructions want them, with no LDS and
+// no shuffles in the loop:
+//   S^T = K Q^T (v_mfma_i32_16x16x64_i8): lane l holds K's token l & 15, bytes
+//     16 (l >> 4) .. + 15 of each 64: one 16-byte load of the cache's row.  The
+//     result has row l & 15 in the lane and tokens 4 (l >> 4) + i.
+//   O^T = V^T P^T (v_mfma_f32_16x16x32_f16): the sum's order is free, so k
+//     index 8 g + j (g = l >> 4) stands for the token the lane's P is of: 4 g + j
+//     of the step's first 16 tokens, 4 g + j - 4 of its second.  P is used where
+//     it lies.  V^T wants 8 tokens of one d a lane: the lane loads dim/16
+//     bytes of each of its 8 tokens' rows (16 lanes read a whole row) and takes
+//     byte e of all eight for product e, so d = dim/16 (l & 15) + e.
+// The next step's loads are under way while a step is computed: 32 tokens are 8 KB
+// a wave at dim 128, and 12 waves a CU keep 96 KB in flight.  The four waves
+// of a block take every fourth step of its split and join in LDS.
+#include <type_traits>
+
+#include "paged_attention.hpp"
+
+namespace phi_dev {
+
+namespace {
+
+constexpr int kWaves = 4;
+constexpr int kStep = 32;  // tokens a wave and step
+
+template <int BYTES> struct VWord;
+template <> struct VWord<4> { typedef uint32_t type __attribute__((ext_vector_type(1))); };
+template <> struct VWord<8> { typedef uint32_t type __attribute__((ext_vector_type(2))); };
+template <> struct VWord<16> { typedef uint32_t type __attribute__((ext_vector_type(4))); };
+
+// One step's operands: two tiles of 16 tokens.
+template <int DP> struct Step {
+    v4i k[2][DP / 64];
+    typename VWord<DP / 16>::type v[2][4];
+    v4f sk[2], sv[2];
+    bool ok[2][4];  // the table has a block for the token (PAGE16: of the tile)
+};
+
+}  // namespace
+
+// DP: dim rounded up to 64, 128 or 256.  F32: fp32 q and out, else bf16.
+// PAGE16: pages of a multiple of 16 tokens with contiguous, 16-byte aligned
+// scales and offsets within a block below 2^31, so that a tile of 16 tokens has
+// one block and its loads one scalar base; otherwise every token finds its own.
+template <int DP, bool F32, bool PAGE16>
+__global__ __launch_bounds__(64 * kWaves) void paged_decode_kernel(KvCache c, PagedAttn p, AttnSplit sp,
+                                                                  const int32_t* __restrict__ table) {
+    constexpr int KS = DP / 64, EB = DP / 16, NT = q_terms<F32>;
+    __shared__ float lo_[kWaves][kDecodeRows][DP];
+    __shared__ float lm[kWaves][kDecodeRows], ll[kWaves][kDecodeRows];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, g = lane >> 4;
+    const int kh = blockIdx.y % c.heads, rt = blockIdx.y / c.heads, b = blockIdx.z;
+    const SeqInfo s = seq_info(p, c.page, b);
+    const int rows = min(s.n, p.max_q) * p.group, r0 = rt * kDecodeRows;
+    const int z0 = blockIdx.x * sp.len;
+    if (r0 >= rows || (blockIdx.x > 0 && z0 >= s.kv)) return;
+    const int D = c.dim;
+
+    // The lane's row of the tile (past the last: the last again, not stored).
+    const int r = min(r0 + col, rows - 1), i = r / p.group, head = kh * p.group + (r - i * p.group);
+    const int64_t token = s.first + i;
+    const int pos = s.pos0 + i;
+    const int pos_first = s.pos0 + r0 / p.group, pos_last = s.pos0 + min(r0 + kDecodeRows - 1, rows - 1) / p.group;
+    const int row_hi = p.causal ? min(s.kv, pos + 1) : s.kv, row_lo = p.window > 0 ? max(0, pos + 1 - p.window) : 0;
+    // Tokens that some row of the tile sees, and that all of them see.
+    const int hi = min(p.causal ? min(s.kv, pos_last + 1) : s.kv, z0 + sp.len);
+    const int lo = max(p.window > 0 ? max(0, pos_first + 1 - p.window) : 0, z0);
+    const int all_hi = p.causal ? min(s.kv, pos_first + 1) : s.kv, all_lo = p.window > 0 ? max(0, pos_last + 1 - p.window) : 0;
+
+    // Q's integer form in the B operand's order.
+    v4i qt[KS][NT];
+    float rq;
+    {
+        float x[KS][16], amax = 0.0f, bad = 0.0f;
+        const float f = p.scale * 1.4426950408889634f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            const int d = 64 * ks + 16 * g;
+            if (d < D) load_q16<F32>(p.q, token * p.q_token + head * p.q_head + d, x[ks]);
+#pragma unroll
+            for (int j = 0; j < 16; j++) {
+                x[ks][j] = d < D ? x[ks][j] * f : 0.0f;
+                amax = fmaxf(amax, fabsf(x[ks][j]));
+                bad += x[ks][j] * 0.0f;  // NaN once an infinity or a NaN is met
+            }
+        }
+        amax = max_x16(max_x32(amax));
+        bad = add_x16(add_x32(bad));
+        const bool some = amax > 1e-30f;
+        const float inv = some ? q_steps<F32> / amax : 0.0f;
+        rq = (some ? amax / q_steps<F32> : 1.0f) + bad;
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) split_q16<F32>(x[ks], inv, qt[ks]);
+    }
+
+    // A lane's bytes past dim read its row's first bytes again: Q is 0 there,
+    // and O's columns past dim are not stored.
+    const int vd = EB * col < D ? EB * col : 0;
+    int kd[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++) kd[ks] = 64 * ks + 16 * g < D ? 64 * ks + 16 * g : 0;
+    const int32_t* trow = table + (int64_t)b * p.table_stride;
+    const int last_page = page_of(c, max(hi - 1, 0));
+
+    auto block_at = [&](int page, bool& ok) {
+        const int blk = trow[min(page, last_page)];
+        ok = blk >= 0 && blk < c.blocks;
+        return ok ? blk : 0;
+    };
+    // Loads of the step at t0; tokens at hi and past it read the last page's, or
+    // block 0's, whatever these hold.
+    auto load = [&](Step<DP>& st, int t0) {
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            const int t = min(t0 + 16 * j, hi - 1);
+            if (PAGE16) {
+                const int page = page_of(c, t), in = (t & ~15) - page * c.page;
+                bool ok;
+                const int64_t blk = block_at(page, ok);
+                const int64_t at = blk * c.block_stride + kh * c.head_stride + (int64_t)in * c.token_stride;
+                const int64_t sat = blk * c.s_block_stride + kh * c.s_head_stride + in;
+                const int8_t* kb = c.k + at;
+                const int8_t* vb = c.v + at;
+                const int ts = (int)c.token_stride;
+                st.ok[j][0] = ok;
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++) st.k[j][ks] = *(const v4i*)(kb + (uint32_t)(col * ts + kd[ks]));
+#pragma unroll
+                for (int n = 0; n < 4; n++) st.v[j][n] = *(const typename VWord<EB>::type*)(vb + (uint32_t)((4 * g + n) * ts + vd));
+                st.sk[j] = *(const v4f*)(c.ks + sat + 4 * g);
+                st.sv[j] = *(const v4f*)(c.vs + sat + 4 * g);
+            } else {
+                // Lane l finds token l & 15; the others' are read from it.
+                const int tk = min(t0 + 16 * j + col, hi - 1), page = page_of(c, tk), in = tk - page * c.page;
+                bool ok;
+                const int64_t blk = block_at(page, ok);
+                const int64_t at = blk * c.block_stride + kh * c.head_stride + in * c.token_stride;
+                const int64_t sat = blk * c.s_block_stride + kh * c.s_head_stride + in * c.s_token_stride;
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++) st.k[j][ks] = *(const v4i*)(c.k + at + kd[ks]);
+#pragma unroll
+                for (int n = 0; n < 4; n++) {
+                    const int64_t av = __shfl(at, 4 * g + n, 64), as = __shfl(sat, 4 * g + n, 64);
+                    st.ok[j][n] = __shfl((int)ok, 4 * g + n, 64);
+                    st.v[j][n] = *(const typename VWord<EB>::type*)(c.v + av + vd);
+                    st.sk[j][n] = c.ks[as];
+                    st.sv[j][n] = c.vs[as];
+                }
+            }
+        }
+    };
+
+    v4f o[EB];
+#pragma unroll
+    for (int e = 0; e < EB; e++) o[e] = v4f{0, 0, 0, 0};
+    float m = kNoMax, l = 0.0f;
+    int vexp = kMinExp;
+    float vlim = ldexpf(1.0f, kMinExp + 1), vmul = ldexpf(1.0f, kPre<F32> - kMinExp);
+
+    auto compute = [&](const Step<DP>& st, int t0) {
+        float t[8], sv[8];
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+            v4i acc[NT];
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                acc[n] = v4i{0, 0, 0, 0};
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++) acc[n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(st.k[j][ks], qt[ks][n], acc[n], 0, 0, 0);
+            }
+#pragma unroll
+            for (int n = 0; n < 4; n++) {
+                int a[NT];
+#pragma unroll
+                for (int k = 0; k < NT; k++) a[k] = acc[k][n];
+                t[4 * j + n] = join_terms<F32>(a) * st.sk[j][n];
+                sv[4 * j + n] = st.sv[j][n];
+            }
+        }
+        bool ok = true;
+#pragma unroll
+        for (int j = 0; j < 2; j++)
+#pragma unroll
+            for (int n = 0; n < (PAGE16 ? 1 : 4); n++) ok &= st.ok[j][n];
+        const bool whole = t0 >= all_lo && t0 + kStep <= min(all_hi, hi) && t0 >= lo && (PAGE16 ? ok : __all(ok));
+        uint32_t seen = 0xff;
+        if (!whole) {
+            seen = 0;
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const int tok = t0 + 16 * (k >> 2) + 4 * g + (k & 3);
+                const bool in = tok >= max(row_lo, lo) && tok < min(row_hi, hi) && st.ok[k >> 2][PAGE16 ? 0 : k & 3];
+                seen |= in ? 1u << k : 0u;
+                t[k] = in ? t[k] : -INFINITY;
+                sv[k] = in ? sv[k] : 0.0f;
+            }
+        }
+        // A larger |sv| than the running power of two covers: move it.
+        float vmax = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; k++) vmax = fmaxf(vmax, fabsf(sv[k]));
+        float keep_v = 1.0f;
+        if (__builtin_expect(__any(vmax >= vlim), 0)) {
+            float top = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 8; k++) top = fmaxf(top, __builtin_isfinite(sv[k]) ? fabsf(sv[k]) : 0.0f);
+#pragma unroll
+            for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+            const int e = max(vexp, __builtin_amdgcn_readfirstlane((int)(__float_as_uint(top) >> 23) - 127));
+            keep_v = ldexpf(1.0f, vexp - e);
+            vexp = e;
+            vlim = ldexpf(1.0f, e + 1);
+            vmul = ldexpf(1.0f, kPre<F32> - e);
+        }
+        float top = t[0];
+#pragma unroll
+        for (int k = 1; k < 8; k++) top = fmaxf(top, t[k]);
+        const float xm = top * rq;
+        const bool grow = xm > m + (float)kHead<F32>;
+        if (__any(grow) || keep_v != 1.0f) {
+            const float m2 = fmaxf(m, max_x16(max_x32(xm)));
+            const float keep = __builtin_amdgcn_exp2f(m - m2);
+            m = m2;
+            l *= keep;
+#pragma unroll
+            for (int e = 0; e < EB; e++)
+#pragma unroll
+                for (int n = 0; n < 4; n++) o[e][n] *= keep * keep_v;
+        }
+        float pv[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            const float e = __builtin_amdgcn_exp2f(fmaf(t[k], rq, -m));
+            l += e;
+            pv[k] = e * (sv[k] * vmul);
+        }
+        if (!whole) {
+#pragma unroll
+            for (int k = 0; k < 8; k++) pv[k] = seen >> k & 1 ? pv[k] : 0.0f;
+        }
+        h8 ph, pl;
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            ph[k] = (_Float16)pv[k];
+            if (F32) pl[k] = (_Float16)(pv[k] - (float)ph[k]);
+        }
+        typename VWord<EB>::type v[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) v[k] = st.v[k >> 2][k & 3] ^ 0x80808080u;
+#pragma unroll
+        for (int w = 0; w < EB / 4; w++) {
+            auto product = [&](auto bc) {
+                constexpr int B = decltype(bc)::value;
+                const h2 a0 = cvt_pair<B>(v[0][w], v[1][w]), a1 = cvt_pair<B>(v[2][w], v[3][w]);
+                const h2 a2 = cvt_pair<B>(v[4][w], v[5][w]), a3 = cvt_pair<B>(v[6][w], v[7][w]);
+                const h8 a = {a0[0], a0[1], a1[0], a1[1], a2[0], a2[1], a3[0], a3[1]};
+                o[4 * w + B] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ph, o[4 * w + B], 0, 0, 0);
+                if (F32) o[4 * w + B] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pl, o[4 * w + B], 0, 0, 0);
+            };
+            product(std::integral_constant<int, 0>{});
+            product(std::integral_constant<int, 1>{});
+            product(std::integral_constant<int, 2>{});
+            product(std::integral_constant<int, 3>{});
+        }
+    };
+
+    // Two steps in registers, one loading.  Loads run ahead of hi - 1 at most by
+    // being clamped to it.
+    const int begin = (lo & ~(kStep - 1)) + kStep * wave, stride = kStep * kWaves;
+    if (begin < hi) {
+        Step<DP> a, b2;
+        load(a, begin);
+        for (int t0 = begin; t0 < hi; t0 += 2 * stride) {
+            load(b2, t0 + stride);
+            compute(a, t0);
+            if (t0 + stride >= hi) break;
+            load(a, t0 + 2 * stride);
+            compute(b2, t0 + stride);
+        }
+    }
+
+    // Join the four waves.  The largest m of a row decides; a wave without a
+    // token has l = 0, o = 0.
+    l = add_x16(add_x32(l));
+    if (g == 0) lm[wave][col] = m, ll[wave][col] = l;
+    __syncthreads();
+    float top = lm[0][col];
+#pragma unroll
+    for (int w = 1; w < kWaves; w++) top = fmaxf(top, lm[w][col]);
+    const float unit = __builtin_amdgcn_exp2f(m - top) * ldexpf(kVUnit, vexp - kPre<F32>);
+#pragma unroll
+    for (int n = 0; n < 4; n++)
+#pragma unroll
+        for (int e = 0; e < EB; e += 4)
+            *(v4f*)&lo_[wave][col][EB * (4 * g + n) + e] =
+                v4f{o[e][n] * unit, o[e + 1][n] * unit, o[e + 2][n] * unit, o[e + 3][n] * unit};
+    __syncthreads();
+    const int row = threadIdx.x / 16, part = threadIdx.x & 15;  // a row a team of 16
+    if (r0 + row >= rows) return;
+    const int ri = (r0 + row) / p.group, rhead = kh * p.group + (r0 + row - ri * p.group);
+    const int64_t rtok = s.first + ri;
+    float rm = lm[0][row];
+#pragma unroll
+    for (int w = 1; w < kWaves; w++) rm = fmaxf(rm, lm[w][row]);
+    float rl = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWaves; w++) rl = fmaf(ll[w][row], __builtin_amdgcn_exp2f(lm[w][row] - rm), rl);
+    const int64_t at = ((int64_t)blockIdx.x * p.tokens + rtok) * p.q_heads + rhead;
+    const float inv = sp.count > 1 ? 1.0f : rl != 0.0f ? 1.0f / rl : 0.0f;
+    if (sp.count > 1 && part == 0) sp.ml[2 * at] = rm, sp.ml[2 * at + 1] = rl;
+#pragma unroll
+    for (int q4 = 0; q4 < DP / 64; q4++) {
+        const int d = 4 * (part + 16 * q4);
+        if (d >= D) break;
+        v4f x = *(const v4f*)&lo_[0][row][d];
+#pragma unroll
+        for (int w = 1; w < kWaves; w++) x += *(const v4f*)&lo_[w][row][d];
+        x *= inv;
+        if (sp.count > 1) {
+            *(v4f*)(sp.o + at * D + d) = x;
+        } else {
+            const int64_t to = rtok * p.out_token + rhead * p.out_head + d;
+            if (F32) *(v4f*)((float*)p.out + to) = x;
+            else *(uint2*)((uint16_t*)p.out + to) = make_uint2(f32x2_to_bf16x2(x[0], x[1]), f32x2_to_bf16x2(x[2], x[3]));
+        }
+    }
+}
+
+template <int DP, bool F32>
+static hipError_t launch_dp(hipStream_t stream, const KvCache& c, const PagedAttn& p, const AttnSplit& s) {
+    const int tiles = (int)(((int64_t)p.max_q * p.group + kDecodeRows - 1) / kDecodeRows);
+    const dim3 grid((unsigned)s.count, (unsigned)(tiles * c.heads), (unsigned)p.batch);
+    const bool page16 = c.page % 16 == 0 && c.s_token_stride == 1 && c.s_block_stride % 4 == 0 && c.s_head_stride % 4 == 0 &&
+                        (uintptr_t)c.ks % 16 == 0 && (uintptr_t)c.vs % 16 == 0 && 16 * c.token_stride < ((int64_t)1 << 31);
+    if (page16) hipLaunchKernelGGL((paged_decode_kernel<DP, F32, true>), grid, dim3(64 * kWaves), 0, stream, c, p, s, p.table);
+    else hipLaunchKernelGGL((paged_decode_kernel<DP, F32, false>), grid, dim3(64 * kWaves), 0, stream, c, p, s, p.table);
+    return hipGetLastError();
+}
+
+hipError_t launch_paged_decode(hipStream_t stream, const KvCache& c, const PagedAttn& p, const AttnSplit& s) {
+    if (c.dim <= 64) return p.bf16 ? launch_dp<64, false>(stream, c, p, s) : launch_dp<64, true>(stream, c, p, s);
+    if (c.dim <= 128) return p.bf16 ? launch_dp<128, false>(stream, c, p, s) : launch_dp<128, true>(stream, c, p, s);
+    return p.bf16 ? launch_dp<256, false>(stream, c, p, s) : launch_dp<256, true>(stream, c, p, s);
+}
+
+}  // namespace phi_dev
