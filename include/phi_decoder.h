@@ -122,10 +122,12 @@ phi_status phi_hip_kv_cache_read(phi_stream_t stream, const phi_kv_cache* cache,
  *                (NULL when that is 0)
  * q_start, kv_len and block_table are read on the device, so a captured graph
  * serves growing sequences up to max_kv.
- * Arithmetic: q is held as integers of 16 bits (PHI_BF16) or 24 bits (PHI_F32)
- * relative to the row's largest |q|, k and v as their codes, exactly; products
- * are summed exactly (q.k) or in fp32 (p.v), the softmax is fp32, and p enters
- * p.v with 11 (PHI_BF16) or 22 (PHI_F32) bits.
+ * Arithmetic.  Sums, maxima and the softmax are fp32 or exact integers.  q is
+ * held as integers of 16 bits (PHI_BF16) or 24 bits (PHI_F32) relative to the
+ * row's largest |q|, k and v as their codes, exactly, and p enters p.v with 16
+ * or 24 bits.  PHI_BF16 sequences of more than 128 rows (new tokens x query heads
+ * a key/value head) round each element of k and v to 11 bits instead, and p
+ * to 11 bits or an error of 2^-39 of the row's largest p.
  */
 phi_status phi_hip_paged_attention(phi_stream_t stream, const void* q, int dtype, int64_t q_token_stride,
                                    int64_t q_head_stride, int64_t tokens, int64_t q_heads, const phi_kv_cache* cache,

@@ -11,11 +11,10 @@
 // 16-bit ones: two products of half the cost, no conversion of K, and less
 // error than q itself has (2^-16 of the row's largest element).
 //
-// p.v takes V's codes, exact in fp16, against p_t sv_t in fp16 (11 bits; fp32 q:
-// a second fp16 holds the next 11).  fp16 rather than bf16 for its three more
-// bits; its range is enough because both factors are kept in range: p by the
-// running maximum m, sv by a running power of two (V_SCALE below), with
-// kHead bits above for p to grow before m has to move.
+// p.v: paged_decode.hip, bound by memory, has V's codes exactly in bf16 against
+// p_t sv_t as a sum of two bf16 (16 bits; fp32 q: three, 24 bits), which have
+// fp32's whole range.  paged_chunk.hip, bound by the matrix cores, has one
+// product of fp16 (11 bits), both factors kept in its range.
 #pragma once
 
 #include "decoder.hpp"
@@ -23,9 +22,7 @@
 
 namespace phi_dev {
 
-typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-typedef float v16f __attribute__((ext_vector_type(16)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 
 // m of a row that has seen nothing: finite, so that exp2(-inf - m) is 0 and
 // exp2(m - m) is 1, and below every logit that matters.
@@ -61,9 +58,21 @@ struct AttnSplit {
     float* ml;
 };
 
-hipError_t launch_paged_decode(hipStream_t stream, const KvCache& c, const PagedAttn& p, const AttnSplit& s);
-// Rows (query heads of a key/value head x new tokens) that a block's tile holds.
+// A sequence's rows are the query heads of a key/value head x its new tokens, in
+// that order.  launch_paged_decode takes the sequences of at most `rows` rows;
+// launch_paged_chunk (bf16 queries only) those of more.
+hipError_t launch_paged_decode(hipStream_t stream, const KvCache& c, const PagedAttn& p, const AttnSplit& s, int64_t rows);
+hipError_t launch_paged_chunk(hipStream_t stream, const KvCache& c, const PagedAttn& p, const AttnSplit& s, int64_t rows);
+// Rows of a block's tile.
 constexpr int kDecodeRows = 16;
+constexpr int kChunkRows = 256, kChunkRowsWide = 128;  // dim to 128, above
+
+// Whether 16 tokens from a multiple of 16 lie in one block, their scales in a
+// row at 16-byte alignment and their codes' offsets in it within 31 bits.
+inline bool tiles_of_16(const KvCache& c) {
+    return c.page % 16 == 0 && c.s_token_stride == 1 && c.s_block_stride % 4 == 0 && c.s_head_stride % 4 == 0 &&
+           (uintptr_t)c.ks % 16 == 0 && (uintptr_t)c.vs % 16 == 0 && 16 * c.token_stride < ((int64_t)1 << 31);
+}
 
 // The maximum over lanes l, l ^ 16, l ^ 32, l ^ 48, and over l, l ^ 32.
 __device__ __forceinline__ float max_x32(float v) {
@@ -137,24 +146,8 @@ __device__ __forceinline__ float join_terms(const int (&c)[q_terms<F32>]) {
     return (float)(c[1] * 256 + c[0]);
 }
 
-// p sv enters fp16 as p * sv * 2^(kPre - E), 2^E <= the largest |sv| so far <
-// 2^(E+1), so it is below 2^(kHead + kPre + 1) <= 2^15.  For fp32 q, p never
-// exceeds 1 and the bits above go to the second half's range.
-template <bool F32> constexpr int kHead = F32 ? 0 : 7;
-template <bool F32> constexpr int kPre = F32 ? 14 : 7;
-constexpr int kMinExp = -100;  // E's floor: the factor stays finite
-
-// V's codes as fp16 enter p.v as code * 2^-9 (cvt_pair).
-constexpr float kVUnit = 0x1p9f;
-
-// Byte b of two words of codes biased by 128 as two fp16 values code * 2^-9:
-// the byte alone in 16 bits is the subnormal (code + 128) 2^-24, and one
-// packed fma, exact, takes off the bias.
-template <int B>
-__device__ __forceinline__ h2 cvt_pair(uint32_t lo, uint32_t hi) {
-    const uint32_t u = __builtin_amdgcn_perm(hi, lo, 0x0c000c00u | (uint32_t)((4 + B) << 16) | (uint32_t)B);
-    const h2 x = __builtin_bit_cast(h2, u), mul = {(_Float16)32768.0f, (_Float16)32768.0f}, off = {(_Float16)-0.25f, (_Float16)-0.25f};
-    return __builtin_elementwise_fma(x, mul, off);
-}
+// How far above the running maximum a logit may lie (as a power of two) before
+// that moves: sums are fp32, so p may well exceed 1.
+constexpr float kHead = 8.0f;
 
 }  // namespace phi_dev

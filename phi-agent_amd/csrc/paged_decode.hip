@@ -7,7 +7,7 @@
 //   S^T = K Q^T (v_mfma_i32_16x16x64_i8): lane l holds K's token l & 15, bytes
 //     16 (l >> 4) .. + 15 of each 64: one 16-byte load of the cache's row.  The
 //     result has row l & 15 in the lane and tokens 4 (l >> 4) + i.
-//   O^T = V^T P^T (v_mfma_f32_16x16x32_f16): the sum's order is free, so k
+//   O^T = V^T P^T (v_mfma_f32_16x16x32_bf16): the sum's order is free, so k
 //     index 8 g + j (g = l >> 4) stands for the token the lane's P is of: 4 g + j
 //     of the step's first 16 tokens, 4 g + j - 4 of its second.  P is used where
 //     it lies.  V^T wants 8 tokens of one d a lane: the lane loads dim/16
@@ -16,7 +16,7 @@
 // The next step's loads are under way while a step is computed: 32 tokens are 8 KB
 // a wave at dim 128, and 12 waves a CU keep 96 KB in flight.  The four waves
 // of a block take every fourth step of its split and join in LDS.
-#include <type_traits>
+#include <algorithm>
 
 #include "paged_attention.hpp"
 
@@ -43,22 +43,21 @@ template <int DP> struct Step {
 }  // namespace
 
 // DP: dim rounded up to 64, 128 or 256.  F32: fp32 q and out, else bf16.
-// PAGE16: pages of a multiple of 16 tokens with contiguous, 16-byte aligned
-// scales and offsets within a block below 2^31, so that a tile of 16 tokens has
-// one block and its loads one scalar base; otherwise every token finds its own.
+// PAGE16: tiles_of_16, so that a tile of 16 tokens has one block and its loads
+// one scalar base; otherwise every token finds its own.
 template <int DP, bool F32, bool PAGE16>
-__global__ __launch_bounds__(64 * kWaves) void paged_decode_kernel(KvCache c, PagedAttn p, AttnSplit sp,
+__global__ __launch_bounds__(64 * kWaves) void paged_decode_kernel(KvCache c, PagedAttn p, AttnSplit sp, int max_rows,
                                                                   const int32_t* __restrict__ table) {
-    constexpr int KS = DP / 64, EB = DP / 16, NT = q_terms<F32>;
+    constexpr int KS = DP / 64, EB = DP / 16, NT = q_terms<F32>, NP = F32 ? 3 : 2;
     __shared__ float lo_[kWaves][kDecodeRows][DP];
     __shared__ float lm[kWaves][kDecodeRows], ll[kWaves][kDecodeRows];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
-    const int kh = blockIdx.y % c.heads, rt = blockIdx.y / c.heads, b = blockIdx.z;
+    const int kh = blockIdx.x % c.heads, rt = blockIdx.x / c.heads, z = blockIdx.y, b = blockIdx.z;
     const SeqInfo s = seq_info(p, c.page, b);
     const int rows = min(s.n, p.max_q) * p.group, r0 = rt * kDecodeRows;
-    const int z0 = blockIdx.x * sp.len;
-    if (r0 >= rows || (blockIdx.x > 0 && z0 >= s.kv)) return;
+    const int z0 = z * sp.len;
+    if (r0 >= rows || rows > max_rows || (z > 0 && z0 >= s.kv)) return;
     const int D = c.dim;
 
     // The lane's row of the tile (past the last: the last again, not stored).
@@ -159,8 +158,6 @@ __global__ __launch_bounds__(64 * kWaves) void paged_decode_kernel(KvCache c, Pa
 #pragma unroll
     for (int e = 0; e < EB; e++) o[e] = v4f{0, 0, 0, 0};
     float m = kNoMax, l = 0.0f;
-    int vexp = kMinExp;
-    float vlim = ldexpf(1.0f, kMinExp + 1), vmul = ldexpf(1.0f, kPre<F32> - kMinExp);
 
     auto compute = [&](const Step<DP>& st, int t0) {
         float t[8], sv[8];
@@ -200,72 +197,43 @@ __global__ __launch_bounds__(64 * kWaves) void paged_decode_kernel(KvCache c, Pa
                 sv[k] = in ? sv[k] : 0.0f;
             }
         }
-        // A larger |sv| than the running power of two covers: move it.
-        float vmax = 0.0f;
-#pragma unroll
-        for (int k = 0; k < 8; k++) vmax = fmaxf(vmax, fabsf(sv[k]));
-        float keep_v = 1.0f;
-        if (__builtin_expect(__any(vmax >= vlim), 0)) {
-            float top = 0.0f;
-#pragma unroll
-            for (int k = 0; k < 8; k++) top = fmaxf(top, __builtin_isfinite(sv[k]) ? fabsf(sv[k]) : 0.0f);
-#pragma unroll
-            for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
-            const int e = max(vexp, __builtin_amdgcn_readfirstlane((int)(__float_as_uint(top) >> 23) - 127));
-            keep_v = ldexpf(1.0f, vexp - e);
-            vexp = e;
-            vlim = ldexpf(1.0f, e + 1);
-            vmul = ldexpf(1.0f, kPre<F32> - e);
-        }
         float top = t[0];
 #pragma unroll
         for (int k = 1; k < 8; k++) top = fmaxf(top, t[k]);
         const float xm = top * rq;
-        const bool grow = xm > m + (float)kHead<F32>;
-        if (__any(grow) || keep_v != 1.0f) {
+        if (__any(xm > m + kHead)) {
             const float m2 = fmaxf(m, max_x16(max_x32(xm)));
             const float keep = __builtin_amdgcn_exp2f(m - m2);
             m = m2;
             l *= keep;
 #pragma unroll
-            for (int e = 0; e < EB; e++)
-#pragma unroll
-                for (int n = 0; n < 4; n++) o[e][n] *= keep * keep_v;
+            for (int e = 0; e < EB; e++) o[e] *= keep;
         }
-        float pv[8];
+        b8 pt[NP];  // p sv, highest bits first
 #pragma unroll
         for (int k = 0; k < 8; k++) {
             const float e = __builtin_amdgcn_exp2f(fmaf(t[k], rq, -m));
             l += e;
-            pv[k] = e * (sv[k] * vmul);
+            float x = whole || (seen >> k & 1) ? e * sv[k] : 0.0f;
+#pragma unroll
+            for (int n = 0; n < NP; n++) {
+                pt[n][k] = (__bf16)x;
+                x -= (float)pt[n][k];
+            }
         }
-        if (!whole) {
+        // Byte e of each token's word, as bf16 (a code's 7 bits are exact, so the
+        // upper half of its fp32 is it).
 #pragma unroll
-            for (int k = 0; k < 8; k++) pv[k] = seen >> k & 1 ? pv[k] : 0.0f;
-        }
-        h8 ph, pl;
+        for (int e = 0; e < EB; e++) {
+            v4i a;
 #pragma unroll
-        for (int k = 0; k < 8; k++) {
-            ph[k] = (_Float16)pv[k];
-            if (F32) pl[k] = (_Float16)(pv[k] - (float)ph[k]);
-        }
-        typename VWord<EB>::type v[8];
+            for (int k = 0; k < 4; k++) {
+                const float f0 = (float)(int8_t)(st.v[k >> 1][2 * (k & 1)][e / 4] >> 8 * (e % 4));
+                const float f1 = (float)(int8_t)(st.v[k >> 1][2 * (k & 1) + 1][e / 4] >> 8 * (e % 4));
+                a[k] = (int)__builtin_amdgcn_perm(__float_as_uint(f1), __float_as_uint(f0), 0x07060302u);
+            }
 #pragma unroll
-        for (int k = 0; k < 8; k++) v[k] = st.v[k >> 2][k & 3] ^ 0x80808080u;
-#pragma unroll
-        for (int w = 0; w < EB / 4; w++) {
-            auto product = [&](auto bc) {
-                constexpr int B = decltype(bc)::value;
-                const h2 a0 = cvt_pair<B>(v[0][w], v[1][w]), a1 = cvt_pair<B>(v[2][w], v[3][w]);
-                const h2 a2 = cvt_pair<B>(v[4][w], v[5][w]), a3 = cvt_pair<B>(v[6][w], v[7][w]);
-                const h8 a = {a0[0], a0[1], a1[0], a1[1], a2[0], a2[1], a3[0], a3[1]};
-                o[4 * w + B] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ph, o[4 * w + B], 0, 0, 0);
-                if (F32) o[4 * w + B] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pl, o[4 * w + B], 0, 0, 0);
-            };
-            product(std::integral_constant<int, 0>{});
-            product(std::integral_constant<int, 1>{});
-            product(std::integral_constant<int, 2>{});
-            product(std::integral_constant<int, 3>{});
+            for (int n = 0; n < NP; n++) o[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), pt[n], o[e], 0, 0, 0);
         }
     };
 
@@ -292,7 +260,7 @@ __global__ __launch_bounds__(64 * kWaves) void paged_decode_kernel(KvCache c, Pa
     float top = lm[0][col];
 #pragma unroll
     for (int w = 1; w < kWaves; w++) top = fmaxf(top, lm[w][col]);
-    const float unit = __builtin_amdgcn_exp2f(m - top) * ldexpf(kVUnit, vexp - kPre<F32>);
+    const float unit = __builtin_amdgcn_exp2f(m - top);
 #pragma unroll
     for (int n = 0; n < 4; n++)
 #pragma unroll
@@ -310,7 +278,7 @@ __global__ __launch_bounds__(64 * kWaves) void paged_decode_kernel(KvCache c, Pa
     float rl = 0.0f;
 #pragma unroll
     for (int w = 0; w < kWaves; w++) rl = fmaf(ll[w][row], __builtin_amdgcn_exp2f(lm[w][row] - rm), rl);
-    const int64_t at = ((int64_t)blockIdx.x * p.tokens + rtok) * p.q_heads + rhead;
+    const int64_t at = ((int64_t)z * p.tokens + rtok) * p.q_heads + rhead;
     const float inv = sp.count > 1 ? 1.0f : rl != 0.0f ? 1.0f / rl : 0.0f;
     if (sp.count > 1 && part == 0) sp.ml[2 * at] = rm, sp.ml[2 * at + 1] = rl;
 #pragma unroll
@@ -332,20 +300,19 @@ __global__ __launch_bounds__(64 * kWaves) void paged_decode_kernel(KvCache c, Pa
 }
 
 template <int DP, bool F32>
-static hipError_t launch_dp(hipStream_t stream, const KvCache& c, const PagedAttn& p, const AttnSplit& s) {
-    const int tiles = (int)(((int64_t)p.max_q * p.group + kDecodeRows - 1) / kDecodeRows);
-    const dim3 grid((unsigned)s.count, (unsigned)(tiles * c.heads), (unsigned)p.batch);
-    const bool page16 = c.page % 16 == 0 && c.s_token_stride == 1 && c.s_block_stride % 4 == 0 && c.s_head_stride % 4 == 0 &&
-                        (uintptr_t)c.ks % 16 == 0 && (uintptr_t)c.vs % 16 == 0 && 16 * c.token_stride < ((int64_t)1 << 31);
-    if (page16) hipLaunchKernelGGL((paged_decode_kernel<DP, F32, true>), grid, dim3(64 * kWaves), 0, stream, c, p, s, p.table);
-    else hipLaunchKernelGGL((paged_decode_kernel<DP, F32, false>), grid, dim3(64 * kWaves), 0, stream, c, p, s, p.table);
+static hipError_t launch_dp(hipStream_t stream, const KvCache& c, const PagedAttn& p, const AttnSplit& s, int64_t rows) {
+    const int64_t most = std::min(rows, (int64_t)p.max_q * p.group), tiles = (most + kDecodeRows - 1) / kDecodeRows;
+    const dim3 grid((unsigned)(tiles * c.heads), (unsigned)s.count, (unsigned)p.batch), block(64 * kWaves);
+    const int lim = (int)std::min<int64_t>(rows, INT32_MAX);
+    if (tiles_of_16(c)) hipLaunchKernelGGL((paged_decode_kernel<DP, F32, true>), grid, block, 0, stream, c, p, s, lim, p.table);
+    else hipLaunchKernelGGL((paged_decode_kernel<DP, F32, false>), grid, block, 0, stream, c, p, s, lim, p.table);
     return hipGetLastError();
 }
 
-hipError_t launch_paged_decode(hipStream_t stream, const KvCache& c, const PagedAttn& p, const AttnSplit& s) {
-    if (c.dim <= 64) return p.bf16 ? launch_dp<64, false>(stream, c, p, s) : launch_dp<64, true>(stream, c, p, s);
-    if (c.dim <= 128) return p.bf16 ? launch_dp<128, false>(stream, c, p, s) : launch_dp<128, true>(stream, c, p, s);
-    return p.bf16 ? launch_dp<256, false>(stream, c, p, s) : launch_dp<256, true>(stream, c, p, s);
+hipError_t launch_paged_decode(hipStream_t stream, const KvCache& c, const PagedAttn& p, const AttnSplit& s, int64_t rows) {
+    if (c.dim <= 64) return p.bf16 ? launch_dp<64, false>(stream, c, p, s, rows) : launch_dp<64, true>(stream, c, p, s, rows);
+    if (c.dim <= 128) return p.bf16 ? launch_dp<128, false>(stream, c, p, s, rows) : launch_dp<128, true>(stream, c, p, s, rows);
+    return p.bf16 ? launch_dp<256, false>(stream, c, p, s, rows) : launch_dp<256, true>(stream, c, p, s, rows);
 }
 
 }  // namespace phi_dev
