@@ -66,6 +66,7 @@ struct PagedAttn {
     int64_t tokens;
     int q_heads, group;  // group: query heads a key/value head
     int batch, max_q, max_kv, table_width, window;
+    int few_rows;  // see paged_attention.hpp
     float scale;
     bool bf16, causal;
 };

@@ -186,7 +186,7 @@ phi_status phi_hip_paged_attention(phi_stream_t stream, const void* q, int dtype
         return fail(PHI_ERR_ARG, "%s: the workspace overlaps q or out", who);
     const phi_dev::PagedAttn p{q, out, block_table, q_start, kv_len, q_token_stride, q_head_stride, out_token_stride,
                                out_head_stride, table_stride, tokens, (int)q_heads, (int)(q_heads / c.heads), (int)batch,
-                               (int)max_q, (int)max_kv, (int)table_width, window > INT32_MAX ? 0 : (int)window, scale,
+                               (int)max_q, (int)max_kv, (int)table_width, window > INT32_MAX ? 0 : (int)window, 0, scale,
                                dtype == PHI_BF16, causal != 0};
     return check_hip(phi_dev::launch_paged_attention((hipStream_t)stream, c, p, workspace), who);
 }

@@ -47,22 +47,31 @@ __device__ __forceinline__ SeqInfo seq_info(const PagedAttn& p, int page, int b)
     return s;
 }
 
-// Where a call's tokens are split over blocks, split z has the tokens
-// [z * len, (z + 1) * len) of each sequence; each leaves, for every row and head
-// (row * q_heads + head), the undivided sum of p v, m and l = sum of p in
-//   o [splits][tokens * q_heads][dim], ml [splits][tokens * q_heads][2]
-// and attn_join_kernel joins them.  One split: no workspace, out is written.
-struct AttnSplit {
+// A sequence's rows are the query heads of a key/value head x its new tokens, in
+// that order.  Sequences of at most few_rows rows go to paged_decode.hip (AttnPart
+// few), those of more to paged_chunk.hip (many; bf16 queries only).
+//
+// A part's blocks share out the (sequence, row tile, split) triples that there
+// are, kv_heads blocks each; the grid is an upper bound of their number and the
+// blocks past it end at once.  (A grid over the longest sequence's tiles and
+// splits leaves working blocks at a fixed stride among idle ones, which the
+// dispatcher deals to the same few compute units: 358 us against 118 for a chunk of
+// 512 tokens over 4352 beside seven empty sequences.)
+//
+// Split z of a sequence has its tokens [z * len, (z + 1) * len).  With count > 1
+// each leaves for its rows the undivided sum of p v, o [splits][rows][dim], and
+// the maximum and the sum of p, ml [splits][rows][2], for attn_join_kernel.
+struct AttnPart {
     int len, count;
+    int64_t rows;   // rows of o and ml a split
+    int row_pitch;  // few: rows a (sequence, key/value head) in them
+    int blocks;     // the grid, over kv_heads
     float* o;
     float* ml;
 };
 
-// A sequence's rows are the query heads of a key/value head x its new tokens, in
-// that order.  launch_paged_decode takes the sequences of at most `rows` rows;
-// launch_paged_chunk (bf16 queries only) those of more.
-hipError_t launch_paged_decode(hipStream_t stream, const KvCache& c, const PagedAttn& p, const AttnSplit& s, int64_t rows);
-hipError_t launch_paged_chunk(hipStream_t stream, const KvCache& c, const PagedAttn& p, const AttnSplit& s, int64_t rows);
+hipError_t launch_paged_decode(hipStream_t stream, const KvCache& c, const PagedAttn& p, const AttnPart& s);
+hipError_t launch_paged_chunk(hipStream_t stream, const KvCache& c, const PagedAttn& p, const AttnPart& s);
 // Rows of a block's tile.
 constexpr int kDecodeRows = 16;
 constexpr int kChunkRows = 256, kChunkRowsWide = 128;  // dim to 128, above
@@ -72,6 +81,41 @@ constexpr int kChunkRows = 256, kChunkRowsWide = 128;  // dim to 128, above
 inline bool tiles_of_16(const KvCache& c) {
     return c.page % 16 == 0 && c.s_token_stride == 1 && c.s_block_stride % 4 == 0 && c.s_head_stride % 4 == 0 &&
            (uintptr_t)c.ks % 16 == 0 && (uintptr_t)c.vs % 16 == 0 && 16 * c.token_stride < ((int64_t)1 << 31);
+}
+
+// Triple number `unit` of a part (the same in all lanes): its sequence, row tile
+// and split; b < 0: there are fewer.  A sequence's triples: late tiles first
+// (they see most tokens), splits inside.  FEW: the sequences of at most few_rows.
+struct AttnUnit {
+    int b, tile, z;
+};
+
+template <bool FEW>
+__device__ __forceinline__ AttnUnit attn_unit(const PagedAttn& p, const AttnPart& s, int page, int tile_rows, int unit) {
+    const int lane = threadIdx.x & 63;
+    for (int b0 = 0; b0 < p.batch; b0 += 64) {
+        int tiles = 0, splits = 1;
+        if (b0 + lane < p.batch) {
+            const SeqInfo q = seq_info(p, page, b0 + lane);
+            const int rows = min(q.n, p.max_q) * p.group;
+            if ((rows <= p.few_rows) == FEW) tiles = (rows + tile_rows - 1) / tile_rows;
+            splits = max(1, (q.kv + s.len - 1) / s.len);
+        }
+        int end = tiles * splits;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+            const int x = __shfl_up(end, off, 64);
+            end += lane >= off ? x : 0;
+        }
+        const uint64_t past = __ballot(end > unit);
+        if (past) {
+            const int at = __builtin_ctzll(past), local = unit - __builtin_amdgcn_readlane(end - tiles * splits, at);
+            const int n = __builtin_amdgcn_readlane(splits, at), tile = local / n;
+            return {b0 + at, __builtin_amdgcn_readlane(tiles, at) - 1 - tile, local - tile * n};
+        }
+        unit -= __builtin_amdgcn_readlane(end, 63);
+    }
+    return {-1, 0, 0};
 }
 
 // The maximum over lanes l, l ^ 16, l ^ 32, l ^ 48, and over l, l ^ 32.

@@ -85,8 +85,7 @@ __device__ __forceinline__ int k_slot(int t, int n) {
 // DP: dim rounded up to 64, 128 or 256; NW waves, 32 rows each; PAGE16 as in
 // paged_decode.hip.
 template <int DP, int NW, bool PAGE16>
-__global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel(KvCache c, PagedAttn p, AttnSplit sp,
-                                                                              int min_rows,
+__global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel(KvCache c, PagedAttn p, AttnPart sp,
                                                                               const int32_t* __restrict__ table) {
     constexpr int KS = DP / 16, OT = DP / 32;
     constexpr int NVI = DP == 256 ? 2 : 1, NKI = DP / 64;  // V's and K's items a lane
@@ -95,12 +94,12 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, h = lane >> 5;
     const int heads = c.heads, D = c.dim;
-    // Late tiles, which see most tokens, first.
-    const int bh = blockIdx.x % (heads * p.batch), tiles = gridDim.x / (heads * p.batch);
-    const int rt = tiles - 1 - blockIdx.x / (heads * p.batch), kh = bh % heads, b = bh / heads;
+    const int kh = blockIdx.x % heads;
+    const AttnUnit unit_of = attn_unit<false>(p, sp, c.page, 32 * NW, blockIdx.x / heads);
+    if (unit_of.b < 0) return;
+    const int b = unit_of.b, z = unit_of.z;
     const SeqInfo s = seq_info(p, c.page, b);
-    const int rows = min(s.n, p.max_q) * p.group, r0 = rt * 32 * NW, z0 = blockIdx.y * sp.len;
-    if (r0 >= rows || rows <= min_rows || (blockIdx.y > 0 && z0 >= s.kv)) return;
+    const int rows = min(s.n, p.max_q) * p.group, r0 = unit_of.tile * 32 * NW, z0 = z * sp.len;
 
     // The lane's row, and the ranges of the wave's rows and of the block's.
     const int w0 = r0 + 32 * wave;
@@ -160,8 +159,9 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel
     uint32_t vraw[NVI][8];
     float vsc[NVI][8];
     v4i kraw[NKI];
-    float ksc[NKI];
-    uint32_t there = 0;  // K's wave: the group's tokens, a bit each
+    float ksc[NKI], kvs[NKI];
+    uint32_t vok = 0, kok = 0;  // bit n: item or token n of the above is there
+    uint32_t there = 0;         // K's wave: the group's tokens, a bit each
     auto block_at = [&](int page, bool& ok) {
         const int blk = trow[min(page, last_page)];
         ok = blk >= 0 && blk < c.blocks;
@@ -169,8 +169,9 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel
     };
     const bool page4 = c.page % 4 == 0;
 
-    // Codes and scales of a tile's group; a token at hi or past it, or without a
-    // block, reads whatever lies in the last page or block 0 and counts as scale 0.
+    // Codes and scales of a tile's group, not looked at before they are staged; a
+    // token at hi or past it, or without a block, reads whatever lies in the last
+    // page or block 0 and counts as scale 0.
     auto load = [&](int t0) {
         const int g0 = t0 + 16 * group;
         int64_t at = 0, sat = 0;
@@ -196,6 +197,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel
             return ok && g0 + n < hi;
         };
         if (does_v) {
+            vok = 0;
 #pragma unroll
             for (int it = 0; it < NVI; it++) {
                 const int item = (it * 64 + lane) % (DP / 2), ih = item / (DP / 4), dq = item % (DP / 4);
@@ -216,23 +218,23 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel
                             ok &= on;
                         }
                         vraw[it][4 * half + j] = *(const uint32_t*)(c.v + a + d);
-                        const float x = c.vs[sa];
-                        vsc[it][4 * half + j] = ok && __builtin_isfinite(x) ? x : 0.0f;
+                        vsc[it][4 * half + j] = c.vs[sa];
+                        vok |= ok ? 1u << (8 * it + 4 * half + j) : 0u;
                     }
                 }
             }
         }
         if (does_k) {
             int64_t a, sa;
+            kok = 0;
             there = (uint32_t)__ballot(find(lane & 15, a, sa)) & 0xffffu;
 #pragma unroll
             for (int it = 0; it < NKI; it++) {
                 const int item = it * 64 + lane, n = item / (DP / 16), ch = item % (DP / 16);
-                const bool ok = find(n, a, sa);
+                kok |= find(n, a, sa) ? 1u << it : 0u;
                 kraw[it] = *(const v4i*)(c.k + a + (16 * ch < D ? 16 * ch : 0));
-                const float x = c.ks[sa], y = c.vs[sa];
-                // A token whose value is not finite is NaN to the rows that see it.
-                ksc[it] = !ok ? 0.0f : __builtin_isfinite(y) ? x : __builtin_nanf("");
+                ksc[it] = c.ks[sa];
+                kvs[it] = c.vs[sa];
             }
         }
     };
@@ -241,7 +243,10 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel
 #pragma unroll
         for (int it = 0; it < NVI; it++)
 #pragma unroll
-            for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(vsc[it][j]));
+            for (int j = 0; j < 8; j++) {
+                vsc[it][j] = (vok >> (8 * it + j) & 1) && __builtin_isfinite(vsc[it][j]) ? vsc[it][j] : 0.0f;
+                top = fmaxf(top, fabsf(vsc[it][j]));
+            }
         const int e = exp_of(wave_top(top));
         if (lane == 0) to.v_exp[group] = e;
         const float unit = pow2(7 - e);
@@ -271,7 +276,11 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel
     auto stage_k = [&](ChunkTile<DP>& to) {
         float top = 0.0f;
 #pragma unroll
-        for (int it = 0; it < NKI; it++) top = fmaxf(top, __builtin_isfinite(ksc[it]) ? fabsf(ksc[it]) : 0.0f);
+        for (int it = 0; it < NKI; it++) {
+            // A token whose value is not finite is NaN to the rows that see it.
+            ksc[it] = !(kok >> it & 1) ? 0.0f : __builtin_isfinite(kvs[it]) ? ksc[it] : __builtin_nanf("");
+            top = fmaxf(top, __builtin_isfinite(ksc[it]) ? fabsf(ksc[it]) : 0.0f);
+        }
         const int e = exp_of(wave_top(top));
         if (lane == 0) to.k_unit[group] = pow2(e - 7), to.seen[group] = there;
         const float unit = pow2(7 - e);
@@ -402,7 +411,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel
     l = add_x32(l);
     if (w0 + col >= rows) return;
     const bool split = sp.count > 1;
-    const int64_t at = ((int64_t)blockIdx.y * p.tokens + token) * p.q_heads + head;
+    const int64_t at = z * sp.rows + token * p.q_heads + head;
     // O holds sum p v in units of 2^-(kP + 7 - vexp), l of 2^-kP.
     const float unit = pow2(max(-126, vexp - 7)) * (split ? 1.0f / (1 << kP) : l != 0.0f ? 1.0f / l : 0.0f);
     if (split && h == 0) sp.ml[2 * at] = m, sp.ml[2 * at + 1] = l * (1.0f / (1 << kP));
@@ -431,9 +440,8 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel
 }
 
 template <int DP, int NW>
-static hipError_t launch_dp(hipStream_t stream, const KvCache& c, const PagedAttn& p, const AttnSplit& s, int64_t rows) {
-    const int64_t most = (int64_t)p.max_q * p.group, tiles = (most + 32 * NW - 1) / (32 * NW);
-    const dim3 grid((unsigned)(tiles * c.heads * p.batch), (unsigned)s.count);
+static hipError_t launch_dp(hipStream_t stream, const KvCache& c, const PagedAttn& p, const AttnPart& s) {
+    const dim3 grid((unsigned)s.blocks * (unsigned)c.heads), block(64 * NW);
     const bool page16 = tiles_of_16(c);
     const void* f = page16 ? (const void*)paged_chunk_kernel<DP, NW, true> : (const void*)paged_chunk_kernel<DP, NW, false>;
     const size_t lds = 2 * sizeof(ChunkTile<DP>);
@@ -441,15 +449,15 @@ static hipError_t launch_dp(hipStream_t stream, const KvCache& c, const PagedAtt
         const hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (e != hipSuccess) return e;
     }
-    if (page16) hipLaunchKernelGGL((paged_chunk_kernel<DP, NW, true>), grid, dim3(64 * NW), lds, stream, c, p, s, (int)rows, p.table);
-    else hipLaunchKernelGGL((paged_chunk_kernel<DP, NW, false>), grid, dim3(64 * NW), lds, stream, c, p, s, (int)rows, p.table);
+    if (page16) hipLaunchKernelGGL((paged_chunk_kernel<DP, NW, true>), grid, block, lds, stream, c, p, s, p.table);
+    else hipLaunchKernelGGL((paged_chunk_kernel<DP, NW, false>), grid, block, lds, stream, c, p, s, p.table);
     return hipGetLastError();
 }
 
-hipError_t launch_paged_chunk(hipStream_t stream, const KvCache& c, const PagedAttn& p, const AttnSplit& s, int64_t rows) {
-    if (c.dim <= 64) return launch_dp<64, kChunkRows / 32>(stream, c, p, s, rows);
-    if (c.dim <= 128) return launch_dp<128, kChunkRows / 32>(stream, c, p, s, rows);
-    return launch_dp<256, kChunkRowsWide / 32>(stream, c, p, s, rows);
+hipError_t launch_paged_chunk(hipStream_t stream, const KvCache& c, const PagedAttn& p, const AttnPart& s) {
+    if (c.dim <= 64) return launch_dp<64, kChunkRows / 32>(stream, c, p, s);
+    if (c.dim <= 128) return launch_dp<128, kChunkRows / 32>(stream, c, p, s);
+    return launch_dp<256, kChunkRowsWide / 32>(stream, c, p, s);
 }
 
 }  // namespace phi_dev

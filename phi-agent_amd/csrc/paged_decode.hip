@@ -16,8 +16,6 @@
 // The next step's loads are under way while a step is computed: 32 tokens are 8 KB
 // a wave at dim 128, and 12 waves a CU keep 96 KB in flight.  The four waves
 // of a block take every fourth step of its split and join in LDS.
-#include <algorithm>
-
 #include "paged_attention.hpp"
 
 namespace phi_dev {
@@ -46,18 +44,19 @@ template <int DP> struct Step {
 // PAGE16: tiles_of_16, so that a tile of 16 tokens has one block and its loads
 // one scalar base; otherwise every token finds its own.
 template <int DP, bool F32, bool PAGE16>
-__global__ __launch_bounds__(64 * kWaves) void paged_decode_kernel(KvCache c, PagedAttn p, AttnSplit sp, int max_rows,
+__global__ __launch_bounds__(64 * kWaves) void paged_decode_kernel(KvCache c, PagedAttn p, AttnPart sp,
                                                                   const int32_t* __restrict__ table) {
     constexpr int KS = DP / 64, EB = DP / 16, NT = q_terms<F32>, NP = F32 ? 3 : 2;
     __shared__ float lo_[kWaves][kDecodeRows][DP];
     __shared__ float lm[kWaves][kDecodeRows], ll[kWaves][kDecodeRows];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
-    const int kh = blockIdx.x % c.heads, rt = blockIdx.x / c.heads, z = blockIdx.y, b = blockIdx.z;
+    const int kh = blockIdx.x % c.heads;
+    const AttnUnit unit = attn_unit<true>(p, sp, c.page, kDecodeRows, blockIdx.x / c.heads);
+    if (unit.b < 0) return;
+    const int b = unit.b, z = unit.z;
     const SeqInfo s = seq_info(p, c.page, b);
-    const int rows = min(s.n, p.max_q) * p.group, r0 = rt * kDecodeRows;
-    const int z0 = z * sp.len;
-    if (r0 >= rows || rows > max_rows || (z > 0 && z0 >= s.kv)) return;
+    const int rows = min(s.n, p.max_q) * p.group, r0 = unit.tile * kDecodeRows, z0 = z * sp.len;
     const int D = c.dim;
 
     // The lane's row of the tile (past the last: the last again, not stored).
@@ -260,13 +259,13 @@ __global__ __launch_bounds__(64 * kWaves) void paged_decode_kernel(KvCache c, Pa
     float top = lm[0][col];
 #pragma unroll
     for (int w = 1; w < kWaves; w++) top = fmaxf(top, lm[w][col]);
-    const float unit = __builtin_amdgcn_exp2f(m - top);
+    const float share = __builtin_amdgcn_exp2f(m - top);
 #pragma unroll
     for (int n = 0; n < 4; n++)
 #pragma unroll
         for (int e = 0; e < EB; e += 4)
             *(v4f*)&lo_[wave][col][EB * (4 * g + n) + e] =
-                v4f{o[e][n] * unit, o[e + 1][n] * unit, o[e + 2][n] * unit, o[e + 3][n] * unit};
+                v4f{o[e][n] * share, o[e + 1][n] * share, o[e + 2][n] * share, o[e + 3][n] * share};
     __syncthreads();
     const int row = threadIdx.x / 16, part = threadIdx.x & 15;  // a row a team of 16
     if (r0 + row >= rows) return;
@@ -278,7 +277,7 @@ __global__ __launch_bounds__(64 * kWaves) void paged_decode_kernel(KvCache c, Pa
     float rl = 0.0f;
 #pragma unroll
     for (int w = 0; w < kWaves; w++) rl = fmaf(ll[w][row], __builtin_amdgcn_exp2f(lm[w][row] - rm), rl);
-    const int64_t at = ((int64_t)z * p.tokens + rtok) * p.q_heads + rhead;
+    const int64_t at = z * sp.rows + ((int64_t)b * c.heads + kh) * sp.row_pitch + r0 + row;
     const float inv = sp.count > 1 ? 1.0f : rl != 0.0f ? 1.0f / rl : 0.0f;
     if (sp.count > 1 && part == 0) sp.ml[2 * at] = rm, sp.ml[2 * at + 1] = rl;
 #pragma unroll
@@ -300,19 +299,17 @@ __global__ __launch_bounds__(64 * kWaves) void paged_decode_kernel(KvCache c, Pa
 }
 
 template <int DP, bool F32>
-static hipError_t launch_dp(hipStream_t stream, const KvCache& c, const PagedAttn& p, const AttnSplit& s, int64_t rows) {
-    const int64_t most = std::min(rows, (int64_t)p.max_q * p.group), tiles = (most + kDecodeRows - 1) / kDecodeRows;
-    const dim3 grid((unsigned)(tiles * c.heads), (unsigned)s.count, (unsigned)p.batch), block(64 * kWaves);
-    const int lim = (int)std::min<int64_t>(rows, INT32_MAX);
-    if (tiles_of_16(c)) hipLaunchKernelGGL((paged_decode_kernel<DP, F32, true>), grid, block, 0, stream, c, p, s, lim, p.table);
-    else hipLaunchKernelGGL((paged_decode_kernel<DP, F32, false>), grid, block, 0, stream, c, p, s, lim, p.table);
+static hipError_t launch_dp(hipStream_t stream, const KvCache& c, const PagedAttn& p, const AttnPart& s) {
+    const dim3 grid((unsigned)s.blocks * (unsigned)c.heads), block(64 * kWaves);
+    if (tiles_of_16(c)) hipLaunchKernelGGL((paged_decode_kernel<DP, F32, true>), grid, block, 0, stream, c, p, s, p.table);
+    else hipLaunchKernelGGL((paged_decode_kernel<DP, F32, false>), grid, block, 0, stream, c, p, s, p.table);
     return hipGetLastError();
 }
 
-hipError_t launch_paged_decode(hipStream_t stream, const KvCache& c, const PagedAttn& p, const AttnSplit& s, int64_t rows) {
-    if (c.dim <= 64) return p.bf16 ? launch_dp<64, false>(stream, c, p, s, rows) : launch_dp<64, true>(stream, c, p, s, rows);
-    if (c.dim <= 128) return p.bf16 ? launch_dp<128, false>(stream, c, p, s, rows) : launch_dp<128, true>(stream, c, p, s, rows);
-    return p.bf16 ? launch_dp<256, false>(stream, c, p, s, rows) : launch_dp<256, true>(stream, c, p, s, rows);
+hipError_t launch_paged_decode(hipStream_t stream, const KvCache& c, const PagedAttn& p, const AttnPart& s) {
+    if (c.dim <= 64) return p.bf16 ? launch_dp<64, false>(stream, c, p, s) : launch_dp<64, true>(stream, c, p, s);
+    if (c.dim <= 128) return p.bf16 ? launch_dp<128, false>(stream, c, p, s) : launch_dp<128, true>(stream, c, p, s);
+    return p.bf16 ? launch_dp<256, false>(stream, c, p, s) : launch_dp<256, true>(stream, c, p, s);
 }
 
 }  // namespace phi_dev
