@@ -77,10 +77,13 @@ constexpr int kDecodeRows = 16;
 constexpr int kChunkRows = 256, kChunkRowsWide = 128;  // dim to 128, above
 
 // Whether 16 tokens from a multiple of 16 lie in one block, their scales in a
-// row at 16-byte alignment and their codes' offsets in it within 31 bits.
+// row at 16-byte alignment, with offsets in the block and strides of blocks
+// within 31 bits.
 inline bool tiles_of_16(const KvCache& c) {
+    const int64_t lim = (int64_t)1 << 31;
     return c.page % 16 == 0 && c.s_token_stride == 1 && c.s_block_stride % 4 == 0 && c.s_head_stride % 4 == 0 &&
-           (uintptr_t)c.ks % 16 == 0 && (uintptr_t)c.vs % 16 == 0 && 16 * c.token_stride < ((int64_t)1 << 31);
+           (uintptr_t)c.ks % 16 == 0 && (uintptr_t)c.vs % 16 == 0 && c.page * c.token_stride < lim && c.block_stride < lim &&
+           c.s_block_stride < lim;
 }
 
 // Triple number `unit` of a part (the same in all lanes): its sequence, row tile

@@ -1,23 +1,30 @@
 // Attention of chunks of new tokens over the paged int8 cache (bf16 queries).
 //
-// Bound by the matrix cores, and next by LDS reads and the softmax's vector
-// work, all within a factor of 1.3 of each other, so each is kept small:
+// Bound by the matrix cores, and next to them by LDS reads and vector work, all
+// near each other, so each is kept small and they are made to overlap:
 //   - A block holds 32 rows a wave (query heads of one key/value head x new
 //     tokens, in that order, so that heads share the cache's tokens) and walks
 //     the tokens in tiles of 64.  Q, O and the softmax stay in registers.
 //   - K and V are made fp16 once a block: the tile's codes come to registers one
-//     tile ahead, become code * scale * 2^E (E: a power of two for every 16
-//     tokens, so that all of them use fp16's range) in one instruction a code,
-//     and go to the other half of a double buffer in LDS in the order in
-//     which the products read them, without bank conflicts.  A logit so has one
-//     rounding to 11 bits for each k_d, at random sides; with q exact in fp16
-//     (8 bits, scaled by a power of two) its error is some 2^-13 |s| / sqrt(dim).
-//     int8 products, exact, cost the same on the matrix cores but three more
-//     vector instructions for every logit (join, convert, scale).
+//     tile ahead, become code * scale in the unit of a power of two for every 16
+//     tokens (so that all of them use fp16's range), and go to a double buffer in
+//     LDS in the order in which the products read them, without bank
+//     conflicts.  K: one fp32 product and one rounding to 11 bits a code, at
+//     random sides, so that a logit is off by some 2^-13 |s| / sqrt(dim) (q is
+//     exact in fp16).  V: the scale has 11 bits too, which makes it one packed
+//     instruction for two codes.
+//     int8 products for q.k, exact, cost the matrix cores the same but the
+//     vector unit three more instructions for every logit (join, convert, scale).
 //   - S^T = K Q^T and O^T = V^T P^T (v_mfma_f32_32x32x16_f16): the logits' layout
 //     is already that of P's operand, as in paged_decode.hip.
-//   - The running maximum moves only when a logit exceeds it by a factor of 2^kUp, and
-//     masks are looked at only in tiles that a mask or the length cuts.
+//   - The running maximum moves only when a logit exceeds it by a factor of 2^kUp,
+//     and masks are looked at only in tiles that a mask or the length cuts.
+//   - Waves 0-3 and 4-7 (one of each on a SIMD) run half a tile apart: while one
+//     group has its products, the other has its softmax and stages the next
+//     tiles, waves 0-3 V's and 4-7 K's.
+#include <type_traits>
+#include <utility>
+
 #include "paged_attention.hpp"
 
 namespace phi_dev {
@@ -32,6 +39,8 @@ constexpr int kGroups = kTile / 16;
 // and an absolute error of 2^-39 of it from there.
 constexpr int kP = 14, kUp = 1;
 constexpr int kMinExp = -100;  // of a group's unit: its inverse stays finite
+// V's fp16 is code * M 2^-24, M = scale * 2^(kM - E) below 2^15.
+constexpr int kM = 14;
 
 typedef uint32_t u2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
@@ -46,19 +55,36 @@ __device__ __forceinline__ void lds_barrier() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-// Two codes, biased by 128, that lie alone in the halves of u: code * f + 0 as
-// fp16, the bias taken off in the same fma (f24 = f 2^24: the halves are
-// subnormals (code + 128) 2^-24).
-__device__ __forceinline__ h2 scale_pair(uint32_t u, float f24a, float fa, float f24b, float fb) {
-    const h2 x = __builtin_bit_cast(h2, u);
-    return h2{(_Float16)fmaf((float)x[0], f24a, -128.0f * fa), (_Float16)fmaf((float)x[1], f24b, -128.0f * fb)};
+// Two codes, biased by 128, that lie alone in the halves of u: code * f as
+// fp16, the bias taken off in the same fma (the halves are the subnormals (code +
+// 128) 2^-24; f24 = f 2^24, off = -128 f).
+__device__ __forceinline__ uint32_t scale_pair(uint32_t u, float f24, float off) {
+    uint32_t r;
+    asm("v_fma_mixlo_f16 %0, %1, %2, %3 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(u), "v"(f24), "v"(off));
+    asm("v_fma_mixhi_f16 %0, %1, %2, %3 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "+v"(r) : "v"(u), "v"(f24), "v"(off));
+    return r;
 }
 
-// max over a wave's lanes of a value >= 0, uniform.
-__device__ __forceinline__ float wave_top(float v) {
-#pragma unroll
-    for (int off = 8; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
-    return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(max_x16(max_x32(v)))));
+template <int N> using int_c = std::integral_constant<int, N>;
+
+// f(0), f(1), .. f(N - 1), each with its number as a type.
+template <class F, int... I>
+__device__ __forceinline__ void each_of(F f, std::integer_sequence<int, I...>) {
+    (f(int_c<I>{}), ...);
+}
+template <int N, class F>
+__device__ __forceinline__ void each(F f) {
+    each_of(f, std::make_integer_sequence<int, N>{});
+}
+
+// max over 16 lanes of a value >= 0; uniform where every 16 lanes hold the same values.
+__device__ __forceinline__ float row_top(float v) {
+    uint32_t u = __float_as_uint(v);
+    u = max(u, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u, 0xB1, 0xF, 0xF, false));   // quad_perm 1,0,3,2
+    u = max(u, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u, 0x4E, 0xF, 0xF, false));   // quad_perm 2,3,0,1
+    u = max(u, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u, 0x141, 0xF, 0xF, false));  // row_half_mirror
+    u = max(u, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u, 0x140, 0xF, 0xF, false));  // row_mirror
+    return __uint_as_float(__builtin_amdgcn_readfirstlane(u));
 }
 
 // E of a group of scales: 2^E <= top < 2^(E+1), within [kMinExp, 127].
@@ -70,11 +96,19 @@ __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)
 }  // namespace
 
 template <int DP> struct ChunkTile {
-    _Float16 k[kTile * DP];  // rows of DP, 16-byte chunk n of row t in slot n ^ swizzle(t)
+    _Float16 k[kTile * DP];  // rows of DP, 16-byte chunk n of row t in slot k_slot(t, n)
     _Float16 v[kTile * DP];  // [2 group + half][slot][8 tokens], slot = (d % 4) DP / 4 + d / 4
-    float k_unit[kGroups];   // 2^(Ek - 7)
-    int v_exp[kGroups];      // Ev
-    uint32_t seen[kGroups];  // bit t: token t of the group is there
+};
+// Of a tile's 16-token groups: 2^(Ek - 7), Ev, and bit t: token t is there.
+struct ChunkMeta {
+    float k_unit[kGroups];
+    int v_exp[kGroups];
+    uint32_t seen[kGroups];
+};
+template <int DP> struct ChunkLds {
+    ChunkTile<DP> tile[2];
+    // Of tile n in n % 4, staged with its K.
+    ChunkMeta meta[4];
 };
 
 template <int DP>
@@ -90,7 +124,8 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel
     constexpr int KS = DP / 16, OT = DP / 32;
     constexpr int NVI = DP == 256 ? 2 : 1, NKI = DP / 64;  // V's and K's items a lane
     extern __shared__ __align__(16) uint8_t lds_raw[];
-    ChunkTile<DP>* tile = (ChunkTile<DP>*)lds_raw;
+    ChunkLds<DP>& lds = *(ChunkLds<DP>*)lds_raw;
+    ChunkTile<DP>* tile = lds.tile;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, h = lane >> 5;
     const int heads = c.heads, D = c.dim;
@@ -111,7 +146,6 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel
     auto hi_of = [&](int ps) { return min(p.causal ? min(s.kv, ps + 1) : s.kv, z0 + sp.len); };
     auto lo_of = [&](int ps) { return max(p.window > 0 ? max(0, ps + 1 - p.window) : 0, z0); };
     const int hi = hi_of(pos_of(r0 + 32 * NW - 1)), lo = lo_of(pos_of(r0));
-    const int wave_hi = w0 < rows ? hi_of(pos_of(w0 + 31)) : 0, wave_lo = lo_of(pos_of(w0));
     const int all_hi = hi_of(pos_of(w0)), all_lo = lo_of(pos_of(w0 + 31));
 
     // Q in fp16, exactly but for elements below 2^-21 of the row's largest,
@@ -151,154 +185,191 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel
         }
     }
 
-    // ---- the tile's codes: wave w takes 16 tokens, V's or (four waves: and) K's ----
-    const bool does_v = NW == 4 || wave < 4, does_k = NW == 4 || wave >= 4;
-    const int group = wave & 3;
+    // ---- the tile's codes: a wave takes 16 tokens, V's or (four waves: and) K's.
+    // Lane l finds token l & 15 and has its scales; a token at hi or past it, or
+    // without a block, reads whatever lies in the last page or block 0 and counts
+    // as scale 0.  Loads run a tile ahead of what is being staged, and the table's
+    // entry for them two; nothing loaded is looked at before.
+    const int group = wave & 3, n16 = lane & 15;
     const int32_t* trow = table + (int64_t)b * p.table_stride;
     const int last_page = page_of(c, max(hi - 1, 0));
-    uint32_t vraw[NVI][8];
-    float vsc[NVI][8];
-    v4i kraw[NKI];
-    float ksc[NKI], kvs[NKI];
-    uint32_t vok = 0, kok = 0;  // bit n: item or token n of the above is there
-    uint32_t there = 0;         // K's wave: the group's tokens, a bit each
-    auto block_at = [&](int page, bool& ok) {
-        const int blk = trow[min(page, last_page)];
-        ok = blk >= 0 && blk < c.blocks;
-        return (int64_t)(ok ? blk : 0);
+    struct Raw {
+        uint32_t w[8 * NVI > 4 * NKI ? 8 * NVI : 4 * NKI];  // V's items' 8 words, K's items' 4
+        float vs, ks;
+        int ok;   // token l & 15 is there
+        int blk;  // the next load's block, fetched one load ahead
     };
-    const bool page4 = c.page % 4 == 0;
+    // V's (and, with eight waves, K's in its place), K's: being staged, and loading.
+    Raw raw_of[NW == 8 ? 1 : 2], next_of[NW == 8 ? 1 : 2];
+    Raw &raw_v = raw_of[0], &raw_k = raw_of[NW == 8 ? 0 : 1], &next_v = next_of[0], &next_k = next_of[NW == 8 ? 0 : 1];
+    // A vector load, also where the entry is uniform: a scalar one would have the
+    // LDS reads around it wait for each other.
+    int lane0 = 0;
+    asm("" : "+v"(lane0));
+    auto fetch = [&](Raw& raw, int t0) __attribute__((always_inline)) {
+        const int t = min(t0 + 16 * group + (PAGE16 ? 0 : n16), hi - 1);
+        raw.blk = trow[min(page_of(c, t), last_page) + lane0];
+    };
+    // V's item of a lane: 4 d of 8 tokens; K's: 16 codes of a token.
+    auto v_item = [&](int it) { return (it * 64 + lane) % (DP / 2); };
+    auto k_token = [&](int it) { return (it * 64 + lane) / (DP / 16); };
+    auto k_chunk = [&](int it) { return (it * 64 + lane) % (DP / 16); };
+    auto token_of = [](int ih, int j) { return 8 * (j >> 2) + 4 * ih + (j & 3); };
+    const int ts = (int)c.token_stride;
+    uint32_t v_off[NVI], k_off[NKI];  // PAGE16: a lane's offset in its group's rows
+#pragma unroll
+    for (int it = 0; it < NVI; it++) {
+        const int dq = v_item(it) % (DP / 4);
+        v_off[it] = (PAGE16 ? 4 * (v_item(it) / (DP / 4)) * ts : 0) + (4 * dq < D ? 4 * dq : 0);
+    }
+#pragma unroll
+    for (int it = 0; it < NKI; it++) k_off[it] = (PAGE16 ? k_token(it) * ts : 0) + (16 * k_chunk(it) < D ? 16 * k_chunk(it) : 0);
 
-    // Codes and scales of a tile's group, not looked at before they are staged; a
-    // token at hi or past it, or without a block, reads whatever lies in the last
-    // page or block 0 and counts as scale 0.
-    auto load = [&](int t0) {
+    // Codes and scales of the group's tokens from t0 on: V's or K's.
+    const int64_t s_head = kh * c.s_head_stride;
+    auto load = [&](Raw& raw, int t0, bool is_k) __attribute__((always_inline)) {
         const int g0 = t0 + 16 * group;
-        int64_t at = 0, sat = 0;
-        bool gok = true;
+        const int8_t* codes = (is_k ? c.k : c.v) + kh * c.head_stride;
+        const int entry = PAGE16 ? __builtin_amdgcn_readfirstlane(raw.blk) : raw.blk;
+        const bool ok = entry >= 0 && entry < c.blocks;
+        const int64_t blk = ok ? entry : 0;
+        raw.ok = ok && g0 + n16 < hi;
+        const int t = min(g0 + (PAGE16 ? 0 : n16), hi - 1), in = (PAGE16 ? t & ~15 : t) - page_of(c, t) * c.page;
         if (PAGE16) {
-            const int t = min(g0, hi - 1), page = page_of(c, t), in = (t & ~15) - page * c.page;
-            const int64_t blk = block_at(page, gok);
-            at = blk * c.block_stride + kh * c.head_stride + (int64_t)in * c.token_stride;
-            sat = blk * c.s_block_stride + kh * c.s_head_stride + in;
-        }
-        // Token n (0..15) of the group: its codes' offset, its scales', whether it is there.
-        auto find = [&](int n, int64_t& a, int64_t& sa) {
-            if (PAGE16) {
-                a = at + (uint32_t)(n * (int)c.token_stride);
-                sa = sat + n;
-                return gok && g0 + n < hi;
-            }
-            const int t = min(g0 + n, hi - 1), page = page_of(c, t), in = t - page * c.page;
-            bool ok;
-            const int64_t blk = block_at(page, ok);
-            a = blk * c.block_stride + kh * c.head_stride + in * c.token_stride;
-            sa = blk * c.s_block_stride + kh * c.s_head_stride + in * c.s_token_stride;
-            return ok && g0 + n < hi;
-        };
-        if (does_v) {
-            vok = 0;
+            // 32-bit strides within a block and of blocks (tiles_of_16); the lane's
+            // offsets stay 32-bit beside a scalar base.
+            codes += (uint64_t)(uint32_t)blk * (uint32_t)c.block_stride + (uint32_t)in * (uint32_t)ts;
+            const int64_t sat = (int64_t)((uint64_t)(uint32_t)blk * (uint32_t)c.s_block_stride) + s_head + in;
+            uint32_t at = n16;
+            asm("" : "+v"(at));
+            raw.vs = (c.vs + sat)[at];
+            if (is_k) {
+                raw.ks = (c.ks + sat)[at];
 #pragma unroll
-            for (int it = 0; it < NVI; it++) {
-                const int item = (it * 64 + lane) % (DP / 2), ih = item / (DP / 4), dq = item % (DP / 4);
-                const int d = 4 * dq < D ? 4 * dq : 0;
+                for (int it = 0; it < NKI; it++) {
+                    uint32_t off = k_off[it];
+                    asm("" : "+v"(off));
+                    *(v4i*)&raw.w[4 * it] = *(const v4i*)(codes + off);
+                }
+            } else {
 #pragma unroll
-                for (int half = 0; half < 2; half++) {
-                    int64_t a = 0, sa = 0;
-                    bool ok = false;
+                for (int j = 0; j < 8; j++) {
+                    const int8_t* row = codes + (uint32_t)(token_of(0, j) * ts);
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const int n = 8 * half + 4 * ih + j;
-                        if (PAGE16 || !page4 || j == 0) {
-                            ok = find(n, a, sa);
-                        } else {  // in the block of the first of the four, if before hi
-                            const bool on = g0 + n < hi;
-                            a += on ? c.token_stride : 0;
-                            sa += on ? c.s_token_stride : 0;
-                            ok &= on;
-                        }
-                        vraw[it][4 * half + j] = *(const uint32_t*)(c.v + a + d);
-                        vsc[it][4 * half + j] = c.vs[sa];
-                        vok |= ok ? 1u << (8 * it + 4 * half + j) : 0u;
+                    for (int it = 0; it < NVI; it++) {
+                        uint32_t off = v_off[it];
+                        asm("" : "+v"(off));
+                        raw.w[8 * it + j] = *(const uint32_t*)(row + off);
                     }
                 }
             }
-        }
-        if (does_k) {
-            int64_t a, sa;
-            kok = 0;
-            there = (uint32_t)__ballot(find(lane & 15, a, sa)) & 0xffffu;
+        } else {
+            const int64_t at = blk * c.block_stride + in * c.token_stride;
+            const int64_t sat = blk * c.s_block_stride + s_head + in * c.s_token_stride;
+            raw.vs = c.vs[sat];
+            if (is_k) {
+                raw.ks = c.ks[sat];
 #pragma unroll
-            for (int it = 0; it < NKI; it++) {
-                const int item = it * 64 + lane, n = item / (DP / 16), ch = item % (DP / 16);
-                kok |= find(n, a, sa) ? 1u << it : 0u;
-                kraw[it] = *(const v4i*)(c.k + a + (16 * ch < D ? 16 * ch : 0));
-                ksc[it] = c.ks[sa];
-                kvs[it] = c.vs[sa];
+                for (int it = 0; it < NKI; it++) *(v4i*)&raw.w[4 * it] = *(const v4i*)(codes + __shfl(at, k_token(it), 64) + k_off[it]);
+            } else {
+#pragma unroll
+                for (int it = 0; it < NVI; it++)
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        raw.w[8 * it + j] = *(const uint32_t*)(codes + __shfl(at, token_of(v_item(it) / (DP / 4), j), 64) + v_off[it]);
+            }
+        }
+        fetch(raw, t0 + kTile);
+    };
+    // E of the group's V scales, the same from V's wave and K's: 2^E <= the
+    // largest that is there and finite.
+    auto v_exp_of = [&](const Raw& raw, float& f) __attribute__((always_inline)) {
+        f = (raw.ok != 0) & __builtin_isfinite(raw.vs) ? raw.vs : 0.0f;
+        return exp_of(row_top(fabsf(f)));
+    };
+    // Staging in pieces without a branch and of a few instructions each, which the
+    // turn of products takes one at a time between its own.  Both kinds: take what
+    // was loaded, load the tile after, the scales; then an eighth of an item's
+    // codes each.
+    constexpr int kVPieces = 5 + 8 * NVI, kKPieces = 5 + 8 * NKI;
+    int v_e = 0;
+    float v_f = 0.0f;
+    h2 v_mul[NVI][4], v_sub[NVI][4];
+    h8 v_out;
+    auto v_piece = [&](auto index, ChunkTile<DP>& to, int next_t0) __attribute__((always_inline)) {
+        constexpr int P = decltype(index)::value;
+        if constexpr (P == 0) {
+            raw_v = next_v;
+        } else if constexpr (P == 1) {
+            load(next_v, next_t0, false);
+        } else if constexpr (P == 2) {
+            v_e = v_exp_of(raw_v, v_f);
+        } else if constexpr (P == 3) {
+            // Lane l has the factors of tokens l & 15 and the next, as a pair.
+            const float m0 = v_f * pow2(kM - v_e);
+            const float m1 = __uint_as_float(__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(m0), 0xF5, 0xF, 0xF, false));  // quad_perm 1,1,3,3
+            const int pair = (int)__builtin_bit_cast(uint32_t, h2{(_Float16)m0, (_Float16)m1});
+#pragma unroll
+            for (int it = 0; it < NVI; it++)
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    v_mul[it][j] = __builtin_bit_cast(h2, __builtin_amdgcn_ds_bpermute(4 * token_of(v_item(it) / (DP / 4), 2 * j), pair));
+        } else if constexpr (P == 4) {
+#pragma unroll
+            for (int it = 0; it < NVI; it++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) v_sub[it][j] = v_mul[it][j] * h2{(_Float16)-0x1p-17f, (_Float16)-0x1p-17f};
+        } else {
+            constexpr int it = (P - 5) / 8, e4 = (P - 5) % 8 / 2, half = (P - 5) % 2;
+            const uint32_t sel = 0x0c000c00u | (uint32_t)((4 + e4) << 16) | (uint32_t)e4;
+#pragma unroll
+            for (int j = 2 * half; j < 2 * half + 2; j++) {
+                if constexpr (e4 == 0) raw_v.w[8 * it + 2 * j] ^= 0x80808080u, raw_v.w[8 * it + 2 * j + 1] ^= 0x80808080u;
+                // code 2^-24 M = (code + 128) 2^-24 M - M 2^-17.
+                const h2 u = __builtin_bit_cast(h2, __builtin_amdgcn_perm(raw_v.w[8 * it + 2 * j + 1], raw_v.w[8 * it + 2 * j], sel));
+                const h2 y = __builtin_elementwise_fma(u, v_mul[it][j], v_sub[it][j]);
+                v_out[2 * j] = y[0], v_out[2 * j + 1] = y[1];
+            }
+            if constexpr (half) {
+                const int ih = v_item(it) / (DP / 4), dq = v_item(it) % (DP / 4);
+                *(h8*)(to.v + (((2 * group + ih) * DP + e4 * (DP / 4) + dq) * 8)) = v_out;
             }
         }
     };
-    auto stage_v = [&](ChunkTile<DP>& to) {
-        float top = 0.0f;
-#pragma unroll
-        for (int it = 0; it < NVI; it++)
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                vsc[it][j] = (vok >> (8 * it + j) & 1) && __builtin_isfinite(vsc[it][j]) ? vsc[it][j] : 0.0f;
-                top = fmaxf(top, fabsf(vsc[it][j]));
-            }
-        const int e = exp_of(wave_top(top));
-        if (lane == 0) to.v_exp[group] = e;
-        const float unit = pow2(7 - e);
-#pragma unroll
-        for (int it = 0; it < NVI; it++) {
-            const int item = (it * 64 + lane) % (DP / 2), ih = item / (DP / 4), dq = item % (DP / 4);
-            float f[8], f24[8];
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                f[j] = vsc[it][j] * unit;
-                f24[j] = f[j] * 0x1p24f;
-                vraw[it][j] ^= 0x80808080u;
-            }
-#pragma unroll
-            for (int e4 = 0; e4 < 4; e4++) {
-                const uint32_t sel = 0x0c000c00u | (uint32_t)((4 + e4) << 16) | (uint32_t)e4;
-                h8 x;
-#pragma unroll
-                for (int j = 0; j < 8; j += 2) {
-                    const h2 y = scale_pair(__builtin_amdgcn_perm(vraw[it][j + 1], vraw[it][j], sel), f24[j], f[j], f24[j + 1], f[j + 1]);
-                    x[j] = y[0], x[j + 1] = y[1];
-                }
-                *(h8*)(to.v + (((2 * group + ih) * DP + e4 * (DP / 4) + dq) * 8)) = x;
-            }
-        }
-    };
-    auto stage_k = [&](ChunkTile<DP>& to) {
-        float top = 0.0f;
-#pragma unroll
-        for (int it = 0; it < NKI; it++) {
+    float k_f = 0.0f, k_mul[NKI];
+    int k_e = 0, k_ev = 0;
+    uint32_t k_out[4];
+    auto k_piece = [&](auto index, int tile_n, int next_t0) __attribute__((always_inline)) {
+        constexpr int P = decltype(index)::value;
+        if constexpr (P == 0) {
+            raw_k = next_k;
+        } else if constexpr (P == 1) {
+            load(next_k, next_t0, true);
+        } else if constexpr (P == 2) {
+            float fv;
+            k_ev = v_exp_of(raw_k, fv);
             // A token whose value is not finite is NaN to the rows that see it.
-            ksc[it] = !(kok >> it & 1) ? 0.0f : __builtin_isfinite(kvs[it]) ? ksc[it] : __builtin_nanf("");
-            top = fmaxf(top, __builtin_isfinite(ksc[it]) ? fabsf(ksc[it]) : 0.0f);
-        }
-        const int e = exp_of(wave_top(top));
-        if (lane == 0) to.k_unit[group] = pow2(e - 7), to.seen[group] = there;
-        const float unit = pow2(7 - e);
+            const float fk = __builtin_isfinite(raw_k.vs) ? raw_k.ks : __builtin_nanf("");
+            k_f = raw_k.ok != 0 ? fk : 0.0f;
+            k_e = exp_of(row_top(__builtin_isfinite(k_f) ? fabsf(k_f) : 0.0f));
+        } else if constexpr (P == 3) {
+            const float own = k_f * pow2(7 - k_e) * 0x1p24f;
 #pragma unroll
-        for (int it = 0; it < NKI; it++) {
-            const int item = it * 64 + lane, n = item / (DP / 16), ch = item % (DP / 16), t = 16 * group + n;
-            const float f = ksc[it] * unit, f24 = f * 0x1p24f;
-            h8 x[2];
-#pragma unroll
-            for (int w = 0; w < 4; w++) {
-                const uint32_t u = (uint32_t)kraw[it][w] ^ 0x80808080u;
-                const h2 y0 = scale_pair(__builtin_amdgcn_perm(u, u, 0x0c010c00u), f24, f, f24, f);
-                const h2 y1 = scale_pair(__builtin_amdgcn_perm(u, u, 0x0c030c02u), f24, f, f24, f);
-                x[w >> 1][4 * (w & 1)] = y0[0], x[w >> 1][4 * (w & 1) + 1] = y0[1];
-                x[w >> 1][4 * (w & 1) + 2] = y1[0], x[w >> 1][4 * (w & 1) + 3] = y1[1];
+            for (int it = 0; it < NKI; it++) k_mul[it] = __uint_as_float(__builtin_amdgcn_ds_bpermute(4 * k_token(it), (int)__float_as_uint(own)));
+        } else if constexpr (P == 4) {
+            ChunkMeta& meta = lds.meta[tile_n & 3];  // the same from all lanes
+            meta.k_unit[group] = pow2(k_e - 7), meta.v_exp[group] = k_ev;
+            meta.seen[group] = (uint32_t)__ballot(raw_k.ok != 0) & 0xffffu;
+        } else {
+            constexpr int it = (P - 5) / 8, w = (P - 5) % 8 / 2, half = (P - 5) % 2;
+            const float f24 = k_mul[it], off = f24 * -0x1p-17f;
+            if constexpr (half == 0) raw_k.w[4 * it + w] ^= 0x80808080u;
+            const uint32_t u = raw_k.w[4 * it + w];
+            k_out[2 * (w & 1) + half] = scale_pair(__builtin_amdgcn_perm(u, u, half ? 0x0c030c02u : 0x0c010c00u), f24, off);
+            if constexpr ((w & 1) && half) {
+                const int t = 16 * group + k_token(it);
+                *(uint4*)(tile[tile_n & 1].k + t * DP + 8 * k_slot<DP>(t, 2 * k_chunk(it) + (w >> 1))) = make_uint4(k_out[0], k_out[1], k_out[2], k_out[3]);
             }
-#pragma unroll
-            for (int m = 0; m < 2; m++) *(h8*)(to.k + t * DP + 8 * k_slot<DP>(t, 2 * ch + m)) = x[m];
         }
     };
 
@@ -310,17 +381,61 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel
     float m = kNoMax, l = 0.0f;
     int vexp = kMinExp;
 
-    auto compute = [&](const ChunkTile<DP>& ct, int t0) {
-        v16f x[2];
-#pragma unroll
-        for (int u = 0; u < 2; u++) {
-#pragma unroll
-            for (int j = 0; j < 16; j++) x[u][j] = 0.0f;
+    // Products: P V of a tile (the first kNV) and S of the next.  Each takes 16
+    // bytes a lane of LDS.
+    constexpr int kNV = kGroups * OT, kNS = 2 * KS;
+    v16f x[2];
+    h8 ph[kGroups];
+    auto operand = [&](auto index, const ChunkTile<DP>& v_of, const ChunkTile<DP>& k_of) __attribute__((always_inline)) {
+        constexpr int P = decltype(index)::value;
+        if constexpr (P < kNV) {
+            return *(const h8*)(v_of.v + ((2 * (P / OT) + h) * DP + 32 * (P % OT) + col) * 8);
+        } else {
+            constexpr int ks = (P - kNV) / 2, u = (P - kNV) % 2;
             const int t = 32 * u + col;
-#pragma unroll
-            for (int ks = 0; ks < KS; ks++)
-                x[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const h8*)(ct.k + t * DP + 8 * k_slot<DP>(t, 2 * ks + h)), q[ks], x[u], 0, 0, 0);
+            return *(const h8*)(k_of.k + t * DP + 8 * k_slot<DP>(t, 2 * ks + h));
         }
+    };
+    auto product = [&](auto index, h8 a) __attribute__((always_inline)) {
+        constexpr int P = decltype(index)::value;
+        if constexpr (P < kNV) {
+            o[P % OT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ph[P / OT], o[P % OT], 0, 0, 0);
+        } else {
+            constexpr int ks = (P - kNV) / 2, u = (P - kNV) % 2;
+            const v16f zero = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+            x[u] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, q[ks], ks == 0 ? zero : x[u], 0, 0, 0);
+        }
+    };
+    // Products FROM .. TO - 1 with their operands read kAhead before, and beside
+    // each the piece of other work that beside(product) does.  The scheduling
+    // barriers keep that order (left alone, the compiler has the other work
+    // first and the operands read one by one: 3150 clocks a turn, against
+    // 1024 of the matrix cores).
+    auto products = [&](auto from, auto to, const ChunkTile<DP>& v_of, const ChunkTile<DP>& k_of, auto beside) __attribute__((always_inline)) {
+        constexpr int F = decltype(from)::value, T = decltype(to)::value, kAhead = 4;
+        h8 a[kAhead];
+        each<kAhead>([&](auto n) __attribute__((always_inline)) { a[n] = operand(int_c<F + decltype(n)::value>{}, v_of, k_of); });
+        each<T - F>([&](auto n) __attribute__((always_inline)) {
+            constexpr int P = F + decltype(n)::value, S = decltype(n)::value % kAhead;
+            __builtin_amdgcn_sched_barrier(0);
+            product(int_c<P>{}, a[S]);
+            if constexpr (P + kAhead < T) a[S] = operand(int_c<P + kAhead>{}, v_of, k_of);
+            beside(int_c<P>{});
+        });
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto nothing = [](auto) __attribute__((always_inline)) {};
+    ChunkMeta ct;  // the next softmax's tile
+    auto read_meta = [&](int tile_n) __attribute__((always_inline)) {
+        const ChunkMeta& from = lds.meta[tile_n & 3];
+#pragma unroll
+        for (int g = 0; g < kGroups; g++) {
+            ct.k_unit[g] = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(from.k_unit[g])));
+            ct.v_exp[g] = __builtin_amdgcn_readfirstlane(from.v_exp[g]);
+            ct.seen[g] = __builtin_amdgcn_readfirstlane(from.seen[g]);
+        }
+    };
+    auto softmax = [&](int t0) __attribute__((always_inline)) {
         float ru[kGroups];
         uint32_t holes = 0;
         int e = vexp;
@@ -330,8 +445,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel
             holes |= ct.seen[g] ^ 0xffffu;
             e = max(e, ct.v_exp[g]);
         }
-        e = __builtin_amdgcn_readfirstlane(e);
-        if (t0 < all_lo || t0 + kTile > all_hi || __builtin_amdgcn_readfirstlane(holes)) {
+        if (t0 < all_lo || t0 + kTile > all_hi || holes) {
             const int a = max(row_lo, lo) - t0 - 4 * h, z = min(row_hi, hi) - t0 - 4 * h;
 #pragma unroll
             for (int g = 0; g < kGroups; g++) {
@@ -363,7 +477,6 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel
 #pragma unroll
                 for (int j = 0; j < 16; j++) o[n][j] *= ko;
         }
-        h8 ph[kGroups];
 #pragma unroll
         for (int g = 0; g < kGroups; g++) {
             // p in units of 2^-kP and of the group's own power of two for sv.
@@ -378,42 +491,76 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel
             }
             l = fmaf(sum, pow2(-de), l);
         }
-#pragma unroll
-        for (int g = 0; g < kGroups; g++)
-#pragma unroll
-            for (int n = 0; n < OT; n++)
-                o[n] = __builtin_amdgcn_mfma_f32_32x32x16_f16(*(const h8*)(ct.v + ((2 * g + h) * DP + 32 * n + col) * 8), ph[g], o[n], 0, 0, 0);
+        asm volatile("" : "+v"(l));  // summed here, not beside the products
     };
 
-    // Tile n is computed from one buffer while n + 1 goes from registers to the
-    // other and n + 2 comes to registers.  V's waves stage before they
-    // compute and K's after, so that one kind's vector work lies beside the
-    // other's products.
-    const int begin = lo & ~(kTile - 1);
-    if (begin < hi) {
-        load(begin);
-        if (does_v) stage_v(tile[0]);
-        if (does_k) stage_k(tile[0]);
-        if (begin + kTile < hi) load(begin + kTile);
+    // A wave has, in turn, the softmax of tile n, and the products P V of n and S of
+    // n + 1 with its staging among them: waves 0-3 V's, 4-7 K's.  Of eight waves
+    // the second four are half a tile behind, and then
+    //   waves 0-3 have the softmax of n in turn 2n + 1 and the products in 2n + 2,
+    //   waves 4-7 in turns 2n + 2 and 2n + 3;
+    //   S reads K of n in turns 2n and 2n + 1, P V reads V of n in 2n + 2 and 2n + 3;
+    //   turn 2n + 2 stages V of n + 1 over n - 1, read until 2n + 1;
+    //   turn 2n + 3 stages K of n + 2 over n, read until 2n + 1, and what belongs to
+    //   it over that of n - 2, which the softmax read until 2n - 2;
+    // a barrier ends every turn.  Four waves have one turn a tile.  Tiles staged
+    // past the last are never read.
+    const int begin = lo & ~(kTile - 1), count = begin < hi ? (hi - begin + kTile - 1) / kTile : 0;
+    auto start = [&](int n) { return begin + n * kTile; };
+    auto walk = [&](auto with_v, auto with_k) __attribute__((always_inline)) {
+        constexpr bool V = decltype(with_v)::value, K = decltype(with_k)::value;
+        if (V) {
+            fetch(next_v, start(0));
+            load(next_v, start(0), false);
+            each<kVPieces>([&](auto i) __attribute__((always_inline)) { v_piece(i, tile[0], start(1)); });
+        }
+        if (K) {
+            fetch(next_k, start(0));
+            load(next_k, start(0), true);
+            for (int n = 0; n < 2; n++)
+                each<kKPieces>([&](auto i) __attribute__((always_inline)) { k_piece(i, n, start(n + 1)); });
+        }
         lds_barrier();
-        int cur = 0;
-        for (int t0 = begin; t0 < hi; t0 += kTile, cur ^= 1) {
-            const bool next = t0 + kTile < hi, more = t0 + 2 * kTile < hi;
-            if (next && does_v) stage_v(tile[cur ^ 1]);
-            if (NW == 8 && does_v && more) load(t0 + 2 * kTile);
-            if (t0 < wave_hi && t0 + kTile > wave_lo) compute(tile[cur], t0);
-            if (next && does_k) stage_k(tile[cur ^ 1]);
-            if ((NW == 4 || does_k) && more) load(t0 + 2 * kTile);
+        if (NW == 8 && K) lds_barrier();
+        products(int_c<kNV>{}, int_c<kNV + kNS>{}, tile[0], tile[0], nothing);
+        read_meta(0);
+        lds_barrier();
+        for (int n = 0; n + 1 < count; n++) {
+            softmax(start(n));
+            if (NW == 8) lds_barrier();
+            __builtin_amdgcn_s_setprio(1);  // before the other group's softmax, which takes every slot
+            products(int_c<0>{}, int_c<kNV + kNS>{}, tile[n & 1], tile[(n + 1) & 1], [&](auto at) __attribute__((always_inline)) {
+                // The pieces evenly over the products.
+                constexpr int P = decltype(at)::value, N = kNV + kNS, pieces = (V ? kVPieces : 0) + (K ? kKPieces : 0);
+                constexpr int first = (P * pieces + N - 1) / N, end = ((P + 1) * pieces + N - 1) / N;
+                static_assert(pieces <= N, "a piece a product");
+                if constexpr (end > first) {
+                    if constexpr (V && first < kVPieces) v_piece(int_c<first>{}, tile[(n + 1) & 1], start(n + 2));
+                    else k_piece(int_c<first - (V ? kVPieces : 0)>{}, n + 2, start(n + 3));
+                }
+                if constexpr (P == N - 8) read_meta(n + 1);
+            });
+            __builtin_amdgcn_s_setprio(0);
             lds_barrier();
         }
+        softmax(start(count - 1));
+        if (NW == 8 && V) lds_barrier();  // as many as the waves behind
+        products(int_c<0>{}, int_c<kNV>{}, tile[(count - 1) & 1], tile[0], nothing);
+    };
+    if (count > 0) {
+        constexpr std::true_type yes;
+        constexpr std::false_type no;
+        if constexpr (NW == 4) walk(yes, yes);
+        else if (wave < 4) walk(yes, no);
+        else walk(no, yes);
     }
 
     l = add_x32(l);
     if (w0 + col >= rows) return;
     const bool split = sp.count > 1;
     const int64_t at = z * sp.rows + token * p.q_heads + head;
-    // O holds sum p v in units of 2^-(kP + 7 - vexp), l of 2^-kP.
-    const float unit = pow2(max(-126, vexp - 7)) * (split ? 1.0f / (1 << kP) : l != 0.0f ? 1.0f / l : 0.0f);
+    // O holds sum p v in units of 2^(kP + kM - 24 - vexp), l of 2^kP.
+    const float unit = ldexpf(1.0f, vexp + 24 - kM) * (split ? 1.0f / (1 << kP) : l != 0.0f ? 1.0f / l : 0.0f);
     if (split && h == 0) sp.ml[2 * at] = m, sp.ml[2 * at + 1] = l * (1.0f / (1 << kP));
     // Value n, j is of slot 32 n + 8 (j / 4) + 4 h + j % 4, so d = 4 (slot % (DP/4))
     // + slot / (DP/4): the four d of a slot % (DP/4) together.
@@ -444,7 +591,7 @@ static hipError_t launch_dp(hipStream_t stream, const KvCache& c, const PagedAtt
     const dim3 grid((unsigned)s.blocks * (unsigned)c.heads), block(64 * NW);
     const bool page16 = tiles_of_16(c);
     const void* f = page16 ? (const void*)paged_chunk_kernel<DP, NW, true> : (const void*)paged_chunk_kernel<DP, NW, false>;
-    const size_t lds = 2 * sizeof(ChunkTile<DP>);
+    const size_t lds = sizeof(ChunkLds<DP>);
     if (lds > 65536) {
         const hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (e != hipSuccess) return e;
