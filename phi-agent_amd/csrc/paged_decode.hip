@@ -44,7 +44,7 @@ template <int DP> struct Step {
 // PAGE16: tiles_of_16, so that a tile of 16 tokens has one block and its loads
 // one scalar base; otherwise every token finds its own.
 template <int DP, bool F32, bool PAGE16>
-__global__ __launch_bounds__(64 * kWaves) void paged_decode_kernel(KvCache c, PagedAttn p, AttnPart sp,
+__global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void paged_decode_kernel(KvCache c, PagedAttn p, AttnPart sp,
                                                                   const int32_t* __restrict__ table) {
     constexpr int KS = DP / 64, EB = DP / 16, NT = q_terms<F32>, NP = F32 ? 3 : 2;
     __shared__ float lo_[kWaves][kDecodeRows][DP];
@@ -105,52 +105,70 @@ __global__ __launch_bounds__(64 * kWaves) void paged_decode_kernel(KvCache c, Pa
     const int32_t* trow = table + (int64_t)b * p.table_stride;
     const int last_page = page_of(c, max(hi - 1, 0));
 
-    auto block_at = [&](int page, bool& ok) {
-        const int blk = trow[min(page, last_page)];
-        ok = blk >= 0 && blk < c.blocks;
-        return ok ? blk : 0;
+    // The table's entries of a step's tiles (a lane's token's), fetched a step
+    // before its loads.
+    int entry[2];
+    auto fetch = [&](int t0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < 2; j++) entry[j] = trow[min(page_of(c, min(t0 + 16 * j + (PAGE16 ? 0 : col), hi - 1)), last_page)];
     };
-    // Loads of the step at t0; tokens at hi and past it read the last page's, or
-    // block 0's, whatever these hold.
-    auto load = [&](Step<DP>& st, int t0) {
+    // A lane's offsets in a tile's rows; kept opaque in the loop, so that they stay
+    // 32-bit beside a scalar base.
+    const int ts = (int)c.token_stride;
+    uint32_t k_off[KS], v_off[4];
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++) k_off[ks] = (PAGE16 ? col * ts : 0) + kd[ks];
+#pragma unroll
+    for (int n = 0; n < 4; n++) v_off[n] = (PAGE16 ? (4 * g + n) * ts : 0) + vd;
+    // Loads of the step at t0, the next call's being of t0 + kStep * kWaves; tokens
+    // at hi and past it read the last page's, or block 0's, whatever these hold.
+    const int64_t s_head = kh * c.s_head_stride;
+    auto load = [&](Step<DP>& st, int t0) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < 2; j++) {
-            const int t = min(t0 + 16 * j, hi - 1);
+            const int8_t* kb = c.k + kh * c.head_stride;
+            const int8_t* vb = c.v + kh * c.head_stride;
+            const bool ok = entry[j] >= 0 && entry[j] < c.blocks;
+            const int64_t blk = ok ? entry[j] : 0;
             if (PAGE16) {
-                const int page = page_of(c, t), in = (t & ~15) - page * c.page;
-                bool ok;
-                const int64_t blk = block_at(page, ok);
-                const int64_t at = blk * c.block_stride + kh * c.head_stride + (int64_t)in * c.token_stride;
-                const int64_t sat = blk * c.s_block_stride + kh * c.s_head_stride + in;
-                const int8_t* kb = c.k + at;
-                const int8_t* vb = c.v + at;
-                const int ts = (int)c.token_stride;
+                const int t = min(t0 + 16 * j, hi - 1), in = (t & ~15) - page_of(c, t) * c.page;
+                const uint64_t at = (uint64_t)(uint32_t)blk * (uint32_t)c.block_stride + (uint32_t)in * (uint32_t)ts;
+                const int64_t sat = (int64_t)((uint64_t)(uint32_t)blk * (uint32_t)c.s_block_stride) + s_head + in;
                 st.ok[j][0] = ok;
 #pragma unroll
-                for (int ks = 0; ks < KS; ks++) st.k[j][ks] = *(const v4i*)(kb + (uint32_t)(col * ts + kd[ks]));
+                for (int ks = 0; ks < KS; ks++) {
+                    uint32_t off = k_off[ks];
+                    asm("" : "+v"(off));
+                    st.k[j][ks] = *(const v4i*)(kb + at + off);
+                }
 #pragma unroll
-                for (int n = 0; n < 4; n++) st.v[j][n] = *(const typename VWord<EB>::type*)(vb + (uint32_t)((4 * g + n) * ts + vd));
-                st.sk[j] = *(const v4f*)(c.ks + sat + 4 * g);
-                st.sv[j] = *(const v4f*)(c.vs + sat + 4 * g);
+                for (int n = 0; n < 4; n++) {
+                    uint32_t off = v_off[n];
+                    asm("" : "+v"(off));
+                    st.v[j][n] = *(const typename VWord<EB>::type*)(vb + at + off);
+                }
+                uint32_t off = 4 * g;
+                asm("" : "+v"(off));
+                st.sk[j] = *(const v4f*)(c.ks + sat + off);
+                st.sv[j] = *(const v4f*)(c.vs + sat + off);
             } else {
-                // Lane l finds token l & 15; the others' are read from it.
-                const int tk = min(t0 + 16 * j + col, hi - 1), page = page_of(c, tk), in = tk - page * c.page;
-                bool ok;
-                const int64_t blk = block_at(page, ok);
-                const int64_t at = blk * c.block_stride + kh * c.head_stride + in * c.token_stride;
-                const int64_t sat = blk * c.s_block_stride + kh * c.s_head_stride + in * c.s_token_stride;
+                // Lane l has token l & 15; the others' are read from it.
+                const int tk = min(t0 + 16 * j + col, hi - 1), in = tk - page_of(c, tk) * c.page;
+                const int64_t at = blk * c.block_stride + in * c.token_stride;
+                const int64_t sat = blk * c.s_block_stride + s_head + in * c.s_token_stride;
 #pragma unroll
-                for (int ks = 0; ks < KS; ks++) st.k[j][ks] = *(const v4i*)(c.k + at + kd[ks]);
+                for (int ks = 0; ks < KS; ks++) st.k[j][ks] = *(const v4i*)(kb + at + k_off[ks]);
 #pragma unroll
                 for (int n = 0; n < 4; n++) {
                     const int64_t av = __shfl(at, 4 * g + n, 64), as = __shfl(sat, 4 * g + n, 64);
                     st.ok[j][n] = __shfl((int)ok, 4 * g + n, 64);
-                    st.v[j][n] = *(const typename VWord<EB>::type*)(c.v + av + vd);
+                    st.v[j][n] = *(const typename VWord<EB>::type*)(vb + av + v_off[n]);
                     st.sk[j][n] = c.ks[as];
                     st.sv[j][n] = c.vs[as];
                 }
             }
         }
+        fetch(t0 + kStep * kWaves);
     };
 
     v4f o[EB];
@@ -158,7 +176,7 @@ __global__ __launch_bounds__(64 * kWaves) void paged_decode_kernel(KvCache c, Pa
     for (int e = 0; e < EB; e++) o[e] = v4f{0, 0, 0, 0};
     float m = kNoMax, l = 0.0f;
 
-    auto compute = [&](const Step<DP>& st, int t0) {
+    auto compute = [&](const Step<DP>& st, int t0) __attribute__((always_inline)) {
         float t[8], sv[8];
 #pragma unroll
         for (int j = 0; j < 2; j++) {
@@ -241,6 +259,7 @@ __global__ __launch_bounds__(64 * kWaves) void paged_decode_kernel(KvCache c, Pa
     const int begin = (lo & ~(kStep - 1)) + kStep * wave, stride = kStep * kWaves;
     if (begin < hi) {
         Step<DP> a, b2;
+        fetch(begin);
         load(a, begin);
         for (int t0 = begin; t0 < hi; t0 += 2 * stride) {
             load(b2, t0 + stride);
