@@ -17,6 +17,8 @@
 // product of fp16 (11 bits), both factors kept in its range.
 #pragma once
 
+#include <climits>
+
 #include "decoder.hpp"
 #include "device_common.hpp"
 
@@ -51,30 +53,33 @@ __device__ __forceinline__ SeqInfo seq_info(const PagedAttn& p, int page, int b)
 // that order.  Sequences of at most few_rows rows go to paged_decode.hip (AttnPart
 // few), those of more to paged_chunk.hip (many; bf16 queries only).
 //
-// A part's blocks share out the (sequence, row tile, split) triples that there
-// are, kv_heads blocks each; the grid is an upper bound of their number and the
-// blocks past it end at once.  (A grid over the longest sequence's tiles and
+// A part's blocks take the (sequence, row tile, split of the tokens) triples that
+// there are, kv_heads blocks each; the grid is an upper bound of their number and
+// the blocks past it end at once.  (A grid over the longest sequence's tiles and
 // splits leaves working blocks at a fixed stride among idle ones, which the
 // dispatcher deals to the same few compute units: 358 us against 118 for a chunk of
 // 512 tokens over 4352 beside seven empty sequences.)
 //
-// Split z of a sequence has its tokens [z * len, (z + 1) * len).  With count > 1
-// each leaves for its rows the undivided sum of p v, o [splits][rows][dim], and
-// the maximum and the sum of p, ml [splits][rows][2], for attn_join_kernel.
+// A tile of more than one split leaves for its rows, split by split, the undivided
+// sum of p v, o [..][dim], and the maximum and the sum of p, ml [..][2], for
+// attn_join_kernel.
 struct AttnPart {
-    int len, count;
-    int64_t rows;   // rows of o and ml a split
-    int row_pitch;  // few: rows a (sequence, key/value head) in them
-    int blocks;     // the grid, over kv_heads
+    // many: tokens a split, from a multiple of it on.  few: tokens a step.
+    int len;
+    int count;     // many: splits a sequence at most
+    int shares;    // few: a split has at least 1 / shares of all tiles' steps; 0: no splits
+    int64_t rows;  // many: rows of o and ml a split.  few: slots of 16 rows a key/value head
+    int blocks;    // the grid, over kv_heads; 0: does not run
     float* o;
     float* ml;
 };
 
-hipError_t launch_paged_decode(hipStream_t stream, const KvCache& c, const PagedAttn& p, const AttnPart& s);
-hipError_t launch_paged_chunk(hipStream_t stream, const KvCache& c, const PagedAttn& p, const AttnPart& s);
 // Rows of a block's tile.
 constexpr int kDecodeRows = 16;
 constexpr int kChunkRows = 256, kChunkRowsWide = 128;  // dim to 128, above
+
+hipError_t launch_paged_decode(hipStream_t stream, const KvCache& c, const PagedAttn& p, const AttnPart& s);
+hipError_t launch_paged_chunk(hipStream_t stream, const KvCache& c, const PagedAttn& p, const AttnPart& s);
 
 // Whether 16 tokens from a multiple of 16 lie in one block, their scales in a
 // row at 16-byte alignment, with offsets in the block and strides of blocks
@@ -86,39 +91,142 @@ inline bool tiles_of_16(const KvCache& c) {
            c.s_block_stride < lim;
 }
 
-// Triple number `unit` of a part (the same in all lanes): its sequence, row tile
-// and split; b < 0: there are fewer.  A sequence's triples: late tiles first
-// (they see most tokens), splits inside.  FEW: the sequences of at most few_rows.
-struct AttnUnit {
-    int b, tile, z;
+// The splits (few: steps) that hold what some row of a sequence sees.  A window
+// leaves out those before it: count is for the window's length then, not for max_kv.
+struct SplitRange {
+    int first, n;
 };
 
-template <bool FEW>
-__device__ __forceinline__ AttnUnit attn_unit(const PagedAttn& p, const AttnPart& s, int page, int tile_rows, int unit) {
+__device__ __forceinline__ SplitRange splits_of(const PagedAttn& p, const AttnPart& s, const SeqInfo& q) {
+    const int hi = p.causal ? min(q.kv, q.pos0 + min(q.n, p.max_q)) : q.kv;
+    const int first = p.window > 0 ? min(max(0, q.pos0 + 1 - p.window), p.max_kv) / s.len : 0;
+    const int end = hi > 0 ? (hi - 1) / s.len + 1 : 0;
+    return {first, min(max(1, end - first), s.count)};
+}
+
+// The work of block number `unit` of a part (the same in all lanes): row tile `tile`
+// of sequence b, tokens from z0 to z1, split z of the sequence's (few: the slot, -1:
+// no other split).  b < 0: there are fewer.
+struct AttnUnit {
+    int b, tile, z, z0, z1;
+    SeqInfo s;
+};
+
+__device__ __forceinline__ SeqInfo seq_of_lane(const SeqInfo& q, int at) {
+    return {__builtin_amdgcn_readlane(q.first, at), __builtin_amdgcn_readlane(q.n, at), __builtin_amdgcn_readlane(q.kv, at),
+            __builtin_amdgcn_readlane(q.pos0, at)};
+}
+
+// The sum over lanes up to the own: within rows of 16, then rows 0 and 2's onto the
+// next, then the first half's onto the second.
+__device__ __forceinline__ int lanes_sum(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr:1
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31
+    return v;
+}
+
+// Sequences of many rows: late tiles first (they see most tokens), splits inside.
+__device__ __forceinline__ AttnUnit many_unit(const PagedAttn& p, const AttnPart& s, int page, int tile_rows, int unit) {
     const int lane = threadIdx.x & 63;
     for (int b0 = 0; b0 < p.batch; b0 += 64) {
-        int tiles = 0, splits = 1;
+        int tiles = 0;
+        SeqInfo q{};
+        SplitRange r{0, 1};
         if (b0 + lane < p.batch) {
-            const SeqInfo q = seq_info(p, page, b0 + lane);
+            q = seq_info(p, page, b0 + lane);
             const int rows = min(q.n, p.max_q) * p.group;
-            if ((rows <= p.few_rows) == FEW) tiles = (rows + tile_rows - 1) / tile_rows;
-            splits = max(1, (q.kv + s.len - 1) / s.len);
+            if (rows > p.few_rows) tiles = (rows + tile_rows - 1) / tile_rows;
+            r = splits_of(p, s, q);
         }
-        int end = tiles * splits;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const int x = __shfl_up(end, off, 64);
-            end += lane >= off ? x : 0;
-        }
+        const int end = lanes_sum(tiles * r.n);
         const uint64_t past = __ballot(end > unit);
         if (past) {
-            const int at = __builtin_ctzll(past), local = unit - __builtin_amdgcn_readlane(end - tiles * splits, at);
-            const int n = __builtin_amdgcn_readlane(splits, at), tile = local / n;
-            return {b0 + at, __builtin_amdgcn_readlane(tiles, at) - 1 - tile, local - tile * n};
+            const int at = __builtin_ctzll(past), local = unit - __builtin_amdgcn_readlane(end - tiles * r.n, at);
+            const int n = __builtin_amdgcn_readlane(r.n, at), tile = local / n, z = local - tile * n;
+            const int z0 = (__builtin_amdgcn_readlane(r.first, at) + z) * s.len;
+            return {b0 + at, __builtin_amdgcn_readlane(tiles, at) - 1 - tile, z, z0, z0 + s.len, seq_of_lane(q, at)};
         }
         unit -= __builtin_amdgcn_readlane(end, 63);
     }
-    return {-1, 0, 0};
+    return {-1, 0, 0, 0, 0, {}};
+}
+
+// Sequences of few rows, 64 at a time, one a lane.  How long a split is follows from
+// the steps there are, so that the splits that are not their tile's last, all of one
+// length, are at most `shares`.  These come first among the 64 sequences' blocks,
+// then the last ones, longer before shorter by quarters of that length, so that the
+// work evens out whatever the lengths.
+struct FewScan {
+    int b0 = -64, base = 0;  // the first lane's sequence, blocks before its
+    int len, total = 0;      // steps a split, 0: being counted; steps in all
+    SeqInfo q;
+    int tiles, first, n, k;  // n steps from `first` on, k splits a tile
+    int full_end = 0, last = 0;  // splits but the last up to the lane's own; its tiles' first last split
+    int lasts = 0;               // last splits
+
+    __device__ __forceinline__ explicit FewScan(const AttnPart& s) : len(s.shares ? 0 : 1 << 30) {}
+    __device__ __forceinline__ int fulls() const { return __builtin_amdgcn_readlane(full_end, 63); }
+    __device__ __forceinline__ int blocks() const { return fulls() + lasts; }
+    // On to the next 64; false: there are none.
+    __device__ __forceinline__ bool next(const PagedAttn& p, const AttnPart& s, int page) {
+        for (;;) {
+            const bool counted = b0 + 64 >= p.batch;
+            if (counted) {
+                if (len) return false;
+                len = max(1, (total + s.shares - 1) / s.shares);
+                if (b0 > 0) b0 = -64;
+            }
+            if (!counted || b0 < 0) {
+                base += blocks();
+                b0 += 64;
+                const int at = b0 + (threadIdx.x & 63);
+                q = SeqInfo{}, tiles = 0;
+                SplitRange r{0, 1};
+                if (at < p.batch) {
+                    q = seq_info(p, page, at);
+                    const int rows = min(q.n, p.max_q) * p.group;
+                    if (rows <= p.few_rows) tiles = (rows + kDecodeRows - 1) / kDecodeRows;
+                    r = splits_of(p, s, q);
+                }
+                first = r.first, n = r.n;
+                if (!len) {
+                    total += __builtin_amdgcn_readlane(lanes_sum(tiles * n), 63);
+                    continue;
+                }
+            }
+            k = (n - 1) / len + 1;
+            full_end = lanes_sum(tiles * (k - 1));
+            lasts = 0;
+            const int quarter = (4 * (n - (k - 1) * len) - 1) / len;
+#pragma unroll
+            for (int c = 3; c >= 0; c--) {
+                const int t = c == 3 ? (quarter >= 3 ? tiles : 0) : quarter == c ? tiles : 0, sum = lanes_sum(t);
+                last = t ? lasts + sum - t : last;
+                lasts += __builtin_amdgcn_readlane(sum, 63);
+            }
+            return true;
+        }
+    }
+};
+
+__device__ __forceinline__ AttnUnit few_unit(const PagedAttn& p, const AttnPart& s, int page, int unit) {
+    FewScan f(s);
+    while (f.next(p, s, page)) {
+        const int local = unit - f.base;
+        if (local >= f.blocks()) continue;
+        const bool full = local < f.fulls();
+        const int off = full ? local : local - f.fulls(), begin = full ? f.full_end - f.tiles * (f.k - 1) : f.last;
+        const int at = __builtin_ctzll(__ballot(begin <= off && off < (full ? f.full_end : begin + f.tiles)));
+        const int k = __builtin_amdgcn_readlane(f.k, at), in = off - __builtin_amdgcn_readlane(begin, at);
+        const int tile = full ? in / (k - 1) : in, z = full ? in - tile * (k - 1) : k - 1;
+        const int z0 = (__builtin_amdgcn_readlane(f.first, at) + z * f.len) * s.len;
+        return {f.b0 + at, tile, k > 1 ? unit : -1, z0, full ? z0 + f.len * s.len : INT_MAX, seq_of_lane(f.q, at)};
+    }
+    return {-1, 0, 0, 0, 0, {}};
 }
 
 // The maximum over lanes l, l ^ 16, l ^ 32, l ^ 48, and over l, l ^ 32.
@@ -139,24 +247,22 @@ __device__ __forceinline__ float add_x16(float v) {
     return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// Sixteen elements of a query vector at element offset off, as fp32.
+// Sixteen elements of a query vector as they lie in memory, and element j.
+template <bool F32> struct Q16 {
+    uint32_t w[F32 ? 16 : 8];
+};
 template <bool F32>
-__device__ __forceinline__ void load_q16(const void* __restrict__ q, int64_t off, float (&x)[16]) {
-    if (F32) {
+__device__ __forceinline__ void load_q16(const void* __restrict__ q, int64_t off, Q16<F32>& x) {
+    const uint4* src = F32 ? (const uint4*)((const float*)q + off) : (const uint4*)((const uint16_t*)q + off);
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float4 t = *(const float4*)((const float*)q + off + 4 * i);
-            x[4 * i] = t.x, x[4 * i + 1] = t.y, x[4 * i + 2] = t.z, x[4 * i + 3] = t.w;
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            const uint4 t = *(const uint4*)((const uint16_t*)q + off + 8 * i);
-            const uint32_t w[4] = {t.x, t.y, t.z, t.w};
-#pragma unroll
-            for (int j = 0; j < 4; j++) x[8 * i + 2 * j] = bf16_to_f32(w[j] & 0xffffu), x[8 * i + 2 * j + 1] = bf16_to_f32(w[j] >> 16);
-        }
+    for (int i = 0; i < (F32 ? 4 : 2); i++) {
+        const uint4 t = src[i];
+        x.w[4 * i] = t.x, x.w[4 * i + 1] = t.y, x.w[4 * i + 2] = t.z, x.w[4 * i + 3] = t.w;
     }
+}
+template <bool F32>
+__device__ __forceinline__ float elem_q16(const Q16<F32>& x, int j) {
+    return __uint_as_float(F32 ? x.w[j] : j & 1 ? x.w[j >> 1] & 0xffff0000u : x.w[j >> 1] << 16);
 }
 
 // The integer form's terms (2 or 3 signed bytes an element) and its largest
@@ -165,23 +271,28 @@ __device__ __forceinline__ void load_q16(const void* __restrict__ q, int64_t off
 template <bool F32> constexpr int q_terms = F32 ? 3 : 2;
 template <bool F32> constexpr float q_steps = F32 ? 8355584.0f : 32639.0f;
 
-// Sixteen elements x * inv as integers, byte-split, term 0 the low one.
+// Sixteen elements x * inv as integers, byte-split, term 0 the low one.  An
+// integer with 128 added to each byte but the highest has its terms as bytes, those
+// below the highest with their sign bit turned.
 template <bool F32>
-__device__ __forceinline__ void split_q16(const float (&x)[16], float inv, v4i (&out)[q_terms<F32>]) {
+__device__ __forceinline__ void split_q16(const Q16<F32>& x, float inv, v4i (&out)[q_terms<F32>]) {
 #pragma unroll
     for (int w = 0; w < 4; w++) {
-        int b[q_terms<F32>][4];
+        uint32_t r[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            int r = (int)rintf(x[4 * w + j] * inv);
-#pragma unroll
-            for (int t = 0; t < q_terms<F32>; t++) {
-                b[t][j] = (int)(int8_t)r;
-                r = (r - b[t][j]) >> 8;
-            }
+            const float v = elem_q16<F32>(x, 4 * w + j);
+            // 1.5 2^23 + 128: the integer part as the sum's low 16 bits.
+            r[j] = F32 ? (uint32_t)((int)rintf(v * inv) + 0x8080) : __float_as_uint(fmaf(v, inv, 12583040.0f));
         }
-#pragma unroll
-        for (int t = 0; t < q_terms<F32>; t++) out[t][w] = (int)pack4(b[t][0], b[t][1], b[t][2], b[t][3]);
+        const uint32_t a = __builtin_amdgcn_perm(r[1], r[0], 0x05010400u), b = __builtin_amdgcn_perm(r[3], r[2], 0x05010400u);
+        out[0][w] = (int)(__builtin_amdgcn_perm(b, a, 0x05040100u) ^ 0x80808080u);
+        const uint32_t second = __builtin_amdgcn_perm(b, a, 0x07060302u);
+        out[1][w] = (int)(F32 ? second ^ 0x80808080u : second);
+        if constexpr (F32) {
+            const uint32_t e = __builtin_amdgcn_perm(r[1], r[0], 0x0c0c0602u), f = __builtin_amdgcn_perm(r[3], r[2], 0x0c0c0602u);
+            out[2][w] = (int)__builtin_amdgcn_perm(f, e, 0x05040100u);
+        }
     }
 }
 

@@ -130,11 +130,11 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel
     const int col = lane & 31, h = lane >> 5;
     const int heads = c.heads, D = c.dim;
     const int kh = blockIdx.x % heads;
-    const AttnUnit unit_of = attn_unit<false>(p, sp, c.page, 32 * NW, blockIdx.x / heads);
+    const AttnUnit unit_of = many_unit(p, sp, c.page, 32 * NW, blockIdx.x / heads);
     if (unit_of.b < 0) return;
-    const int b = unit_of.b, z = unit_of.z;
-    const SeqInfo s = seq_info(p, c.page, b);
-    const int rows = min(s.n, p.max_q) * p.group, r0 = unit_of.tile * 32 * NW, z0 = z * sp.len;
+    const int b = unit_of.b, z = unit_of.z, z0 = unit_of.z0;
+    const SeqInfo s = unit_of.s;
+    const int rows = min(s.n, p.max_q) * p.group, r0 = unit_of.tile * 32 * NW;
 
     // The lane's row, and the ranges of the wave's rows and of the block's.
     const int w0 = r0 + 32 * wave;
@@ -143,7 +143,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel
     const int pos = s.pos0 + i;
     const int row_hi = p.causal ? min(s.kv, pos + 1) : s.kv, row_lo = p.window > 0 ? max(0, pos + 1 - p.window) : 0;
     auto pos_of = [&](int row) { return s.pos0 + min(row, rows - 1) / p.group; };
-    auto hi_of = [&](int ps) { return min(p.causal ? min(s.kv, ps + 1) : s.kv, z0 + sp.len); };
+    auto hi_of = [&](int ps) { return min(p.causal ? min(s.kv, ps + 1) : s.kv, unit_of.z1); };
     auto lo_of = [&](int ps) { return max(p.window > 0 ? max(0, ps + 1 - p.window) : 0, z0); };
     const int hi = hi_of(pos_of(r0 + 32 * NW - 1)), lo = lo_of(pos_of(r0));
     const int all_hi = hi_of(pos_of(w0)), all_lo = lo_of(pos_of(w0 + 31));

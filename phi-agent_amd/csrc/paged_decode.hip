@@ -13,9 +13,13 @@
 //     it lies.  V^T wants 8 tokens of one d a lane: the lane loads dim/16
 //     bytes of each of its 8 tokens' rows (16 lanes read a whole row) and takes
 //     byte e of all eight for product e, so d = dim/16 (l & 15) + e.
-// The next step's loads are under way while a step is computed: 32 tokens are 8 KB
-// a wave at dim 128, and 12 waves a CU keep 96 KB in flight.  The four waves
-// of a block take every fourth step of its split and join in LDS.
+// The next step's loads are under way while a step is computed, the table's entries
+// for those two steps ahead: 32 tokens are 8 KB a wave at dim 128, and the two blocks
+// a compute unit holds keep 64 KB in flight.  The four waves of a block take every
+// fourth step of its split and join in LDS.
+// 64 sequences of 4096 tokens, 32 heads over 8 of 128, pages of 16: 103 us with the
+// join, 5.4 TB/s of the 6.2 that reading reaches; one step of one sequence 7.8 us,
+// launch, three dependent loads and the join of the waves.
 #include "paged_attention.hpp"
 
 namespace phi_dev {
@@ -52,11 +56,11 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void paged_decode_k
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
     const int kh = blockIdx.x % c.heads;
-    const AttnUnit unit = attn_unit<true>(p, sp, c.page, kDecodeRows, blockIdx.x / c.heads);
+    const AttnUnit unit = few_unit(p, sp, c.page, blockIdx.x / c.heads);
     if (unit.b < 0) return;
-    const int b = unit.b, z = unit.z;
-    const SeqInfo s = seq_info(p, c.page, b);
-    const int rows = min(s.n, p.max_q) * p.group, r0 = unit.tile * kDecodeRows, z0 = z * sp.len;
+    const int b = unit.b, slot = unit.z, z0 = unit.z0;
+    const SeqInfo s = unit.s;
+    const int rows = min(s.n, p.max_q) * p.group, r0 = unit.tile * kDecodeRows;
     const int D = c.dim;
 
     // The lane's row of the tile (past the last: the last again, not stored).
@@ -66,35 +70,9 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void paged_decode_k
     const int pos_first = s.pos0 + r0 / p.group, pos_last = s.pos0 + min(r0 + kDecodeRows - 1, rows - 1) / p.group;
     const int row_hi = p.causal ? min(s.kv, pos + 1) : s.kv, row_lo = p.window > 0 ? max(0, pos + 1 - p.window) : 0;
     // Tokens that some row of the tile sees, and that all of them see.
-    const int hi = min(p.causal ? min(s.kv, pos_last + 1) : s.kv, z0 + sp.len);
+    const int hi = min(p.causal ? min(s.kv, pos_last + 1) : s.kv, unit.z1);
     const int lo = max(p.window > 0 ? max(0, pos_first + 1 - p.window) : 0, z0);
     const int all_hi = p.causal ? min(s.kv, pos_first + 1) : s.kv, all_lo = p.window > 0 ? max(0, pos_last + 1 - p.window) : 0;
-
-    // Q's integer form in the B operand's order.
-    v4i qt[KS][NT];
-    float rq;
-    {
-        float x[KS][16], amax = 0.0f, bad = 0.0f;
-        const float f = p.scale * 1.4426950408889634f;
-#pragma unroll
-        for (int ks = 0; ks < KS; ks++) {
-            const int d = 64 * ks + 16 * g;
-            if (d < D) load_q16<F32>(p.q, token * p.q_token + head * p.q_head + d, x[ks]);
-#pragma unroll
-            for (int j = 0; j < 16; j++) {
-                x[ks][j] = d < D ? x[ks][j] * f : 0.0f;
-                amax = fmaxf(amax, fabsf(x[ks][j]));
-                bad += x[ks][j] * 0.0f;  // NaN once an infinity or a NaN is met
-            }
-        }
-        amax = max_x16(max_x32(amax));
-        bad = add_x16(add_x32(bad));
-        const bool some = amax > 1e-30f;
-        const float inv = some ? q_steps<F32> / amax : 0.0f;
-        rq = (some ? amax / q_steps<F32> : 1.0f) + bad;
-#pragma unroll
-        for (int ks = 0; ks < KS; ks++) split_q16<F32>(x[ks], inv, qt[ks]);
-    }
 
     // A lane's bytes past dim read its row's first bytes again: Q is 0 there,
     // and O's columns past dim are not stored.
@@ -171,6 +149,41 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void paged_decode_k
         fetch(t0 + kStep * kWaves);
     };
 
+    // The first step's loads are under way beside Q's (fp32: Q takes their registers).
+    const int begin = (lo & ~(kStep - 1)) + kStep * wave, stride = kStep * kWaves;
+    Step<DP> first;
+    if (begin < hi) fetch(begin);
+    Q16<F32> x[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++) {
+        const int d = 64 * ks + 16 * g;
+        if (d < D) load_q16<F32>(p.q, token * p.q_token + head * p.q_head + d, x[ks]);
+        else x[ks] = Q16<F32>{};
+    }
+    if (!F32 && begin < hi) load(first, begin);
+
+    // Q's integer form in the B operand's order.
+    v4i qt[KS][NT];
+    float amax = 0.0f, bad = 0.0f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            const float v = elem_q16<F32>(x[ks], j);
+            amax = fmaxf(amax, fabsf(v));
+            bad = fmaf(v, 0.0f, bad);  // NaN once an infinity or a NaN is met
+        }
+    amax = max_x16(max_x32(amax));
+    bad = add_x16(add_x32(bad));
+    const float f = p.scale * 1.4426950408889634f;
+    float inv = 0.0f, rq = amax / q_steps<F32> * fabsf(f);
+    if (amax > 1e-30f && rq > 0x1p-126f) inv = copysignf(q_steps<F32> / amax, f);
+    else rq = 1.0f;  // every logit is 0
+    rq += bad;
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++) split_q16<F32>(x[ks], inv, qt[ks]);
+    if (F32 && begin < hi) load(first, begin);
+
     v4f o[EB];
 #pragma unroll
     for (int e = 0; e < EB; e++) o[e] = v4f{0, 0, 0, 0};
@@ -204,6 +217,7 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void paged_decode_k
         const bool whole = t0 >= all_lo && t0 + kStep <= min(all_hi, hi) && t0 >= lo && (PAGE16 ? ok : __all(ok));
         uint32_t seen = 0xff;
         if (!whole) {
+            asm volatile("");  // keeps this a branch: 80 instructions that few steps need
             seen = 0;
 #pragma unroll
             for (int k = 0; k < 8; k++) {
@@ -256,17 +270,14 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void paged_decode_k
 
     // Two steps in registers, one loading.  Loads run ahead of hi - 1 at most by
     // being clamped to it.
-    const int begin = (lo & ~(kStep - 1)) + kStep * wave, stride = kStep * kWaves;
     if (begin < hi) {
-        Step<DP> a, b2;
-        fetch(begin);
-        load(a, begin);
+        Step<DP> second;
         for (int t0 = begin; t0 < hi; t0 += 2 * stride) {
-            load(b2, t0 + stride);
-            compute(a, t0);
+            load(second, t0 + stride);
+            compute(first, t0);
             if (t0 + stride >= hi) break;
-            load(a, t0 + 2 * stride);
-            compute(b2, t0 + stride);
+            load(first, t0 + 2 * stride);
+            compute(second, t0 + stride);
         }
     }
 
@@ -296,9 +307,9 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void paged_decode_k
     float rl = 0.0f;
 #pragma unroll
     for (int w = 0; w < kWaves; w++) rl = fmaf(ll[w][row], __builtin_amdgcn_exp2f(lm[w][row] - rm), rl);
-    const int64_t at = z * sp.rows + ((int64_t)b * c.heads + kh) * sp.row_pitch + r0 + row;
-    const float inv = sp.count > 1 ? 1.0f : rl != 0.0f ? 1.0f / rl : 0.0f;
-    if (sp.count > 1 && part == 0) sp.ml[2 * at] = rm, sp.ml[2 * at + 1] = rl;
+    const int64_t at = (kh * sp.rows + slot) * kDecodeRows + row;
+    const float div = slot >= 0 ? 1.0f : rl != 0.0f ? 1.0f / rl : 0.0f;
+    if (slot >= 0 && part == 0) sp.ml[2 * at] = rm, sp.ml[2 * at + 1] = rl;
 #pragma unroll
     for (int q4 = 0; q4 < DP / 64; q4++) {
         const int d = 4 * (part + 16 * q4);
@@ -306,8 +317,8 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void paged_decode_k
         v4f x = *(const v4f*)&lo_[0][row][d];
 #pragma unroll
         for (int w = 1; w < kWaves; w++) x += *(const v4f*)&lo_[w][row][d];
-        x *= inv;
-        if (sp.count > 1) {
+        x *= div;
+        if (slot >= 0) {
             *(v4f*)(sp.o + at * D + d) = x;
         } else {
             const int64_t to = rtok * p.out_token + rhead * p.out_head + d;
