@@ -60,16 +60,15 @@ __device__ __forceinline__ SeqInfo seq_info(const PagedAttn& p, int page, int b)
 // dispatcher deals to the same few compute units: 358 us against 118 for a chunk of
 // 512 tokens over 4352 beside seven empty sequences.)
 //
-// A tile of more than one split leaves for its rows, split by split, the undivided
-// sum of p v, o [..][dim], and the maximum and the sum of p, ml [..][2], for
-// attn_join_kernel.
+// A tile of more than one split leaves for its rows, split by split in a slot each,
+// the undivided sum of p v, o [kv_heads][slots][tile's rows][dim], and the maximum
+// and the sum of p, ml [..][2], for attn_join_kernel.
 struct AttnPart {
-    // many: tokens a split, from a multiple of it on.  few: tokens a step.
-    int len;
-    int count;     // many: splits a sequence at most
-    int shares;    // few: a split has at least 1 / shares of all tiles' steps; 0: no splits
-    int64_t rows;  // many: rows of o and ml a split.  few: slots of 16 rows a key/value head
-    int blocks;    // the grid, over kv_heads; 0: does not run
+    int step;     // tokens
+    int shares;   // a split has at least 1 / shares of all tiles' steps; 0: no splits
+    int slots;    // a key/value head
+    int rows;     // a tile
+    int blocks;   // the grid, over kv_heads; 0: does not run
     float* o;
     float* ml;
 };
@@ -91,24 +90,11 @@ inline bool tiles_of_16(const KvCache& c) {
            c.s_block_stride < lim;
 }
 
-// The splits (few: steps) that hold what some row of a sequence sees.  A window
-// leaves out those before it: count is for the window's length then, not for max_kv.
-struct SplitRange {
-    int first, n;
-};
-
-__device__ __forceinline__ SplitRange splits_of(const PagedAttn& p, const AttnPart& s, const SeqInfo& q) {
-    const int hi = p.causal ? min(q.kv, q.pos0 + min(q.n, p.max_q)) : q.kv;
-    const int first = p.window > 0 ? min(max(0, q.pos0 + 1 - p.window), p.max_kv) / s.len : 0;
-    const int end = hi > 0 ? (hi - 1) / s.len + 1 : 0;
-    return {first, min(max(1, end - first), s.count)};
-}
-
 // The work of block number `unit` of a part (the same in all lanes): row tile `tile`
-// of sequence b, tokens from z0 to z1, split z of the sequence's (few: the slot, -1:
-// no other split).  b < 0: there are fewer.
+// of sequence b, tokens from z0 to z1, to be left in a slot (-1: there is no other
+// split, so written out).  b < 0: there are fewer.
 struct AttnUnit {
-    int b, tile, z, z0, z1;
+    int b, tile, slot, z0, z1;
     SeqInfo s;
 };
 
@@ -129,38 +115,12 @@ __device__ __forceinline__ int lanes_sum(int v) {
     return v;
 }
 
-// Sequences of many rows: late tiles first (they see most tokens), splits inside.
-__device__ __forceinline__ AttnUnit many_unit(const PagedAttn& p, const AttnPart& s, int page, int tile_rows, int unit) {
-    const int lane = threadIdx.x & 63;
-    for (int b0 = 0; b0 < p.batch; b0 += 64) {
-        int tiles = 0;
-        SeqInfo q{};
-        SplitRange r{0, 1};
-        if (b0 + lane < p.batch) {
-            q = seq_info(p, page, b0 + lane);
-            const int rows = min(q.n, p.max_q) * p.group;
-            if (rows > p.few_rows) tiles = (rows + tile_rows - 1) / tile_rows;
-            r = splits_of(p, s, q);
-        }
-        const int end = lanes_sum(tiles * r.n);
-        const uint64_t past = __ballot(end > unit);
-        if (past) {
-            const int at = __builtin_ctzll(past), local = unit - __builtin_amdgcn_readlane(end - tiles * r.n, at);
-            const int n = __builtin_amdgcn_readlane(r.n, at), tile = local / n, z = local - tile * n;
-            const int z0 = (__builtin_amdgcn_readlane(r.first, at) + z) * s.len;
-            return {b0 + at, __builtin_amdgcn_readlane(tiles, at) - 1 - tile, z, z0, z0 + s.len, seq_of_lane(q, at)};
-        }
-        unit -= __builtin_amdgcn_readlane(end, 63);
-    }
-    return {-1, 0, 0, 0, 0, {}};
-}
-
-// Sequences of few rows, 64 at a time, one a lane.  How long a split is follows from
-// the steps there are, so that the splits that are not their tile's last, all of one
+// The sequences of a part, 64 at a time, one a lane (FEW: those of at most few_rows
+// rows).  How long a split is follows from the steps there are, so that the splits that are not their tile's last, all of one
 // length, are at most `shares`.  These come first among the 64 sequences' blocks,
 // then the last ones, longer before shorter by quarters of that length, so that the
 // work evens out whatever the lengths.
-struct FewScan {
+template <bool FEW> struct AttnScan {
     int b0 = -64, base = 0;  // the first lane's sequence, blocks before its
     int len, total = 0;      // steps a split, 0: being counted; steps in all
     SeqInfo q;
@@ -168,7 +128,7 @@ struct FewScan {
     int full_end = 0, last = 0;  // splits but the last up to the lane's own; its tiles' first last split
     int lasts = 0;               // last splits
 
-    __device__ __forceinline__ explicit FewScan(const AttnPart& s) : len(s.shares ? 0 : 1 << 30) {}
+    __device__ __forceinline__ explicit AttnScan(const AttnPart& s) : len(s.shares ? 0 : 1 << 30) {}
     __device__ __forceinline__ int fulls() const { return __builtin_amdgcn_readlane(full_end, 63); }
     __device__ __forceinline__ int blocks() const { return fulls() + lasts; }
     // On to the next 64; false: there are none.
@@ -185,14 +145,16 @@ struct FewScan {
                 b0 += 64;
                 const int at = b0 + (threadIdx.x & 63);
                 q = SeqInfo{}, tiles = 0;
-                SplitRange r{0, 1};
+                first = 0, n = 1;
                 if (at < p.batch) {
                     q = seq_info(p, page, at);
                     const int rows = min(q.n, p.max_q) * p.group;
-                    if (rows <= p.few_rows) tiles = (rows + kDecodeRows - 1) / kDecodeRows;
-                    r = splits_of(p, s, q);
+                    if ((rows <= p.few_rows) == FEW) tiles = (rows + s.rows - 1) / s.rows;
+                    // The steps that hold what some row sees.
+                    const int hi = p.causal ? min(q.kv, q.pos0 + min(q.n, p.max_q)) : q.kv;
+                    if (p.window > 0) first = min(max(0, q.pos0 + 1 - p.window), p.max_kv) / s.step;
+                    n = max(1, (hi > 0 ? (hi - 1) / s.step + 1 : 0) - first);
                 }
-                first = r.first, n = r.n;
                 if (!len) {
                     total += __builtin_amdgcn_readlane(lanes_sum(tiles * n), 63);
                     continue;
@@ -213,8 +175,9 @@ struct FewScan {
     }
 };
 
-__device__ __forceinline__ AttnUnit few_unit(const PagedAttn& p, const AttnPart& s, int page, int unit) {
-    FewScan f(s);
+template <bool FEW>
+__device__ __forceinline__ AttnUnit attn_unit(const PagedAttn& p, const AttnPart& s, int page, int unit) {
+    AttnScan<FEW> f(s);
     while (f.next(p, s, page)) {
         const int local = unit - f.base;
         if (local >= f.blocks()) continue;
@@ -223,8 +186,9 @@ __device__ __forceinline__ AttnUnit few_unit(const PagedAttn& p, const AttnPart&
         const int at = __builtin_ctzll(__ballot(begin <= off && off < (full ? f.full_end : begin + f.tiles)));
         const int k = __builtin_amdgcn_readlane(f.k, at), in = off - __builtin_amdgcn_readlane(begin, at);
         const int tile = full ? in / (k - 1) : in, z = full ? in - tile * (k - 1) : k - 1;
-        const int z0 = (__builtin_amdgcn_readlane(f.first, at) + z * f.len) * s.len;
-        return {f.b0 + at, tile, k > 1 ? unit : -1, z0, full ? z0 + f.len * s.len : INT_MAX, seq_of_lane(f.q, at)};
+        const int z0 = (__builtin_amdgcn_readlane(f.first, at) + z * f.len) * s.step;
+        // Late tiles first: they see most tokens.
+        return {f.b0 + at, __builtin_amdgcn_readlane(f.tiles, at) - 1 - tile, k > 1 ? unit : -1, z0, full ? z0 + f.len * s.step : INT_MAX, seq_of_lane(f.q, at)};
     }
     return {-1, 0, 0, 0, 0, {}};
 }

@@ -130,9 +130,9 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel
     const int col = lane & 31, h = lane >> 5;
     const int heads = c.heads, D = c.dim;
     const int kh = blockIdx.x % heads;
-    const AttnUnit unit_of = many_unit(p, sp, c.page, 32 * NW, blockIdx.x / heads);
+    const AttnUnit unit_of = attn_unit<false>(p, sp, c.page, blockIdx.x / heads);
     if (unit_of.b < 0) return;
-    const int b = unit_of.b, z = unit_of.z, z0 = unit_of.z0;
+    const int b = unit_of.b, z0 = unit_of.z0;
     const SeqInfo s = unit_of.s;
     const int rows = min(s.n, p.max_q) * p.group, r0 = unit_of.tile * 32 * NW;
 
@@ -557,8 +557,8 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel
 
     l = add_x32(l);
     if (w0 + col >= rows) return;
-    const bool split = sp.count > 1;
-    const int64_t at = z * sp.rows + token * p.q_heads + head;
+    const bool split = unit_of.slot >= 0;
+    const int64_t at = ((int64_t)kh * sp.slots + unit_of.slot) * (32 * NW) + 32 * wave + col;
     // O holds sum p v in units of 2^(kP + kM - 24 - vexp), l of 2^kP.
     const float unit = ldexpf(1.0f, vexp + 24 - kM) * (split ? 1.0f / (1 << kP) : l != 0.0f ? 1.0f / l : 0.0f);
     if (split && h == 0) sp.ml[2 * at] = m, sp.ml[2 * at + 1] = l * (1.0f / (1 << kP));

@@ -56,9 +56,9 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void paged_decode_k
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
     const int kh = blockIdx.x % c.heads;
-    const AttnUnit unit = few_unit(p, sp, c.page, blockIdx.x / c.heads);
+    const AttnUnit unit = attn_unit<true>(p, sp, c.page, blockIdx.x / c.heads);
     if (unit.b < 0) return;
-    const int b = unit.b, slot = unit.z, z0 = unit.z0;
+    const int b = unit.b, slot = unit.slot, z0 = unit.z0;
     const SeqInfo s = unit.s;
     const int rows = min(s.n, p.max_q) * p.group, r0 = unit.tile * kDecodeRows;
     const int D = c.dim;
@@ -307,7 +307,7 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void paged_decode_k
     float rl = 0.0f;
 #pragma unroll
     for (int w = 0; w < kWaves; w++) rl = fmaf(ll[w][row], __builtin_amdgcn_exp2f(lm[w][row] - rm), rl);
-    const int64_t at = (kh * sp.rows + slot) * kDecodeRows + row;
+    const int64_t at = ((int64_t)kh * sp.slots + slot) * kDecodeRows + row;
     const float div = slot >= 0 ? 1.0f : rl != 0.0f ? 1.0f / rl : 0.0f;
     if (slot >= 0 && part == 0) sp.ml[2 * at] = rm, sp.ml[2 * at + 1] = rl;
 #pragma unroll
