@@ -3,9 +3,8 @@
 //   (q, s) = rotate + quantise of y (quant_rotate.hip).
 //
 // Bound by memory: 2 to 4 bytes of x, 4 to 8 of the residual stream and 1 of q an
-// element, about 25 vector instructions.  So one pass: a lane holds 16
-// consecutive elements of a 256-group a round, a wave four groups a round, and the
-// row stays in registers through both of its reductions (the sum of squares, a
+// element, about 25 vector instructions.  So one pass: a lane holds 16 elements of a
+// 256-group a round, a wave four groups a round, and the row stays in registers through both of its reductions (the sum of squares, a
 // wave's by shuffles and the row's waves' through LDS; the largest |z| the same
 // way).  The rotation is that of qr_tiles.hpp, on a 16 x 16 tile of LDS private to
 // the group's 16 lanes, and so are the scale and the codes: q and s are to the
@@ -13,9 +12,10 @@
 //
 // Rows may start at any element: loads and stores are 16 bytes at the elements'
 // own alignment (the hardware takes them unaligned; aligned ones are the same
-// instructions), and only the lane with the row's last, partial 16 elements goes
-// one by one.  4352 rows of 5120 in bf16 onto an fp32 stream: 55 us, 4.4 TB/s of the
-// 4.9 that a copy reaches; 154 us with the row in LDS, an element a thread.
+// instructions).  4352 rows of 5120 in bf16 onto an fp32 stream: 54 us, 4.6 TB/s of
+// the 4.9 that a copy reaches; 154 us with the row in LDS, an element a thread.  777 rows
+// of 5003 in fp32 without the rotation: 15 us; 19 us with 16 consecutive elements a
+// lane, whose four loads each touch every line.
 #include "decoder.hpp"
 #include "qr_tiles.hpp"
 
@@ -24,54 +24,77 @@ namespace phi_dev {
 namespace {
 
 typedef uint32_t u4a1 __attribute__((ext_vector_type(4), aligned(1)));
+typedef uint32_t u2a2 __attribute__((ext_vector_type(2), aligned(2)));
+typedef uint32_t u1a1 __attribute__((aligned(1)));
 typedef uint32_t u4a2 __attribute__((ext_vector_type(4), aligned(2)));
 typedef float f4a4 __attribute__((ext_vector_type(4), aligned(4)));
 
-// Elements e0 .. e0 + 15 of p's row at element offset `row`, 0 from K on.
-template <bool BF16>
+// A lane's 16 elements of a row: e0 .. e0 + 15 (ROT: the rotation wants them together,
+// K is a multiple of 16) or, v[4 i + j], e0 + 64 i + j (the 16 lanes' loads are one
+// piece; the row's last piece goes one by one).
+template <bool ROT> __device__ __forceinline__ int at16(int e0, int j) { return e0 + (ROT ? j : 64 * (j / 4) + j % 4); }
+
+// Of p's row at element offset `row`; 0 from K on.
+template <bool ROT, bool BF16>
 __device__ __forceinline__ void load_row16(const void* __restrict__ p, int64_t row, int e0, int K, float (&v)[16]) {
-    if (e0 + 16 <= K) {
-        if (BF16) {
+    const uint16_t* h = (const uint16_t*)p + row;
+    const float* f = (const float*)p + row;
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const u4a2 t = *(const u4a2*)((const uint16_t*)p + row + e0 + 8 * i);
+    for (int j = 0; j < 16; j++) v[j] = 0.0f;
+    if (BF16 && ROT) {
 #pragma unroll
-                for (int j = 0; j < 4; j++) v[8 * i + 2 * j] = __uint_as_float(t[j] << 16), v[8 * i + 2 * j + 1] = __uint_as_float(t[j] & 0xffff0000u);
-            }
-        } else {
+        for (int i = 0; i < 2; i++) {
+            const u4a2 t = e0 < K ? *(const u4a2*)(h + e0 + 8 * i) : u4a2{0, 0, 0, 0};
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const f4a4 t = *(const f4a4*)((const float*)p + row + e0 + 4 * i);
+            for (int j = 0; j < 4; j++) v[8 * i + 2 * j] = __uint_as_float(t[j] << 16), v[8 * i + 2 * j + 1] = __uint_as_float(t[j] & 0xffff0000u);
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int e = at16<ROT>(e0, 4 * i);
+        if (ROT ? e0 < K : e + 4 <= K) {
+            if (BF16) {
+                const u2a2 t = *(const u2a2*)(h + e);
+#pragma unroll
+                for (int j = 0; j < 2; j++) v[4 * i + 2 * j] = __uint_as_float(t[j] << 16), v[4 * i + 2 * j + 1] = __uint_as_float(t[j] & 0xffff0000u);
+            } else {
+                const f4a4 t = *(const f4a4*)(f + e);
 #pragma unroll
                 for (int j = 0; j < 4; j++) v[4 * i + j] = t[j];
             }
-        }
-    } else {
+        } else if (!ROT) {
 #pragma unroll
-        for (int j = 0; j < 16; j++) {
-            v[j] = 0.0f;
-            if (e0 + j < K) v[j] = BF16 ? bf16_to_f32(((const uint16_t*)p)[row + e0 + j]) : ((const float*)p)[row + e0 + j];
+            for (int j = 0; j < 4; j++)
+                if (e + j < K) v[4 * i + j] = BF16 ? bf16_to_f32(h[e + j]) : f[e + j];
         }
     }
 }
 
+template <bool ROT>
 __device__ __forceinline__ void store_row16(void* p, bool bf16, int64_t row, int e0, int K, const float (&v)[16]) {
-    if (e0 + 16 <= K) {
-        if (bf16) {
+    uint16_t* h = (uint16_t*)p + row;
+    float* f = (float*)p + row;
+    if (bf16 && ROT) {
 #pragma unroll
-            for (int i = 0; i < 2; i++)
-                *(u4a2*)((uint16_t*)p + row + e0 + 8 * i) =
-                    u4a2{f32x2_to_bf16x2(v[8 * i], v[8 * i + 1]), f32x2_to_bf16x2(v[8 * i + 2], v[8 * i + 3]),
-                         f32x2_to_bf16x2(v[8 * i + 4], v[8 * i + 5]), f32x2_to_bf16x2(v[8 * i + 6], v[8 * i + 7])};
-        } else {
+        for (int i = 0; i < 2; i++)
+            if (e0 < K)
+                *(u4a2*)(h + e0 + 8 * i) = u4a2{f32x2_to_bf16x2(v[8 * i], v[8 * i + 1]), f32x2_to_bf16x2(v[8 * i + 2], v[8 * i + 3]),
+                                                f32x2_to_bf16x2(v[8 * i + 4], v[8 * i + 5]), f32x2_to_bf16x2(v[8 * i + 6], v[8 * i + 7])};
+        return;
+    }
 #pragma unroll
-            for (int i = 0; i < 4; i++) *(f4a4*)((float*)p + row + e0 + 4 * i) = f4a4{v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
-        }
-    } else {
+    for (int i = 0; i < 4; i++) {
+        const int e = at16<ROT>(e0, 4 * i);
+        if (ROT ? e0 < K : e + 4 <= K) {
+            if (bf16) *(u2a2*)(h + e) = u2a2{f32x2_to_bf16x2(v[4 * i], v[4 * i + 1]), f32x2_to_bf16x2(v[4 * i + 2], v[4 * i + 3])};
+            else *(f4a4*)(f + e) = f4a4{v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
+        } else if (!ROT) {
 #pragma unroll
-        for (int j = 0; j < 16; j++) {
-            if (e0 + j < K && bf16) ((uint16_t*)p)[row + e0 + j] = (uint16_t)f32_to_bf16(v[j]);
-            if (e0 + j < K && !bf16) ((float*)p)[row + e0 + j] = v[j];
+            for (int j = 0; j < 4; j++) {
+                if (e + j < K && bf16) h[e + j] = (uint16_t)f32_to_bf16(v[4 * i + j]);
+                if (e + j < K && !bf16) f[e + j] = v[4 * i + j];
+            }
         }
     }
 }
@@ -96,16 +119,16 @@ __global__ __launch_bounds__(1024) void rms_norm_quant_kernel(RmsNorm p) {
     const int K = p.K;
     const int64_t row = (int64_t)blockIdx.x * blockDim.y + ty, rr = min(row, p.rows - 1);
     const bool live = row < p.rows;
-    auto e0_of = [&](int r) { return (wr * 4 * R + team + 4 * r) * 256 + tl * 16; };
+    auto e0_of = [&](int r) { return (wr * 4 * R + team + 4 * r) * 256 + tl * (ROT ? 16 : 4); };
 
     float v[R][16], sum = 0.0f;
 #pragma unroll
-    for (int r = 0; r < R; r++) load_row16<XB>(p.x, rr * p.ldx, e0_of(r), K, v[r]);
+    for (int r = 0; r < R; r++) load_row16<ROT, XB>(p.x, rr * p.ldx, e0_of(r), K, v[r]);
     if (RES != RES_NONE) {
 #pragma unroll
         for (int r = 0; r < R; r++) {
             float t[16];
-            load_row16<RES == RES_BF16>(p.residual, rr * p.ldr, e0_of(r), K, t);
+            load_row16<ROT, RES == RES_BF16>(p.residual, rr * p.ldr, e0_of(r), K, t);
 #pragma unroll
             for (int j = 0; j < 16; j++) v[r][j] += t[j];
         }
@@ -124,7 +147,7 @@ __global__ __launch_bounds__(1024) void rms_norm_quant_kernel(RmsNorm p) {
     }
     if (RES != RES_NONE && p.residual_out && live) {
 #pragma unroll
-        for (int r = 0; r < R; r++) store_row16(p.residual_out, RES == RES_BF16, row * p.ldr, e0_of(r), K, v[r]);
+        for (int r = 0; r < R; r++) store_row16<ROT>(p.residual_out, RES == RES_BF16, row * p.ldr, e0_of(r), K, v[r]);
     }
     const float rstd = 1.0f / sqrtf(sum / (float)K + p.eps);
     bool fine = __builtin_isfinite(sum) && __builtin_isfinite(rstd);
@@ -136,19 +159,19 @@ __global__ __launch_bounds__(1024) void rms_norm_quant_kernel(RmsNorm p) {
         for (int j = 0; j < 16; j++) v[r][j] *= rstd;
         if (p.weight) {
             float t[16];
-            if (p.w_bf16) load_row16<true>(p.weight, 0, e0, K, t);
-            else load_row16<false>(p.weight, 0, e0, K, t);
+            if (p.w_bf16) load_row16<ROT, true>(p.weight, 0, e0, K, t);
+            else load_row16<ROT, false>(p.weight, 0, e0, K, t);
 #pragma unroll
             for (int j = 0; j < 16; j++) v[r][j] *= t[j];
         }
         if (p.shift) {
             float t[16];
-            if (p.w_bf16) load_row16<true>(p.shift, 0, e0, K, t);
-            else load_row16<false>(p.shift, 0, e0, K, t);
+            if (p.w_bf16) load_row16<ROT, true>(p.shift, 0, e0, K, t);
+            else load_row16<ROT, false>(p.shift, 0, e0, K, t);
 #pragma unroll
             for (int j = 0; j < 16; j++) v[r][j] += t[j];
         }
-        if (p.y && live) store_row16(p.y, p.y_bf16, row * p.ldy, e0, K, v[r]);
+        if (p.y && live) store_row16<ROT>(p.y, p.y_bf16, row * p.ldy, e0, K, v[r]);
         float bad = 0.0f;
 #pragma unroll
         for (int j = 0; j < 16; j++) bad = fmaf(v[r][j], 0.0f, bad);  // NaN once an infinity or a NaN is met
@@ -229,13 +252,19 @@ __global__ __launch_bounds__(1024) void rms_norm_quant_kernel(RmsNorm p) {
                 packed[k] = cvt_pack4(d[0], d[1], d[2], d[3]);
             }
         }
-        int8_t* dst = p.q + row * p.ldq + e0;
-        if (e0 + 16 <= K) {
-            *(u4a1*)dst = u4a1{packed[0], packed[1], packed[2], packed[3]};
-        } else {
+        int8_t* dst = p.q + row * p.ldq;
+        if (ROT) {
+            if (e0 < K) *(u4a1*)(dst + e0) = u4a1{packed[0], packed[1], packed[2], packed[3]};
+            continue;
+        }
 #pragma unroll
-            for (int j = 0; j < 16; j++)
-                if (e0 + j < K) dst[j] = (int8_t)(packed[j / 4] >> 8 * (j % 4));
+        for (int i = 0; i < 4; i++) {
+            const int e = at16<ROT>(e0, 4 * i);
+            if (e + 4 <= K) *(u1a1*)(dst + e) = packed[i];
+            else
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (e + j < K) dst[e + j] = (int8_t)(packed[i] >> 8 * j);
         }
     }
 }
