@@ -115,8 +115,8 @@ phi_status phi_hip_kv_cache_read(phi_stream_t stream, const phi_kv_cache* cache,
  *   q_start      [batch + 1] int32, ascending from 0 to tokens
  *   kv_len       [batch] int32
  *   max_q        at least the longest sequence's n: rows past it are left as they are
- *   max_kv       at least the longest kv_len, at most table_width * page: tokens
- *                past it are not seen
+ *   max_kv       at least the longest kv_len, at most table_width * page and 2^30:
+ *                tokens past it are not seen
  *   window       0, or with causal the number of tokens seen, the row's own included
  *   workspace    phi_hip_paged_attention_workspace_bytes() bytes, 16-byte aligned
  *                (NULL when that is 0)
@@ -126,8 +126,12 @@ phi_status phi_hip_kv_cache_read(phi_stream_t stream, const phi_kv_cache* cache,
  * held as integers of 16 bits (PHI_BF16) or 24 bits (PHI_F32) relative to the
  * row's largest |q|, k and v as their codes, exactly, and p enters p.v with 16
  * or 24 bits.  PHI_BF16 sequences of more than 128 rows (new tokens x query heads
- * a key/value head) round each element of k and v to 11 bits instead, and p
- * to 11 bits or an error of 2^-39 of the row's largest p.
+ * a key/value head) have q exactly (elements below 2^-21 of the row's largest
+ * apart), k's elements rounded to 11 bits, v's scales and v's elements to 11 bits
+ * each or an error of 2^-23 of the largest of 16 tokens, and p's to 11 bits or an
+ * error of 2^-39 of the row's largest p.
+ * The order of sums, and so a result's last bits, depends on the sizes, the lengths
+ * and max_q, max_kv and batch; the same call gives the same bits.
  */
 phi_status phi_hip_paged_attention(phi_stream_t stream, const void* q, int dtype, int64_t q_token_stride,
                                    int64_t q_head_stride, int64_t tokens, int64_t q_heads, const phi_kv_cache* cache,
@@ -138,7 +142,7 @@ phi_status phi_hip_paged_attention(phi_stream_t stream, const void* q, int dtype
                                    size_t ws_bytes);
 
 /* Workspace of phi_hip_paged_attention for these sizes (0 when a call does not
- * split its tokens). */
+ * split its tokens; one with a window may need less). */
 size_t phi_hip_paged_attention_workspace_bytes(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t dim,
                                                int64_t batch, int64_t max_q, int64_t max_kv, int dtype);
 

@@ -4,15 +4,13 @@
 //
 // Bound by memory.  A team of lanes has a vector, 16 elements a lane in pieces of 16
 // bytes, each piece of all lanes together; the largest |x| by shuffles within the
-// team.
-// A wave's teams have consecutive tokens of a head, whose codes and scales lie
+// team.  A wave's teams have consecutive tokens of a head, whose codes and scales lie
 // together in a page; consecutive waves have the heads of k, then of v, whose
-// elements lie together in the projection's output.  32760 tokens of 8 heads of
-// 128 in bf16: 49 us for the write (4.1 TB/s, of 4.9 that a copy reaches) and 37 for
-// the read (5.5).  With a token's k and v in one team, 56 and 37; with all tokens
-// of one head before the next head's, so that elements are read in pieces of 256
-// bytes, 64 and 34; with an element a lane and a
-// wave a vector 189 and 139.
+// elements lie together in the projection's output.  32760 tokens of 8 heads of 128 in
+// bf16: 49 us for the write (4.1 TB/s, of 4.9 that a copy reaches) and 37 for the read
+// (5.5).  With a token's k and v in one team, 56 and 37; with all tokens of one head
+// before the next head's, so that elements are read in pieces of 256 bytes, 64 and 34;
+// with an element a lane and a wave a vector, 189 and 139.
 #include "decoder.hpp"
 #include "device_common.hpp"
 

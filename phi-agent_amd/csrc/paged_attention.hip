@@ -109,7 +109,8 @@ __global__ __launch_bounds__(256) void attn_join_kernel(PagedAttn p, AttnPart fe
 
 namespace {
 
-// bf16 sequences of more rows than this go to the chunk kernel.
+// bf16 sequences of more rows than this go to the chunk kernel (8 sequences over 8192:
+// 64 rows take 77 us and 128 rows 130 here, 136 rows 110 there).
 constexpr int kFewRows = 128;
 
 // Sequences of few rows are split so that about kShares blocks have work, the two

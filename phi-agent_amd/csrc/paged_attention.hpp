@@ -260,8 +260,8 @@ __device__ __forceinline__ void split_q16(const Q16<F32>& x, float inv, v4i (&ou
     }
 }
 
-// c_t in fp32 (exactly, for bf16 q's two terms at dim <= 256: below 2^31) from
-// the terms' products.
+// c_t in fp32, rounded once for bf16 q (its two terms' sum is exact, below 2^31 at
+// dim <= 256), three times for fp32 q.
 template <bool F32>
 __device__ __forceinline__ float join_terms(const int (&c)[q_terms<F32>]) {
     if (F32) return fmaf((float)c[q_terms<F32> - 1], 65536.0f, fmaf((float)c[1], 256.0f, (float)c[0]));
