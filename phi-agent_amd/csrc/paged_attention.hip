@@ -131,7 +131,8 @@ constexpr int kSplitTiles = 256, kSplitBlocks = 2048;
 // 256 shares).
 constexpr int kSplitChunks = 256, kSharesChunks = 256;
 // Nor up to kWhole tokens: a second launch for the join costs the host 4 us, and the
-// GPU gains 1.9 at 1024 tokens (14.8 to 12.9), 1 at 777 and loses 2.4 at 512.
+// GPU gains 1.5 us for one sequence of 1024 (14.2 to 12.7), 1 at 777, loses 0.8 at 600,
+// and 2.5 for eight of 1024.
 constexpr int kWhole = 1024;
 
 // Up to this many rows x heads, a row's join takes four waves (one sequence of 32768,

@@ -42,6 +42,10 @@ template <int DP> struct Step {
     bool ok[2][4];  // the table has a block for the token (PAGE16: of the tile)
 };
 
+// Byte n of w, signed, as fp32: one instruction in this form, two from a cast of a
+// byte, which took 64 a step of 280 (one sequence of 777 tokens: 14.5 us to 13.4).
+__device__ __forceinline__ float byte_f32(uint32_t w, int n) { return (float)((int32_t)(w << (24 - 8 * n)) >> 24); }
+
 }  // namespace
 
 // DP: dim rounded up to 64, 128 or 256.  F32: fp32 q and out, else bf16.
@@ -259,8 +263,8 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void paged_decode_k
             v4i a;
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                const float f0 = (float)(int8_t)(st.v[k >> 1][2 * (k & 1)][e / 4] >> 8 * (e % 4));
-                const float f1 = (float)(int8_t)(st.v[k >> 1][2 * (k & 1) + 1][e / 4] >> 8 * (e % 4));
+                const float f0 = byte_f32(st.v[k >> 1][2 * (k & 1)][e / 4], e % 4);
+                const float f1 = byte_f32(st.v[k >> 1][2 * (k & 1) + 1][e / 4], e % 4);
                 a[k] = (int)__builtin_amdgcn_perm(__float_as_uint(f1), __float_as_uint(f0), 0x07060302u);
             }
 #pragma unroll
