@@ -25,6 +25,8 @@ def _empty(shape, dtype, like: torch.Tensor, stream) -> torch.Tensor:
 
 def _row_pitch(name: str, t: torch.Tensor, shape) -> int:
     """The pitch of a [rows, K] tensor with contiguous rows (of one row: any from K on)."""
+    if t.shape == shape and t.is_contiguous():
+        return shape[1]
     if t.shape != shape:
         raise ValueError(f"rms_norm_quant: {name} is {tuple(t.shape)}, not {tuple(shape)}")
     pitch, step = t.stride()
