@@ -11,8 +11,12 @@
 //     LDS in the order in which the products read them, without bank
 //     conflicts.  K: one fp32 product and one rounding to 11 bits a code, at
 //     random sides, so that a logit is off by some 2^-13 |s| / sqrt(dim) (q is
-//     exact in fp16).  V: the scale has 11 bits too, which makes it one packed
-//     instruction for two codes.
+//     exact in fp16).  V: the scale has 11 bits too, which makes it two packed
+//     instructions for two codes, the first of which makes the codes exact in a unit
+//     that leaves the product fp16's range.  (With one, code * scale less the bias, the
+//     bias loses its bits: a token of 2^-12 of its 16 tokens' largest scale is off by 0.2 %,
+//     to one side, one of 2^-20 by 40 %.  The second costs 0.8 % of the time below, 1.3 % at
+//     dim 256; fp32 scales in v_fma_mix, as for K, 3 % and 7 %.)
 //     int8 products for q.k, exact, cost the matrix cores the same but the
 //     vector unit three more instructions for every logit (join, convert, scale).
 //   - S^T = K Q^T and O^T = V^T P^T (v_mfma_f32_32x32x16_f16): the logits' layout
@@ -45,7 +49,8 @@ constexpr int kGroups = kTile / 16;
 // and an absolute error of 2^-39 of it from there.
 constexpr int kP = 14, kUp = 1;
 constexpr int kMinExp = -100;  // of a group's unit: its inverse stays finite
-// V's fp16 is code * M 2^-24, M = scale * 2^(kM - E) below 2^15.
+// V's fp16 is code 2^-9 * M, M = scale * 2^(kM - E) below 2^15, both factors in fp16: below
+// 2^13, with 11 bits down to 2^-20 of the unit 2^E of its 16 tokens.
 constexpr int kM = 14;
 
 typedef uint32_t u2 __attribute__((ext_vector_type(2)));
@@ -297,10 +302,10 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel
     // turn of products takes one at a time between its own.  Both kinds: take what
     // was loaded, load the tile after, the scales; then an eighth of an item's
     // codes each.
-    constexpr int kVPieces = 5 + 8 * NVI, kKPieces = 5 + 8 * NKI;
+    constexpr int kVPieces = 4 + 8 * NVI, kKPieces = 5 + 8 * NKI;
     int v_e = 0;
     float v_f = 0.0f;
-    h2 v_mul[NVI][4], v_sub[NVI][4];
+    h2 v_mul[NVI][4];
     h8 v_out;
     auto v_piece = [&](auto index, ChunkTile<DP>& to, int next_t0) __attribute__((always_inline)) {
         constexpr int P = decltype(index)::value;
@@ -320,20 +325,15 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel
 #pragma unroll
                 for (int j = 0; j < 4; j++)
                     v_mul[it][j] = __builtin_bit_cast(h2, __builtin_amdgcn_ds_bpermute(4 * token_of(v_item(it) / (DP / 4), 2 * j), pair));
-        } else if constexpr (P == 4) {
-#pragma unroll
-            for (int it = 0; it < NVI; it++)
-#pragma unroll
-                for (int j = 0; j < 4; j++) v_sub[it][j] = v_mul[it][j] * h2{(_Float16)-0x1p-17f, (_Float16)-0x1p-17f};
         } else {
-            constexpr int it = (P - 5) / 8, e4 = (P - 5) % 8 / 2, half = (P - 5) % 2;
+            constexpr int it = (P - 4) / 8, e4 = (P - 4) % 8 / 2, half = (P - 4) % 2;
             const uint32_t sel = 0x0c000c00u | (uint32_t)((4 + e4) << 16) | (uint32_t)e4;
 #pragma unroll
             for (int j = 2 * half; j < 2 * half + 2; j++) {
                 if constexpr (e4 == 0) raw_v.w[8 * it + 2 * j] ^= 0x80808080u, raw_v.w[8 * it + 2 * j + 1] ^= 0x80808080u;
-                // code 2^-24 M = (code + 128) 2^-24 M - M 2^-17.
+                // The halves (code + 128) 2^-24 to code 2^-9, exactly; a factor a token.
                 const h2 u = __builtin_bit_cast(h2, __builtin_amdgcn_perm(raw_v.w[8 * it + 2 * j + 1], raw_v.w[8 * it + 2 * j], sel));
-                const h2 y = __builtin_elementwise_fma(u, v_mul[it][j], v_sub[it][j]);
+                const h2 y = __builtin_elementwise_fma(u, h2{(_Float16)0x1p15f, (_Float16)0x1p15f}, h2{(_Float16)-0.25f, (_Float16)-0.25f}) * v_mul[it][j];
                 v_out[2 * j] = y[0], v_out[2 * j + 1] = y[1];
             }
             if constexpr (half) {
@@ -565,8 +565,8 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel
     if (w0 + col >= rows) return;
     const bool split = unit_of.slot >= 0;
     const int64_t at = ((int64_t)kh * sp.slots + unit_of.slot) * (32 * NW) + 32 * wave + col;
-    // O holds sum p v in units of 2^(kP + kM - 24 - vexp), l of 2^kP.
-    const float unit = ldexpf(1.0f, vexp + 24 - kM) * (split ? 1.0f / (1 << kP) : l != 0.0f ? 1.0f / l : 0.0f);
+    // O holds sum p v in units of 2^(kP + kM - 9 - vexp), l of 2^kP.
+    const float unit = pow2(vexp + 9 - kM), share = split ? 1.0f / (1 << kP) : l != 0.0f ? 1.0f / l : 0.0f;
     if (split && h == 0) sp.ml[2 * at] = m, sp.ml[2 * at + 1] = l * (1.0f / (1 << kP));
     // Value n, j is of slot 32 n + 8 (j / 4) + 4 h + j % 4, so d = 4 (slot % (DP/4))
     // + slot / (DP/4): the four d of a slot % (DP/4) together.
@@ -581,7 +581,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel
 #pragma unroll
         for (int e4 = 0; e4 < 4; e4++) {
             const int slot = e4 * Q + 8 * blk + jj;  // less 4 h, which the lane's registers carry
-            y[e4] = o[slot >> 5][4 * ((slot & 31) >> 3) + (slot & 3)] * unit;
+            y[e4] = o[slot >> 5][4 * ((slot & 31) >> 3) + (slot & 3)] * share * unit;
         }
         if (split) {
             *(v4f*)(sp.o + at * D + 4 * dq) = y;

@@ -1,0 +1,134 @@
+"""Paged attention of chunks (bf16 sequences of more than 128 rows) on values at the
+ends of their ranges.
+
+The oracle is a plain softmax in 64 bits, a sequence and head at a time.  Beside each
+value stands how far the kernel's arithmetic may be from it:
+  k   fp16, in a unit in which 16 tokens' largest scale is 2^7 to 2^8: 2^-11 of an
+      element, or half a subnormal's step, 2^-25 of 2^7 at least: 2^-32 of that scale
+  v   fp16 of its scale's fp16 (2^-11 each), in a unit in which 16 tokens' largest scale
+      is 2^5 to 2^6: 2^-30 of that scale from v's step and 2^-32 from a scale's own
+  q   exact, but half a subnormal's step (2^-25 where the row's largest is 2^7 or more)
+  p   fp16 in 2^14 at the row's largest: 2^-11 of it, or 2^-25 / 2^14 = 2^-39 of the
+      largest p, for a v of up to 128 times the largest scale that its blocks see
+  sums in fp32 (2^-20 of the sum of magnitudes), the logit's own roundings (five, in
+  units of 2^-24) and exp2's, 2^-22; the output's bf16."""
+import math
+
+import pytest
+import torch
+
+import decoder_ref as R
+import phi_qlinear as Q
+
+pytestmark = pytest.mark.gpu
+
+BF16 = torch.bfloat16
+
+
+def groups_top(scales, codes, live):
+    """Of [tokens] scales: the largest |scale| among a token's 16, of those that are live
+    and have a nonzero code."""
+    s = torch.where(live & codes.ne(0).any(dim=1), scales.double().abs(), 0.0)
+    pad = -len(s) % 16
+    top = torch.cat([s, torch.zeros(pad, dtype=s.dtype)]).view(-1, 16).max(dim=1)[0]
+    return top.repeat_interleave(16)[:len(s)]
+
+
+def oracle(c, *, scale, causal=True, window=0):
+    """(out, bound) in 64 bits; NaN for rows of no sequence and rows that see a scale of NaN."""
+    q, k, v, ks, vs, table = (c[x] for x in ("q", "k", "v", "ks", "vs", "table"))
+    T, Hq, D = q.shape
+    blocks, H, page, _ = k.shape
+    G = Hq // H
+    out, bound = (torch.full((T, Hq, D), math.nan, dtype=torch.float64) for _ in range(2))
+    for b, kv in enumerate(c["kv_len"]):
+        s0, n = c["starts"][b], c["starts"][b + 1] - c["starts"][b]
+        t = torch.arange(kv)
+        blk = table[b][t // page].long() if kv else t
+        live = (blk >= 0) & (blk < blocks)
+        pos = kv - n + torch.arange(n)[:, None]
+        seen = live[None, :].expand(n, -1)
+        if causal:
+            seen = seen & (t <= pos)
+        if window:
+            seen = seen & (t > pos - window)
+        some = seen.any(0)
+        blk, at = blk.clamp(0, blocks - 1), t % page
+        for h in range(Hq):
+            g = h // G
+            if not bool(some.any()):
+                out[s0:s0 + n, h], bound[s0:s0 + n, h] = 0.0, 0.0
+                continue
+            (kd, k_top), (vd, v_top) = (
+                (torch.where(some[:, None], x[blk, g, at].double() * s[blk, g, at].double()[:, None], 0.0),
+                 groups_top(s[blk, g, at], x[blk, g, at], some)) for x, s in ((k, ks), (v, vs)))
+            qd = q[s0:s0 + n, h].double()
+            logit = qd @ kd.T * scale
+            p = torch.where(seen, torch.exp(logit - torch.where(seen, logit, -math.inf).max(1, keepdim=True)[0].clamp(min=-1e300)), 0.0)
+            p = p / p.sum(1, keepdim=True).clamp(min=1e-300)
+            e = 2.0 ** -11 * (qd.abs() @ kd.abs().T) + 2.0 ** -32 * (qd.abs().sum(1)[:, None] * k_top + qd.abs().max(1)[0][:, None] * kd.abs().sum(1))
+            # A weight is off by the factor of its own logit's error, their sum by the mean of these.
+            e = p * torch.expm1(torch.where(seen, abs(scale) * e + 5 * 2.0 ** -24 * 1.4427 * logit.abs(), 0.0) + 2.0 ** -22)
+            weight, off = p @ vd.abs(), e.sum(1)[:, None]
+            least = 2.0 ** -29 * (p @ v_top) + 2.0 ** -39 * 256 * float(v_top.max()) * p.max(1)[0] * seen.sum(1)
+            o = p @ vd
+            out[s0:s0 + n, h] = o
+            bound[s0:s0 + n, h] = (e @ vd.abs() + off * weight) / (1 - off) + (3 * 2.0 ** -11 + 2.0 ** -20) * weight + least[:, None] + 2.0 ** -8 * o.abs()
+    return out, bound
+
+
+def run(dev, c, *, max_q=None, **kw):
+    to = lambda t: torch.empty_strided(t.shape, t.stride(), dtype=t.dtype, device=dev).copy_(t)  # noqa: E731
+    cache = Q.KvCache(*(to(c[x]) for x in ("k", "v", "ks", "vs")))
+    starts, lens = (torch.tensor(c[x], dtype=torch.int32, device=dev) for x in ("starts", "kv_len"))
+    n = max(b - a for a, b in zip(c["starts"], c["starts"][1:]))
+    got = Q.paged_attention(to(c["q"]), cache, c["table"].to(dev), starts, lens, max_q=max_q or n, max_kv=max(c["kv_len"]), **kw)
+    return got.cpu()
+
+
+def check(dev, c, *, max_q=None, out=None, **kw):
+    assert (c["starts"][1] - c["starts"][0]) * (c["q"].shape[1] // c["k"].shape[1]) > 128
+    kw.setdefault("scale", c["q"].shape[2] ** -0.5)
+    got = run(dev, c, max_q=max_q, out=out, **kw)
+    want, bound = oracle(c, **kw)
+    err = (got.double() - want).abs()
+    nan = want.isnan()
+    assert torch.equal(got.isnan(), nan), f"{int(got.isnan().sum())} values are NaN, {int(nan.sum())} should be"
+    worst = float((err / bound.clamp(min=1e-300))[~nan].max())
+    assert worst <= 1.0, f"{worst:.3g} times the bound"
+    return got
+
+
+def case(lens, D=128, page=16, Hq=1, H=1, seed=1, **kw):
+    return R.make_case(lens, Hq=Hq, H=H, D=D, page=page, dtype=BF16, seed=seed, **kw)
+
+
+def place(c, b, t):
+    """Token t of sequence b in the cache: an index of ks and vs (head 0)."""
+    page = c["k"].shape[2]
+    return int(c["table"][b, t // page]), 0, t % page
+
+
+# ------------------------------------------------------------------ scales of v
+@pytest.mark.parametrize("D,page", [(128, 16), (64, 8), (80, 24), (256, 64)])
+@pytest.mark.parametrize("bits", [6, 10, 12, 14, 16, 20, 24])
+def test_small_values_beside_large_ones(dev, D, page, bits):
+    """One token of every 16 has values 2^bits of the others' and no weight to speak of."""
+    c = case([(150, 500)], D=D, page=page, seed=bits)
+    c["q"][:, 0, 0] = 16
+    c["k"][..., 0] = 0
+    c["vs"] = c["vs"].clamp(min=0.03) * 2.0 ** -bits
+    for t in range(5, 500, 16):
+        at = place(c, 0, t)
+        c["k"][at] = 0
+        c["k"][at][0], c["ks"][at], c["vs"][at] = -127, 0.5, 0.05
+    check(dev, c)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("top", [2.0 ** 117, 2.0 ** 118, 1e36, 2.0 ** -100, 1e-31])
+def test_largest_and_smallest_value_scales(dev, D, top):
+    """Scales to 2^119.6, whose values to 2^126.6 fp32 holds, and down to 4e-33."""
+    c = case([(140, 333)], D=D, seed=D)
+    c["vs"] *= top / 0.052
+    check(dev, c)
