@@ -447,7 +447,9 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel
         int e = vexp;
 #pragma unroll
         for (int g = 0; g < kGroups; g++) {
-            ru[g] = rq * ct.k_unit[g];
+            // Above 0 whatever the units (a row of zeros, 16 tokens that are not there), so
+            // that a masked logit stays -inf; 2^-149 more is nothing to the others.
+            ru[g] = fmaf(rq, ct.k_unit[g], 0x1p-149f);
             holes |= ct.seen[g] ^ 0xffffu;
             e = max(e, ct.v_exp[g]);
         }

@@ -132,3 +132,37 @@ def test_largest_and_smallest_value_scales(dev, D, top):
     c = case([(140, 333)], D=D, seed=D)
     c["vs"] *= top / 0.052
     check(dev, c)
+
+
+# ------------------------------------------------------------------ query rows of nothing
+@pytest.mark.parametrize("D,page", [(64, 16), (128, 16), (128, 24), (80, 32), (256, 16), (192, 7)])
+@pytest.mark.parametrize("n,kv", [(140, 228), (150, 150), (200, 1301), (130, 47)])
+def test_zero_and_tiny_query_rows(dev, D, page, n, kv):
+    """Equal weights for all that a row of zeros sees, wherever the last tile of 64 ends."""
+    c = case([(n, kv)], D=D, page=page, seed=D + kv)
+    for i, x in enumerate((0.0, 1e-8, 1e-12, 1e-20, 1e-30, 1e-38, -0.0)):
+        c["q"][i::11] *= x
+    check(dev, c)
+    check(dev, c, causal=False)
+    check(dev, c, window=33)
+
+
+@pytest.mark.parametrize("page", [16, 8])
+def test_zero_query_rows_over_holes(dev, page):
+    """Whole groups of 16 tokens that are not there, at the ends of tiles and within them."""
+    c = case([(160, 700), (140, 333)], page=page)
+    c["q"][::2], c["q"][1::4] = 0, c["q"][1::4] * 1e-13
+    c["table"][0, 32 // page:64 // page], c["table"][0, 400 // page], c["table"][1, 0:16 // page] = -1, 1 << 20, -5
+    check(dev, c)
+
+
+@pytest.mark.parametrize("q,k", [(1e-20, 1e-20), (1e-30, 1e30), (1e25, 1e-25), (1.0, 1e-33), (1e-12, 1e8)])
+def test_units_of_q_and_k_apart(dev, q, k):
+    """Rows and keys of sizes whose product is 1, or all but nothing, beside groups that are not there."""
+    c = case([(140, 420)], page=8, seed=7)
+    c["q"][::3] *= q
+    c["ks"] *= k
+    c["q"][1::3] *= min(1.0, 1.0 / k)
+    c["q"][2::3] = 0
+    c["table"][0, 4:10], c["table"][0, 30] = -1, -1
+    check(dev, c)
