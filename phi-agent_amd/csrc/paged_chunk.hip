@@ -201,6 +201,8 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel
     // without a block, reads whatever lies in the last page or block 0 and counts
     // as scale 0.  Loads run a tile ahead of what is being staged, and the table's
     // entry for them two; nothing loaded is looked at before.
+    const int begin = lo & ~(kTile - 1), count = begin < hi ? (hi - begin + kTile - 1) / kTile : 0;
+    auto start = [&](int n) { return begin + n * kTile; };
     const int group = wave & 3, n16 = lane & 15;
     const int32_t* trow = table + (int64_t)b * p.table_stride;
     const int last_page = page_of(c, max(hi - 1, 0));
@@ -292,13 +294,30 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel
         }
         fetch(raw, t0 + kTile);
     };
-    // E of the group's V scales, the same from V's wave and K's: 2^E <= the
-    // largest that is there and finite.
-    auto v_exp_of = [&](const Raw& raw, float& f) __attribute__((always_inline)) {
+    // E of the group's V scales, the same from V's wave and K's: 2^E <= the largest that
+    // is there and finite and no zeros'.  The cache has a vector of zeros at the scale
+    // 1, whatever its neighbours' are, so the codes of tokens with that scale are looked
+    // at, a quarter of a vector's pieces a lane.  (Rare, so by loads of its own: the
+    // branch costs 1 %, 2 % at dim 256, and 20 % where every tenth vector is zeros; a test of
+    // all codes as V is staged 5 % to 10 %.)
+    auto v_exp_of = [&](const Raw& raw, int tile_n, float& f) __attribute__((always_inline)) {
         f = (raw.ok != 0) & __builtin_isfinite(raw.vs) ? raw.vs : 0.0f;
+        if (__any(f == 1.0f)) {
+            int codes = 0;
+            if (f == 1.0f) {
+                const int t = start(tile_n) + 16 * group + n16, page = page_of(c, t);
+                const int8_t* row = c.v + kh * c.head_stride + trow[page] * c.block_stride + (t - page * c.page) * c.token_stride;
+                for (int d = 16 * (lane >> 4); d < D; d += 64) {
+                    const v4i w = *(const v4i*)(row + d);
+                    codes |= w[0] | w[1] | w[2] | w[3];
+                }
+            }
+            const uint64_t some = __ballot(codes != 0), half = some | some >> 32;
+            f = (half | half >> 16) >> n16 & 1 ? f : f == 1.0f ? 0.0f : f;
+        }
         return exp_of(row_top(fabsf(f)));
     };
-    // Staging in pieces without a branch and of a few instructions each, which the
+    // Staging in pieces without a branch (but that) and of a few instructions each, which the
     // turn of products takes one at a time between its own.  Both kinds: take what
     // was loaded, load the tile after, the scales; then an eighth of an item's
     // codes each.
@@ -307,14 +326,14 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel
     float v_f = 0.0f;
     h2 v_mul[NVI][4];
     h8 v_out;
-    auto v_piece = [&](auto index, ChunkTile<DP>& to, int next_t0) __attribute__((always_inline)) {
+    auto v_piece = [&](auto index, int tile_n, int next_t0) __attribute__((always_inline)) {
         constexpr int P = decltype(index)::value;
         if constexpr (P == 0) {
             raw_v = next_v;
         } else if constexpr (P == 1) {
             load(next_v, next_t0, false);
         } else if constexpr (P == 2) {
-            v_e = v_exp_of(raw_v, v_f);
+            v_e = v_exp_of(raw_v, tile_n, v_f);
         } else if constexpr (P == 3) {
             // Lane l has the factors of tokens l & 15 and the next, as a pair.
             const float m0 = v_f * pow2(kM - v_e);
@@ -338,7 +357,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel
             }
             if constexpr (half) {
                 const int ih = v_item(it) / (DP / 4), dq = v_item(it) % (DP / 4);
-                *(h8*)(to.v + (((2 * group + ih) * DP + e4 * (DP / 4) + dq) * 8)) = v_out;
+                *(h8*)(tile[tile_n & 1].v + (((2 * group + ih) * DP + e4 * (DP / 4) + dq) * 8)) = v_out;
             }
         }
     };
@@ -353,7 +372,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel
             load(next_k, next_t0, true);
         } else if constexpr (P == 2) {
             float fv;
-            k_ev = v_exp_of(raw_k, fv);
+            k_ev = v_exp_of(raw_k, tile_n, fv);
             // A token whose value is not finite is NaN to the rows that see it.
             const float fk = __builtin_isfinite(raw_k.vs) ? raw_k.ks : __builtin_nanf("");
             k_f = raw_k.ok != 0 ? fk : 0.0f;
@@ -513,14 +532,12 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel
     //   it over that of n - 2, which the softmax read until 2n - 2;
     // a barrier ends every turn.  Four waves have one turn a tile.  Tiles staged
     // past the last are never read.
-    const int begin = lo & ~(kTile - 1), count = begin < hi ? (hi - begin + kTile - 1) / kTile : 0;
-    auto start = [&](int n) { return begin + n * kTile; };
     auto walk = [&](auto with_v, auto with_k) __attribute__((always_inline)) {
         constexpr bool V = decltype(with_v)::value, K = decltype(with_k)::value;
         if (V) {
             fetch(next_v, start(0));
             load(next_v, start(0), false);
-            each<kVPieces>([&](auto i) __attribute__((always_inline)) { v_piece(i, tile[0], start(1)); });
+            each<kVPieces>([&](auto i) __attribute__((always_inline)) { v_piece(i, 0, start(1)); });
         }
         if (K) {
             fetch(next_k, start(0));
@@ -543,7 +560,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel
                 constexpr int first = (P * pieces + N - 1) / N, end = ((P + 1) * pieces + N - 1) / N;
                 static_assert(pieces <= N, "a piece a product");
                 if constexpr (end > first) {
-                    if constexpr (V && first < kVPieces) v_piece(int_c<first>{}, tile[(n + 1) & 1], start(n + 2));
+                    if constexpr (V && first < kVPieces) v_piece(int_c<first>{}, n + 1, start(n + 2));
                     else k_piece(int_c<first - (V ? kVPieces : 0)>{}, n + 2, start(n + 3));
                 }
                 if constexpr (P == N - 8) read_meta(n + 1);

@@ -166,3 +166,34 @@ def test_units_of_q_and_k_apart(dev, q, k):
     c["q"][2::3] = 0
     c["table"][0, 4:10], c["table"][0, 30] = -1, -1
     check(dev, c)
+
+
+# ------------------------------------------------------------------ vectors of zeros
+@pytest.mark.parametrize("D,page", [(128, 16), (64, 8), (80, 24), (256, 16), (192, 7)])
+@pytest.mark.parametrize("bits", [12, 16, 20, 30, 40, 90])
+def test_zero_values_beside_small_ones(dev, D, page, bits):
+    """A vector of zeros has the scale 1, whatever its neighbours have."""
+    c = case([(150, 500)], D=D, page=page, seed=bits)
+    c["vs"] *= 2.0 ** -bits
+    for t in (*range(3, 500, 16), *range(200, 250)):
+        at = place(c, 0, t)
+        c["v"][at], c["vs"][at] = 0, 1.0
+    check(dev, c)
+    check(dev, c, window=100)
+
+
+@pytest.mark.parametrize("size", [1.0, 1e-4, 1e-8, 1e-20])
+def test_written_zero_vectors(dev, size):
+    """As the cache's own quantiser writes them, keys of zeros among them too."""
+    H, D, page, kv, n = 2, 128, 16, 400, 150
+    g = torch.Generator().manual_seed(3)
+    k, v = (torch.randn((kv, H, D), generator=g) for _ in range(2))
+    v *= size
+    for x in (k, v):
+        x[torch.rand((kv, H), generator=g) < 0.1] = 0
+    v[-70:-60] = 0
+    cache = Q.kv_cache_empty(kv // page, page, H, D, dev)
+    Q.kv_cache_write(cache, k.to(BF16).to(dev), v.to(BF16).to(dev), torch.arange(kv, device=dev))
+    c = dict(q=torch.randn((n, 2 * H, D), generator=g).to(BF16), table=torch.arange(kv // page, dtype=torch.int32)[None],
+             starts=[0, n], kv_len=[kv], **{x: t.cpu() for x, t in zip(("k", "v", "ks", "vs"), cache)})
+    check(dev, c)
