@@ -129,8 +129,10 @@ phi_status phi_hip_kv_cache_read(phi_stream_t stream, const phi_kv_cache* cache,
  * a key/value head) have q exactly (elements below 2^-21 of the row's largest
  * apart), k's elements rounded to 11 bits or an error of 2^-32 of the largest scale
  * of k of 16 tokens, v's scales and v's elements to 11 bits each or an error of 2^-29
- * of the largest scale of v of 16 tokens (vectors of zeros apart), and p's to 11 bits or an error of 2^-39 of
- * the row's largest p.
+ * of the largest scale of v of 16 tokens (vectors of zeros apart), and p's to 11
+ * bits or an error of 2^-39 of the row's largest p, times the ratio of the largest
+ * scale of v to that of the 16 tokens.  The largest are those of the tokens that some
+ * row of a block of 256 (dim above 128: 128) sees.
  * The order of sums, and so a result's last bits, depends on the sizes, the lengths
  * and max_q, max_kv and batch; the same call gives the same bits.
  */

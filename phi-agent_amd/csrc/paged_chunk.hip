@@ -197,9 +197,9 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel
     }
 
     // ---- the tile's codes: a wave takes 16 tokens, V's or (four waves: and) K's.
-    // Lane l finds token l & 15 and has its scales; a token at hi or past it, or
-    // without a block, reads whatever lies in the last page or block 0 and counts
-    // as scale 0.  Loads run a tile ahead of what is being staged, and the table's
+    // Lane l finds token l & 15 and has its scales; a token below lo, at hi or past it,
+    // or without a block, reads whatever lies there, in the last page or in block 0
+    // and counts as scale 0.  Loads run a tile ahead of what is being staged, and the table's
     // entry for them two; nothing loaded is looked at before.
     const int begin = lo & ~(kTile - 1), count = begin < hi ? (hi - begin + kTile - 1) / kTile : 0;
     auto start = [&](int n) { return begin + n * kTile; };
@@ -537,11 +537,13 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel
         if (V) {
             fetch(next_v, start(0));
             load(next_v, start(0), false);
+            next_v.ok &= start(0) + 16 * group + n16 >= lo;  // only the first tile has tokens below lo
             each<kVPieces>([&](auto i) __attribute__((always_inline)) { v_piece(i, 0, start(1)); });
         }
         if (K) {
             fetch(next_k, start(0));
             load(next_k, start(0), true);
+            next_k.ok &= start(0) + 16 * group + n16 >= lo;
             for (int n = 0; n < 2; n++)
                 each<kKPieces>([&](auto i) __attribute__((always_inline)) { k_piece(i, n, start(n + 1)); });
         }

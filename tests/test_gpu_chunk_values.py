@@ -197,3 +197,24 @@ def test_written_zero_vectors(dev, size):
     c = dict(q=torch.randn((n, 2 * H, D), generator=g).to(BF16), table=torch.arange(kv // page, dtype=torch.int32)[None],
              starts=[0, n], kv_len=[kv], **{x: t.cpu() for x, t in zip(("k", "v", "ks", "vs"), cache)})
     check(dev, c)
+
+
+# ------------------------------------------------------------------ places that no row sees
+@pytest.mark.parametrize("D,page", [(128, 16), (64, 8), (80, 24), (256, 16)])
+@pytest.mark.parametrize("junk", [1e30, -1e30, 3e38, math.inf, math.nan])
+def test_junk_below_the_window(dev, D, page, junk):
+    """What lies before the first row's window, in its tile or far before it, may hold anything."""
+    n, kv, window = 150, 700, 90
+    c = case([(n, kv)], D=D, page=page, seed=D)
+    for t in range(kv - n + 1 - window):
+        c["ks"][place(c, 0, t)] = c["vs"][place(c, 0, t)] = junk
+    check(dev, c, window=window)
+
+
+@pytest.mark.parametrize("junk", [1e30, math.inf, math.nan])
+def test_junk_past_the_end_and_in_other_blocks(dev, junk):
+    c = case([(150, 300), (140, 190)], page=24, seed=3, blocks_extra=4)
+    for x in ("ks", "vs"):
+        c[x] = torch.where(c[x].isnan(), torch.full_like(c[x], junk), c[x])
+    c["table"][0, 3] = -1
+    check(dev, c)
