@@ -101,7 +101,7 @@ __device__ __forceinline__ float row_top(float v) {
 // E of a group of scales: 2^E <= top < 2^(E+1), within [kMinExp, 127].
 __device__ __forceinline__ int exp_of(float top) { return max(kMinExp, (int)(__float_as_uint(top) >> 23) - 127); }
 
-// 2^e, |e| < 127.
+// 2^e, -127 < e < 128.
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
 }  // namespace
@@ -182,7 +182,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel
         amax = max_x32(amax);
         bad = add_x32(bad);
         const int e = exp_of(amax);
-        const float f = p.scale * 1.4426950408889634f, unit = pow2(min(e, 126)) * 0.0078125f;
+        const float f = p.scale * 1.4426950408889634f, unit = pow2(min(e, 127)) * 0.0078125f;
         float mul = pow2(7 - e);
         rq = fabsf(f) * unit;
         if (!(rq > 0x1p-126f)) mul = 0.0f, rq = 1.0f;  // every logit is 0

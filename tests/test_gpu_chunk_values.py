@@ -218,3 +218,15 @@ def test_junk_past_the_end_and_in_other_blocks(dev, junk):
         c[x] = torch.where(c[x].isnan(), torch.full_like(c[x], junk), c[x])
     c["table"][0, 3] = -1
     check(dev, c)
+
+
+# ------------------------------------------------------------------ far ends
+@pytest.mark.parametrize("e", [126, 127])
+def test_largest_query_rows(dev, e):
+    """Rows whose largest element has bf16's largest exponents keep their logits' size."""
+    c = case([(140, 333)], seed=e)
+    scale = 2.0 ** -e
+    c["q"][::2] = (c["q"][::2].float().clamp(-1.9, 1.9) * 2.0 ** e).to(BF16)
+    c["q"][::2, 0, 0] = 1.5 * 2.0 ** e
+    c["q"][1::2] = (c["q"][1::2].float() * 2.0 ** (e - 3)).to(BF16)
+    check(dev, c, scale=scale)
