@@ -112,7 +112,8 @@ phi_status phi_hip_kv_cache_read(phi_stream_t stream, const phi_kv_cache* cache,
  *                share memory with q
  *   block_table  [batch, table_stride] int32, `table_width` entries a row; the
  *                tokens of an entry that is no block of the cache are not seen
- *   q_start      [batch + 1] int32, ascending from 0 to tokens
+ *   q_start      [batch + 1] int32, ascending from 0 to at most tokens: rows past the
+ *                last sequence's are left as they are
  *   kv_len       [batch] int32
  *   max_q        at least the longest sequence's n: rows past it are left as they are
  *   max_kv       at least the longest kv_len, at most table_width * page and 2^30:
@@ -126,7 +127,7 @@ phi_status phi_hip_kv_cache_read(phi_stream_t stream, const phi_kv_cache* cache,
  * held as integers of 16 bits (PHI_BF16) or 24 bits (PHI_F32) relative to the
  * row's largest |q|, k and v as their codes, exactly, and p enters p.v with 16
  * or 24 bits.  PHI_BF16 sequences of more than 128 rows (new tokens x query heads
- * a key/value head) have q exactly (elements below 2^-21 of the row's largest
+ * a key/value head; a batch of one: where max_q allows as many) have q exactly (elements below 2^-21 of the row's largest
  * apart), k's elements rounded to 11 bits or an error of 2^-32 of the largest scale
  * of k of 16 tokens, v's scales and v's elements to 11 bits each or an error of 2^-29
  * of the largest scale of v of 16 tokens (vectors of zeros apart), and p's to 11

@@ -157,7 +157,8 @@ Plan attn_plan(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t dim, i
                int64_t window, bool bf16) {
     const int64_t group = q_heads / kv_heads, rows = max_q * group, span = window > 0 ? std::min(max_kv, window + max_q - 1) : max_kv;
     Plan a{};
-    a.few_rows = bf16 ? kFewRows : INT32_MAX;
+    // A lone sequence takes one kernel, whose launch has to serve all its lengths to max_q.
+    a.few_rows = !bf16 ? INT32_MAX : batch == 1 && rows > kFewRows ? 0 : kFewRows;
     for (AttnPart* s : {&a.few, &a.many}) {
         const bool few = s == &a.few;
         if (few ? rows > a.few_rows && batch == 1 : rows <= a.few_rows) continue;

@@ -230,3 +230,34 @@ def test_largest_query_rows(dev, e):
     c["q"][::2, 0, 0] = 1.5 * 2.0 ** e
     c["q"][1::2] = (c["q"][1::2].float() * 2.0 ** (e - 3)).to(BF16)
     check(dev, c, scale=scale)
+
+
+# ------------------------------------------------------------------ a lone sequence of few rows
+@pytest.mark.parametrize("n", [1, 5, 64, 128, 129, 0])
+@pytest.mark.parametrize("kv", [300, 2500])
+def test_lone_sequence_shorter_than_its_bound(dev, n, kv):
+    """A buffer of 200 tokens of which q_start says that n are there: a prompt's last
+    chunk.  One captured call serves all n; rows of no sequence are left as they are."""
+    D, T = 128, 200
+    c = case([(T, kv)], D=D, seed=n)
+    to = lambda t: t.to(dev)  # noqa: E731
+    cache = Q.KvCache(*(to(c[x]) for x in ("k", "v", "ks", "vs")))
+    q, table, lens = to(c["q"]), to(c["table"]), torch.tensor([kv], dtype=torch.int32, device=dev)
+    starts, out = torch.tensor([0, T], dtype=torch.int32, device=dev), torch.empty_like(q)
+    ws = Q.paged_attention_workspace(T, 1, 1, D, 1, T, kv, BF16, dev)
+    call = lambda: Q.paged_attention(q, cache, table, starts, lens, max_q=T, max_kv=kv, out=out, workspace=ws)  # noqa: E731
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    c["starts"] = [0, n]
+    want, bound = oracle(dict(c, q=c["q"][:n]), scale=D ** -0.5)
+    for run_it in (call, graph.replay, call, graph.replay):
+        starts.copy_(torch.tensor([0, n], dtype=torch.int32))
+        out.fill_(7.0)
+        run_it()
+        got = out.cpu()
+        assert bool(((got[:n].double() - want).abs() <= bound).all()) and bool((got[n:] == 7).all())
+        starts[1] = T
+        graph.replay()  # the whole buffer between
