@@ -195,7 +195,7 @@ def paged_attention(q: torch.Tensor, cache: KvCache, block_table: torch.Tensor, 
             workspace = _empty((wn,), torch.uint8, q, stream)
     wp, wn = _ws(workspace)
     _check(L.phi_hip_paged_attention(_stream(stream), q.data_ptr(), dt, qt, qh, T, Hq, cache._desc, block_table.data_ptr(),
-                                     width, max(pitch, width), q_start.data_ptr(), kv_len.data_ptr(), B, max_q, max_kv,
+                                     width, pitch if B > 1 else width, q_start.data_ptr(), kv_len.data_ptr(), B, max_q, max_kv,
                                      D ** -0.5 if scale is None else scale, 1 if causal else 0, window, out.data_ptr(),
                                      ot, oh, wp, wn))
     return out
