@@ -145,8 +145,8 @@ phi_status phi_hip_paged_attention(phi_stream_t stream, const void* q, int dtype
                                    int64_t out_token_stride, int64_t out_head_stride, void* workspace,
                                    size_t ws_bytes);
 
-/* Workspace of phi_hip_paged_attention for these sizes (0 when a call does not
- * split its tokens; one with a window may need less). */
+/* Workspace of phi_hip_paged_attention for these sizes, with a window or without (0
+ * when a call does not split its tokens, and for sizes that no call may have). */
 size_t phi_hip_paged_attention_workspace_bytes(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t dim,
                                                int64_t batch, int64_t max_q, int64_t max_kv, int dtype);
 

@@ -196,6 +196,7 @@ size_t phi_hip_paged_attention_workspace_bytes(int64_t tokens, int64_t q_heads, 
                                                int64_t batch, int64_t max_q, int64_t max_kv, int dtype) {
     if (tokens <= 0 || q_heads <= 0 || kv_heads <= 0 || dim <= 0 || batch <= 0 || max_q <= 0 || max_kv <= 0) return 0;
     if (tokens > INT32_MAX || q_heads > 65535 || dim > 256 || batch > 65535 || max_q > tokens || max_kv > kMaxKv) return 0;
+    if (q_heads % kv_heads != 0) return 0;
     return phi_dev::paged_attention_workspace(tokens, (int)q_heads, (int)kv_heads, (int)dim, (int)batch, (int)max_q,
                                               (int)max_kv, dtype == PHI_BF16);
 }
