@@ -115,7 +115,8 @@ phi_status phi_hip_kv_cache_read(phi_stream_t stream, const phi_kv_cache* cache,
  *   q_start      [batch + 1] int32, ascending from 0 to at most tokens: rows past the
  *                last sequence's are left as they are
  *   kv_len       [batch] int32
- *   max_q        at least the longest sequence's n: rows past it are left as they are
+ *   max_q        at least the longest sequence's n, at most tokens, and 2^30 times key/value
+ *                heads over query heads: rows past it are left as they are
  *   max_kv       at least the longest kv_len, at most table_width * page and 2^30:
  *                tokens past it are not seen
  *   window       0, or with causal the number of tokens seen, the row's own included

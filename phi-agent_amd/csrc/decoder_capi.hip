@@ -24,6 +24,7 @@ bool meet(const void* a, int64_t an, const void* b, int64_t bn) {
 }
 
 constexpr int64_t kMaxKv = 1 << 30;  // a sequence's tokens: positions and steps past them stay 32-bit
+constexpr int64_t kMaxRows = 1 << 30;  // a sequence's new tokens x query heads a key/value head, the same
 constexpr int64_t kMaxK = 32768;      // columns of a norm's row (held on chip)
 constexpr int64_t kMaxPage = 1 << 20;
 constexpr int64_t kMaxPitch = (int64_t)1 << 29;    // elements: 2^31 rows of it stay within 63 bits
@@ -166,6 +167,8 @@ phi_status phi_hip_paged_attention(phi_stream_t stream, const void* q, int dtype
     if (tokens == 0 || batch == 0 || max_q == 0) return ok();
     if (tokens > INT32_MAX || batch > 65535 || max_q > tokens || max_kv > kMaxKv)
         return fail(PHI_ERR_SHAPE, "%s: tokens=%lld batch=%lld max_q=%lld max_kv=%lld out of range", who, (long long)tokens, (long long)batch, (long long)max_q, (long long)max_kv);
+    if (max_q * (q_heads / c.heads) > kMaxRows)
+        return fail(PHI_ERR_SHAPE, "%s: max_q=%lld at %lld query heads a key/value head is out of range", who, (long long)max_q, (long long)(q_heads / c.heads));
     if (max_kv > 0 && (table_width > INT32_MAX || max_kv > table_width * c.page))
         return fail(PHI_ERR_SHAPE, "%s: max_kv=%lld exceeds the block table's %lld x %d tokens", who, (long long)max_kv, (long long)table_width, c.page);
     if (table_stride < table_width || table_stride > kMaxStride) return fail(PHI_ERR_SHAPE, "%s: block table's stride is smaller than its row", who);
@@ -196,7 +199,7 @@ size_t phi_hip_paged_attention_workspace_bytes(int64_t tokens, int64_t q_heads, 
                                                int64_t batch, int64_t max_q, int64_t max_kv, int dtype) {
     if (tokens <= 0 || q_heads <= 0 || kv_heads <= 0 || dim <= 0 || batch <= 0 || max_q <= 0 || max_kv <= 0) return 0;
     if (tokens > INT32_MAX || q_heads > 65535 || dim > 256 || batch > 65535 || max_q > tokens || max_kv > kMaxKv) return 0;
-    if (q_heads % kv_heads != 0) return 0;
+    if (q_heads % kv_heads != 0 || max_q * (q_heads / kv_heads) > kMaxRows) return 0;
     return phi_dev::paged_attention_workspace(tokens, (int)q_heads, (int)kv_heads, (int)dim, (int)batch, (int)max_q,
                                               (int)max_kv, dtype == PHI_BF16);
 }
