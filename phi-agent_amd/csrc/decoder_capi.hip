@@ -18,9 +18,32 @@ bool is_float(int dtype) { return dtype == PHI_F32 || dtype == PHI_BF16; }
 
 int64_t elem(int dtype) { return dtype == PHI_BF16 ? 2 : 4; }
 
-// Whether [a, a + an) and [b, b + bn) meet (null: no).
-bool meet(const void* a, int64_t an, const void* b, int64_t bn) {
-    return a && b && (uintptr_t)a < (uintptr_t)b + (uintptr_t)bn && (uintptr_t)b < (uintptr_t)a + (uintptr_t)an;
+// n1 x n2 pieces of `bytes` bytes at strides of s1 and s2 bytes (null p: none).
+struct Pieces {
+    const void* p;
+    int64_t bytes, n1 = 1, s1 = 0, n2 = 1, s2 = 0;
+    int64_t extent() const { return (n1 - 1) * s1 + (n2 - 1) * s2 + bytes; }
+    // All pieces lie in the first `width` bytes of periods of P from p on.
+    int64_t width(int64_t P) const { return (s1 % P ? (n1 - 1) * s1 : 0) + (s2 % P ? (n2 - 1) * s2 : 0) + bytes; }
+};
+
+// Whether a piece of a may meet one of b: not where the memory they span is apart, nor
+// where a common period holds them side by side (columns of one buffer).
+bool meet(const Pieces& a, const Pieces& b) {
+    const uintptr_t pa = (uintptr_t)a.p, pb = (uintptr_t)b.p;
+    if (!pa || !pb || pa >= pb + (uintptr_t)b.extent() || pb >= pa + (uintptr_t)a.extent()) return false;
+    for (const int64_t P : {a.s1, a.s2, b.s1, b.s2}) {
+        if (P <= 0) continue;
+        const int64_t wa = a.width(P), wb = b.width(P), d = (int64_t)(pb % (uintptr_t)P) - (int64_t)(pa % (uintptr_t)P), at = d < 0 ? d + P : d;
+        if (wa <= at && at + wb <= P) return false;
+    }
+    return true;
+}
+
+// rows of K elements, and [tokens, heads, dim] vectors.
+Pieces rows_of(const void* p, int64_t rows, int64_t K, int64_t pitch, int64_t elem) { return {p, K * elem, rows, pitch * elem}; }
+Pieces vectors_of(const void* p, int64_t tokens, int64_t token_stride, int64_t heads, int64_t head_stride, int64_t dim, int64_t elem) {
+    return {p, dim * elem, tokens, token_stride * elem, heads, head_stride * elem};
 }
 
 constexpr int64_t kMaxKv = 1 << 30;  // a sequence's tokens: positions and steps past them stay 32-bit
@@ -100,15 +123,15 @@ phi_status phi_hip_rms_norm_quant(phi_stream_t stream, const void* x, int x_dtyp
     if (!aligned(x, elem(x_dtype)) || !aligned(s, 4) || (residual && (!aligned(residual, elem(res_dtype)) || !aligned(residual_out, elem(res_dtype)))) ||
         (weight && !aligned(weight, elem(w_dtype))) || (shift && !aligned(shift, elem(w_dtype))) || (y && !aligned(y, elem(y_dtype))))
         return fail(PHI_ERR_ALIGN, "%s: a pointer is not aligned to its type", who);
-    const int64_t xn = ((rows - 1) * ldx + K) * elem(x_dtype), rn = ((rows - 1) * ldr + K) * elem(res_dtype);
-    const int64_t yn = ((rows - 1) * ldy + K) * elem(y_dtype), qn = (rows - 1) * ldq + K, wn = K * elem(w_dtype);
-    const struct { const void* p; int64_t n; } in[] = {{x, xn}, {residual, rn}, {weight, wn}, {shift, wn}}, out[] = {{residual_out, rn}, {y, yn}, {q, qn}, {s, rows * 4}};
+    const int64_t re = elem(res_dtype);
+    const Pieces in[] = {rows_of(x, rows, K, ldx, elem(x_dtype)), rows_of(residual, rows, K, ldr, re), {weight, K * elem(w_dtype)}, {shift, K * elem(w_dtype)}};
+    const Pieces out[] = {rows_of(residual_out, rows, K, ldr, re), rows_of(y, rows, K, ldy, elem(y_dtype)), rows_of(q, rows, K, ldq, 1), {s, rows * 4}};
     for (const auto& o : out) {
         for (const auto& i : in)
-            if (meet(o.p, o.n, i.p, i.n) && !(o.p == residual_out && i.p == residual && o.p == i.p))
+            if (meet(o, i) && !(o.p == residual_out && i.p == residual && o.p == i.p))
                 return fail(PHI_ERR_ARG, "%s: an output overlaps an input", who);
         for (const auto& o2 : out)
-            if (&o < &o2 && meet(o.p, o.n, o2.p, o2.n)) return fail(PHI_ERR_ARG, "%s: two outputs overlap", who);
+            if (&o < &o2 && meet(o, o2)) return fail(PHI_ERR_ARG, "%s: two outputs overlap", who);
     }
     const phi_dev::RmsNorm p{x, residual, residual_out, weight, shift, y, q, s, ldx, ldr, ldy, ldq, rows, (int)K, eps, qmax,
                              x_dtype == PHI_BF16, res_dtype == PHI_BF16, w_dtype == PHI_BF16, y_dtype == PHI_BF16,
@@ -179,14 +202,14 @@ phi_status phi_hip_paged_attention(phi_stream_t stream, const void* q, int dtype
     if (st != PHI_OK) return st;
     if ((max_kv > 0 && !block_table) || !q_start || !kv_len) return fail(PHI_ERR_ARG, "%s: null pointer", who);
     if (!aligned(block_table, 4) || !aligned(q_start, 4) || !aligned(kv_len, 4)) return fail(PHI_ERR_ALIGN, "%s: block_table, q_start or kv_len is misaligned", who);
-    const int64_t qn = ((tokens - 1) * q_token_stride + (q_heads - 1) * q_head_stride + c.dim) * elem(dtype);
-    const int64_t on = ((tokens - 1) * out_token_stride + (q_heads - 1) * out_head_stride + c.dim) * elem(dtype);
-    if (meet(q, qn, out, on)) return fail(PHI_ERR_ARG, "%s: out overlaps q", who);
+    const Pieces qs = vectors_of(q, tokens, q_token_stride, q_heads, q_head_stride, c.dim, elem(dtype));
+    const Pieces os = vectors_of(out, tokens, out_token_stride, q_heads, out_head_stride, c.dim, elem(dtype));
+    if (meet(qs, os)) return fail(PHI_ERR_ARG, "%s: out overlaps q", who);
     const size_t need = phi_hip_paged_attention_workspace_bytes(tokens, q_heads, c.heads, c.dim, batch, max_q, max_kv, dtype);
     if (need > 0 && (!workspace || ws_bytes < need))
         return fail(PHI_ERR_WORKSPACE, "%s: needs %zu bytes of workspace, got %zu", who, need, workspace ? ws_bytes : (size_t)0);
     if (need > 0 && !aligned(workspace, 16)) return fail(PHI_ERR_ALIGN, "%s: the workspace must be 16-byte aligned", who);
-    if (need > 0 && (meet(workspace, (int64_t)need, q, qn) || meet(workspace, (int64_t)need, out, on)))
+    if (need > 0 && (meet({workspace, (int64_t)need}, qs) || meet({workspace, (int64_t)need}, os)))
         return fail(PHI_ERR_ARG, "%s: the workspace overlaps q or out", who);
     const phi_dev::PagedAttn p{q, out, block_table, q_start, kv_len, q_token_stride, q_head_stride, out_token_stride,
                                out_head_stride, table_stride, tokens, (int)q_heads, (int)(q_heads / c.heads), (int)batch,

@@ -1,0 +1,78 @@
+"""Which tensors' memory the decoder operators' C entries take as shared, on the CPU.
+Where nothing is shared a call passes these checks and ends at the launch, for want
+of a device."""
+import ctypes
+import itertools
+
+import pytest
+import torch
+
+import phi_qlinear as Q
+
+BASE = 0x7000000000  # of made-up buffers; never dereferenced
+
+
+def at(byte, buffer=0):
+    return ctypes.c_void_p(BASE + (buffer << 32) + byte)
+
+
+def norm(lib, *, x, ldx, q, ldq, rows=6, K=64, res=None, out=None, ldr=64, y=None, ldy=64, s=at(0, 9)):
+    rc = lib.phi_hip_rms_norm_quant(None, x, Q.BF16, ldx, res, out, Q.BF16, ldr, None, None, Q.F32, 1e-6, rows, K, y, Q.BF16, ldy,
+                                    q, ldq, s, 127.0, 0, 0)
+    return rc, Q.last_error()
+
+
+def overlaps(rc_text):
+    rc, text = rc_text
+    assert ("overlap" in text) == (rc == 1), text
+    return rc == 1
+
+
+no_device = pytest.mark.skipif(torch.cuda.is_available(), reason="addresses are made up")
+
+
+@no_device
+@pytest.mark.parametrize("x,res,y,shared", [(0, 64, 128, False), (128, 0, 64, False), (0, 63, 128, True), (0, 64, 127, True),
+                                            (0, 128, 64, False), (129, 0, 64, True), (64, 64, 0, False)])
+def test_norm_on_columns_of_one_buffer(lib, x, res, y, shared):
+    """x, residual (updated in place) and y are 64 columns each of a buffer of 192."""
+    r = at(2 * res)
+    got = overlaps(norm(lib, x=at(2 * x), ldx=192, res=r, out=None if x == res else r, ldr=192, y=at(2 * y), ldy=192, q=at(0, 1), ldq=64))
+    assert got == shared
+
+
+@no_device
+def test_norm_on_columns_of_different_types(lib):
+    """Codes in the last 64 bytes of rows whose first 128 are x; a byte earlier they meet."""
+    for first, shared in ((128, False), (127, True), (129, True)):
+        assert overlaps(norm(lib, x=at(0), ldx=96, q=at(first), ldq=192)) == shared
+
+
+def brute(a, b):
+    """Whether two sets of pieces (start, bytes, n1, s1, n2, s2) share a byte."""
+    covered = [{start + i * s1 + j * s2 + k for i in range(n1) for j in range(n2) for k in range(w)} for start, w, n1, s1, n2, s2 in (a, b)]
+    return bool(covered[0] & covered[1])
+
+
+@no_device
+def test_attention_beside_its_queries(lib):
+    """out and q as parts of one buffer, against the bytes themselves: nothing shared is
+    never missed, and the usual layouts that share nothing are taken."""
+    T, H, D = 3, 2, 16
+    cache = Q.KvCacheDesc(k=0x100000, v=0x200000, k_scale=0x300000, v_scale=0x400000, blocks=10, heads=2, page=16, dim=D, block_stride=512,
+                          head_stride=256, token_stride=16, s_block_stride=32, s_head_stride=16, s_token_stride=1)
+
+    def call(q, qt, qh, o, ot, oh):
+        rc = lib.phi_hip_paged_attention(None, at(2 * q), Q.BF16, qt, qh, T, H, ctypes.byref(cache), at(0, 1), 4, 4, at(0, 2), at(0, 3), 1, T,
+                                         64, 0.25, 1, 0, at(2 * o), ot, oh, None, 0)
+        return overlaps((rc, Q.last_error()))
+
+    for q, o, (qt, qh), (ot, oh) in itertools.product((0, 64), range(0, 200, 8), ((32, 16), (64, 16), (64, 32), (16, 48), (96, 32)),
+                                                      ((32, 16), (64, 16), (64, 32), (16, 48), (96, 32))):
+        shared = brute((q, D, T, qt, H, qh), (o, D, T, ot, H, oh))
+        assert call(q, qt, qh, o, ot, oh) or not shared
+    assert not call(0, 64, 16, 32, 64, 16)  # [T, q | out, H, D]
+    assert not call(0, 64, 32, 16, 64, 32)  # [T, H, q | out, D]
+    assert not call(0, 32, 16, 96, 32, 16)  # one after the other
+    assert not call(0, 16, 96, 48, 16, 96)  # [H, q | out, T, D]
+    assert call(0, 64, 16, 24, 64, 16) and call(0, 64, 32, 0, 64, 32)

@@ -37,3 +37,32 @@ def test_table_rows_that_overlap_are_refused(dev):
     one, want, bound = batch(dev, [(1, 40)])
     table = one.pop("block_table")
     assert near(Q.paged_attention(block_table=torch.as_strided(table, table.shape, (0, 1)), **one), want, bound)
+
+
+@pytest.mark.parametrize("lens", [[(1, 50), (1, 33)], [(140, 200), (3, 90)]])
+@pytest.mark.parametrize("within", ["tokens", "heads"])
+def test_attention_output_beside_its_queries(dev, lens, within):
+    """q and out as columns of one tensor that share no element."""
+    args, want, bound = batch(dev, lens, Hq=4)
+    q = args.pop("q")
+    T, Hq, D = q.shape
+    both = torch.full((T, 2 * Hq, D) if within == "tokens" else (T, Hq, 2 * D), 9.0, dtype=BF16, device=dev)
+    left, right = both.split(Hq, dim=1) if within == "tokens" else both.split(D, dim=2)
+    left.copy_(q)
+    # The plain bound is for exact keys: chunks round them to 11 bits, which 2^-9 of the weights' sum covers here.
+    got = Q.paged_attention(left, out=right, **args)
+    assert got.data_ptr() == right.data_ptr() and torch.equal(left, q)
+    assert torch.equal(right, Q.paged_attention(q, **args)) and bool(((got.cpu().double() - want).abs() <= bound + 2.0 ** -6).all())
+
+
+def test_norm_on_columns_of_one_tensor(dev):
+    """x, its residual stream (updated in place) and the normalised row side by side."""
+    rows, K = 37, 512
+    wide = torch.randn((rows, 3 * K), generator=torch.Generator().manual_seed(2)).to(dev)
+    x, h, y = wide.split(K, dim=1)
+    x0, h0 = x.clone(), h.clone()
+    new, y0 = torch.empty_like(h0), torch.empty_like(h0)
+    w = torch.linspace(0.5, 1.5, K, device=dev)
+    q0, s0 = Q.rms_norm_quant(x0, w, 1e-6, residual=h0, residual_out=new, y=y0)
+    q, s = Q.rms_norm_quant(x, w, 1e-6, residual=h, residual_out=h, y=y)
+    assert torch.equal(q, q0) and torch.equal(s, s0) and torch.equal(x, x0) and torch.equal(h, new) and torch.equal(y, y0)
