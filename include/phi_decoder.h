@@ -92,7 +92,8 @@ phi_status phi_hip_kv_cache_write(phi_stream_t stream, const phi_kv_cache* cache
 
 /* The values of `tokens` slots, k, v [tokens, heads, dim] of dtype (PHI_F32:
  * code * scale; PHI_BF16: that, rounded), strides as for the write; zeros for
- * a slot that is negative or past the cache. */
+ * a slot that is negative or past the cache.  k and v share no memory with each
+ * other or the cache. */
 phi_status phi_hip_kv_cache_read(phi_stream_t stream, const phi_kv_cache* cache, const int64_t* slots, int64_t tokens,
                                  void* k, int64_t k_token_stride, int64_t k_head_stride, void* v,
                                  int64_t v_token_stride, int64_t v_head_stride, int dtype);

@@ -52,6 +52,7 @@ constexpr int64_t kMaxK = 32768;      // columns of a norm's row (held on chip)
 constexpr int64_t kMaxPage = 1 << 20;
 constexpr int64_t kMaxPitch = (int64_t)1 << 29;    // elements: 2^31 rows of it stay within 63 bits
 constexpr int64_t kMaxStride = (int64_t)1 << 40;   // of a cache's blocks, heads and tokens
+constexpr int64_t kMaxSpan = (int64_t)1 << 56;     // more than any memory
 
 phi_status check_cache(const char* who, const phi_kv_cache* c, phi_dev::KvCache* out) {
     if (!c || !c->k || !c->v || !c->k_scale || !c->v_scale) return fail(PHI_ERR_ARG, "%s: null cache", who);
@@ -167,6 +168,15 @@ phi_status phi_hip_kv_cache_read(phi_stream_t stream, const phi_kv_cache* cache,
     if (tokens == 0) return ok();
     st = check_kv_tokens(who, c, k, k_token_stride, k_head_stride, v, v_token_stride, v_head_stride, dtype, slots, tokens);
     if (st != PHI_OK) return st;
+    const Pieces to[] = {vectors_of(k, tokens, k_token_stride, c.heads, k_head_stride, c.dim, elem(dtype)),
+                         vectors_of(v, tokens, v_token_stride, c.heads, v_head_stride, c.dim, elem(dtype))};
+    if (meet(to[0], to[1])) return fail(PHI_ERR_ARG, "%s: k overlaps v", who);
+    auto span = [](int64_t n, int64_t stride) { return n > 1 && stride > kMaxSpan / (n - 1) ? kMaxSpan : (n - 1) * stride; };
+    const int64_t codes = span(c.blocks, c.block_stride) + span(c.heads, c.head_stride) + span(c.page, c.token_stride) + c.dim;
+    const int64_t scales = (span(c.blocks, c.s_block_stride) + span(c.heads, c.s_head_stride) + span(c.page, c.s_token_stride) + 1) * 4;
+    for (const Pieces& x : to)
+        if (meet(x, {c.k, codes}) || meet(x, {c.v, codes}) || meet(x, {c.ks, scales}) || meet(x, {c.vs, scales}))
+            return fail(PHI_ERR_ARG, "%s: k or v overlaps the cache", who);
     const phi_dev::KvTokens t{k, v, k_token_stride, k_head_stride, v_token_stride, v_head_stride, slots, tokens, dtype == PHI_BF16};
     return check_hip(phi_dev::launch_kv_cache_read((hipStream_t)stream, c, t), who);
 }

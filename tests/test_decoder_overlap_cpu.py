@@ -76,3 +76,38 @@ def test_attention_beside_its_queries(lib):
     assert not call(0, 32, 16, 96, 32, 16)  # one after the other
     assert not call(0, 16, 96, 48, 16, 96)  # [H, q | out, T, D]
     assert call(0, 64, 16, 24, 64, 16) and call(0, 64, 32, 0, 64, 32)
+
+
+def read_into(lib, k, v, kt=32, vt=32, kh=16, vh=16, cache=None):
+    """kv_cache_read of 2 heads of 16 into bf16 k and v at these element offsets of a
+    buffer; the cache's arrays are 4 MiB apart in another."""
+    d = dict(k=BASE + (5 << 32), v=BASE + (5 << 32) + (4 << 20), k_scale=BASE + (5 << 32) + (8 << 20), v_scale=BASE + (5 << 32) + (12 << 20),
+             blocks=10, heads=2, page=16, dim=16, block_stride=512, head_stride=256, token_stride=16, s_block_stride=32, s_head_stride=16,
+             s_token_stride=1)
+    d.update(cache or {})
+    to = lambda x: x if isinstance(x, ctypes.c_void_p) else at(2 * x)  # noqa: E731
+    rc = lib.phi_hip_kv_cache_read(None, ctypes.byref(Q.KvCacheDesc(**d)), at(0, 1), 3, to(k), kt, kh, to(v), vt, vh, Q.BF16)
+    return overlaps((rc, Q.last_error()))
+
+
+@no_device
+def test_read_into_overlapping_outputs(lib):
+    for k, v in itertools.product((0, 32), range(0, 200, 8)):
+        for (kt, kh), (vt, vh) in itertools.product(((32, 16), (64, 16), (16, 48)), repeat=2):
+            shared = brute((k, 16, 3, kt, 2, kh), (v, 16, 3, vt, 2, vh))
+            assert read_into(lib, k, v, kt, vt, kh, vh) or not shared
+    assert read_into(lib, 0, 0) and read_into(lib, 0, 16)
+    assert not read_into(lib, 0, 96)  # one after the other
+    assert not read_into(lib, 0, 32, kt=64, vt=64)  # columns of one tensor
+    assert not read_into(lib, 0, 16, kt=64, vt=64, kh=32, vh=32)
+
+
+@no_device
+@pytest.mark.parametrize("array,size", [("k", 5120), ("v", 5120), ("k_scale", 1280), ("v_scale", 1280)])
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_read_into_the_cache(lib, array, size, which):
+    """An output that reaches into one of the cache's arrays, at either end of it; 192 bytes."""
+    start = 6 << 32
+    for byte, shared in ((0, True), (-192, False), (-176, True), (size, False), (size - 16, True)):
+        to = {"k": 0, "v": 1024, which: ctypes.c_void_p(BASE + start + byte)}
+        assert read_into(lib, to["k"], to["v"], cache={array: BASE + start}) == shared
