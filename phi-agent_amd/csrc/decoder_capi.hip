@@ -83,6 +83,12 @@ phi_status check_vectors(const char* who, const char* name, const void* x, int d
     return PHI_OK;
 }
 
+// Outputs: one place for two vectors is no result of either.
+phi_status check_apart(const char* who, const char* name, int64_t tokens, int64_t token_stride, int64_t heads, int64_t head_stride, int64_t dim) {
+    if ((tokens > 1 && token_stride < dim) || (heads > 1 && head_stride < dim)) return fail(PHI_ERR_SHAPE, "%s: %s's vectors overlap", who, name);
+    return PHI_OK;
+}
+
 phi_status check_kv_tokens(const char* who, const phi_dev::KvCache& c, const void* k, int64_t kt, int64_t kh, const void* v,
                            int64_t vt, int64_t vh, int dtype, const int64_t* slots, int64_t tokens) {
     if (!is_float(dtype)) return fail(PHI_ERR_ARG, "%s: k and v must be f32 or bf16", who);
@@ -151,6 +157,10 @@ phi_status phi_hip_kv_cache_write(phi_stream_t stream, const phi_kv_cache* cache
     if (tokens < 0) return fail(PHI_ERR_SHAPE, "%s: negative size", who);
     if (tokens == 0) return ok();
     st = check_kv_tokens(who, c, k, k_token_stride, k_head_stride, v, v_token_stride, v_head_stride, dtype, slots, tokens);
+    if (st == PHI_OK) st = check_apart(who, "the cache", c.page, c.token_stride, c.heads, c.head_stride, c.dim);
+    if (st == PHI_OK) st = check_apart(who, "the cache", c.blocks, c.block_stride, 1, 0, c.dim);
+    if (st == PHI_OK) st = check_apart(who, "the cache", c.page, c.s_token_stride, c.heads, c.s_head_stride, 1);
+    if (st == PHI_OK) st = check_apart(who, "the cache", c.blocks, c.s_block_stride, 1, 0, 1);
     if (st != PHI_OK) return st;
     const phi_dev::KvTokens t{(void*)k, (void*)v, k_token_stride, k_head_stride, v_token_stride, v_head_stride, slots, tokens, dtype == PHI_BF16};
     return check_hip(phi_dev::launch_kv_cache_write((hipStream_t)stream, c, t), who);
@@ -167,6 +177,8 @@ phi_status phi_hip_kv_cache_read(phi_stream_t stream, const phi_kv_cache* cache,
     if (tokens < 0) return fail(PHI_ERR_SHAPE, "%s: negative size", who);
     if (tokens == 0) return ok();
     st = check_kv_tokens(who, c, k, k_token_stride, k_head_stride, v, v_token_stride, v_head_stride, dtype, slots, tokens);
+    if (st == PHI_OK) st = check_apart(who, "k", tokens, k_token_stride, c.heads, k_head_stride, c.dim);
+    if (st == PHI_OK) st = check_apart(who, "v", tokens, v_token_stride, c.heads, v_head_stride, c.dim);
     if (st != PHI_OK) return st;
     const Pieces to[] = {vectors_of(k, tokens, k_token_stride, c.heads, k_head_stride, c.dim, elem(dtype)),
                          vectors_of(v, tokens, v_token_stride, c.heads, v_head_stride, c.dim, elem(dtype))};
@@ -209,6 +221,7 @@ phi_status phi_hip_paged_attention(phi_stream_t stream, const void* q, int dtype
     if (!std::isfinite(scale)) return fail(PHI_ERR_ARG, "%s: scale must be finite", who);
     st = check_vectors(who, "q", q, dtype, q_token_stride, q_head_stride);
     if (st == PHI_OK) st = check_vectors(who, "out", out, dtype, out_token_stride, out_head_stride);
+    if (st == PHI_OK) st = check_apart(who, "out", tokens, out_token_stride, q_heads, out_head_stride, c.dim);
     if (st != PHI_OK) return st;
     if ((max_kv > 0 && !block_table) || !q_start || !kv_len) return fail(PHI_ERR_ARG, "%s: null pointer", who);
     if (!aligned(block_table, 4) || !aligned(q_start, 4) || !aligned(kv_len, 4)) return fail(PHI_ERR_ALIGN, "%s: block_table, q_start or kv_len is misaligned", who);

@@ -111,3 +111,39 @@ def test_read_into_the_cache(lib, array, size, which):
     for byte, shared in ((0, True), (-192, False), (-176, True), (size, False), (size - 16, True)):
         to = {"k": 0, "v": 1024, which: ctypes.c_void_p(BASE + start + byte)}
         assert read_into(lib, to["k"], to["v"], cache={array: BASE + start}) == shared
+
+
+@no_device
+@pytest.mark.parametrize("tokens,ot,oh,refused", [(3, 0, 16, True), (3, 32, 0, True), (3, 8, 48, True), (1, 0, 16, False), (3, 32, 16, False),
+                                                  (3, 16, 48, False)])
+def test_outputs_whose_vectors_overlap(lib, tokens, ot, oh, refused):
+    """Vectors of 16 at smaller strides are written over one another: refused, where there is more than one."""
+    def answer(rc):
+        assert ("'s vectors overlap" in Q.last_error()) == (rc == 2), Q.last_error()
+        return rc == 2
+
+    cache = Q.KvCacheDesc(k=0x100000, v=0x200000, k_scale=0x300000, v_scale=0x400000, blocks=10, heads=2, page=16, dim=16, block_stride=512,
+                          head_stride=256, token_stride=16, s_block_stride=32, s_head_stride=16, s_token_stride=1)
+    assert answer(lib.phi_hip_paged_attention(None, at(0, 4), Q.BF16, 0, 16, tokens, 2, ctypes.byref(cache), at(0, 1), 4, 4, at(0, 2), at(0, 3), 1,
+                                              tokens, 64, 0.25, 1, 0, at(0), ot, oh, None, 0)) == refused
+    for k, v in (((ot, oh), (32, 16)), ((32, 16), (ot, oh))):
+        assert answer(lib.phi_hip_kv_cache_read(None, ctypes.byref(cache), at(0, 1), tokens, at(0), *k, at(0, 4), *v, Q.BF16)) == refused
+    # Inputs may: one vector for all tokens or heads.
+    assert not answer(lib.phi_hip_kv_cache_write(None, ctypes.byref(cache), at(0), ot, oh, at(0, 4), ot, oh, Q.BF16, at(0, 1), tokens))
+
+
+@no_device
+@pytest.mark.parametrize("stride,value,refused", [("block_stride", 0, True), ("head_stride", 0, True), ("token_stride", 0, True),
+                                                  ("s_block_stride", 0, True), ("s_head_stride", 0, True), ("s_token_stride", 0, True),
+                                                  ("token_stride", 16, False)])
+def test_writing_to_a_cache_whose_vectors_overlap(lib, stride, value, refused):
+    """A cache that holds one vector for several places can be read, not written."""
+    d = dict(k=0x100000, v=0x200000, k_scale=0x300000, v_scale=0x400000, blocks=10, heads=2, page=16, dim=16, block_stride=512,
+             head_stride=256, token_stride=16, s_block_stride=32, s_head_stride=16, s_token_stride=1)
+    one = dict(block_stride="blocks", head_stride="heads", token_stride="page", s_block_stride="blocks", s_head_stride="heads", s_token_stride="page")
+    d[stride] = value
+    for n, want in ((d[one[stride]], refused), (1, False)):
+        cache = Q.KvCacheDesc(**{**d, one[stride]: n})
+        rc = lib.phi_hip_kv_cache_write(None, ctypes.byref(cache), at(0), 32, 16, at(0, 4), 32, 16, Q.BF16, at(0, 1), 3)
+        assert (rc == 2 and "cache's vectors overlap" in Q.last_error()) == want
+        assert lib.phi_hip_kv_cache_read(None, ctypes.byref(cache), at(0, 1), 3, at(0), 32, 16, at(0, 4), 32, 16, Q.BF16) != 2
