@@ -46,9 +46,9 @@ extern "C" {
  * Any K from 1 to 32768 without the rotation; any pitch of at least K; every
  * pointer aligned to its own type.  residual_out apart, no output may share
  * memory with an input.  A row with an infinity or a NaN in r, or one
- * whose squares sum past fp32, gets the scale NaN (codes 0), so that what the
- * linear makes of it is NaN too.  rows == 0
- * is a no-op.
+ * whose squares sum past fp32, gets y and the scale NaN (codes 0), so that what a
+ * linear makes of it is NaN too; the scale is NaN also where, with eps 0, the squares
+ * are all 0 in fp32.  rows == 0 is a no-op.
  */
 phi_status phi_hip_rms_norm_quant(phi_stream_t stream, const void* x, int x_dtype, int64_t ldx, const void* residual,
                                   void* residual_out, int res_dtype, int64_t ldr, const void* weight,

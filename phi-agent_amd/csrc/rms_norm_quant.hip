@@ -149,7 +149,8 @@ __global__ __launch_bounds__(1024) void rms_norm_quant_kernel(RmsNorm p) {
 #pragma unroll
         for (int r = 0; r < R; r++) store_row16<ROT>(p.residual_out, RES == RES_BF16, row * p.ldr, e0_of(r), K, v[r]);
     }
-    const float rstd = 1.0f / sqrtf(sum / (float)K + p.eps);
+    // Past fp32 (or not a number): no norm, so that y is none either.
+    const float rstd = __builtin_isfinite(sum) ? 1.0f / sqrtf(sum / (float)K + p.eps) : __builtin_nanf("");
     bool fine = __builtin_isfinite(sum) && __builtin_isfinite(rstd);
     uint32_t top = 0;
 #pragma unroll

@@ -66,3 +66,20 @@ def test_norm_on_columns_of_one_tensor(dev):
     q0, s0 = Q.rms_norm_quant(x0, w, 1e-6, residual=h0, residual_out=new, y=y0)
     q, s = Q.rms_norm_quant(x, w, 1e-6, residual=h, residual_out=h, y=y)
     assert torch.equal(q, q0) and torch.equal(s, s0) and torch.equal(x, x0) and torch.equal(h, new) and torch.equal(y, y0)
+
+
+# ------------------------------------------------------------------ rows without a norm
+@pytest.mark.parametrize("K,rotate", [(512, True), (4096, True), (1000, False), (20480, False)])
+@pytest.mark.parametrize("ydtype", [BF16, F32])
+def test_norm_rows_that_are_not_finite(dev, K, rotate, ydtype):
+    """Where a row's scale is NaN its normalised row is too, in every place: an
+    infinity or a NaN in it, or squares whose sum passes 32 bits."""
+    x = torch.randn((6, K), generator=torch.Generator().manual_seed(K))
+    x[1, 3], x[2, K - 1], x[4, K // 2] = torch.inf, torch.nan, -torch.inf
+    x[3] *= 1e20
+    y = torch.zeros((6, K), dtype=ydtype, device=dev)
+    shift = torch.ones(K, device=dev)
+    q, s = Q.rms_norm_quant(x.to(dev), None, 1e-6, shift=shift, rotate=rotate, y=y)
+    bad = torch.tensor([False, True, True, True, True, False])
+    assert torch.equal(s.cpu().isnan(), bad) and not q.cpu()[bad].any()
+    assert torch.equal(y.cpu().isnan(), bad[:, None].expand(6, K))
