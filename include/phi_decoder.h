@@ -84,7 +84,7 @@ typedef struct phi_kv_cache {
  * vector with an infinity or a NaN gets the scale NaN (codes 0).
  * slots [tokens] int64: block * page + place in the block; one that is
  * negative or past the cache skips its token.  Two tokens with one slot in one
- * call leave either's vector.
+ * call leave a mixture there, codes of either and the scale of either.
  */
 phi_status phi_hip_kv_cache_write(phi_stream_t stream, const phi_kv_cache* cache, const void* k, int64_t k_token_stride,
                                   int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride,

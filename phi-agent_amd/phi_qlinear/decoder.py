@@ -125,8 +125,9 @@ def _kv_tokens(who: str, cache: KvCache, k: torch.Tensor, v: torch.Tensor, slots
 
 def kv_cache_write(cache: KvCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, *, stream=None) -> None:
     """Quantise k, v [tokens, heads, dim] (f32/bf16, any token and head strides)
-    into the cache at slots [tokens] int64 (block * page + place; negative: the
-    token is skipped), one scale a token and head (phi_hip_kv_cache_write)."""
+    into the cache at slots [tokens] int64 (block * page + place, each once;
+    negative: the token is skipped), one scale a token and head
+    (phi_hip_kv_cache_write)."""
     n = slots.numel()
     kt, kh, vt, vh = _kv_tokens("kv_cache_write", cache, k, v, slots, (n, cache._heads, cache._dim))
     _check(load().phi_hip_kv_cache_write(_stream(stream), cache._desc, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, _dt(k),
