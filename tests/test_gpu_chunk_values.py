@@ -67,13 +67,16 @@ def oracle(c, *, scale, causal=True, window=0):
             p = torch.where(seen, torch.exp(logit - torch.where(seen, logit, -math.inf).max(1, keepdim=True)[0].clamp(min=-1e300)), 0.0)
             p = p / p.sum(1, keepdim=True).clamp(min=1e-300)
             e = 2.0 ** -11 * (qd.abs() @ kd.abs().T) + 2.0 ** -32 * (qd.abs().sum(1)[:, None] * k_top + qd.abs().max(1)[0][:, None] * kd.abs().sum(1))
-            # A weight is off by the factor of its own logit's error, their sum by the mean of these.
-            e = p * torch.expm1(torch.where(seen, abs(scale) * e + 5 * 2.0 ** -24 * 1.4427 * logit.abs(), 0.0) + 2.0 ** -22)
+            # A weight is off by the factor of its own logit's error, their sum by the mean of
+            # these; where that is past a half, every weight by the largest error twice.
+            e = torch.where(seen, abs(scale) * e + 5 * 2.0 ** -24 * 1.4427 * logit.abs(), 0.0) + 2.0 ** -22
+            twice, e = torch.expm1(2 * e.max(1)[0].clamp(max=100.0))[:, None], p * torch.expm1(e.clamp(max=100.0))
             weight, off = p @ vd.abs(), e.sum(1)[:, None]
+            soft = torch.where(off < 0.5, (e @ vd.abs() + off * weight) / (1 - off).clamp(min=0.5), twice * weight)
             least = 2.0 ** -29 * (p @ v_top) + 2.0 ** -39 * 256 * float(v_top.max()) * p.max(1)[0] * seen.sum(1)
             o = p @ vd
             out[s0:s0 + n, h] = o
-            bound[s0:s0 + n, h] = (e @ vd.abs() + off * weight) / (1 - off) + (3 * 2.0 ** -11 + 2.0 ** -20) * weight + least[:, None] + 2.0 ** -8 * o.abs()
+            bound[s0:s0 + n, h] = soft + (3 * 2.0 ** -11 + 2.0 ** -20) * weight + least[:, None] + 2.0 ** -8 * o.abs()
     return out, bound
 
 
@@ -261,3 +264,64 @@ def test_lone_sequence_shorter_than_its_bound(dev, n, kv):
         assert bool(((got[:n].double() - want).abs() <= bound).all()) and bool((got[n:] == 7).all())
         starts[1] = T
         graph.replay()  # the whole buffer between
+
+
+# ------------------------------------------------------------------ scales, strides, values that are not finite
+@pytest.mark.parametrize("scale", [-0.3, 0.0, -0.0, 2.5, 40.0, 1e-30])
+def test_scales(dev, scale):
+    check(dev, case([(60, 200), (50, 70)], Hq=6, H=2, D=64, seed=2), scale=scale)
+
+
+@pytest.mark.parametrize("lens", [[(140, 200)], [(150, 1500), (140, 150), (3, 2000)]])
+def test_queries_and_output_in_wider_tensors(dev, lens):
+    """Columns of wider tensors, q's and out's of different widths; what lies beside out stays."""
+    c = case(lens, Hq=4, H=2, D=64, seed=2)
+    T = c["starts"][-1]
+    wide = torch.randn((T, 9, 64), generator=torch.Generator().manual_seed(1)).to(BF16)
+    wide[:, 3:7] = c["q"]
+    c["q"] = wide[:, 3:7]
+    big = torch.full((T, 7, 72), 3.0, dtype=BF16, device=dev)
+    check(dev, c, out=big[:, 1:5, :64])
+    assert bool((big[:, 0] == 3).all()) and bool((big[:, 5:] == 3).all()) and bool((big[..., 64:] == 3).all())
+
+
+@pytest.mark.parametrize("page", [16, 24])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_query_rows_that_are_not_finite(dev, page, bad):
+    """Such a row is NaN, and no other."""
+    c = case([(150, 420)], Hq=2, page=page, seed=6)
+    c["q"][7, 1, 3] = c["q"][149, 0, 127] = bad
+    got = run(dev, c, scale=0.1)
+    want = torch.zeros((150, 2), dtype=torch.bool)
+    want[7, 1] = want[149, 0] = True
+    assert torch.equal(got.isnan(), want[:, :, None].expand_as(got))
+
+
+@pytest.mark.parametrize("page", [16, 24])
+@pytest.mark.parametrize("name", ["ks", "vs"])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("window", [0, 40])
+def test_cache_scales_that_are_not_finite(dev, page, name, bad, window):
+    """The rows that see such a token are NaN, and only they."""
+    n, kv, t = 200, 330, 201
+    c = case([(n, kv)], page=page, seed=6)
+    c[name][place(c, 0, t)] = bad
+    got = run(dev, c, scale=0.1, window=window)
+    pos = kv - n + torch.arange(n)
+    want = (pos >= t) & ((pos - window < t) if window else True)
+    assert torch.equal(got.isnan(), want[:, None, None].expand_as(got))
+
+
+@pytest.mark.parametrize("D,page", [(64, 16), (128, 24), (256, 16)])
+def test_peaks_and_wide_ranges(dev, D, page):
+    """One token far above the rest (a sink), logits of thousands, v scales 30 powers of ten apart."""
+    c = case([(200, 700)], D=D, page=page, seed=16)
+    c["ks"][place(c, 0, 0)] = 0.25
+    check(dev, c)
+    check(dev, c, scale=40.0)
+    for t in range(0, 700, 5):
+        c["vs"][place(c, 0, t)] *= 10.0 ** -(t % 31)
+    check(dev, c)
+    c["vs"] *= 1e30
+    check(dev, c)
+    check(dev, c, causal=False)
