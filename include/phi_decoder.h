@@ -64,7 +64,8 @@ phi_status phi_hip_rms_norm_quant(phi_stream_t stream, const void* x, int x_dtyp
  *   scales  k_scale + b * s_block_stride + h * s_head_stride + t * s_token_stride  (floats)
  * so both [blocks, heads, page, dim] and [blocks, page, heads, dim] fit.  dim:
  * a multiple of 16 from 16 to 256; any page from 1 to 2^20; code strides multiples of
- * 16, k and v 16-byte aligned.  What was never written may hold anything.
+ * 16, k and v 16-byte aligned.  What was never written may hold anything; the scale
+ * of a token that is seen is finite, or NaN, which makes NaN of what sees it.
  */
 typedef struct phi_kv_cache {
     int8_t* k;
@@ -129,13 +130,15 @@ phi_status phi_hip_kv_cache_read(phi_stream_t stream, const phi_kv_cache* cache,
  * held as integers of 16 bits (PHI_BF16) or 24 bits (PHI_F32) relative to the
  * row's largest |q|, k and v as their codes, exactly, and p enters p.v with 16
  * or 24 bits.  PHI_BF16 sequences of more than 128 rows (new tokens x query heads
- * a key/value head; a batch of one: where max_q allows as many) have q exactly (elements below 2^-21 of the row's largest
- * apart), k's elements rounded to 11 bits or an error of 2^-32 of the largest scale
- * of k of 16 tokens, v's scales and v's elements to 11 bits each or an error of 2^-29
- * of the largest scale of v of 16 tokens (vectors of zeros apart), and p's to 11
- * bits or an error of 2^-39 of the row's largest p, times the ratio of the largest
- * scale of v to that of the 16 tokens.  The largest are those of the tokens that some
- * row of a block of 256 (dim above 128: 128) sees.
+ * a key/value head; a batch of one: where max_q allows as many) have q exactly
+ * (elements below 2^-21 of the row's largest apart), k's elements rounded to 11 bits or
+ * an error of 2^-32 of the largest scale of k of 16 tokens, v's scales and v's elements
+ * to 11 bits each or an error of 2^-29 of the largest scale of v of 16 tokens (vectors
+ * of zeros apart), and p's to 11 bits or an error of 2^-39 of the row's largest p,
+ * times the ratio of the largest scale of v to that of the 16 tokens.  The largest are
+ * those of the tokens that some row of a block of 256 (dim above 128: 128) sees.
+ * Sums of p v are fp32 and divided last, with p up to 2^8, so v beyond 2^119 over
+ * the number of tokens may pass them.
  * The order of sums, and so a result's last bits, depends on the sizes, the lengths
  * and max_q, max_kv and batch; the same call gives the same bits.
  */
