@@ -325,3 +325,18 @@ def test_peaks_and_wide_ranges(dev, D, page):
     c["vs"] *= 1e30
     check(dev, c)
     check(dev, c, causal=False)
+
+
+@pytest.mark.parametrize("bits", [8, 16, 22])
+@pytest.mark.parametrize("at", [256, 333])
+def test_small_values_before_large_ones(dev, bits, at):
+    """Rows that see tokens of small v scales only, beside later tokens of large ones."""
+    c = case([(400, 500)], seed=bits)
+    for t in range(at):
+        c["vs"][place(c, 0, t)] *= 2.0 ** -bits
+    got = check(dev, c)
+    # Against the same batch without the later tokens, whose units are the small ones.
+    n = at - 100
+    d = dict(c, q=c["q"][:n], starts=[0, n], kv_len=[at])
+    alone, (want, bound) = run(dev, d, scale=128 ** -0.5), oracle(c, scale=128 ** -0.5)
+    assert bool(((alone.double() - want[:n]).abs() <= bound[:n]).all() and ((got[:n].double() - alone.double()).abs() <= 2 * bound[:n]).all())
