@@ -135,8 +135,9 @@ phi_status phi_hip_kv_cache_read(phi_stream_t stream, const phi_kv_cache* cache,
  * an error of 2^-32 of the largest scale of k of 16 tokens, v's scales and v's elements
  * to 11 bits each or an error of 2^-29 of the largest scale of v of 16 tokens (vectors
  * of zeros apart), and p's to 11 bits or an error of 2^-39 of the row's largest p,
- * times the ratio of the largest scale of v to that of the 16 tokens.  The largest are
- * those of the tokens that some row of a block of 256 (dim above 128: 128) sees.
+ * times the ratio of the largest scale of v, of all 16 tokens that the row sees some of,
+ * to that of p's own 16.  16 tokens' largest is that of those which some row of a
+ * block of 256 (dim above 128: 128) sees.
  * Sums of p v are fp32 and divided last, with p up to 2^8, so v beyond 2^119 over
  * the number of tokens may pass them.
  * The order of sums, and so a result's last bits, depends on the sizes, the lengths

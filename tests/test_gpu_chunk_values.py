@@ -9,7 +9,8 @@ value stands how far the kernel's arithmetic may be from it:
       is 2^5 to 2^6: 2^-30 of that scale from v's step and 2^-32 from a scale's own
   q   exact, but half a subnormal's step (2^-25 where the row's largest is 2^7 or more)
   p   fp16 in 2^14 at the row's largest: 2^-11 of it, or 2^-25 / 2^14 = 2^-39 of the
-      largest p, for a v of up to 128 times the largest scale that its blocks see
+      largest p, for a v of up to 128 times the largest scale of the 16 tokens that it
+      sees some of
   sums in fp32 (2^-20 of the sum of magnitudes), the logit's own roundings (five, in
   units of 2^-24) and exp2's, 2^-22; the output's bf16."""
 import math
@@ -32,6 +33,13 @@ def groups_top(scales, codes, live):
     pad = -len(s) % 16
     top = torch.cat([s, torch.zeros(pad, dtype=s.dtype)]).view(-1, 16).max(dim=1)[0]
     return top.repeat_interleave(16)[:len(s)]
+
+
+def rows_top(seen, top):
+    """Of [rows, tokens] seen and groups_top: the largest of the 16 tokens that a row sees some of."""
+    pad = -len(top) % 16
+    seen = torch.nn.functional.pad(seen, (0, pad)).view(len(seen), -1, 16).any(2)
+    return torch.where(seen, torch.nn.functional.pad(top, (0, pad)).view(-1, 16).max(1)[0], 0.0).max(1)[0]
 
 
 def oracle(c, *, scale, causal=True, window=0):
@@ -73,10 +81,10 @@ def oracle(c, *, scale, causal=True, window=0):
             twice, e = torch.expm1(2 * e.max(1)[0].clamp(max=100.0))[:, None], p * torch.expm1(e.clamp(max=100.0))
             weight, off = p @ vd.abs(), e.sum(1)[:, None]
             soft = torch.where(off < 0.5, (e @ vd.abs() + off * weight) / (1 - off).clamp(min=0.5), twice * weight)
-            least = 2.0 ** -29 * (p @ v_top) + 2.0 ** -39 * 256 * float(v_top.max()) * p.max(1)[0] * seen.sum(1)
+            least = 2.0 ** -29 * (p @ v_top)[:, None] + 2.0 ** -39 * 256 * (rows_top(seen, v_top) * p.max(1)[0] * seen.sum(1))[:, None]
             o = p @ vd
             out[s0:s0 + n, h] = o
-            bound[s0:s0 + n, h] = soft + (3 * 2.0 ** -11 + 2.0 ** -20) * weight + least[:, None] + 2.0 ** -8 * o.abs()
+            bound[s0:s0 + n, h] = soft + (3 * 2.0 ** -11 + 2.0 ** -20) * weight + least + 2.0 ** -8 * o.abs()
     return out, bound
 
 
@@ -327,16 +335,25 @@ def test_peaks_and_wide_ranges(dev, D, page):
     check(dev, c, causal=False)
 
 
-@pytest.mark.parametrize("bits", [8, 16, 22])
-@pytest.mark.parametrize("at", [256, 333])
-def test_small_values_before_large_ones(dev, bits, at):
+@pytest.mark.parametrize("at,bits", [(333, 8), (333, 16), (333, 22), (256, 22), (256, 30), (256, 40), (256, 90)])
+def test_small_values_before_large_ones(dev, at, bits):
     """Rows that see tokens of small v scales only, beside later tokens of large ones."""
     c = case([(400, 500)], seed=bits)
     for t in range(at):
         c["vs"][place(c, 0, t)] *= 2.0 ** -bits
     got = check(dev, c)
-    # Against the same batch without the later tokens, whose units are the small ones.
+    # Against the same batch without the later tokens.
     n = at - 100
-    d = dict(c, q=c["q"][:n], starts=[0, n], kv_len=[at])
-    alone, (want, bound) = run(dev, d, scale=128 ** -0.5), oracle(c, scale=128 ** -0.5)
-    assert bool(((alone.double() - want[:n]).abs() <= bound[:n]).all() and ((got[:n].double() - alone.double()).abs() <= 2 * bound[:n]).all())
+    alone = run(dev, dict(c, q=c["q"][:n], starts=[0, n], kv_len=[at]), scale=128 ** -0.5)
+    want, bound = (x[:n] for x in oracle(c, scale=128 ** -0.5))
+    assert bool(((alone.double() - want).abs() <= bound).all() and ((got[:n].double() - alone.double()).abs() <= 2 * bound).all())
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_large_values_that_windows_leave_behind(dev, D):
+    """Windows of rows in one block that see large values, some, and none."""
+    c = case([(300, 900)], D=D, seed=D)
+    for t in range(900):
+        c["vs"][place(c, 0, t)] *= 2.0 ** -(40 * (t // 16 % 20 != 0))
+    check(dev, c, window=70)
+    check(dev, c, window=200)
