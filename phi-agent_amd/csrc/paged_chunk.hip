@@ -27,9 +27,9 @@
 //     group has its products, the other has its softmax and stages the next
 //     tiles, waves 0-3 V's and 4-7 K's.
 // 4096 tokens over 16384, 32 heads over 8 of 128: 1.08 ms, 890 TFLOP/s of the 1458 that
-// a product of 8192^3 in fp16 reaches; the matrix cores are busy 42 % of the time.  A
+// a product of 8192^3 in fp16 reaches; the matrix cores are busy 43 % of the time.  A
 // tile takes 5400 clocks, of which the matrix cores need 2048 and the vector unit some
-// 3150 (two waves' softmax and staging), and each group's turn waits for the other's.
+// 3300 (two waves' softmax and staging), and each group's turn waits for the other's.
 // A block costs 13 us beside its tiles: the batch's lookup and Q 4, the first tiles 4,
 // O's stores 3 to 8.
 #include <type_traits>

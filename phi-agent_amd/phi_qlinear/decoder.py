@@ -137,7 +137,7 @@ def kv_cache_write(cache: KvCache, k: torch.Tensor, v: torch.Tensor, slots: torc
 def kv_cache_read(cache: KvCache, slots: torch.Tensor, *, out_dtype=torch.bfloat16, k: torch.Tensor | None = None,
                   v: torch.Tensor | None = None, stream=None):
     """The values at slots [tokens] int64 as k, v [tokens, heads, dim] (zeros for
-    a negative slot; phi_hip_kv_cache_read)."""
+    a negative slot; phi_hip_kv_cache_read).  k and v share no memory."""
     n = slots.numel()
     shape = (n, cache._heads, cache._dim)
     if k is None:
@@ -167,7 +167,8 @@ def paged_attention(q: torch.Tensor, cache: KvCache, block_table: torch.Tensor, 
     lie in blocks block_table[b] (int32, as q_start [batch + 1] and kv_len
     [batch]); max_q and max_kv bound the new tokens and the length of any
     sequence.  scale: dim ** -0.5 if not given.  A row that sees no token gives
-    zeros."""
+    zeros; rows of no sequence are left as they are.  out may be columns of the
+    tensor that q is in."""
     _require_device(q, block_table, q_start, kv_len, out, workspace)
     shape = q.shape
     T, Hq, D = shape
