@@ -1,0 +1,81 @@
+/*
+ * phi_serving.h -- what a server of many requests runs beside phi_decoder.h's
+ * operators, in the manner of phi_qlinear.h: every entry point enqueues work on
+ * the caller's HIP stream and returns a phi_status (message:
+ * phi_hip_last_error()), nothing synchronises, nothing allocates device memory.
+ *
+ *   phi_hip_rotary               rotary positions of [tokens, heads, dim] vectors
+ *   phi_hip_rotary_cache_write   the same of a projection's q and k, with k and v
+ *                                quantised into the paged cache
+ *   phi_hip_kv_cache_copy        pages of a cache copied (forked sequences, compaction)
+ *
+ * The reference rotates pairs of half a head's distance on fp32 tensors
+ * (rope_half, core/kernels/attn.cpp:99-); it has no cache.
+ */
+#ifndef PHI_SERVING_H
+#define PHI_SERVING_H
+
+#include "phi_decoder.h"
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+/*
+ * Rotary positions: of each vector's first `rot` elements, pair j (elements j and
+ * j + rot/2, or 2j and 2j + 1 if interleaved) is turned by the angle
+ * t = positions[token] * freq[j]:
+ *   a' = scale (a cos t - b sin t),   b' = scale (b cos t + a sin t)
+ * Elements from rot on are copied.
+ *
+ *   x, out     [tokens, heads, dim] of dtype (PHI_F32 or PHI_BF16), token and head
+ *              strides in elements; any strides of x, vectors of out apart.  out may
+ *              be x itself (the same strides), or must not share memory with it.
+ *   positions  [tokens] int64, any value: negative ones turn back
+ *   freq       [rot / 2] fp64, finite, radians a position: contexts stretched by
+ *              any rule are other frequencies (and a scale)
+ *   dim        from 1 to 1024; rot even, from 2 to dim
+ * The angle is kept as a 64-bit fraction of a turn, position * freq modulo 1 to
+ * 2^-53 of the angle (as fp64 has it) and 2^-64 a position; its cosine and sine are
+ * fp32 to 2^-22, products and sums fp32, rounded once.
+ */
+phi_status phi_hip_rotary(phi_stream_t stream, const void* x, int dtype, int64_t x_token_stride, int64_t x_head_stride,
+                          int64_t tokens, int64_t heads, int64_t dim, const int64_t* positions, const double* freq,
+                          int64_t rot, int interleaved, float scale, void* out, int64_t out_token_stride,
+                          int64_t out_head_stride);
+
+/*
+ * A projection's output on its way to attention, in one launch: q [tokens, q_heads,
+ * cache dim] rotated to q_out (which may be q itself), k [tokens, cache heads, dim]
+ * rotated and v as it is quantised into the cache at slots [tokens], as
+ * phi_hip_kv_cache_write does (k from its fp32 values, not rounded to dtype
+ * between).  All of dtype; strides in elements, vectors 16-byte aligned.  q_heads 0:
+ * no q.  A token whose slot is skipped has its q rotated all the same.  q_out shares
+ * no memory with k, v or the cache.
+ */
+phi_status phi_hip_rotary_cache_write(phi_stream_t stream, const phi_kv_cache* cache, const void* q,
+                                      int64_t q_token_stride, int64_t q_head_stride, int64_t q_heads, void* q_out,
+                                      int64_t q_out_token_stride, int64_t q_out_head_stride, const void* k,
+                                      int64_t k_token_stride, int64_t k_head_stride, const void* v,
+                                      int64_t v_token_stride, int64_t v_head_stride, int dtype,
+                                      const int64_t* positions, const double* freq, int64_t rot, int interleaved,
+                                      float scale, const int64_t* slots, int64_t tokens);
+
+/*
+ * Copy blocks of one cache (codes and scales of k and v, all heads) to blocks of
+ * another, or of the same: for i < n the first tokens[i] tokens (NULL: all; fewer
+ * than 1: none; more than a page: all) of block from_blocks[i] to block to_blocks[i].  A pair with a
+ * block that its cache does not have is skipped.  The caches agree in heads, page and
+ * dim; their strides may differ.  Blocks that are written are written once and not
+ * read in the same call: else they are left with a mixture.  A page of at most 2^26
+ * tokens x heads.
+ */
+phi_status phi_hip_kv_cache_copy(phi_stream_t stream, const phi_kv_cache* from, const phi_kv_cache* to,
+                                 const int32_t* from_blocks, const int32_t* to_blocks, const int32_t* tokens,
+                                 int64_t n);
+
+#ifdef __cplusplus
+}
+#endif
+
+#endif /* PHI_SERVING_H */

@@ -1,107 +1,8 @@
 // C ABI of the decoder layer's operators (include/phi_decoder.h): argument
 // validation and dispatch, under the error contract of capi.hip.
-#include <cmath>
+#include "decoder_checks.hpp"
 
-#include "../../include/phi_decoder.h"
-#include "capi.hpp"
-#include "decoder.hpp"
-
-using phi_capi::check_hip;
-using phi_capi::fail;
-using phi_capi::ok;
-
-namespace {
-
-bool aligned(const void* p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
-
-bool is_float(int dtype) { return dtype == PHI_F32 || dtype == PHI_BF16; }
-
-int64_t elem(int dtype) { return dtype == PHI_BF16 ? 2 : 4; }
-
-// n1 x n2 pieces of `bytes` bytes at strides of s1 and s2 bytes (null p: none).
-struct Pieces {
-    const void* p;
-    int64_t bytes, n1 = 1, s1 = 0, n2 = 1, s2 = 0;
-    int64_t extent() const { return (n1 - 1) * s1 + (n2 - 1) * s2 + bytes; }
-    // All pieces lie in the first `width` bytes of periods of P from p on.
-    int64_t width(int64_t P) const { return (s1 % P ? (n1 - 1) * s1 : 0) + (s2 % P ? (n2 - 1) * s2 : 0) + bytes; }
-};
-
-// Whether a piece of a may meet one of b: not where the memory they span is apart, nor
-// where a common period holds them side by side (columns of one buffer).
-bool meet(const Pieces& a, const Pieces& b) {
-    const uintptr_t pa = (uintptr_t)a.p, pb = (uintptr_t)b.p;
-    if (!pa || !pb || pa >= pb + (uintptr_t)b.extent() || pb >= pa + (uintptr_t)a.extent()) return false;
-    for (const int64_t P : {a.s1, a.s2, b.s1, b.s2}) {
-        if (P <= 0) continue;
-        const int64_t wa = a.width(P), wb = b.width(P), d = (int64_t)(pb % (uintptr_t)P) - (int64_t)(pa % (uintptr_t)P), at = d < 0 ? d + P : d;
-        if (wa <= at && at + wb <= P) return false;
-    }
-    return true;
-}
-
-// rows of K elements, and [tokens, heads, dim] vectors.
-Pieces rows_of(const void* p, int64_t rows, int64_t K, int64_t pitch, int64_t elem) { return {p, K * elem, rows, pitch * elem}; }
-Pieces vectors_of(const void* p, int64_t tokens, int64_t token_stride, int64_t heads, int64_t head_stride, int64_t dim, int64_t elem) {
-    return {p, dim * elem, tokens, token_stride * elem, heads, head_stride * elem};
-}
-
-constexpr int64_t kMaxKv = 1 << 30;  // a sequence's tokens: positions and steps past them stay 32-bit
-constexpr int64_t kMaxRows = 1 << 30;  // a sequence's new tokens x query heads a key/value head, the same
-constexpr int64_t kMaxK = 32768;      // columns of a norm's row (held on chip)
-constexpr int64_t kMaxPage = 1 << 20;
-constexpr int64_t kMaxPitch = (int64_t)1 << 29;    // elements: 2^31 rows of it stay within 63 bits
-constexpr int64_t kMaxStride = (int64_t)1 << 40;   // of a cache's blocks, heads and tokens
-constexpr int64_t kMaxSpan = (int64_t)1 << 56;     // more than any memory
-
-phi_status check_cache(const char* who, const phi_kv_cache* c, phi_dev::KvCache* out) {
-    if (!c || !c->k || !c->v || !c->k_scale || !c->v_scale) return fail(PHI_ERR_ARG, "%s: null cache", who);
-    if (c->blocks <= 0 || c->heads <= 0 || c->page <= 0) return fail(PHI_ERR_SHAPE, "%s: empty cache (blocks=%lld heads=%lld page=%lld)", who, (long long)c->blocks, (long long)c->heads, (long long)c->page);
-    if (c->dim < 16 || c->dim > 256 || c->dim % 16 != 0) return fail(PHI_ERR_SHAPE, "%s: dim=%lld is not a multiple of 16 from 16 to 256", who, (long long)c->dim);
-    if (c->blocks > INT32_MAX || c->heads > 65535 || c->page > kMaxPage) return fail(PHI_ERR_SHAPE, "%s: cache dimension too large", who);
-    const int64_t st[] = {c->block_stride, c->head_stride, c->token_stride, c->s_block_stride, c->s_head_stride, c->s_token_stride};
-    for (int64_t s : st)
-        if (s < 0 || s > kMaxStride) return fail(PHI_ERR_SHAPE, "%s: bad cache stride %lld", who, (long long)s);
-    if (!aligned(c->k, 16) || !aligned(c->v, 16) || c->block_stride % 16 != 0 || c->head_stride % 16 != 0 || c->token_stride % 16 != 0)
-        return fail(PHI_ERR_ALIGN, "%s: the cache's codes must be 16-byte aligned at strides of multiples of 16", who);
-    if (!aligned(c->k_scale, 4) || !aligned(c->v_scale, 4)) return fail(PHI_ERR_ALIGN, "%s: cache scales are misaligned", who);
-    int lg = 0;
-    while ((int64_t)1 << lg < c->page) lg++;
-    *out = phi_dev::KvCache{c->k, c->v, c->k_scale, c->v_scale, c->block_stride, c->head_stride, c->token_stride,
-                            c->s_block_stride, c->s_head_stride, c->s_token_stride, c->blocks * c->page, (int)c->blocks,
-                            (int)c->heads, (int)c->page, (int)c->dim,
-                            (uint32_t)(((uint64_t)1 << (31 + lg)) / (uint64_t)c->page + 1), 31 + lg};
-    return PHI_OK;
-}
-
-phi_status check_vectors(const char* who, const char* name, const void* x, int dtype, int64_t token_stride, int64_t head_stride) {
-    if (!x) return fail(PHI_ERR_ARG, "%s: null %s", who, name);
-    if (token_stride < 0 || head_stride < 0 || token_stride > kMaxPitch || head_stride > kMaxPitch)
-        return fail(PHI_ERR_SHAPE, "%s: bad stride of %s", who, name);
-    if (!aligned(x, 16) || token_stride * elem(dtype) % 16 != 0 || head_stride * elem(dtype) % 16 != 0)
-        return fail(PHI_ERR_ALIGN, "%s: %s's vectors must be 16-byte aligned", who, name);
-    return PHI_OK;
-}
-
-// Outputs: one place for two vectors is no result of either.
-phi_status check_apart(const char* who, const char* name, int64_t tokens, int64_t token_stride, int64_t heads, int64_t head_stride, int64_t dim) {
-    if ((tokens > 1 && token_stride < dim) || (heads > 1 && head_stride < dim)) return fail(PHI_ERR_SHAPE, "%s: %s's vectors overlap", who, name);
-    return PHI_OK;
-}
-
-phi_status check_kv_tokens(const char* who, const phi_dev::KvCache& c, const void* k, int64_t kt, int64_t kh, const void* v,
-                           int64_t vt, int64_t vh, int dtype, const int64_t* slots, int64_t tokens) {
-    if (!is_float(dtype)) return fail(PHI_ERR_ARG, "%s: k and v must be f32 or bf16", who);
-    if (tokens > INT32_MAX) return fail(PHI_ERR_SHAPE, "%s: tokens exceeds 2^31", who);
-    phi_status st = check_vectors(who, "k", k, dtype, kt, kh);
-    if (st == PHI_OK) st = check_vectors(who, "v", v, dtype, vt, vh);
-    if (st != PHI_OK) return st;
-    if (!slots) return fail(PHI_ERR_ARG, "%s: null slots", who);
-    if (!aligned(slots, 8)) return fail(PHI_ERR_ALIGN, "%s: slots is misaligned", who);
-    return PHI_OK;
-}
-
-}  // namespace
+using namespace phi_capi;
 
 extern "C" {
 
@@ -157,10 +58,7 @@ phi_status phi_hip_kv_cache_write(phi_stream_t stream, const phi_kv_cache* cache
     if (tokens < 0) return fail(PHI_ERR_SHAPE, "%s: negative size", who);
     if (tokens == 0) return ok();
     st = check_kv_tokens(who, c, k, k_token_stride, k_head_stride, v, v_token_stride, v_head_stride, dtype, slots, tokens);
-    if (st == PHI_OK) st = check_apart(who, "the cache", c.page, c.token_stride, c.heads, c.head_stride, c.dim);
-    if (st == PHI_OK) st = check_apart(who, "the cache", c.blocks, c.block_stride, 1, 0, c.dim);
-    if (st == PHI_OK) st = check_apart(who, "the cache", c.page, c.s_token_stride, c.heads, c.s_head_stride, 1);
-    if (st == PHI_OK) st = check_apart(who, "the cache", c.blocks, c.s_block_stride, 1, 0, 1);
+    if (st == PHI_OK) st = check_cache_apart(who, c);
     if (st != PHI_OK) return st;
     const phi_dev::KvTokens t{(void*)k, (void*)v, k_token_stride, k_head_stride, v_token_stride, v_head_stride, slots, tokens, dtype == PHI_BF16};
     return check_hip(phi_dev::launch_kv_cache_write((hipStream_t)stream, c, t), who);
@@ -183,11 +81,8 @@ phi_status phi_hip_kv_cache_read(phi_stream_t stream, const phi_kv_cache* cache,
     const Pieces to[] = {vectors_of(k, tokens, k_token_stride, c.heads, k_head_stride, c.dim, elem(dtype)),
                          vectors_of(v, tokens, v_token_stride, c.heads, v_head_stride, c.dim, elem(dtype))};
     if (meet(to[0], to[1])) return fail(PHI_ERR_ARG, "%s: k overlaps v", who);
-    auto span = [](int64_t n, int64_t stride) { return n > 1 && stride > kMaxSpan / (n - 1) ? kMaxSpan : (n - 1) * stride; };
-    const int64_t codes = span(c.blocks, c.block_stride) + span(c.heads, c.head_stride) + span(c.page, c.token_stride) + c.dim;
-    const int64_t scales = (span(c.blocks, c.s_block_stride) + span(c.heads, c.s_head_stride) + span(c.page, c.s_token_stride) + 1) * 4;
     for (const Pieces& x : to)
-        if (meet(x, {c.k, codes}) || meet(x, {c.v, codes}) || meet(x, {c.ks, scales}) || meet(x, {c.vs, scales}))
+        if (meets_cache(x, c))
             return fail(PHI_ERR_ARG, "%s: k or v overlaps the cache", who);
     const phi_dev::KvTokens t{k, v, k_token_stride, k_head_stride, v_token_stride, v_head_stride, slots, tokens, dtype == PHI_BF16};
     return check_hip(phi_dev::launch_kv_cache_read((hipStream_t)stream, c, t), who);

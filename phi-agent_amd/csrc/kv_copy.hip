@@ -1,0 +1,92 @@
+// Blocks of the paged cache copied: forked sequences' last pages, compaction.
+//
+// Bound by memory.  A pair's codes of k, then of v, are pieces of 16 bytes in the order
+// in which they lie (tokens within heads, or heads within tokens), kPieces a thread, all
+// of a thread's loads before its stores; then both scales, a float each.
+#include "device_common.hpp"
+#include "serving.hpp"
+
+namespace phi_dev {
+
+namespace {
+
+constexpr int kPieces = 8;
+
+// n / d as (n * mul) >> shift for 0 <= n < 2^31.
+struct Div {
+    uint32_t d, mul;
+    int shift;
+};
+Div div_by(uint32_t d) {
+    int lg = 0;
+    while (1u << lg < d) lg++;
+    return {d, (uint32_t)(((uint64_t)1 << (31 + lg)) / d + 1), 31 + lg};
+}
+__device__ __forceinline__ uint32_t quotient(const Div& d, uint32_t n) { return (uint32_t)(((uint64_t)n * d.mul) >> d.shift); }
+
+}  // namespace
+
+// inner, outer: the smaller stride's and the larger's counts of a page's vectors;
+// token_inner: the inner are tokens.
+__global__ __launch_bounds__(256) void kv_copy_kernel(KvCopy p, Div vector, Div inner, bool token_inner, int code_parts, int scale_parts) {
+    const int per = 2 * code_parts + scale_parts;
+    const int64_t i = blockIdx.x / per;
+    const int part = blockIdx.x - (int)i * per;
+    const int from = p.from_blocks[i], to = p.to_blocks[i];
+    if (from < 0 || from >= p.from.blocks || to < 0 || to >= p.to.blocks) return;
+    const uint32_t take = (uint32_t)min(max(p.tokens ? p.tokens[i] : p.from.page, 0), p.from.page);
+    const uint32_t vectors = (uint32_t)p.from.heads * (uint32_t)p.from.page;
+    const bool scales = part >= 2 * code_parts;
+    const bool v = !scales && part >= code_parts;
+    const uint32_t first = (uint32_t)(scales ? part - 2 * code_parts : v ? part - code_parts : part) * (256 * kPieces) + threadIdx.x;
+    // Vector n's head and token.
+    auto place = [&](uint32_t n, uint32_t& head, uint32_t& token) {
+        const uint32_t o = quotient(inner, n), in = n - o * inner.d;
+        head = token_inner ? o : in, token = token_inner ? in : o;
+    };
+    if (scales) {
+        for (int j = 0; j < kPieces; j++) {
+            const uint32_t n = first + 256 * j;
+            uint32_t head, token;
+            if (n >= vectors) return;
+            place(n, head, token);
+            if (token >= take) continue;
+            const int64_t a = from * p.from.s_block_stride + head * p.from.s_head_stride + token * p.from.s_token_stride;
+            const int64_t b = to * p.to.s_block_stride + head * p.to.s_head_stride + token * p.to.s_token_stride;
+            p.to.ks[b] = p.from.ks[a];
+            p.to.vs[b] = p.from.vs[a];
+        }
+        return;
+    }
+    const int8_t* src = (v ? p.from.v : p.from.k) + from * p.from.block_stride;
+    int8_t* dst = (v ? p.to.v : p.to.k) + to * p.to.block_stride;
+    v4i x[kPieces];
+    int64_t at[kPieces];
+#pragma unroll
+    for (int j = 0; j < kPieces; j++) {
+        const uint32_t n = first + 256 * j, vec = quotient(vector, n);
+        uint32_t head, token;
+        place(vec, head, token);
+        const bool has = vec < vectors && token < take;
+        const uint32_t in = 16 * (n - vec * vector.d);
+        at[j] = has ? head * p.to.head_stride + token * p.to.token_stride + in : -1;
+        if (has) x[j] = *(const v4i*)(src + head * p.from.head_stride + token * p.from.token_stride + in);
+    }
+#pragma unroll
+    for (int j = 0; j < kPieces; j++)
+        if (at[j] >= 0) *(v4i*)(dst + at[j]) = x[j];
+}
+
+hipError_t launch_kv_cache_copy(hipStream_t stream, const KvCopy& p) {
+    const KvCache& c = p.from;
+    const bool token_inner = c.token_stride <= c.head_stride;
+    const int64_t vectors = (int64_t)c.heads * c.page, pieces = vectors * (c.dim / 16), each = 256 * kPieces;
+    const int code_parts = (int)((pieces + each - 1) / each), scale_parts = (int)((vectors + each - 1) / each);
+    const int64_t grid = p.n * (2 * (int64_t)code_parts + scale_parts);
+    if (grid > INT32_MAX) return hipErrorInvalidConfiguration;
+    hipLaunchKernelGGL(kv_copy_kernel, dim3((unsigned)grid), dim3(256), 0, stream, p, div_by(c.dim / 16),
+                       div_by(token_inner ? c.page : c.heads), token_inner, code_parts, scale_parts);
+    return hipGetLastError();
+}
+
+}  // namespace phi_dev

@@ -1,0 +1,284 @@
+// Rotary positions, alone or with the write of k and v into the paged int8 cache.
+//
+// Bound by memory: every vector is read and written once.  A team of lanes has a
+// vector, 8 pairs a lane; a wave's teams have consecutive tokens of one head, so that
+// a page's codes and scales are written together (kv_cache.hip); a block's waves have
+// neighbouring heads and go over the others with the same tokens, so that a pair's
+// cosine and sine are computed once for all of a block's heads.
+//
+// The angle position * freq is wanted modulo a turn, to fp32 at any position.  With
+// step = freq / 2 pi as a 64-bit fraction of a turn, position * step in 64-bit
+// integers drops whole turns by itself and is exact for the step as it is; its top 32
+// bits, taken about the nearest quarter turn, are an angle within pi/4, for which
+// Taylor's series to x^9 and x^10 are within 2^-29.
+#include "device_common.hpp"
+#include "serving.hpp"
+
+namespace phi_dev {
+
+namespace {
+
+// Cosine and sine of position * freq.
+__device__ __forceinline__ float2 turn_of(int64_t position, double freq) {
+    const double turns = freq * 0.15915494309189533577;
+    // To 2^-63 of a turn, within half a turn either way.
+    const uint64_t step = (uint64_t)(int64_t)((turns - rint(turns)) * 0x1p63) << 1;
+    const uint32_t at = (uint32_t)((step * (uint64_t)position) >> 32) + 0x20000000u;
+    const float x = (float)((int32_t)(at & 0x3fffffffu) - 0x20000000) * 1.4629180792671596e-9f;  // 2 pi / 2^32
+    const float y = x * x;
+    float s = fmaf(y, fmaf(y, fmaf(y, fmaf(y, 1.0f / 362880, -1.0f / 5040), 1.0f / 120), -1.0f / 6), 1.0f);
+    s *= x;
+    const float c = fmaf(y, fmaf(y, fmaf(y, fmaf(y, fmaf(y, -1.0f / 3628800, 1.0f / 40320), -1.0f / 720), 1.0f / 24), -0.5f), 1.0f);
+    const uint32_t quarter = at >> 30;
+    const float a = quarter & 1 ? s : c, b = quarter & 1 ? c : s;
+    return make_float2(quarter == 1 || quarter == 2 ? -a : a, quarter >= 2 ? -b : b);
+}
+
+// Where piece i of a lane's 8 / W pieces lies: W elements at a, W at b.
+struct RotaryPiece {
+    int a, b;
+    bool turned, has_a, has_b;
+};
+
+// A lane's 16 elements as they lie in memory, 2 W of a piece together.
+template <bool BF16, int W> constexpr int kRawWords = BF16 && W > 1 ? 8 : 16;
+
+template <bool BF16, int W>
+__device__ __forceinline__ void load_run(const void* base, int64_t at, uint32_t* w) {
+    if (BF16) {
+        const uint16_t* p = (const uint16_t*)base + at;
+        if (W == 8) {
+            const uint4 t = *(const uint4*)p;
+            w[0] = t.x, w[1] = t.y, w[2] = t.z, w[3] = t.w;
+        } else if (W == 4) {
+            const uint2 t = *(const uint2*)p;
+            w[0] = t.x, w[1] = t.y;
+        } else {
+            w[0] = *p;
+        }
+    } else {
+        const uint32_t* p = (const uint32_t*)base + at;
+        if (W == 1) {
+            w[0] = *p;
+        } else {
+#pragma unroll
+            for (int i = 0; i < W / 4; i++) {
+                const uint4 t = *(const uint4*)(p + 4 * i);
+                w[4 * i] = t.x, w[4 * i + 1] = t.y, w[4 * i + 2] = t.z, w[4 * i + 3] = t.w;
+            }
+        }
+    }
+}
+
+template <bool BF16, int W>
+__device__ __forceinline__ void store_run(void* base, int64_t at, const float* x) {
+    if (BF16) {
+        uint16_t* p = (uint16_t*)base + at;
+        if (W == 8) *(uint4*)p = make_uint4(f32x2_to_bf16x2(x[0], x[1]), f32x2_to_bf16x2(x[2], x[3]), f32x2_to_bf16x2(x[4], x[5]), f32x2_to_bf16x2(x[6], x[7]));
+        else if (W == 4) *(uint2*)p = make_uint2(f32x2_to_bf16x2(x[0], x[1]), f32x2_to_bf16x2(x[2], x[3]));
+        else *p = (uint16_t)f32_to_bf16(x[0]);
+    } else {
+        float* p = (float*)base + at;
+        if (W == 1) {
+            *p = x[0];
+        } else {
+#pragma unroll
+            for (int i = 0; i < W / 4; i++) *(float4*)(p + 4 * i) = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+        }
+    }
+}
+
+template <int W>
+__device__ __forceinline__ void store_codes(int8_t* p, const float* x, float inv) {
+    if (W == 1) {
+        *p = (int8_t)quant_code(x[0], inv, 127.0f, 0);
+    } else {
+#pragma unroll
+        for (int i = 0; i < W / 4; i++)
+            ((uint32_t*)p)[i] = pack4(quant_code(x[4 * i], inv, 127.0f, 0), quant_code(x[4 * i + 1], inv, 127.0f, 0),
+                                      quant_code(x[4 * i + 2], inv, 127.0f, 0), quant_code(x[4 * i + 3], inv, 127.0f, 0));
+    }
+}
+
+}  // namespace
+
+// W: elements an access (see rotary_width).  A block has the heads from part *
+// per_part on of 64 >> lg tokens, `parts` blocks one group of tokens.
+template <bool BF16, bool INTER, bool WRITE, int W>
+__global__ __launch_bounds__(256) void rotary_kernel(Rotary p, KvCache c, int lg, int parts, int per_part) {
+    constexpr int N = 8 / W, RW = kRawWords<BF16, W>;
+    __shared__ float2 turns[512];  // [token][pair]: 64 >> lg tokens of at most 8 << lg pairs
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int tokens = 64 >> lg, half = p.rot >> 1;
+    const int64_t group = blockIdx.x / parts, first = group * tokens;
+    const int part = blockIdx.x - (int)group * parts;
+
+    for (int i = threadIdx.x; i < tokens * half; i += 256) {
+        const int t = i / half;
+        if (first + t < p.tokens) {
+            const float2 v = turn_of(p.positions[first + t], p.freq[i - t * half]);
+            turns[i] = make_float2(v.x * p.scale, v.y * p.scale);
+        }
+    }
+    __syncthreads();
+
+    const int mine = lane >> lg, l = lane & ((1 << lg) - 1);
+    const int64_t token = first + mine;
+    const bool live = token < p.tokens;
+    RotaryPiece at[N];
+    float2 cs[8];
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const int pair = 8 * l + W * i;
+        at[i].turned = pair < half;
+        at[i].a = at[i].turned && !INTER ? pair : 2 * pair;
+        at[i].b = at[i].turned && !INTER ? half + pair : 2 * pair + W;
+        at[i].has_a = live && 2 * pair < p.dim;
+        at[i].has_b = live && (W > 1 ? 2 * pair : 2 * pair + 1) < p.dim;
+#pragma unroll
+        for (int j = 0; j < W; j++) cs[W * i + j] = at[i].turned && live ? turns[mine * half + pair + j] : make_float2(1.0f, 0.0f);
+    }
+    bool keep = false;
+    int64_t code = 0, scale_at = 0;
+    if (WRITE && live) {
+        const int64_t slot = p.slots[token];
+        keep = slot >= 0 && slot < c.slots;
+        const int64_t use = keep ? slot : 0, block = c.slots <= INT32_MAX ? page_of(c, (int)use) : use / c.page, in = use - block * c.page;
+        code = block * c.block_stride + in * c.token_stride;
+        scale_at = block * c.s_block_stride + in * c.s_token_stride;
+    }
+
+    const int heads = p.q.heads + (WRITE ? 2 * c.heads : 0), end = min(heads, (part + 1) * per_part);
+    // U heads of a wave at a time, their loads together.
+    constexpr int U = BF16 && W == 8 ? 4 : 2;
+    for (int h0 = part * per_part + wave; h0 < end; h0 += 4 * U) {
+        uint32_t w[U][RW];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int h = h0 + 4 * u;
+            if (h >= end) break;
+            const int kind = !WRITE || h < p.q.heads ? 0 : h < p.q.heads + c.heads ? 1 : 2;
+            const RotaryHeads& s = kind == 0 ? p.q : kind == 1 ? p.k : p.v;
+            const int head = kind == 0 ? h : kind == 1 ? h - p.q.heads : h - p.q.heads - c.heads;
+            const int64_t from = token * s.in_token + head * s.in_head;
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                constexpr int R = RW / N / 2;
+                if (at[i].has_a) load_run<BF16, W>(s.in, from + at[i].a, &w[u][2 * R * i]);
+                if (at[i].has_b) load_run<BF16, W>(s.in, from + at[i].b, &w[u][2 * R * i + R]);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int h = h0 + 4 * u;
+            if (h >= end) break;
+            const int kind = !WRITE || h < p.q.heads ? 0 : h < p.q.heads + c.heads ? 1 : 2;
+            const int head = kind == 0 ? h : kind == 1 ? h - p.q.heads : h - p.q.heads - c.heads;
+            float x[16];
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                if (!BF16) x[e] = __uint_as_float(w[u][e]);
+                else if (W == 1) x[e] = bf16_to_f32(w[u][e]);
+                else x[e] = bf16_to_f32(e & 1 ? w[u][e / 2 % RW] >> 16 : w[u][e / 2 % RW] & 0xffffu);
+            }
+            if (kind < 2) {
+#pragma unroll
+                for (int i = 0; i < N; i++)
+#pragma unroll
+                    for (int j = 0; j < W; j++) {
+                        const int ea = 2 * W * i + (INTER ? 2 * j : j), eb = INTER ? ea + 1 : ea + W;
+                        const float a = x[ea], b = x[eb], cos = cs[W * i + j].x, sin = cs[W * i + j].y;
+                        x[ea] = at[i].turned ? fmaf(a, cos, -(b * sin)) : a;
+                        x[eb] = at[i].turned ? fmaf(b, cos, a * sin) : b;
+                    }
+            }
+            if (kind == 0) {
+                const int64_t to = token * p.q.out_token + head * p.q.out_head;
+#pragma unroll
+                for (int i = 0; i < N; i++) {
+                    if (at[i].has_a) store_run<BF16, W>(p.q.out, to + at[i].a, &x[2 * W * i]);
+                    if (at[i].has_b) store_run<BF16, W>(p.q.out, to + at[i].b, &x[2 * W * i + W]);
+                }
+            } else if (WRITE) {
+                // As kv_cache.hip quantises.
+                float top = 0.0f, bad = 0.0f;
+#pragma unroll
+                for (int i = 0; i < N; i++)
+#pragma unroll
+                    for (int j = 0; j < 2 * W; j++) {
+                        const float v = (j < W ? at[i].has_a : at[i].has_b) ? x[2 * W * i + j] : 0.0f;
+                        top = fmaxf(top, fabsf(v));
+                        bad = fmaf(v, 0.0f, bad);  // NaN once an infinity or a NaN is met
+                    }
+                for (int off = 1; off < 1 << lg; off <<= 1) {
+                    top = fmaxf(top, __shfl_xor(top, off, 64));
+                    bad += __shfl_xor(bad, off, 64);
+                }
+                if (!keep) continue;
+                const bool fine = bad == 0.0f;
+                const float sc = top > 1e-30f ? top / 127.0f : 1.0f, inv = fine ? 1.0f / sc : 0.0f;
+                if (!fine) {
+#pragma unroll
+                    for (int e = 0; e < 16; e++) x[e] = 0.0f;
+                }
+                int8_t* to = (kind == 1 ? c.k : c.v) + code + head * c.head_stride;
+#pragma unroll
+                for (int i = 0; i < N; i++) {
+                    if (at[i].has_a) store_codes<W>(to + at[i].a, &x[2 * W * i], inv);
+                    if (at[i].has_b) store_codes<W>(to + at[i].b, &x[2 * W * i + W], inv);
+                }
+                if (l == 0) (kind == 1 ? c.ks : c.vs)[scale_at + head * c.s_head_stride] = fine ? sc : __builtin_nanf("");
+            }
+        }
+    }
+}
+
+// Elements an access: 8 pairs of a lane are one run of 8 at each side where the
+// halves and the rest are whole runs and rows lie at 16 bytes; runs of 4 the same; else
+// one by one.
+static int rotary_width(const Rotary& p) {
+    const int e = p.bf16 ? 2 : 4;
+    for (int w : {8, 4}) {
+        const int64_t unit = w * e < 16 ? w * e : 16;
+        bool ok = p.rot % (2 * w) == 0 && p.dim % (2 * w) == 0;
+        for (const RotaryHeads* s : {&p.q, &p.k, &p.v}) {
+            if (!s->heads) continue;
+            ok = ok && (uintptr_t)s->in % unit == 0 && s->in_token * e % unit == 0 && s->in_head * e % unit == 0 &&
+                 (uintptr_t)s->out % unit == 0 && s->out_token * e % unit == 0 && s->out_head * e % unit == 0;
+        }
+        if (ok) return w;
+    }
+    return 1;
+}
+
+template <bool BF16, bool INTER, bool WRITE>
+static hipError_t launch(hipStream_t stream, const Rotary& p, const KvCache& c) {
+    int lg = 0;
+    while (16 << lg < p.dim) lg++;
+    const int64_t groups = (p.tokens + (64 >> lg) - 1) >> (6 - lg);
+    const int heads = p.q.heads + (WRITE ? 2 * c.heads : 0), most = (heads + 3) / 4;
+    // Enough blocks for every compute unit to have eight; beyond, a block's heads share its angles.
+    const int64_t want = (2048 + groups - 1) / groups;
+    const int per_part = 4 * ((most + (int)(want < most ? want : most) - 1) / (int)(want < most ? want : most));
+    const int parts = (heads + per_part - 1) / per_part;
+    if (groups * parts > INT32_MAX) return hipErrorInvalidConfiguration;
+    const dim3 grid((unsigned)(groups * parts)), block(256);
+    switch (rotary_width(p)) {
+        case 8: hipLaunchKernelGGL((rotary_kernel<BF16, INTER, WRITE, 8>), grid, block, 0, stream, p, c, lg, parts, per_part); break;
+        case 4: hipLaunchKernelGGL((rotary_kernel<BF16, INTER, WRITE, 4>), grid, block, 0, stream, p, c, lg, parts, per_part); break;
+        default: hipLaunchKernelGGL((rotary_kernel<BF16, INTER, WRITE, 1>), grid, block, 0, stream, p, c, lg, parts, per_part);
+    }
+    return hipGetLastError();
+}
+
+hipError_t launch_rotary(hipStream_t stream, const Rotary& p, const KvCache& c) {
+    const bool write = p.k.heads > 0;
+    if (p.bf16) {
+        if (p.interleaved) return write ? launch<true, true, true>(stream, p, c) : launch<true, true, false>(stream, p, c);
+        return write ? launch<true, false, true>(stream, p, c) : launch<true, false, false>(stream, p, c);
+    }
+    if (p.interleaved) return write ? launch<false, true, true>(stream, p, c) : launch<false, true, false>(stream, p, c);
+    return write ? launch<false, false, true>(stream, p, c) : launch<false, false, false>(stream, p, c);
+}
+
+}  // namespace phi_dev

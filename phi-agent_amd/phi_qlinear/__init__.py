@@ -1,8 +1,8 @@
 """Python front end of the gfx950 quantized-linear library.
 
 Thin ctypes bindings over the C ABI in ``include/phi_qlinear.h`` and
-``include/phi_decoder.h`` (``lib/libphi_qlinear.so``; the second header's
-operators are in ``decoder.py``).  PyTorch provides device memory and the stream;
+``include/phi_decoder.h`` and ``include/phi_serving.h`` (``lib/libphi_qlinear.so``;
+the second and third header's operators are in ``decoder.py`` and ``serving.py``).  PyTorch provides device memory and the stream;
 every computation runs in the HIP kernels.  There is no fallback: if the
 library is missing or the device is absent the calls raise.
 
@@ -91,7 +91,8 @@ EXPORTS = ["phi_hip_last_error", "phi_hip_abi_version", "phi_hip_quant_rotate", 
            "phi_hip_dequant_fp4_rows", "phi_hip_gemm_plan_set", "phi_hip_gemm_plan_get", "phi_hip_gemm_plan_count",
            "phi_hip_gemm_plan_clear", "phi_hip_gemm_is_small", "phi_hip_w4a8_banded_bytes", "phi_hip_w4a8_pack_banded",
            "phi_hip_w4a8_linear_banded", "phi_hip_rms_norm_quant", "phi_hip_kv_cache_write", "phi_hip_kv_cache_read",
-           "phi_hip_paged_attention", "phi_hip_paged_attention_workspace_bytes"]
+           "phi_hip_paged_attention", "phi_hip_paged_attention_workspace_bytes", "phi_hip_rotary",
+           "phi_hip_rotary_cache_write", "phi_hip_kv_cache_copy"]
 
 _lib = None
 
@@ -168,6 +169,11 @@ def load() -> ctypes.CDLL:
                                           I64, I64, F, I, I64, P, I64, I64, P, SZ]
     L.phi_hip_paged_attention_workspace_bytes.argtypes = [I64, I64, I64, I64, I64, I64, I64, I]
     L.phi_hip_paged_attention_workspace_bytes.restype = SZ
+    KV = ctypes.POINTER(KvCacheDesc)
+    L.phi_hip_rotary.argtypes = [P, P, I, I64, I64, I64, I64, I64, P, P, I64, I, F, P, I64, I64]
+    L.phi_hip_rotary_cache_write.argtypes = [P, KV, P, I64, I64, I64, P, I64, I64, P, I64, I64, P, I64, I64, I, P, P, I64, I,
+                                             F, P, I64]
+    L.phi_hip_kv_cache_copy.argtypes = [P, KV, KV, P, P, P, I64]
     for name in EXPORTS:
         f = getattr(L, name)
         if f.restype is None:
@@ -756,3 +762,4 @@ def q8_linear_kt(x: torch.Tensor, Wkt: torch.Tensor, N: int, sW: torch.Tensor,
 
 from .decoder import (KvCache, kv_cache_empty, kv_cache_read, kv_cache_write, paged_attention,  # noqa: E402,F401
                       paged_attention_workspace, rms_norm_quant)
+from .serving import (KvPages, kv_cache_copy, rotary, rotary_cache_write, rotary_frequencies)  # noqa: E402,F401

@@ -1,0 +1,235 @@
+"""What a server of many requests runs beside the decoder layer's operators
+(include/phi_serving.h).
+
+``rotary`` turns vectors by their positions, ``rotary_cache_write`` does so on
+a projection's way into the paged cache, ``kv_cache_copy`` copies pages of it,
+as ``KvPages`` says when sequences fork or pages move together.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import _check, _dt, _ptr, _stream, load
+from .decoder import KvCache, _empty, _vectors
+
+
+def _here(who: str, stream, *tensors) -> None:
+    """Device tensors, all of the device that the call runs on."""
+    at = {t.get_device() for t in tensors if t is not None}
+    if -1 in at:
+        raise ValueError("phi_qlinear operates on device tensors")
+    dev = torch._C._cuda_getDevice() if stream is None else stream.device.index
+    if at != {dev}:
+        raise ValueError(f"{who}: tensors of device {sorted(at)} in a call on device {dev}")
+
+
+def rotary_frequencies(rot: int, base: float = 10000.0, *, scaling: str | None = None, factor: float = 1.0,
+                       length: int = 8192, slow: float = 1.0, fast: float = 32.0, device="cuda") -> torch.Tensor:
+    """Radians a position of `rot` elements' pairs, fp64 [rot / 2]: base^(-2 j / rot),
+    for a context of `factor` times the trained `length` by one of these rules:
+
+      linear  all of them 1 / factor
+      ntk     another base, base * factor^(rot / (rot - 2)): the last pair's 1 / factor
+      parts   pairs of more than `fast` turns in `length` positions as they are, those
+              of fewer than `slow` turns 1 / factor, between them a mean weighted by
+              the turns
+      ramp    the same, weighted by the pair's number j between those that have `fast`
+              and `slow` turns (rounded to whole pairs)
+    """
+    if rot < 2 or rot % 2:
+        raise ValueError(f"rotary_frequencies: {rot} is no even number from 2 on")
+    j = torch.arange(rot // 2, dtype=torch.float64)
+    if scaling == "ntk":
+        if rot < 4:
+            raise ValueError("rotary_frequencies: ntk needs two pairs")
+        base = base * factor ** (rot / (rot - 2))
+    f = base ** (-2.0 * j / rot)
+    if scaling in (None, "ntk"):
+        return f.to(device)
+    if scaling == "linear":
+        keep = torch.zeros_like(f)
+    elif scaling == "parts":
+        keep = ((length * f / (2 * math.pi) - slow) / (fast - slow)).clamp(0, 1)
+    elif scaling == "ramp":
+        pair = lambda turns: rot * math.log(length / (turns * 2 * math.pi)) / (2 * math.log(base))  # noqa: E731
+        first, last = max(math.floor(pair(fast)), 0), min(math.ceil(pair(slow)), rot - 1)
+        keep = 1 - ((j - first) / max(last - first, 1e-3)).clamp(0, 1)
+    else:
+        raise ValueError(f"rotary_frequencies: no rule {scaling!r}")
+    return (f * (keep + (1 - keep) / factor)).to(device)
+
+
+def _turns(who: str, positions: torch.Tensor, freq: torch.Tensor, tokens: int) -> None:
+    if (positions.dtype != torch.int64 or positions.shape != (tokens,) or not positions.is_contiguous()
+            or freq.dtype != torch.float64 or freq.dim() != 1 or not freq.is_contiguous()):
+        raise ValueError(f"{who}: positions [tokens] int64 and freq [rot / 2] float64, contiguous")
+
+
+def rotary(x: torch.Tensor, positions: torch.Tensor, freq: torch.Tensor, *, interleaved: bool = False,
+           scale: float = 1.0, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """Rotary positions of x [tokens, heads, dim] (f32/bf16, any strides with a
+    contiguous dim; phi_hip_rotary): the pairs of each vector's first 2 len(freq)
+    elements, (j, j + len(freq)) or, interleaved, (2 j, 2 j + 1), turned by
+    positions [tokens] int64 times freq [rot / 2] float64 and scaled; the rest
+    copied.  out may be x."""
+    _here("rotary", stream, x, positions, freq, out)
+    shape = x.shape
+    T, H, D = shape
+    xt, xh = _vectors("rotary", "x", x, shape)
+    _turns("rotary", positions, freq, T)
+    if out is None:
+        out, ot, oh = _empty(shape, x.dtype, x, stream), H * D, D
+    else:
+        ot, oh = _vectors("rotary", "out", out, shape)
+        if out.dtype != x.dtype:
+            raise ValueError("rotary: out and x differ in dtype")
+    _check(load().phi_hip_rotary(_stream(stream), x.data_ptr(), _dt(x), xt, xh, T, H, D, positions.data_ptr(),
+                                 freq.data_ptr(), 2 * freq.shape[0], 1 if interleaved else 0, scale, out.data_ptr(), ot, oh))
+    return out
+
+
+def rotary_cache_write(cache: KvCache, q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
+                       positions: torch.Tensor, freq: torch.Tensor, slots: torch.Tensor, *, interleaved: bool = False,
+                       scale: float = 1.0, out: torch.Tensor | None = None, stream=None) -> torch.Tensor | None:
+    """A projection's output on its way to attention (phi_hip_rotary_cache_write):
+    q [tokens, q_heads, dim] rotated as by `rotary` and returned (out may be q; q
+    None: there is none), k [tokens, heads, dim] rotated and v as it is into the
+    cache at slots [tokens], as by `kv_cache_write`.  q, k and v of one dtype
+    (f32/bf16), vectors 16-byte aligned."""
+    who = "rotary_cache_write"
+    _here(who, stream, cache.k, q, k, v, positions, freq, slots, out)
+    n = slots.numel()
+    shape = (n, cache._heads, cache._dim)
+    if k.dtype != v.dtype or (q is not None and q.dtype != k.dtype) or slots.dtype != torch.int64 or not slots.is_contiguous():
+        raise ValueError(f"{who}: q, k and v of one dtype, slots contiguous int64")
+    kt, kh = _vectors(who, "k", k, shape)
+    vt, vh = _vectors(who, "v", v, shape)
+    _turns(who, positions, freq, n)
+    qp = op = None
+    qt = qh = ot = oh = heads = 0
+    if q is not None:
+        heads = q.shape[1]
+        qt, qh = _vectors(who, "q", q, (n, heads, cache._dim))
+        if out is None:
+            out, ot, oh = _empty(q.shape, q.dtype, q, stream), heads * cache._dim, cache._dim
+        else:
+            ot, oh = _vectors(who, "out", out, q.shape)
+            if out.dtype != q.dtype:
+                raise ValueError(f"{who}: out and q differ in dtype")
+        qp, op = q.data_ptr(), out.data_ptr()
+    elif out is not None:
+        raise ValueError(f"{who}: out without q")
+    _check(load().phi_hip_rotary_cache_write(
+        _stream(stream), cache._desc, qp, qt, qh, heads, op, ot, oh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, _dt(k),
+        positions.data_ptr(), freq.data_ptr(), 2 * freq.shape[0], 1 if interleaved else 0, scale, slots.data_ptr(), n))
+    return out
+
+
+def kv_cache_copy(source: KvCache, target: KvCache, from_blocks: torch.Tensor, to_blocks: torch.Tensor, *,
+                  tokens: torch.Tensor | None = None, stream=None) -> None:
+    """Blocks from_blocks[i] of a cache to blocks to_blocks[i] of another, or of
+    the same (phi_hip_kv_cache_copy): all tokens, or the first tokens[i].  int32,
+    of one length.  A block that is written is written once and not read in the
+    same call; a pair with a block that its cache does not have is skipped."""
+    _here("kv_cache_copy", stream, source.k, target.k, from_blocks, to_blocks, tokens)
+    n = from_blocks.numel()
+    for t in (from_blocks, to_blocks, tokens):
+        if t is not None and (t.dtype != torch.int32 or t.shape != (n,) or not t.is_contiguous()):
+            raise ValueError("kv_cache_copy: from_blocks, to_blocks and tokens are contiguous int32 of one length")
+    _check(load().phi_hip_kv_cache_copy(_stream(stream), source._desc, target._desc, from_blocks.data_ptr(),
+                                        to_blocks.data_ptr(), _ptr(tokens), n))
+
+
+class KvPages:
+    """Who has which pages of a paged cache: pages handed out as sequences grow,
+    shared when they fork, taken back when their last sequence ends, and moved
+    together.  Host side only: `copies` holds what the device has yet to copy,
+    (from, to, tokens), for `flush` to do before the next write or attention.
+
+    A sequence's pages are append-only, so a forked one shares its parent's whole
+    pages and gets a copy of the last where that is not full."""
+
+    def __init__(self, blocks: int, page: int):
+        self.page, self.of, self.length, self.copies = page, {}, {}, []
+        self.users = [0] * blocks
+        self.free = list(range(blocks))[::-1]  # the lowest is handed out first
+
+    def _take(self, n: int) -> list[int]:
+        if n > len(self.free):
+            raise RuntimeError("the cache is full")
+        got = [self.free.pop() for _ in range(n)]
+        for b in got:
+            self.users[b] = 1
+        return got
+
+    def grow(self, seq, tokens: int) -> list[int]:
+        """Room for `tokens` more of a sequence (a new one, if it is not known):
+        their slots.  All or nothing: RuntimeError where there are too few pages."""
+        if tokens < 0:
+            raise ValueError(f"KvPages: {tokens} tokens")
+        at, mine = self.length.get(seq, 0), self.of.get(seq, [])
+        new = self._take(max(0, -(-(at + tokens) // self.page) - len(mine)))
+        self.of[seq] = mine = mine + new
+        self.length[seq] = at + tokens
+        return [mine[t // self.page] * self.page + t % self.page for t in range(at, at + tokens)]
+
+    def fork(self, parent, child) -> None:
+        """A sequence `child` with the parent's tokens."""
+        if child in self.of:
+            raise ValueError(f"KvPages: {child!r} is there already")
+        n, pages = self.length[parent], self.of[parent]
+        whole, rest = divmod(n, self.page)
+        last = self._take(1) if rest else []
+        for b in pages[:whole]:
+            self.users[b] += 1
+        if rest:
+            self.copies.append((pages[whole], last[0], rest))
+        self.of[child], self.length[child] = pages[:whole] + last, n
+
+    def end(self, seq) -> None:
+        """A sequence's pages back, but for those that others share."""
+        for b in self.of.pop(seq, []):
+            self.users[b] -= 1
+            if not self.users[b]:
+                self.free.append(b)
+        self.length.pop(seq, None)
+        self.free.sort(reverse=True)
+
+    def shared(self, seqs) -> int:
+        """How many leading pages all of `seqs` share."""
+        rows = [self.of[s] for s in seqs]
+        n = min(self.length[s] // self.page for s in seqs)
+        return next((i for i in range(n) if any(r[i] != rows[0][i] for r in rows)), n)
+
+    def compact(self) -> int:
+        """Move pages so that those in use are the lowest; the number of them."""
+        used = [b for b, n in enumerate(self.users) if n]
+        high = [b for b in used if b >= len(used)]
+        low = [b for b in range(len(used)) if not self.users[b]]
+        move = dict(zip(high, low))
+        for a, b in move.items():
+            self.users[a], self.users[b] = 0, self.users[a]
+            self.copies.append((a, b, self.page))
+        self.of = {s: [move.get(b, b) for b in pages] for s, pages in self.of.items()}
+        self.free = list(range(len(used), len(self.users)))[::-1]
+        return len(used)
+
+    def flush(self, cache: KvCache, stream=None) -> None:
+        """Have the device do the copies, in as few calls as leave no block in one that
+        is written there and read, or written twice."""
+        if stream is not None:
+            with torch.cuda.stream(stream):
+                return self.flush(cache)
+        left, self.copies = self.copies, []
+        while left:
+            read, written, now, later = set(), set(), [], []
+            for c in left:
+                meets = c[0] in written or c[1] in written or c[1] in read
+                (later if later or meets else now).append(c)
+                read.add(c[0]), written.add(c[1])
+            part = torch.tensor(now, dtype=torch.int32).t().contiguous().to(cache.k.device)
+            kv_cache_copy(cache, cache, part[0], part[1], tokens=part[2])
+            left = later

@@ -1,0 +1,18 @@
+"""Plain 64-bit forms of the serving operators, on the CPU."""
+import torch
+
+
+def rotated(x, positions, freq, interleaved, scale):
+    """x [tokens, heads, dim] turned, in 64 bits, and beside each value the sum of
+    its terms' magnitudes (of what was only copied: 0)."""
+    half = freq.numel()
+    x = x.double()
+    angle = positions.double()[:, None] * freq
+    cos, sin = torch.cos(angle)[:, None] * scale, torch.sin(angle)[:, None] * scale
+    j = torch.arange(half)
+    i, k = (2 * j, 2 * j + 1) if interleaved else (j, j + half)
+    a, b = x[..., i], x[..., k]
+    y, mag = x.clone(), torch.zeros_like(x)
+    y[..., i], y[..., k] = a * cos - b * sin, b * cos + a * sin
+    mag[..., i] = mag[..., k] = abs(scale) * (a.abs() + b.abs())
+    return y, mag
