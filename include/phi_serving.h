@@ -8,9 +8,11 @@
  *   phi_hip_rotary_cache_write   the same of a projection's q and k, with k and v
  *                                quantised into the paged cache
  *   phi_hip_kv_cache_copy        pages of a cache copied (forked sequences, compaction)
+ *   phi_hip_lora_batched         a linear's output plus each row's own low-rank adapter
  *
  * The reference rotates pairs of half a head's distance on fp32 tensors
- * (rope_half, core/kernels/attn.cpp:99-); it has no cache.
+ * (rope_half, core/kernels/attn.cpp:99-) and adds one adapter to all rows
+ * (apply_lora_tail, core/models/model_common.cpp:1667-1700); it has no cache.
  */
 #ifndef PHI_SERVING_H
 #define PHI_SERVING_H
@@ -73,6 +75,36 @@ phi_status phi_hip_rotary_cache_write(phi_stream_t stream, const phi_kv_cache* c
 phi_status phi_hip_kv_cache_copy(phi_stream_t stream, const phi_kv_cache* from, const phi_kv_cache* to,
                                  const int32_t* from_blocks, const int32_t* to_blocks, const int32_t* tokens,
                                  int64_t n);
+
+/*
+ * Low-rank adapters of many requests beside one linear:
+ *   out[m] = base[m] + scale[a] B[a] (A[a] x[m]),   a = adapter[m]
+ * for rows m in any order of adapters; a row whose adapter is below 0 or not below
+ * `adapters` has none: out[m] = base[m].
+ *
+ *   x        [rows, ldx] of x_dtype, K columns
+ *   A, B     [adapters, R, K] and [adapters, N, R] of w_dtype, last dimension
+ *            contiguous, the others' strides in elements.  Adapters of fewer ranks
+ *            have zeros in the rest.
+ *   adapter  [rows] int32; scale [adapters] fp32, or NULL: 1
+ *   base     [rows, ld_base] of out_dtype, N columns: the linear's output; NULL: 0
+ *   out      [rows, ldo] of out_dtype; may be base, else shares no memory with an input
+ *   workspace  phi_hip_lora_batched_workspace_bytes() bytes, 16-byte aligned
+ * All dtypes PHI_F32 or PHI_BF16; every pointer aligned to its own type; R to 256, rows,
+ * K and N to 2^24.  Products of bf16 by bf16 are exact, the others fp32; all sums and A x
+ * itself are fp32, and out is rounded once.  phi_hip_lora_tail has one adapter for
+ * all rows and the reference's order of sums; here a sum's order depends on rows, K
+ * and R alone, so a row's bits do not depend on its neighbours' adapters.
+ */
+phi_status phi_hip_lora_batched(phi_stream_t stream, const void* x, int x_dtype, int64_t ldx, int64_t rows, int64_t K,
+                                const void* A, int64_t a_adapter_stride, int64_t a_row_stride, const void* B,
+                                int64_t b_adapter_stride, int64_t b_row_stride, int w_dtype, int64_t adapters,
+                                int64_t R, int64_t N, const int32_t* adapter, const float* scale, const void* base,
+                                int64_t ld_base, void* out, int out_dtype, int64_t ldo, void* workspace,
+                                size_t ws_bytes);
+
+/* Workspace of phi_hip_lora_batched (0 for sizes that no call may have). */
+size_t phi_hip_lora_batched_workspace_bytes(int64_t rows, int64_t K, int64_t R);
 
 #ifdef __cplusplus
 }

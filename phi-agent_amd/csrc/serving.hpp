@@ -35,4 +35,21 @@ struct KvCopy {
 };
 hipError_t launch_kv_cache_copy(hipStream_t stream, const KvCopy& p);
 
+// out = base + scale[a] B[a] (A[a] x), a = adapter of the row; strides in elements.
+struct LoraBatched {
+    const void* x;
+    const void* A;   // [adapters, R, K]
+    const void* B;   // [adapters, N, R]
+    const int32_t* adapter;
+    const float* scale;  // null: 1
+    const void* base;    // null: 0
+    void* out;
+    float* h;        // [splits][rows][rank_pitch]: parts of A x
+    int64_t ldx, a_adapter, a_row, b_adapter, b_row, ld_base, ldo;
+    int rows, K, N, R, adapters, splits, rank_pitch;
+    bool x_bf16, w_bf16, out_bf16;
+};
+hipError_t launch_lora_batched(hipStream_t stream, LoraBatched p);
+size_t lora_batched_workspace(int64_t rows, int64_t K, int64_t R);
+
 }  // namespace phi_dev

@@ -9,6 +9,8 @@ using namespace phi_capi;
 namespace {
 
 constexpr int64_t kMaxRotaryDim = 1024;   // a wave has a vector
+constexpr int64_t kMaxRank = 256;              // of an adapter: h of 32 rows is held in LDS
+constexpr int64_t kMaxLoraRows = 1 << 24, kMaxLoraK = 1 << 24;  // units and columns counted in 31 bits
 constexpr int64_t kMaxPageVectors = 1 << 26;  // of at most 16 pieces: counted in 31 bits
 
 // [tokens, heads, dim] vectors that are written: one of the strides holds the other's
@@ -125,6 +127,54 @@ phi_status phi_hip_kv_cache_copy(phi_stream_t stream, const phi_kv_cache* from, 
     if (!aligned(from_blocks, 4) || !aligned(to_blocks, 4) || !aligned(tokens, 4)) return fail(PHI_ERR_ALIGN, "%s: blocks or tokens are misaligned", who);
     const phi_dev::KvCopy p{a, b, from_blocks, to_blocks, tokens, n};
     return check_hip(phi_dev::launch_kv_cache_copy((hipStream_t)stream, p), who);
+}
+
+phi_status phi_hip_lora_batched(phi_stream_t stream, const void* x, int x_dtype, int64_t ldx, int64_t rows, int64_t K,
+                                const void* A, int64_t a_adapter_stride, int64_t a_row_stride, const void* B,
+                                int64_t b_adapter_stride, int64_t b_row_stride, int w_dtype, int64_t adapters,
+                                int64_t R, int64_t N, const int32_t* adapter, const float* scale, const void* base,
+                                int64_t ld_base, void* out, int out_dtype, int64_t ldo, void* workspace,
+                                size_t ws_bytes) {
+    static const char* who = "lora_batched";
+    if (device_lost()) return fail(PHI_ERR_DEVICE_LOST, "%s: device was lost earlier", who);
+    if (rows < 0 || K < 0 || N < 0 || R < 0 || adapters < 0) return fail(PHI_ERR_SHAPE, "%s: negative size", who);
+    if (!is_float(x_dtype) || !is_float(w_dtype) || !is_float(out_dtype)) return fail(PHI_ERR_ARG, "%s: dtypes must be f32 or bf16", who);
+    if (rows == 0 || N == 0) return ok();
+    if (K == 0 || R == 0 || adapters == 0) return fail(PHI_ERR_SHAPE, "%s: empty factors (K=%lld R=%lld adapters=%lld)", who, (long long)K, (long long)R, (long long)adapters);
+    if (R > kMaxRank) return fail(PHI_ERR_UNSUPPORTED, "%s: R=%lld exceeds %lld", who, (long long)R, (long long)kMaxRank);
+    if (rows > kMaxLoraRows || K > kMaxLoraK || N > kMaxLoraK || adapters > INT32_MAX)
+        return fail(PHI_ERR_SHAPE, "%s: rows=%lld K=%lld N=%lld adapters=%lld out of range", who, (long long)rows, (long long)K, (long long)N, (long long)adapters);
+    if (!x || !A || !B || !adapter || !out) return fail(PHI_ERR_ARG, "%s: null pointer", who);
+    if (ldx < K || ldo < N || (base && ld_base < N) || a_row_stride < K || b_row_stride < R) return fail(PHI_ERR_SHAPE, "%s: leading dimension smaller than the row", who);
+    if (ldx > kMaxPitch || ldo > kMaxPitch || (base && ld_base > kMaxPitch) || a_row_stride > kMaxPitch || b_row_stride > kMaxPitch)
+        return fail(PHI_ERR_SHAPE, "%s: leading dimension too large", who);
+    for (int64_t s : {a_adapter_stride, b_adapter_stride})
+        if (s < 0 || s > kMaxStride / 2) return fail(PHI_ERR_SHAPE, "%s: bad adapter stride %lld", who, (long long)s);
+    const int64_t xe = elem(x_dtype), we = elem(w_dtype), oe = elem(out_dtype);
+    if (!aligned(x, xe) || !aligned(A, we) || !aligned(B, we) || !aligned(adapter, 4) || !aligned(scale, 4) || !aligned(out, oe) || !aligned(base, oe))
+        return fail(PHI_ERR_ALIGN, "%s: a pointer is not aligned to its type", who);
+    const size_t need = phi_hip_lora_batched_workspace_bytes(rows, K, R);
+    if (!workspace || ws_bytes < need) return fail(PHI_ERR_WORKSPACE, "%s: needs %zu bytes of workspace, got %zu", who, need, workspace ? ws_bytes : (size_t)0);
+    if (!aligned(workspace, 16)) return fail(PHI_ERR_ALIGN, "%s: the workspace must be 16-byte aligned", who);
+    const Pieces to = rows_of(out, rows, N, ldo, oe), from = rows_of(base, rows, N, ld_base, oe), ws{workspace, (int64_t)need};
+    const Pieces in[] = {rows_of(x, rows, K, ldx, xe), {A, K * we, R, a_row_stride * we, adapters, a_adapter_stride * we},
+                         {B, R * we, N, b_row_stride * we, adapters, b_adapter_stride * we}, {adapter, rows * 4}, {scale, adapters * 4}};
+    for (const auto& i : in) {
+        if (meet(to, i)) return fail(PHI_ERR_ARG, "%s: out overlaps an input", who);
+        if (meet(ws, i)) return fail(PHI_ERR_ARG, "%s: the workspace overlaps an operand", who);
+    }
+    if (meet(ws, to) || meet(ws, from)) return fail(PHI_ERR_ARG, "%s: the workspace overlaps an operand", who);
+    const bool same = base == out && (rows == 1 || ld_base == ldo);
+    if (!same && meet(to, from)) return fail(PHI_ERR_ARG, "%s: out overlaps base", who);
+    const phi_dev::LoraBatched p{x, A, B, adapter, scale, base, out, (float*)workspace, ldx, a_adapter_stride, a_row_stride, b_adapter_stride,
+                                 b_row_stride, ld_base, ldo, (int)rows, (int)K, (int)N, (int)R, (int)adapters, 0, 0,
+                                 x_dtype == PHI_BF16, w_dtype == PHI_BF16, out_dtype == PHI_BF16};
+    return check_hip(phi_dev::launch_lora_batched((hipStream_t)stream, p), who);
+}
+
+size_t phi_hip_lora_batched_workspace_bytes(int64_t rows, int64_t K, int64_t R) {
+    if (rows <= 0 || K <= 0 || R <= 0 || rows > kMaxLoraRows || K > kMaxLoraK || R > kMaxRank) return 0;
+    return phi_dev::lora_batched_workspace(rows, K, R);
 }
 
 }  // extern "C"

@@ -3,7 +3,8 @@
 
 ``rotary`` turns vectors by their positions, ``rotary_cache_write`` does so on
 a projection's way into the paged cache, ``kv_cache_copy`` copies pages of it,
-as ``KvPages`` says when sequences fork or pages move together.
+as ``KvPages`` says when sequences fork or pages move together,
+``lora_batched`` adds each request's own adapter to a linear's output.
 """
 from __future__ import annotations
 
@@ -12,7 +13,7 @@ import math
 
 import torch
 
-from . import _check, _dt, _ptr, _stream, load
+from . import _check, _dt, _ptr, _stream, _ws, load
 from .decoder import KvCache, _empty, _vectors
 
 
@@ -233,3 +234,51 @@ class KvPages:
             part = torch.tensor(now, dtype=torch.int32).t().contiguous().to(cache.k.device)
             kv_cache_copy(cache, cache, part[0], part[1], tokens=part[2])
             left = later
+
+
+def lora_batched_workspace(rows: int, K: int, R: int, device) -> torch.Tensor:
+    """A buffer of phi_hip_lora_batched_workspace_bytes bytes."""
+    return torch.empty(load().phi_hip_lora_batched_workspace_bytes(rows, K, R), dtype=torch.uint8, device=device)
+
+
+def _pitch(name: str, t: torch.Tensor, shape) -> int:
+    """The pitch of a [rows, columns] tensor with contiguous rows (of one row: any from the columns on)."""
+    if t.shape != shape or (t.stride(1) != 1 and shape[1] > 1):
+        raise ValueError(f"lora_batched: {name} is {tuple(t.shape)}, not {tuple(shape)} with contiguous rows")
+    return t.stride(0) if shape[0] > 1 else max(t.stride(0), shape[1])
+
+
+def lora_batched(x: torch.Tensor, A: torch.Tensor, B: torch.Tensor, adapter: torch.Tensor, *,
+                 scale: torch.Tensor | None = None, base: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                 out_dtype=None, workspace: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """base + scale[a] B[a] (A[a] x) for rows of x [rows, K], a the row's adapter
+    [rows] int32 (below 0 or not below the adapters: none; phi_hip_lora_batched).
+    A [adapters, R, K] and B [adapters, N, R] of one dtype, scale [adapters] f32
+    (None: 1), base [rows, N] the linear's output (None: 0); out may be base.  out
+    has base's dtype, or out_dtype (x's if neither is given).  All f32/bf16."""
+    _here("lora_batched", stream, x, A, B, adapter, scale, base, out, workspace)
+    M, K = x.shape
+    if A.dim() != 3 or B.dim() != 3 or A.dtype != B.dtype:
+        raise ValueError("lora_batched: A is [adapters, R, K] and B [adapters, N, R], of one dtype")
+    n, R, N = A.shape[0], A.shape[1], B.shape[1]
+    ast, bst = A.stride(), B.stride()
+    if A.shape[2] != K or B.shape[0] != n or B.shape[2] != R or (K > 1 and ast[2] != 1) or (R > 1 and bst[2] != 1):
+        raise ValueError(f"lora_batched: factors of {tuple(A.shape)} and {tuple(B.shape)} for rows of {K}, last dimension contiguous")
+    if adapter.dtype != torch.int32 or adapter.shape != (M,) or not adapter.is_contiguous():
+        raise ValueError("lora_batched: adapter is contiguous int32 [rows]")
+    if scale is not None and (scale.dtype != torch.float32 or scale.shape != (n,) or not scale.is_contiguous()):
+        raise ValueError("lora_batched: scale is contiguous f32 [adapters]")
+    shape = (M, N)
+    if out is None:
+        out = _empty(shape, out_dtype or (x if base is None else base).dtype, x, stream)
+    if (base is not None and base.dtype != out.dtype) or (out_dtype is not None and out.dtype != out_dtype):
+        raise ValueError("lora_batched: base and out differ in dtype")
+    L = load()
+    if workspace is None:
+        workspace = _empty((L.phi_hip_lora_batched_workspace_bytes(M, K, R),), torch.uint8, x, stream)
+    wp, wn = _ws(workspace)
+    _check(L.phi_hip_lora_batched(
+        _stream(stream), x.data_ptr(), _dt(x), _pitch("x", x, (M, K)), M, K, A.data_ptr(), ast[0], ast[1] if R > 1 else max(ast[1], K),
+        B.data_ptr(), bst[0], bst[1] if N > 1 else max(bst[1], R), _dt(A), n, R, N, adapter.data_ptr(), _ptr(scale), _ptr(base),
+        0 if base is None else _pitch("base", base, shape), out.data_ptr(), _dt(out), _pitch("out", out, shape), wp, wn))
+    return out

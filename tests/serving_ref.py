@@ -16,3 +16,19 @@ def rotated(x, positions, freq, interleaved, scale):
     y[..., i], y[..., k] = a * cos - b * sin, b * cos + a * sin
     mag[..., i] = mag[..., k] = abs(scale) * (a.abs() + b.abs())
     return y, mag
+
+
+def adapted(x, A, B, adapter, scale, base):
+    """base + scale B (A x) of each row's adapter in 64 bits and, beside each value,
+    the sum of its terms' magnitudes through both products (0: none)."""
+    n, R, K = A.shape
+    M, N = x.shape[0], B.shape[1]
+    y = torch.zeros((M, N), dtype=torch.float64) if base is None else base.double()
+    mag = torch.zeros((M, N), dtype=torch.float64)
+    for a in range(n):
+        mine = adapter == a
+        s = 1.0 if scale is None else scale[a].double()
+        xa, Aa, Ba = x[mine].double(), A[a].double(), B[a].double()
+        y[mine] += (xa @ Aa.t()) @ Ba.t() * s
+        mag[mine] = (xa.abs() @ Aa.abs().t()) @ Ba.abs().t() * abs(s)
+    return y, mag

@@ -157,6 +157,68 @@ def test_copy_of_nothing(lib):
     assert copy(lib, far(), far(), frm=None, to=None, n=0) == 0 and Q.last_error() == ""
 
 
+def adapt(lib, x=A, xd=Q.BF16, ldx=512, rows=4, K=512, a=B, aa=16 * 512, ar=512, b=C, ba=256 * 16, br=16, wd=Q.BF16, n=3, rank=16, N=256,
+          adapter=D, scale=E, base=F, ldb=256, out=G, od=Q.BF16, ldo=256, ws=ctypes.c_void_p(8 << 28), wn=1 << 20):
+    return lib.phi_hip_lora_batched(None, x, xd, ldx, rows, K, a, aa, ar, b, ba, br, wd, n, rank, N, adapter, scale, base, ldb, out, od,
+                                    ldo, ws, wn)
+
+
+@pytest.mark.parametrize("rc,text,kw", [
+    (2, "negative", dict(rows=-1)),
+    (2, "negative", dict(rank=-1)),
+    (2, "negative", dict(n=-1)),
+    (1, "dtypes", dict(xd=Q.F16)),
+    (1, "dtypes", dict(wd=Q.I8)),
+    (1, "dtypes", dict(od=Q.I32)),
+    (2, "empty factors", dict(K=0)),
+    (2, "empty factors", dict(rank=0)),
+    (2, "empty factors", dict(n=0)),
+    (7, "exceeds", dict(rank=257, br=257)),
+    (2, "out of range", dict(rows=(1 << 24) + 1)),
+    (2, "out of range", dict(N=(1 << 24) + 1, ldo=1 << 25, ldb=1 << 25)),
+    (2, "out of range", dict(n=1 << 31)),
+    (1, "null", dict(x=None)),
+    (1, "null", dict(a=None)),
+    (1, "null", dict(b=None)),
+    (1, "null", dict(adapter=None)),
+    (1, "null", dict(out=None)),
+    (2, "leading", dict(ldx=511)),
+    (2, "leading", dict(ldo=255)),
+    (2, "leading", dict(ldb=255)),
+    (2, "leading", dict(ar=511)),
+    (2, "leading", dict(br=15)),
+    (2, "too large", dict(ldx=1 << 30)),
+    (2, "adapter stride", dict(aa=-1)),
+    (2, "adapter stride", dict(ba=1 << 41)),
+    (3, "aligned", dict(x=ODD)),
+    (3, "aligned", dict(out=ODD)),
+    (3, "aligned", dict(adapter=ctypes.c_void_p((4 << 28) + 2))),
+    (3, "aligned", dict(scale=ctypes.c_void_p((5 << 28) + 2))),
+    (4, "workspace", dict(ws=None)),
+    (4, "workspace", dict(wn=100)),
+    (3, "workspace", dict(ws=ctypes.c_void_p((8 << 28) + 8))),
+    (1, "out overlaps an input", dict(out=ctypes.c_void_p((1 << 28) + 64))),
+    (1, "out overlaps an input", dict(out=ctypes.c_void_p((2 << 28) + 2 * 16 * 512 * 2 - 64))),
+    (1, "out overlaps an input", dict(out=C)),
+    (1, "out overlaps an input", dict(adapter=G)),
+    (1, "out overlaps base", dict(out=ctypes.c_void_p((6 << 28) + 256))),
+    (1, "out overlaps base", dict(out=F, ldo=512)),
+    (1, "workspace overlaps", dict(ws=F)),
+    (1, "workspace overlaps", dict(ws=G)),
+    (1, "workspace overlaps", dict(ws=A)),
+])
+def test_adapters_refuse(lib, rc, text, kw):
+    assert adapt(lib, **kw) == rc and text in Q.last_error() and "lora_batched" in Q.last_error()
+
+
+def test_adapters_of_nothing(lib):
+    for kw in (dict(rows=0), dict(N=0)):
+        assert adapt(lib, x=None, out=None, ws=None, **kw) == 0 and Q.last_error() == ""
+    size = lib.phi_hip_lora_batched_workspace_bytes
+    assert size(0, 5, 5) == size(5, 0, 5) == size(5, 5, 0) == size(5, 5, 257) == size(1 << 25, 5, 5) == 0
+    assert size(1, 1, 1) >= 4 and size(1000, 4096, 16) >= 1000 * 16 * 4
+
+
 def test_python_refusals():
     t = torch.zeros((2, 3, 64))
     with pytest.raises(ValueError, match="device"):
