@@ -8,6 +8,7 @@
  *   phi_hip_rotary_cache_write   the same of a projection's q and k, with k and v
  *                                quantised into the paged cache
  *   phi_hip_kv_cache_copy        pages of a cache copied (forked sequences, compaction)
+ *   phi_hip_paged_attention_shared  attention of sequences that share prefixes
  *   phi_hip_lora_batched         a linear's output plus each row's own low-rank adapter
  *
  * The reference rotates pairs of half a head's distance on fp32 tensors
@@ -75,6 +76,45 @@ phi_status phi_hip_rotary_cache_write(phi_stream_t stream, const phi_kv_cache* c
 phi_status phi_hip_kv_cache_copy(phi_stream_t stream, const phi_kv_cache* from, const phi_kv_cache* to,
                                  const int32_t* from_blocks, const int32_t* to_blocks, const int32_t* tokens,
                                  int64_t n);
+
+/*
+ * phi_hip_paged_attention (causal) for a batch whose sequences share prefixes, each
+ * prefix read once for all rows that see it.  Group g's prefix, prefix_len[g] tokens in the blocks
+ * prefix_table[g][0..], comes before the own tokens of the sequences
+ * group_start[g] .. group_start[g+1] - 1: all of their rows see all of it.  A
+ * sequence's own tokens, kv_len[b] with the new ones last, lie in the blocks
+ * block_table[b][0..], from the first block's first place on; of these its row i sees
+ * t <= kv_len[b] - n + i.  With n = q_start[b+1] - q_start[b],
+ *   out = sum softmax(scale * q . k) v   over both, one softmax.
+ * A row that sees nothing gives zeros.
+ *
+ *   groups       from 1 to 65535; group_start [groups + 1] int32, ascending from 0 on
+ *                to at most batch: sequences before the first group's or past the last's
+ *                have no prefix
+ *   prefix_table [groups, prefix_stride] int32, `prefix_width` entries a row, as block_table
+ *   prefix_len   [groups] int32; max_prefix at least the longest, at most
+ *                prefix_width * page and 2^30: tokens past it are not seen
+ *   tokens       at most 2^30 times key/value heads over query heads
+ *   workspace    phi_hip_paged_attention_shared_workspace_bytes() bytes, 16-byte aligned
+ * All else as phi_hip_paged_attention, its arithmetic too, a group's rows over their
+ * prefix being one sequence of it; the parts are joined in fp32.  Lengths, starts and
+ * tables are read on the device, so a captured graph serves growing sequences and
+ * other groups.
+ */
+phi_status phi_hip_paged_attention_shared(phi_stream_t stream, const void* q, int dtype, int64_t q_token_stride,
+                                          int64_t q_head_stride, int64_t tokens, int64_t q_heads,
+                                          const phi_kv_cache* cache, const int32_t* prefix_table,
+                                          int64_t prefix_width, int64_t prefix_stride, const int32_t* prefix_len,
+                                          const int32_t* group_start, int64_t groups, int64_t max_prefix,
+                                          const int32_t* block_table, int64_t table_width, int64_t table_stride,
+                                          const int32_t* q_start, const int32_t* kv_len, int64_t batch, int64_t max_q,
+                                          int64_t max_kv, float scale, void* out, int64_t out_token_stride,
+                                          int64_t out_head_stride, void* workspace, size_t ws_bytes);
+
+/* Workspace of phi_hip_paged_attention_shared (0 for sizes that no call may have). */
+size_t phi_hip_paged_attention_shared_workspace_bytes(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t dim,
+                                                      int64_t groups, int64_t batch, int64_t max_prefix,
+                                                      int64_t max_q, int64_t max_kv, int dtype);
 
 /*
  * Low-rank adapters of many requests beside one linear:

@@ -69,9 +69,23 @@ struct PagedAttn {
     int few_rows;  // see paged_attention.hpp
     float scale;
     bool bf16, causal;
+    // Prefixes that sequences group_start[g] .. group_start[g + 1] - 1 share (groups 0:
+    // none).  With them `batch` counts groups, first, and sequences, `max_q` bounds a
+    // group's rows, and own_q and max_kv a sequence's; prefix_at: prefix tables from
+    // `table` on, in elements.
+    const int32_t* prefix_len;
+    const int32_t* group_start;
+    int64_t prefix_at, prefix_stride;
+    int groups, max_prefix, prefix_width, own_q;
+    struct AttnRow* own_rows;
+    struct AttnRow* prefix_rows;
 };
 hipError_t launch_paged_attention(hipStream_t stream, const KvCache& c, const PagedAttn& p, void* workspace);
 size_t paged_attention_workspace(int64_t tokens, int q_heads, int kv_heads, int dim, int batch, int max_q, int max_kv,
                                  bool bf16);
+// p as a caller has it: batch, max_q of the sequences.
+hipError_t launch_paged_attention_shared(hipStream_t stream, const KvCache& c, const PagedAttn& p, void* workspace);
+size_t paged_attention_shared_workspace(int64_t tokens, int q_heads, int kv_heads, int dim, int groups, int batch, int max_prefix,
+                                        int max_q, int max_kv, bool bf16);
 
 }  // namespace phi_dev

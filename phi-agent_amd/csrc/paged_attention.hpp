@@ -38,15 +38,30 @@ struct SeqInfo {
     int pos0;      // position of its first new token (below 0: rows before any token)
 };
 
+// With shared prefixes a group's prefix is a sequence too, the groups' before the
+// batch's own: its rows are those of all its sequences, each past all of its tokens.
 __device__ __forceinline__ SeqInfo seq_info(const PagedAttn& p, int page, int b) {
     SeqInfo s;
-    const int64_t a = p.q_start[b], e = p.q_start[b + 1], T = p.tokens;
+    const bool prefix = b < p.groups;
+    int from = b - p.groups, to = from + 1;
+    if (prefix) {
+        const int batch = p.batch - p.groups;
+        from = min(max(p.group_start[b], 0), batch), to = min(max(p.group_start[b + 1], 0), batch);
+    }
+    const int64_t a = p.q_start[from], e = p.q_start[to], T = p.tokens;
     s.first = (int)(a < 0 ? 0 : a > T ? T : a);
     s.n = max(0, (int)(e < 0 ? 0 : e > T ? T : e) - s.first);
-    const int kv = max(0, p.kv_len[b]);
-    s.kv = (int)min((int64_t)min(kv, p.max_kv), (int64_t)p.table_width * page);
-    s.pos0 = kv - s.n;
+    const int kv = max(0, prefix ? p.prefix_len[b] : p.kv_len[from]);
+    s.kv = (int)min((int64_t)min(kv, prefix ? p.max_prefix : p.max_kv), (int64_t)(prefix ? p.prefix_width : p.table_width) * page);
+    s.pos0 = prefix ? s.kv : kv - s.n;
+    if (p.groups && !prefix) s.n = min(s.n, p.own_q);
     return s;
+}
+
+// A sequence's row of the block table; prefixes' lie prefix_at further on.
+__device__ __forceinline__ const int32_t* table_row(const PagedAttn& p, const int32_t* table, int b) {
+    const int64_t at = b < p.groups ? p.prefix_at + b * p.prefix_stride : (b - p.groups) * p.table_stride;
+    return table + at;
 }
 
 // A sequence's rows are the query heads of a key/value head x its new tokens, in
@@ -93,10 +108,28 @@ inline bool tiles_of_16(const KvCache& c) {
 // The work of block number `unit` of a part (the same in all lanes): row tile `tile`
 // of sequence b, tokens from z0 to z1, to be left in a slot (-1: there is no other
 // split, so written out).  b < 0: there are fewer.
+// Of its tile's `splits`, those but the last are in slots from `first` on.
 struct AttnUnit {
     int b, tile, slot, z0, z1;
     SeqInfo s;
+    int first, splits;
+    bool last;
 };
+
+// Where a row's partial results are: for shared prefixes the last split of a tile
+// leaves this for each of its rows, [tokens][group], a prefix's apart from an own
+// one's.  `id` (of the group or sequence) tells a row that nothing was left for.
+struct AttnRow {
+    int first, last;  // slots: from first on, splits - 1 of them, and last
+    uint32_t where;   // splits | row of the tile << 16 | chunk kernel's << 31
+    int id;
+};
+__device__ __forceinline__ void leave_row(const PagedAttn& p, const AttnUnit& u, int r, int in, bool many) {
+    const bool prefix = u.b < p.groups;
+    const int i = r / p.group;
+    (prefix ? p.prefix_rows : p.own_rows)[(int64_t)(u.s.first + i) * p.group + (r - i * p.group)] =
+        {u.first, u.slot, (uint32_t)u.splits | (uint32_t)in << 16 | (many ? 1u << 31 : 0u), prefix ? u.b : u.b - p.groups};
+}
 
 __device__ __forceinline__ SeqInfo seq_of_lane(const SeqInfo& q, int at) {
     return {__builtin_amdgcn_readlane(q.first, at), __builtin_amdgcn_readlane(q.n, at), __builtin_amdgcn_readlane(q.kv, at),
@@ -182,15 +215,17 @@ __device__ __forceinline__ AttnUnit attn_unit(const PagedAttn& p, const AttnPart
         const int local = unit - f.base;
         if (local >= f.blocks()) continue;
         const bool full = local < f.fulls();
-        const int off = full ? local : local - f.fulls(), begin = full ? f.full_end - f.tiles * (f.k - 1) : f.last;
+        const int full_begin = f.full_end - f.tiles * (f.k - 1);
+        const int off = full ? local : local - f.fulls(), begin = full ? full_begin : f.last;
         const int at = __builtin_ctzll(__ballot(begin <= off && off < (full ? f.full_end : begin + f.tiles)));
         const int k = __builtin_amdgcn_readlane(f.k, at), in = off - __builtin_amdgcn_readlane(begin, at);
         const int tile = full ? in / (k - 1) : in, z = full ? in - tile * (k - 1) : k - 1;
         const int z0 = (__builtin_amdgcn_readlane(f.first, at) + z * f.len) * s.step;
         // Late tiles first: they see most tokens.
-        return {f.b0 + at, __builtin_amdgcn_readlane(f.tiles, at) - 1 - tile, k > 1 ? unit : -1, z0, full ? z0 + f.len * s.step : INT_MAX, seq_of_lane(f.q, at)};
+        return {f.b0 + at, __builtin_amdgcn_readlane(f.tiles, at) - 1 - tile, k > 1 || p.groups ? unit : -1, z0, full ? z0 + f.len * s.step : INT_MAX, seq_of_lane(f.q, at),
+                f.base + __builtin_amdgcn_readlane(full_begin, at) + tile * (k - 1), k, !full};
     }
-    return {-1, 0, 0, 0, 0, {}};
+    return {-1, 0, 0, 0, 0, {}, 0, 0, false};
 }
 
 // The maximum over lanes l, l ^ 16, l ^ 32, l ^ 48, and over l, l ^ 32.

@@ -206,7 +206,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel
     const int begin = lo & ~(kTile - 1), count = begin < hi ? (hi - begin + kTile - 1) / kTile : 0;
     auto start = [&](int n) { return begin + n * kTile; };
     const int group = wave & 3, n16 = lane & 15;
-    const int32_t* trow = table + (int64_t)b * p.table_stride;
+    const int32_t* trow = table_row(p, table, b);
     const int last_page = page_of(c, max(hi - 1, 0));
     struct Raw {
         uint32_t w[8 * NVI > 4 * NKI ? 8 * NVI : 4 * NKI];  // V's items' 8 words, K's items' 4
@@ -599,6 +599,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel
     const int64_t at = ((int64_t)kh * sp.slots + unit_of.slot) * (32 * NW) + 32 * wave + col;
     // O holds sum p v in units of 2^(kP + kM - 9 - vexp), l of 2^kP.
     const float unit = pow2(vexp + 9 - kM), share = split ? 1.0f / (1 << kP) : l != 0.0f ? 1.0f / l : 0.0f;
+    if (p.groups && unit_of.last && kh == 0 && h == 0) leave_row(p, unit_of, w0 + col, 32 * wave + col, true);
     if (split && h == 0) sp.ml[2 * at] = m, sp.ml[2 * at + 1] = l * (1.0f / (1 << kP));
     // Value n, j is of slot 32 n + 8 (j / 4) + 4 h + j % 4, so d = 4 (slot % (DP/4))
     // + slot / (DP/4): the four d of a slot % (DP/4) together.

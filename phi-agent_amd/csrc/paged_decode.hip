@@ -86,7 +86,7 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void paged_decode_k
     int kd[KS];
 #pragma unroll
     for (int ks = 0; ks < KS; ks++) kd[ks] = 64 * ks + 16 * g < D ? 64 * ks + 16 * g : 0;
-    const int32_t* trow = table + (int64_t)b * p.table_stride;
+    const int32_t* trow = table_row(p, table, b);
     const int last_page = page_of(c, max(hi - 1, 0));
 
     // The table's entries of a step's tiles (a lane's token's), fetched a step
@@ -316,6 +316,7 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void paged_decode_k
     const int64_t at = ((int64_t)kh * sp.slots + slot) * kDecodeRows + row;
     const float div = slot >= 0 ? 1.0f : rl != 0.0f ? 1.0f / rl : 0.0f;
     if (slot >= 0 && part == 0) sp.ml[2 * at] = rm, sp.ml[2 * at + 1] = rl;
+    if (p.groups && unit.last && kh == 0 && part == 0) leave_row(p, unit, r0 + row, row, false);
 #pragma unroll
     for (int q4 = 0; q4 < DP / 64; q4++) {
         const int d = 4 * (part + 16 * q4);

@@ -129,6 +129,73 @@ phi_status phi_hip_kv_cache_copy(phi_stream_t stream, const phi_kv_cache* from, 
     return check_hip(phi_dev::launch_kv_cache_copy((hipStream_t)stream, p), who);
 }
 
+phi_status phi_hip_paged_attention_shared(phi_stream_t stream, const void* q, int dtype, int64_t q_token_stride,
+                                          int64_t q_head_stride, int64_t tokens, int64_t q_heads,
+                                          const phi_kv_cache* cache, const int32_t* prefix_table,
+                                          int64_t prefix_width, int64_t prefix_stride, const int32_t* prefix_len,
+                                          const int32_t* group_start, int64_t groups, int64_t max_prefix,
+                                          const int32_t* block_table, int64_t table_width, int64_t table_stride,
+                                          const int32_t* q_start, const int32_t* kv_len, int64_t batch, int64_t max_q,
+                                          int64_t max_kv, float scale, void* out, int64_t out_token_stride,
+                                          int64_t out_head_stride, void* workspace, size_t ws_bytes) {
+    static const char* who = "paged_attention_shared";
+    if (device_lost()) return fail(PHI_ERR_DEVICE_LOST, "%s: device was lost earlier", who);
+    phi_dev::KvCache c;
+    phi_status st = check_cache(who, cache, &c);
+    if (st != PHI_OK) return st;
+    if (tokens < 0 || groups < 0 || batch < 0 || max_q < 0 || max_kv < 0 || max_prefix < 0 || table_width < 0 || prefix_width < 0)
+        return fail(PHI_ERR_SHAPE, "%s: negative size", who);
+    if (!is_float(dtype)) return fail(PHI_ERR_ARG, "%s: q must be f32 or bf16", who);
+    if (q_heads <= 0 || q_heads % c.heads != 0 || q_heads > 65535)
+        return fail(PHI_ERR_SHAPE, "%s: %lld query heads for %d key/value heads", who, (long long)q_heads, c.heads);
+    if (tokens == 0 || batch == 0 || max_q == 0) return ok();
+    if (tokens > INT32_MAX || batch > 65535 || groups > 65535 || max_q > tokens || max_kv > kMaxKv || max_prefix > kMaxKv)
+        return fail(PHI_ERR_SHAPE, "%s: tokens=%lld groups=%lld batch=%lld max_prefix=%lld max_q=%lld max_kv=%lld out of range", who, (long long)tokens,
+                    (long long)groups, (long long)batch, (long long)max_prefix, (long long)max_q, (long long)max_kv);
+    if (tokens * (q_heads / c.heads) > kMaxRows)
+        return fail(PHI_ERR_SHAPE, "%s: tokens=%lld at %lld query heads a key/value head is out of range", who, (long long)tokens, (long long)(q_heads / c.heads));
+    if (groups == 0) return fail(PHI_ERR_SHAPE, "%s: no groups", who);
+    if (max_kv > 0 && (table_width > INT32_MAX || max_kv > table_width * c.page))
+        return fail(PHI_ERR_SHAPE, "%s: max_kv=%lld exceeds the block table's %lld x %d tokens", who, (long long)max_kv, (long long)table_width, c.page);
+    if (max_prefix > 0 && (prefix_width > INT32_MAX || max_prefix > prefix_width * c.page))
+        return fail(PHI_ERR_SHAPE, "%s: max_prefix=%lld exceeds the prefix table's %lld x %d tokens", who, (long long)max_prefix, (long long)prefix_width, c.page);
+    if (table_stride < table_width || table_stride > kMaxStride || prefix_stride < prefix_width || prefix_stride > kMaxStride)
+        return fail(PHI_ERR_SHAPE, "%s: a table's stride is smaller than its row", who);
+    if (!std::isfinite(scale)) return fail(PHI_ERR_ARG, "%s: scale must be finite", who);
+    st = check_vectors(who, "q", q, dtype, q_token_stride, q_head_stride);
+    if (st == PHI_OK) st = check_vectors(who, "out", out, dtype, out_token_stride, out_head_stride);
+    if (st == PHI_OK) st = check_layout(who, "out", tokens, out_token_stride, q_heads, out_head_stride, c.dim);
+    if (st != PHI_OK) return st;
+    if ((max_kv > 0 && !block_table) || (max_prefix > 0 && !prefix_table) || !prefix_len || !group_start || !q_start || !kv_len)
+        return fail(PHI_ERR_ARG, "%s: null pointer", who);
+    if (!aligned(block_table, 4) || !aligned(prefix_table, 4) || !aligned(prefix_len, 4) || !aligned(group_start, 4) || !aligned(q_start, 4) || !aligned(kv_len, 4))
+        return fail(PHI_ERR_ALIGN, "%s: a table, lengths or starts are misaligned", who);
+    const Pieces qs = vectors_of(q, tokens, q_token_stride, q_heads, q_head_stride, c.dim, elem(dtype));
+    const Pieces os = vectors_of(out, tokens, out_token_stride, q_heads, out_head_stride, c.dim, elem(dtype));
+    if (meet(qs, os)) return fail(PHI_ERR_ARG, "%s: out overlaps q", who);
+    const size_t need = phi_hip_paged_attention_shared_workspace_bytes(tokens, q_heads, c.heads, c.dim, groups, batch, max_prefix, max_q, max_kv, dtype);
+    if (!workspace || ws_bytes < need)
+        return fail(PHI_ERR_WORKSPACE, "%s: needs %zu bytes of workspace, got %zu", who, need, workspace ? ws_bytes : (size_t)0);
+    if (!aligned(workspace, 16)) return fail(PHI_ERR_ALIGN, "%s: the workspace must be 16-byte aligned", who);
+    const Pieces ws{workspace, (int64_t)need};
+    if (meet(ws, qs) || meet(ws, os)) return fail(PHI_ERR_ARG, "%s: the workspace overlaps q or out", who);
+    phi_dev::PagedAttn p{q, out, block_table, q_start, kv_len, q_token_stride, q_head_stride, out_token_stride, out_head_stride, table_stride,
+                         tokens, (int)q_heads, (int)(q_heads / c.heads), (int)batch, (int)max_q, (int)max_kv, (int)table_width, 0, 0, scale,
+                         dtype == PHI_BF16, true, prefix_len, group_start, ((int64_t)(uintptr_t)prefix_table - (int64_t)(uintptr_t)block_table) / 4, prefix_stride, (int)groups,
+                         (int)max_prefix, (int)prefix_width, (int)max_q, nullptr, nullptr};
+    return check_hip(phi_dev::launch_paged_attention_shared((hipStream_t)stream, c, p, workspace), who);
+}
+
+size_t phi_hip_paged_attention_shared_workspace_bytes(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t dim,
+                                                      int64_t groups, int64_t batch, int64_t max_prefix,
+                                                      int64_t max_q, int64_t max_kv, int dtype) {
+    if (tokens <= 0 || q_heads <= 0 || kv_heads <= 0 || dim <= 0 || groups <= 0 || batch <= 0 || max_q <= 0 || max_kv < 0 || max_prefix < 0) return 0;
+    if (tokens > INT32_MAX || q_heads > 65535 || dim > 256 || groups > 65535 || batch > 65535 || max_q > tokens || max_kv > kMaxKv || max_prefix > kMaxKv) return 0;
+    if (q_heads % kv_heads != 0 || tokens * (q_heads / kv_heads) > kMaxRows) return 0;
+    return phi_dev::paged_attention_shared_workspace(tokens, (int)q_heads, (int)kv_heads, (int)dim, (int)groups, (int)batch, (int)max_prefix, (int)max_q,
+                                                     (int)max_kv, dtype == PHI_BF16);
+}
+
 phi_status phi_hip_lora_batched(phi_stream_t stream, const void* x, int x_dtype, int64_t ldx, int64_t rows, int64_t K,
                                 const void* A, int64_t a_adapter_stride, int64_t a_row_stride, const void* B,
                                 int64_t b_adapter_stride, int64_t b_row_stride, int w_dtype, int64_t adapters,

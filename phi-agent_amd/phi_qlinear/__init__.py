@@ -92,7 +92,8 @@ EXPORTS = ["phi_hip_last_error", "phi_hip_abi_version", "phi_hip_quant_rotate", 
            "phi_hip_gemm_plan_clear", "phi_hip_gemm_is_small", "phi_hip_w4a8_banded_bytes", "phi_hip_w4a8_pack_banded",
            "phi_hip_w4a8_linear_banded", "phi_hip_rms_norm_quant", "phi_hip_kv_cache_write", "phi_hip_kv_cache_read",
            "phi_hip_paged_attention", "phi_hip_paged_attention_workspace_bytes", "phi_hip_rotary",
-           "phi_hip_rotary_cache_write", "phi_hip_kv_cache_copy", "phi_hip_lora_batched", "phi_hip_lora_batched_workspace_bytes"]
+           "phi_hip_rotary_cache_write", "phi_hip_kv_cache_copy", "phi_hip_lora_batched", "phi_hip_lora_batched_workspace_bytes",
+           "phi_hip_paged_attention_shared", "phi_hip_paged_attention_shared_workspace_bytes"]
 
 _lib = None
 
@@ -174,6 +175,10 @@ def load() -> ctypes.CDLL:
     L.phi_hip_rotary_cache_write.argtypes = [P, KV, P, I64, I64, I64, P, I64, I64, P, I64, I64, P, I64, I64, I, P, P, I64, I,
                                              F, P, I64]
     L.phi_hip_kv_cache_copy.argtypes = [P, KV, KV, P, P, P, I64]
+    L.phi_hip_paged_attention_shared.argtypes = [P, P, I, I64, I64, I64, I64, KV, P, I64, I64, P, P, I64, I64, P, I64, I64, P, P,
+                                                 I64, I64, I64, F, P, I64, I64, P, SZ]
+    L.phi_hip_paged_attention_shared_workspace_bytes.argtypes = [I64] * 9 + [I]
+    L.phi_hip_paged_attention_shared_workspace_bytes.restype = SZ
     L.phi_hip_lora_batched.argtypes = [P, P, I, I64, I64, I64, P, I64, I64, P, I64, I64, I, I64, I64, I64, P, P, P, I64, P, I,
                                        I64, P, SZ]
     L.phi_hip_lora_batched_workspace_bytes.argtypes = [I64, I64, I64]
@@ -766,5 +771,5 @@ def q8_linear_kt(x: torch.Tensor, Wkt: torch.Tensor, N: int, sW: torch.Tensor,
 
 from .decoder import (KvCache, kv_cache_empty, kv_cache_read, kv_cache_write, paged_attention,  # noqa: E402,F401
                       paged_attention_workspace, rms_norm_quant)
-from .serving import (KvPages, kv_cache_copy, lora_batched, lora_batched_workspace, rotary, rotary_cache_write,
-                      rotary_frequencies)  # noqa: E402,F401
+from .serving import (KvPages, kv_cache_copy, lora_batched, lora_batched_workspace, paged_attention_shared,
+                      paged_attention_shared_workspace, rotary, rotary_cache_write, rotary_frequencies)  # noqa: E402,F401

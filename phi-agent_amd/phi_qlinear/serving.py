@@ -4,6 +4,7 @@
 ``rotary`` turns vectors by their positions, ``rotary_cache_write`` does so on
 a projection's way into the paged cache, ``kv_cache_copy`` copies pages of it,
 as ``KvPages`` says when sequences fork or pages move together,
+``paged_attention_shared`` attends over prefixes that sequences share and their own tokens,
 ``lora_batched`` adds each request's own adapter to a linear's output.
 """
 from __future__ import annotations
@@ -13,7 +14,7 @@ import math
 
 import torch
 
-from . import _check, _dt, _ptr, _stream, _ws, load
+from . import _DTYPES, _check, _dt, _ptr, _stream, _ws, load
 from .decoder import KvCache, _empty, _vectors
 
 
@@ -234,6 +235,64 @@ class KvPages:
             part = torch.tensor(now, dtype=torch.int32).t().contiguous().to(cache.k.device)
             kv_cache_copy(cache, cache, part[0], part[1], tokens=part[2])
             left = later
+
+
+def paged_attention_shared_workspace(tokens: int, q_heads: int, kv_heads: int, dim: int, groups: int, batch: int, max_prefix: int,
+                                     max_q: int, max_kv: int, dtype: torch.dtype, device) -> torch.Tensor:
+    """A buffer of phi_hip_paged_attention_shared_workspace_bytes bytes."""
+    n = load().phi_hip_paged_attention_shared_workspace_bytes(tokens, q_heads, kv_heads, dim, groups, batch, max_prefix, max_q,
+                                                              max_kv, _DTYPES[dtype])
+    return torch.empty(n, dtype=torch.uint8, device=device)
+
+
+def _table(name: str, t: torch.Tensor, rows: int) -> int:
+    """The pitch of a table [rows, width] int32 with contiguous rows."""
+    pitch, step = t.stride()
+    if t.dtype != torch.int32 or t.shape[0] != rows or (step != 1 and t.shape[1] > 1):
+        raise ValueError(f"paged_attention_shared: {name} is [{rows}, width] int32 with contiguous rows")
+    return pitch if rows > 1 else t.shape[1]
+
+
+def paged_attention_shared(q: torch.Tensor, cache: KvCache, prefix_table: torch.Tensor, prefix_len: torch.Tensor,
+                           group_start: torch.Tensor, block_table: torch.Tensor, q_start: torch.Tensor,
+                           kv_len: torch.Tensor, *, max_prefix: int, max_q: int, max_kv: int, scale: float | None = None,
+                           out: torch.Tensor | None = None, workspace: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """Causal attention of new tokens q [tokens, q_heads, dim] (bf16/f32) over
+    prefixes that sequences share and their own tokens
+    (phi_hip_paged_attention_shared).  Sequences group_start[g] ..
+    group_start[g + 1] - 1 see prefix_len[g] tokens in blocks prefix_table[g],
+    then their own as by `paged_attention`: kv_len[b] in blocks block_table[b],
+    the last of them rows q_start[b] .. q_start[b + 1] - 1 of q.  All int32;
+    max_prefix, max_q and max_kv bound a prefix, the new tokens and the own tokens
+    of any sequence.  scale: dim ** -0.5 if not given."""
+    who = "paged_attention_shared"
+    _here(who, stream, q, cache.k, prefix_table, prefix_len, group_start, block_table, q_start, kv_len, out, workspace)
+    shape = q.shape
+    T, Hq, D = shape
+    G, B, i32 = prefix_len.numel(), kv_len.numel(), torch.int32
+    if D != cache._dim:
+        raise ValueError(f"{who}: q is {tuple(shape)}, the cache's vectors have {cache._dim} elements")
+    qt, qh = _vectors(who, "q", q, shape)
+    for name, t, n in (("prefix_len", prefix_len, G), ("group_start", group_start, G + 1), ("q_start", q_start, B + 1), ("kv_len", kv_len, B)):
+        if t.dtype != i32 or t.shape != (n,) or not t.is_contiguous():
+            raise ValueError(f"{who}: {name} is contiguous int32 [{n}]")
+    prefix_pitch, pitch = _table("prefix_table", prefix_table, G), _table("block_table", block_table, B)
+    if out is None:
+        out, ot, oh = _empty(shape, q.dtype, q, stream), Hq * D, D
+    else:
+        ot, oh = _vectors(who, "out", out, shape)
+        if out.dtype != q.dtype:
+            raise ValueError(f"{who}: out and q differ in dtype")
+    L, dt = load(), _dt(q)
+    if workspace is None:
+        wn = L.phi_hip_paged_attention_shared_workspace_bytes(T, Hq, cache._heads, D, G, B, max_prefix, max_q, max_kv, dt)
+        workspace = _empty((wn,), torch.uint8, q, stream)
+    wp, wn = _ws(workspace)
+    _check(L.phi_hip_paged_attention_shared(
+        _stream(stream), q.data_ptr(), dt, qt, qh, T, Hq, cache._desc, prefix_table.data_ptr(), prefix_table.shape[1], prefix_pitch,
+        prefix_len.data_ptr(), group_start.data_ptr(), G, max_prefix, block_table.data_ptr(), block_table.shape[1], pitch,
+        q_start.data_ptr(), kv_len.data_ptr(), B, max_q, max_kv, D ** -0.5 if scale is None else scale, out.data_ptr(), ot, oh, wp, wn))
+    return out
 
 
 def lora_batched_workspace(rows: int, K: int, R: int, device) -> torch.Tensor:

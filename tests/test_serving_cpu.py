@@ -219,6 +219,71 @@ def test_adapters_of_nothing(lib):
     assert size(1, 1, 1) >= 4 and size(1000, 4096, 16) >= 1000 * 16 * 4
 
 
+H = ctypes.c_void_p(8 << 28)
+
+
+def shared(lib, c, q=A, dtype=Q.BF16, qt=256, qh=64, tokens=8, heads=4, ptable=B, pwidth=6, pstride=6, plen=C, first=D, groups=2, max_prefix=96,
+           table=E, width=4, stride=4, start=F, lens=F, batch=3, max_q=4, max_kv=64, scale=0.1, out=G, ot=256, oh=64, ws=H, wn=1 << 28):
+    return lib.phi_hip_paged_attention_shared(None, q, dtype, qt, qh, tokens, heads, ctypes.byref(c) if c else None, ptable, pwidth, pstride, plen,
+                                              first, groups, max_prefix, table, width, stride, start, lens, batch, max_q, max_kv, scale, out, ot, oh,
+                                              ws, wn)
+
+
+@pytest.mark.parametrize("rc,text,kw", [
+    (2, "negative", dict(tokens=-1)),
+    (2, "negative", dict(groups=-1)),
+    (2, "negative", dict(max_prefix=-1)),
+    (1, "f32 or bf16", dict(dtype=Q.F16)),
+    (2, "5 query heads for 2", dict(heads=5)),
+    (2, "out of range", dict(max_q=9)),
+    (2, "out of range", dict(batch=70000)),
+    (2, "out of range", dict(groups=70000)),
+    (2, "out of range", dict(max_prefix=(1 << 30) + 1)),
+    (2, "out of range", dict(tokens=(1 << 29) + 1)),
+    (2, "no groups", dict(groups=0)),
+    (2, "block table", dict(max_kv=65)),
+    (2, "prefix table", dict(max_prefix=97)),
+    (2, "stride", dict(stride=3)),
+    (2, "stride", dict(pstride=5)),
+    (1, "scale", dict(scale=math.inf)),
+    (1, "null q", dict(q=None)),
+    (1, "null out", dict(out=None)),
+    (1, "null pointer", dict(table=None)),
+    (1, "null pointer", dict(ptable=None)),
+    (1, "null pointer", dict(plen=None)),
+    (1, "null pointer", dict(first=None)),
+    (1, "null pointer", dict(start=None)),
+    (1, "null pointer", dict(lens=None)),
+    (3, "aligned", dict(qt=257)),
+    (3, "misaligned", dict(plen=ODD)),
+    (3, "misaligned", dict(ptable=ODD)),
+    (2, "vectors overlap", dict(ot=128)),
+    (1, "out overlaps q", dict(out=ctypes.c_void_p((1 << 28) + 1024))),
+    (4, "workspace", dict(ws=None)),
+    (4, "workspace", dict(wn=64)),
+    (3, "workspace", dict(ws=ctypes.c_void_p((8 << 28) + 8))),
+    (1, "workspace overlaps", dict(ws=A)),
+    (1, "workspace overlaps", dict(ws=G)),
+])
+def test_shared_attention_refuses(lib, rc, text, kw):
+    assert shared(lib, far(), **kw) == rc and text in Q.last_error() and "paged_attention_shared" in Q.last_error()
+
+
+@pytest.mark.parametrize("rc,text,kw", BAD_CACHES)
+def test_shared_attention_of_bad_caches(lib, rc, text, kw):
+    assert shared(lib, cache(**kw)) == rc and text in Q.last_error()
+
+
+def test_shared_attention_of_nothing(lib):
+    for kw in (dict(tokens=0), dict(batch=0), dict(max_q=0)):
+        assert shared(lib, far(), q=None, out=None, ws=None, **kw) == 0 and Q.last_error() == ""
+    size = lib.phi_hip_paged_attention_shared_workspace_bytes
+    for bad in ((0, 4, 2, 64, 1, 1, 10, 1, 10), (8, 5, 2, 64, 1, 1, 10, 1, 10), (8, 4, 2, 64, 0, 1, 10, 1, 10), (8, 4, 2, 64, 1, 1, 10, 9, 10),
+                (8, 4, 2, 64, 1, 70000, 10, 1, 10)):
+        assert size(*bad, Q.BF16) == 0
+    assert size(8, 4, 2, 64, 1, 8, 10, 1, 0, Q.BF16) > 0
+
+
 def test_python_refusals():
     t = torch.zeros((2, 3, 64))
     with pytest.raises(ValueError, match="device"):
