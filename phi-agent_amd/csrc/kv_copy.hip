@@ -10,7 +10,7 @@ namespace phi_dev {
 
 namespace {
 
-constexpr int kPieces = 8;
+constexpr int kPieces = 4;
 
 // n / d as (n * mul) >> shift for 0 <= n < 2^31.
 struct Div {
@@ -28,7 +28,7 @@ __device__ __forceinline__ uint32_t quotient(const Div& d, uint32_t n) { return 
 
 // inner, outer: the smaller stride's and the larger's counts of a page's vectors;
 // token_inner: the inner are tokens.
-__global__ __launch_bounds__(256) void kv_copy_kernel(KvCopy p, Div vector, Div inner, bool token_inner, int code_parts, int scale_parts) {
+__global__ __launch_bounds__(256, 8) void kv_copy_kernel(KvCopy p, Div vector, Div inner, bool token_inner, bool dense, int code_parts, int scale_parts) {
     const int per = 2 * code_parts + scale_parts;
     const int64_t i = blockIdx.x / per;
     const int part = blockIdx.x - (int)i * per;
@@ -60,7 +60,16 @@ __global__ __launch_bounds__(256) void kv_copy_kernel(KvCopy p, Div vector, Div 
     }
     const int8_t* src = (v ? p.from.v : p.from.k) + from * p.from.block_stride;
     int8_t* dst = (v ? p.to.v : p.to.k) + to * p.to.block_stride;
+    const uint32_t pieces = vectors * vector.d;
     v4i x[kPieces];
+    if (dense && take == (uint32_t)p.from.page) {
+#pragma unroll
+        for (int j = 0; j < kPieces; j++) x[j] = first + 256 * j < pieces ? *(const v4i*)(src + 16 * (uint64_t)(first + 256 * j)) : v4i{0, 0, 0, 0};
+#pragma unroll
+        for (int j = 0; j < kPieces; j++)
+            if (first + 256 * j < pieces) *(v4i*)(dst + 16 * (uint64_t)(first + 256 * j)) = x[j];
+        return;
+    }
     int64_t at[kPieces];
 #pragma unroll
     for (int j = 0; j < kPieces; j++) {
@@ -80,12 +89,14 @@ __global__ __launch_bounds__(256) void kv_copy_kernel(KvCopy p, Div vector, Div 
 hipError_t launch_kv_cache_copy(hipStream_t stream, const KvCopy& p) {
     const KvCache& c = p.from;
     const bool token_inner = c.token_stride <= c.head_stride;
+    const int64_t inner = token_inner ? c.token_stride : c.head_stride, outer = token_inner ? c.head_stride : c.token_stride;
+    const bool dense = inner == c.dim && outer == (token_inner ? c.page : c.heads) * inner && p.to.token_stride == c.token_stride && p.to.head_stride == c.head_stride;
     const int64_t vectors = (int64_t)c.heads * c.page, pieces = vectors * (c.dim / 16), each = 256 * kPieces;
     const int code_parts = (int)((pieces + each - 1) / each), scale_parts = (int)((vectors + each - 1) / each);
     const int64_t grid = p.n * (2 * (int64_t)code_parts + scale_parts);
     if (grid > INT32_MAX) return hipErrorInvalidConfiguration;
     hipLaunchKernelGGL(kv_copy_kernel, dim3((unsigned)grid), dim3(256), 0, stream, p, div_by(c.dim / 16),
-                       div_by(token_inner ? c.page : c.heads), token_inner, code_parts, scale_parts);
+                       div_by(token_inner ? c.page : c.heads), token_inner, dense, code_parts, scale_parts);
     return hipGetLastError();
 }
 

@@ -1,91 +1,215 @@
 // Low-rank adapters of many requests beside one linear:
 //   out[m] = base[m] + scale[a] B[a] (A[a] x[m]),   a = adapter[m].
 //
-// Two passes, h = A[a] x[m] and the update.  A tile of 64 rows has its rows sorted
-// into classes, those of one adapter; a block takes up to 32 rows of a class as the
+// Two passes, h = A[a] x[m] and the update.  A tile of 128 rows has its rows sorted
+// into classes, those of one adapter; a block takes rows of one class as the
 // columns of its products, so that an adapter's factors are read once for all of a
-// class's rows however they are mixed, and a row's values meet no other adapter's.
-// Both operands come straight from memory in the order of the matrix instructions: a
-// lane has 8 consecutive k of a row, which are one v_mfma_f32_16x16x32_bf16 or, in
-// fp32, eight v_mfma_f32_16x16x4_f32 (k 8 g + e in the e-th, g = lane / 16, on both
-// sides).
+// class's rows however they are mixed, and a row's values meet no other adapter's.  The
+// first pass leaves the classes for the second.
+// An operand of a matrix instruction is 16 rows of 32 k, 8 consecutive k of row l % 16 in
+// lane l: one v_mfma_f32_16x16x32_bf16 or, in fp32, eight v_mfma_f32_16x16x4_f32 (k 8 g + e
+// in the e-th, g = l / 16, on both sides).
 // h is fp32 throughout: against bf16 factors it enters the second product as three
 // bf16, all of its 24 bits.
 #include <algorithm>
+#include <type_traits>
 
 #include "device_common.hpp"
 #include "serving.hpp"
 
 namespace phi_dev {
 
+constexpr int kLoraTile = 128;  // rows
+
+// A tile's classes as the first pass leaves them for the second.
+struct LoraClass {
+    uint64_t rows[2];
+    int adapter, pad[3];
+};
+
 namespace {
 
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 
-constexpr int kCols = 32;  // rows of x a block, two tiles of columns
 constexpr int kSplits = 8;
+constexpr int kSpread = 32;  // tiles, from which on each XCD has neighbours
 
-// Unit u of a tile of 64 rows: up to kCols rows of one class, from the skip-th on.
+// Up to `most` rows of one class, from the skip-th on.
 struct LoraUnit {
     int adapter;  // below 0: none
-    uint64_t rows;
-    int skip, n;
+    int index;    // of the class; where there is no unit, the number of classes
+    int skip, n;  // n 0: there is none
+    uint64_t rows[2];
 };
 
-__device__ __forceinline__ bool lora_unit(const LoraBatched& p, int tile, int u, LoraUnit& got) {
-    const int row = tile * 64 + (threadIdx.x & 63);
-    int a = row < p.rows ? p.adapter[row] : 0;
-    a = a >= 0 && a < p.adapters ? a : -1;
-    uint64_t left = __ballot(row < p.rows);
-    while (left) {
-        const int one = __builtin_amdgcn_readlane(a, __builtin_ctzll(left));
-        const uint64_t mine = __ballot(a == one) & left;
-        const int n = __popcll(mine), groups = (n + kCols - 1) / kCols;
-        if (u < groups) {
-            got = {one, mine, kCols * u, min(n - kCols * u, kCols)};
-            return true;
+// A tile's classes, as one wave finds them: two rows a lane, the first row of each class by
+// the lowest number in a table of adapters (those that fall on one place of it in turns).
+// (Class by class from the first row left, 0.2 us each: 7.7 us to the last of 28.)
+constexpr int kPlaces = 1024;
+struct LoraTable {
+    int place[kPlaces], key[kLoraTile], count[kLoraTile];
+};
+struct LoraClasses {
+    int a[2], count[2];  // a row's adapter and, of a class's first row, its rows
+    uint64_t some[2], first[2];
+
+    __device__ __forceinline__ void find(const LoraBatched& p, int tile, LoraTable& t) {
+        const int lane = threadIdx.x & 63;
+        bool left[2], mine[2] = {false, false};
+#pragma unroll
+        for (int i = 0; i < kPlaces / 256; i++) *(int4*)(t.place + 4 * (lane + 64 * i)) = make_int4(kLoraTile, kLoraTile, kLoraTile, kLoraTile);
+        int at[2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int row = tile * kLoraTile + 64 * h + lane;
+            left[h] = row < p.rows;
+            some[h] = __ballot(left[h]);
+            a[h] = left[h] ? p.adapter[row] : 0;
+            a[h] = a[h] >= 0 && a[h] < p.adapters ? a[h] : -1;
+            at[h] = (a[h] + 1) & (kPlaces - 1);
+            t.key[64 * h + lane] = a[h], t.count[64 * h + lane] = 0;
         }
-        u -= groups;
-        left &= ~mine;
+        // A wave's LDS accesses are done in order; the fences keep the compiler's.
+        auto fence = [] {
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup", "local");
+        };
+        do {
+            fence();
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+                if (left[h]) atomicMin(&t.place[at[h]], 64 * h + lane);
+            fence();
+            int won[2];
+#pragma unroll
+            for (int h = 0; h < 2; h++) won[h] = t.place[at[h]];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                if (!left[h] || t.key[won[h]] != a[h]) continue;
+                mine[h] = won[h] == 64 * h + lane;
+                atomicAdd(&t.count[won[h]], 1);
+                left[h] = false;
+            }
+            fence();
+            // For the next turn, those that are left begin anew.
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+                if (left[h]) t.place[at[h]] = kLoraTile;
+        } while (__any(left[0] || left[1]));
+        fence();
+#pragma unroll
+        for (int h = 0; h < 2; h++) first[h] = __ballot(mine[h]), count[h] = t.count[64 * h + lane];
     }
-    return false;
-}
+    // Unit u: all classes' first `most` rows, then the next of those that have more, and so on.
+    __device__ __forceinline__ LoraUnit unit(int u, int most) const {
+        const uint64_t below = ((uint64_t)1 << (threadIdx.x & 63)) - 1;
+        const int classes = __popcll(first[0]) + __popcll(first[1]);
+#pragma unroll 1
+        for (int skip = 0; skip < kLoraTile; skip += most) {
+            const uint64_t of[2] = {__ballot(count[0] > skip) & first[0], __ballot(count[1] > skip) & first[1]};
+            const int n0 = __popcll(of[0]), n = n0 + __popcll(of[1]);
+            if (u >= n) {
+                u -= n;
+                continue;
+            }
+            const int h = u >= n0;
+            const uint64_t mask = of[h], got = __ballot((mask & ~below & (below + 1)) && (int)__popcll(mask & below) == u - (h ? n0 : 0));
+            const int lane = __builtin_ctzll(got), one = __builtin_amdgcn_readlane(a[h], lane), all = __builtin_amdgcn_readlane(count[h], lane);
+            const uint64_t before = ((uint64_t)1 << lane) - 1;
+            return {one, (int)(h ? __popcll(first[0]) + __popcll(first[1] & before) : __popcll(first[0] & before)), skip, min(all - skip, most),
+                    {__ballot(a[0] == one) & some[0], __ballot(a[1] == one) & some[1]}};
+        }
+        return {0, classes, 0, 0, {0, 0}};
+    }
+};
 
-// The unit's rows, in LDS; every wave writes the same.
-__device__ __forceinline__ void unit_rows(const LoraUnit& u, int tile, int* rows) {
+// Tile number `id` of `around`: where these are 8 ceil(tiles / 8), neighbours, which often
+// have one adapter, on one XCD, whose L2 keeps its factors (blocks go round the eight).
+__device__ __forceinline__ int lora_tile(int id, int around, int tiles) { return around >= kSpread ? (id & 7) * (around >> 3) + (id >> 3) : id; }
+
+// Rows of a class from the skip-th on, `most` of them, in LDS; every wave writes the same.
+__device__ __forceinline__ void class_rows(const uint64_t (&mask)[2], int tile, int skip, int most, int* rows) {
     const int lane = threadIdx.x & 63;
-    const int at = __popcll(u.rows & (((uint64_t)1 << lane) - 1)) - u.skip;
-    if ((u.rows >> lane & 1) && at >= 0 && at < kCols) rows[at] = tile * 64 + lane;
+    const uint64_t below = ((uint64_t)1 << lane) - 1;
+    const int at[2] = {(int)__popcll(mask[0] & below), (int)(__popcll(mask[0]) + __popcll(mask[1] & below))};
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+        if ((mask[h] >> lane & 1) && at[h] >= skip && at[h] < skip + most) rows[at[h] - skip] = tile * kLoraTile + 64 * h + lane;
 }
 
-// Eight elements k.. of a row of K, zeros past its end.  VEC: K % 8 == 0 and rows at
-// 16 bytes.
+// Rows may lie at any of their elements: loads are of 16 bytes all the same, which the
+// memory path takes at any address.
+typedef uint32_t any4 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t any2 __attribute__((ext_vector_type(2), aligned(2)));
+
 template <bool B16> struct Eight {
     uint32_t w[B16 ? 4 : 8];
 };
-template <bool B16, bool VEC>
-__device__ __forceinline__ Eight<B16> load_eight(const char* row, int k, int K) {
+template <bool B16>
+__device__ __forceinline__ Eight<B16> load_eight(const char* row, int k) {
     Eight<B16> e;
-    if (VEC) {
-        const uint4* p = (const uint4*)(row + (size_t)(k < K ? k : 0) * (B16 ? 2 : 4));
+    const char* p = row + (size_t)(uint32_t)k * (B16 ? 2 : 4);
 #pragma unroll
-        for (int i = 0; i < (B16 ? 1 : 2); i++) {
-            const uint4 t = p[i];
-            e.w[4 * i] = k < K ? t.x : 0, e.w[4 * i + 1] = k < K ? t.y : 0, e.w[4 * i + 2] = k < K ? t.z : 0, e.w[4 * i + 3] = k < K ? t.w : 0;
-        }
-        return e;
+    for (int i = 0; i < (B16 ? 1 : 2); i++) {
+        const any4 t = *(const any4*)(p + 16 * i);
+        e.w[4 * i] = t[0], e.w[4 * i + 1] = t[1], e.w[4 * i + 2] = t[2], e.w[4 * i + 3] = t[3];
     }
-    uint32_t t[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const int at = k + i < K ? k + i : 0;
-        const uint32_t v = B16 ? ((const uint16_t*)row)[at] : ((const uint32_t*)row)[at];
-        t[i] = k + i < K ? v : 0;
-    }
-#pragma unroll
-    for (int i = 0; i < (B16 ? 4 : 8); i++) e.w[i] = B16 ? t[2 * i] | t[2 * i + 1] << 16 : t[i];
     return e;
 }
+// The same from k on in a row of K, zeros past its end.  What lies behind the row is read
+// with it and dropped, but not from `end`, the operand's, on: there one by one, in a loop
+// that costs few registers.
+template <bool B16>
+__device__ __forceinline__ Eight<B16> load_masked(const char* row, int k, int K, const char* end) {
+    constexpr int E = B16 ? 2 : 4;
+    Eight<B16> e{};
+    const char* p = row + (size_t)(uint32_t)k * E;
+    if (__any(k < K && p + 8 * E > end)) {
+#pragma unroll 1
+        for (int i = 0; i < 8; i++) {
+            const int at = min(k + i, K - 1);
+            const uint32_t v = B16 ? ((const uint16_t*)row)[at] : ((const uint32_t*)row)[at], x = k + i < K ? v : 0;
+#pragma unroll
+            for (int j = 0; j < (B16 ? 4 : 8); j++) {
+                const uint32_t above = j + 1 < (B16 ? 4 : 8) ? e.w[(j + 1) % (B16 ? 4 : 8)] : x;
+                e.w[j] = B16 ? __builtin_amdgcn_alignbit(above, e.w[j], 16) : above;
+            }
+        }
+    } else if (k < K) {
+        e = load_eight<B16>(row, k);
+#pragma unroll
+        for (int j = 0; j < (B16 ? 4 : 8); j++) {
+            if (B16) e.w[j] &= (k + 2 * j < K ? 0xffffu : 0u) | (k + 2 * j + 1 < K ? 0xffff0000u : 0u);
+            else e.w[j] = k + j < K ? e.w[j] : 0;
+        }
+    }
+    return e;
+}
+
+// 16 rows of 32 H k on their way through LDS: loaded with a row's lanes side by side
+// (16 lanes that meet 16 rows are taken one by one by the address path).
+template <bool B16, int H> struct Rows {
+    static constexpr int kLanes = (B16 ? 4 : 8) * H, kLoads = kLanes / 4, kPitch = 16 * kLanes + 16, kBytes = 16 * kPitch;
+    any4 w[kLoads];
+    static __device__ __forceinline__ int row(int i) { return (threadIdx.x & 63) / kLanes + 64 / kLanes * i; }
+    static __device__ __forceinline__ int k() { return (threadIdx.x & (kLanes - 1)) * (B16 ? 8 : 4); }
+    // rows[i]: row(i)'s.
+    __device__ __forceinline__ void load(const char* const (&rows)[kLoads], int k0) {
+#pragma unroll
+        for (int i = 0; i < kLoads; i++) w[i] = *(const any4*)(rows[i] + (size_t)(uint32_t)(k0 + k()) * (B16 ? 2 : 4));
+    }
+    __device__ __forceinline__ void to(uint8_t* lds) const {
+#pragma unroll
+        for (int i = 0; i < kLoads; i++) *(uint4*)(lds + row(i) * kPitch + 16 * (threadIdx.x & (kLanes - 1))) = make_uint4(w[i][0], w[i][1], w[i][2], w[i][3]);
+    }
+    // The operand of k from 32 h on.
+    static __device__ __forceinline__ Eight<B16> from(const uint8_t* lds, int h) {
+        const int lane = threadIdx.x & 63, n = B16 ? 1 : 2;
+        Eight<B16> e;
+#pragma unroll
+        for (int i = 0; i < n; i++) *(uint4*)(e.w + 4 * i) = *(const uint4*)(lds + (lane & 15) * kPitch + 64 * n * h + 16 * n * (lane >> 4) + 16 * i);
+        return e;
+    }
+};
 template <bool B16>
 __device__ __forceinline__ float value(const Eight<B16>& e, int i) {
     return __uint_as_float(B16 ? i & 1 ? e.w[i >> 1] & 0xffff0000u : e.w[i >> 1] << 16 : e.w[i]);
@@ -104,186 +228,482 @@ __device__ __forceinline__ v4f product(const Eight<AB>& a, const Eight<BB>& b, v
 
 }  // namespace
 
-// RT tiles of 16 ranks from 16 RT blockIdx.z on.
-template <bool XB, bool WB, bool VEC, int RT>
-__global__ __launch_bounds__(256) void lora_batched_down_kernel(LoraBatched p, int tiles) {
-    constexpr int P = 16 * RT + 4;
-    __shared__ int rows[kCols];
-    __shared__ float part[4][kCols][P];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int tile = blockIdx.x % tiles, split = blockIdx.y, r0 = 16 * RT * blockIdx.z;
-    LoraUnit u;
-    if (!lora_unit(p, tile, blockIdx.x / tiles, u) || u.adapter < 0) return;
-    unit_rows(u, tile, rows);
-    __syncthreads();
-    const int col = lane & 15, g = lane >> 4;
-    const char* xs[2];
-    const char* as[RT];
-#pragma unroll
-    for (int c = 0; c < 2; c++) xs[c] = (const char*)p.x + (int64_t)rows[min(16 * c + col, u.n - 1)] * p.ldx * (XB ? 2 : 4);
-#pragma unroll
-    for (int r = 0; r < RT; r++)
-        as[r] = (const char*)p.A + (u.adapter * p.a_adapter + min(r0 + 16 * r + col, p.R - 1) * p.a_row) * (WB ? 2 : 4);
-    const int steps = (p.K + 31) / 32, parts = 4 * p.splits, me = 4 * split + wave;
-    const int s0 = (int)((int64_t)steps * me / parts), s1 = (int)((int64_t)steps * (me + 1) / parts);
-    const bool two = u.n > 16;
-    v4f acc[2][RT];
-#pragma unroll
-    for (int c = 0; c < 2; c++)
-#pragma unroll
-        for (int r = 0; r < RT; r++) acc[c][r] = v4f{0, 0, 0, 0};
-    for (int s = s0; s < s1; s++) {
-        const int k = 32 * s + 8 * g;
-        Eight<XB> x[2];
-        Eight<WB> a[RT];
-        x[0] = load_eight<XB, VEC>(xs[0], k, p.K);
-        if (two) x[1] = load_eight<XB, VEC>(xs[1], k, p.K);
-#pragma unroll
-        for (int r = 0; r < RT; r++) a[r] = load_eight<WB, VEC>(as[r], k, p.K);
-#pragma unroll
-        for (int r = 0; r < RT; r++) acc[0][r] = product(a[r], x[0], acc[0][r]);
-        if (two) {
-#pragma unroll
-            for (int r = 0; r < RT; r++) acc[1][r] = product(a[r], x[1], acc[1][r]);
-        }
-    }
-#pragma unroll
-    for (int c = 0; c < 2; c++)
-#pragma unroll
-        for (int r = 0; r < RT; r++) *(v4f*)&part[wave][16 * c + col][16 * r + 4 * g] = acc[c][r];
-    __syncthreads();
-    for (int i = threadIdx.x; i < u.n * 4 * RT; i += 256) {
-        const int c = i / (4 * RT), r = 4 * (i % (4 * RT));
-        if (r0 + r >= p.rank_pitch) continue;
-        v4f sum = *(const v4f*)&part[0][c][r];
-#pragma unroll
-        for (int w = 1; w < 4; w++) sum += *(const v4f*)&part[w][c][r];
-        *(v4f*)(p.h + ((int64_t)split * p.rows + rows[c]) * p.rank_pitch + r0 + r) = sum;
-    }
-}
+// h of few rows: RT tiles of 16 ranks from 16 RT blockIdx.z on for up to 32 rows of a class,
+// every `parts`-th unit of a tile a block.  Each wave has a stretch of K, U steps of 32 at
+// a time straight from memory.
+constexpr int kFewCols = 32;
 
-// A wave has 64 columns n of out, as four tiles of the matrix instruction whose rows
-// are so chosen that a lane's results are 16 consecutive n: row r of tile t stands
-// for n = 16 (r / 4) + 4 t + r % 4.  A block has 256 `chunks` columns.
-template <bool WB, bool OB, bool VECB, bool VECO>
-__global__ __launch_bounds__(256) void lora_batched_up_kernel(LoraBatched p, int tiles, int chunks) {
-    constexpr int T = WB ? 3 : 1;  // terms of h
-    __shared__ int rows[kCols];
-    extern __shared__ __align__(16) uint8_t lds[];
+template <bool XB, bool WB, int RT>
+__global__ __launch_bounds__(256, 2) void lora_batched_down_kernel(LoraBatched p, int tiles, int around, int parts) {
+    constexpr int P = 16 * RT + 4, U = XB && WB ? 4 : 2;
+    __shared__ int rows[kFewCols];
+    __shared__ float part[4][kFewCols][P];
+    __shared__ LoraTable table;
+    __shared__ LoraUnit found;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int tile = blockIdx.x % tiles;
-    LoraUnit u;
-    if (!lora_unit(p, tile, blockIdx.x / tiles, u)) return;
-    const bool some = u.adapter >= 0;
-    if (!some && p.out == p.base) return;
-    unit_rows(u, tile, rows);
-    __syncthreads();
-    const int ranks = (p.R + 31) / 32 * 32, pitch = ranks + (WB ? 8 : 4);
-    uint16_t* hb = (uint16_t*)lds;  // [term][column][pitch]
-    float* hf = (float*)lds;        // [column][pitch]
+    const int tile = lora_tile(blockIdx.x % around, around, tiles), split = blockIdx.y, r0 = 16 * RT * blockIdx.z;
+    if (tile >= tiles) return;
     const int col = lane & 15, g = lane >> 4;
-    if (some) {
-        const float scale = p.scale ? p.scale[u.adapter] : 1.0f;
-        for (int i = threadIdx.x; i < kCols * ranks / 4; i += 256) {
-            const int c = i / (ranks / 4), r = 4 * (i - c * (ranks / 4));
-            v4f sum = {0, 0, 0, 0};
-            if (c < u.n && r < p.R) {
-                const float* from = p.h + (int64_t)rows[c] * p.rank_pitch + r;
-                for (int s = 0; s < p.splits; s++) sum += *(const v4f*)(from + (int64_t)s * p.rows * p.rank_pitch);
-#pragma unroll
-                for (int e = 0; e < 4; e++) sum[e] = r + e < p.R ? sum[e] * scale : 0.0f;
-            }
-            if constexpr (WB) {
-#pragma unroll
-                for (int t = 0; t < T; t++) {
-                    const uint32_t lo = f32x2_to_bf16x2(sum[0], sum[1]), hi = f32x2_to_bf16x2(sum[2], sum[3]);
-                    *(uint2*)(hb + (t * kCols + c) * pitch + r) = make_uint2(lo, hi);
-                    // What an infinity leaves is 0, not NaN.
-                    const float y[4] = {bf16_to_f32(lo & 0xffffu), bf16_to_f32(lo >> 16), bf16_to_f32(hi & 0xffffu), bf16_to_f32(hi >> 16)};
-#pragma unroll
-                    for (int e = 0; e < 4; e++) sum[e] = __builtin_isfinite(y[e]) ? sum[e] - y[e] : 0.0f;
-                }
-            } else {
-                *(v4f*)(hf + c * pitch + r) = sum;
-            }
+    const int steps = (p.K + 31) / 32, waves = 4 * p.splits, me = 4 * split + wave;
+    const int s0 = (int)((int64_t)steps * me / waves), s1 = (int)((int64_t)steps * (me + 1) / waves), whole = min(s1, p.K / 32);
+    const bool tells = split == 0 && blockIdx.z == 0 && threadIdx.x == 0;
+    LoraClasses classes;
+    if (wave == 0) classes.find(p, tile, table);
+#pragma unroll 1
+    for (int unit = blockIdx.x / around;; unit += parts) {
+        if (wave == 0) {
+            const LoraUnit u = classes.unit(unit, kFewCols);
+            if (lane == 0) found = u;
         }
         __syncthreads();
-    }
-    const int tiles_n = u.n > 16 ? 2 : 1;
-    for (int chunk = 0; chunk < chunks; chunk++) {
-        const int n0 = (blockIdx.y * chunks + chunk) * 256 + 64 * wave;
-        if (n0 >= p.N) break;
-        v4f acc[2][4];
+        const LoraUnit u = found;
+        if (!u.n) {
+            if (tells) p.counts[tile] = u.index;
+            return;
+        }
+        if (tells && u.skip == 0) p.classes[(int64_t)tile * kLoraTile + u.index] = {{u.rows[0], u.rows[1]}, u.adapter, {}};
+        if (u.adapter < 0) {
+            __syncthreads();
+            continue;
+        }
+        class_rows(u.rows, tile, u.skip, kFewCols, rows);
+        __syncthreads();
+        const bool two = u.n > 16;
+        const char* xs[2];
+        const char* as[RT];
+#pragma unroll
+        for (int c = 0; c < 2; c++) xs[c] = (const char*)p.x + (int64_t)rows[min(16 * c + col, u.n - 1)] * p.ldx * (XB ? 2 : 4);
+#pragma unroll
+        for (int r = 0; r < RT; r++)
+            as[r] = (const char*)p.A + (u.adapter * p.a_adapter + min(r0 + 16 * r + col, p.R - 1) * p.a_row) * (WB ? 2 : 4);
+        v4f acc[2][RT];
 #pragma unroll
         for (int c = 0; c < 2; c++)
 #pragma unroll
-            for (int t = 0; t < 4; t++) acc[c][t] = v4f{0, 0, 0, 0};
-        if (some) {
-            const char* bs[4];
+            for (int r = 0; r < RT; r++) acc[c][r] = v4f{0, 0, 0, 0};
+        auto multiply = [&](const Eight<XB> (&x)[2], const Eight<WB> (&a)[RT]) __attribute__((always_inline)) {
 #pragma unroll
-            for (int t = 0; t < 4; t++)
-                bs[t] = (const char*)p.B + (u.adapter * p.b_adapter + min(n0 + 16 * (col >> 2) + 4 * t + (col & 3), p.N - 1) * p.b_row) * (WB ? 2 : 4);
-            for (int k0 = 0; k0 < ranks; k0 += 32) {
-                const int k = k0 + 8 * g;
-                Eight<WB> b[4];
+            for (int r = 0; r < RT; r++) acc[0][r] = product(a[r], x[0], acc[0][r]);
+            if (two) {
 #pragma unroll
-                for (int t = 0; t < 4; t++) b[t] = load_eight<WB, VECB>(bs[t], k, p.R);
-#pragma unroll
-                for (int c = 0; c < 2; c++) {
-                    if (c >= tiles_n) break;
-#pragma unroll
-                    for (int term = T - 1; term >= 0; term--) {
-                        Eight<WB> h;
-                        if (WB) {
-                            *(uint4*)h.w = *(const uint4*)(hb + (term * kCols + 16 * c + col) * pitch + k);
-                        } else {
-                            *(v4f*)h.w = *(const v4f*)(hf + (16 * c + col) * pitch + k);
-                            *(v4f*)(h.w + (WB ? 0 : 4)) = *(const v4f*)(hf + (16 * c + col) * pitch + k + 4);
-                        }
-#pragma unroll
-                        for (int t = 0; t < 4; t++) acc[c][t] = product(b[t], h, acc[c][t]);
-                    }
-                }
+                for (int r = 0; r < RT; r++) acc[1][r] = product(a[r], x[1], acc[1][r]);
             }
+        };
+#pragma unroll 1
+        for (int s = s0; s < whole; s += U) {
+            Eight<XB> x[U][2];
+            Eight<WB> a[U][RT];
+#pragma unroll
+            for (int i = 0; i < U; i++) {
+                const int k = 32 * min(s + i, whole - 1) + 8 * g;  // past the last: unused
+                x[i][0] = load_eight<XB>(xs[0], k);
+                if (two) x[i][1] = load_eight<XB>(xs[1], k);
+#pragma unroll
+                for (int r = 0; r < RT; r++) a[i][r] = load_eight<WB>(as[r], k);
+            }
+#pragma unroll
+            for (int i = 0; i < U; i++)
+                if (s + i < whole) multiply(x[i], a[i]);
+        }
+        if (whole < s1) {  // the last of K
+            const int k = 32 * whole + 8 * g;
+            Eight<XB> x[2];
+            Eight<WB> a[RT];
+#pragma unroll
+            for (int c = 0; c < 2; c++) x[c] = load_masked<XB>(xs[c], k, p.K, p.x_end);
+#pragma unroll
+            for (int r = 0; r < RT; r++) a[r] = load_masked<WB>(as[r], k, p.K, p.a_end);
+            multiply(x, a);
         }
 #pragma unroll
-        for (int c = 0; c < 2; c++) {
-            if (16 * c + col >= u.n) continue;
-            const int64_t row = rows[16 * c + col];
-            const int n = n0 + 16 * g;
-            if (n >= p.N) continue;
-            const int64_t to = row * p.ldo + n, from = row * p.ld_base + n;
-            float y[16];
+        for (int c = 0; c < 2; c++)
 #pragma unroll
-            for (int j = 0; j < 16; j++) y[j] = acc[c][j >> 2][j & 3];
-            if (VECO) {
-                if (p.base) {
-                    const uint4* b = OB ? (const uint4*)((const uint16_t*)p.base + from) : (const uint4*)((const float*)p.base + from);
+            for (int r = 0; r < RT; r++) *(v4f*)&part[wave][16 * c + col][16 * r + 4 * g] = acc[c][r];
+        __syncthreads();
+#pragma unroll 1
+        for (int i = threadIdx.x; i < u.n * 4 * RT; i += 256) {
+            const int c = i / (4 * RT), r = 4 * (i % (4 * RT));
+            if (r0 + r >= p.rank_pitch) continue;
+            v4f sum = *(const v4f*)&part[0][c][r];
 #pragma unroll
-                    for (int i = 0; i < (OB ? 2 : 4); i++) {
-                        const uint4 v = b[i];
-                        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+            for (int w = 1; w < 4; w++) sum += *(const v4f*)&part[w][c][r];
+            *(v4f*)(p.h + ((int64_t)split * p.rows + rows[c]) * p.rank_pitch + r0 + r) = sum;
+        }
+        __syncthreads();
+    }
+}
+
+// h of many rows, up to a tile's 128 of a class a block, so that A is read a fourth as often:
+// blocks of one adapter meet in L2, where A's second reading cost more than x from memory
+// (4352 rows of 5120 on 64 ranks: 35 us in units of 32 rows, 15 with A from a few lines).
+// Waves 0-3 have 32 rows each of the first half of the block's stretch of K, waves 4-7 of the
+// second; a half's four waves share A's step of H 32 k in LDS, two steps' in turn, and
+// load two steps ahead.
+template <bool XB, bool WB, int RT>
+__global__ __launch_bounds__(512, 2) void lora_batched_down_wide_kernel(LoraBatched p, int tiles, int around, int parts) {
+    constexpr int H = XB && WB ? 2 : 1, kStep = 32 * H, P = 16 * RT + 4;
+    typedef Rows<XB, H> RX;
+    typedef Rows<WB, H> RA;
+    constexpr int kA = RT * RA::kBytes, kX = 2 * RX::kBytes, kStage = 2 * 2 * kA + 8 * kX, kJoin = kLoraTile * P * 4;
+    // A's rows to load: RT tiles by four waves.
+    constexpr int kMine = RT * RA::kLoads / 4 > 0 ? RT * RA::kLoads / 4 : 1;
+    __shared__ int rows[kLoraTile];
+    __shared__ __align__(16) uint8_t lds[kStage > kJoin ? kStage : kJoin];
+    __shared__ LoraTable table;
+    __shared__ LoraUnit found;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = wave >> 2, w = wave & 3;
+    const int tile = lora_tile(blockIdx.x % around, around, tiles), split = blockIdx.y, r0 = 16 * RT * blockIdx.z;
+    if (tile >= tiles) return;
+    const int col = lane & 15, g = lane >> 4;
+    const int steps = (p.K + kStep - 1) / kStep, ranges = 2 * p.splits, me = 2 * split + half;
+    const int s0 = (int)((int64_t)steps * me / ranges), s1 = (int)((int64_t)steps * (me + 1) / ranges);
+    // Both halves go round as often.
+    const int turns = max(s1 - s0, (int)((int64_t)steps * (2 * split + 2 - half) / ranges) - (int)((int64_t)steps * (2 * split + 1 - half) / ranges));
+    const bool tells = split == 0 && blockIdx.z == 0 && threadIdx.x == 0;
+    uint8_t* const lds_x = lds + 4 * kA + wave * kX;
+    LoraClasses classes;
+    if (wave == 0) classes.find(p, tile, table);
+#pragma unroll 1
+    for (int unit = blockIdx.x / around;; unit += parts) {
+        if (wave == 0) {
+            const LoraUnit u = classes.unit(unit, kLoraTile);
+            if (lane == 0) found = u;
+        }
+        __syncthreads();
+        const LoraUnit u = found;
+        if (!u.n) {
+            if (tells) p.counts[tile] = u.index;
+            return;
+        }
+        if (tells && u.skip == 0) p.classes[(int64_t)tile * kLoraTile + u.index] = {{u.rows[0], u.rows[1]}, u.adapter, {}};
+        if (u.adapter < 0) {
+            __syncthreads();
+            continue;
+        }
+        class_rows(u.rows, tile, 0, kLoraTile, rows);
+        __syncthreads();
+        const bool mine = 32 * w < u.n;
+        const char* xs[2][RX::kLoads];
+        const char* as[kMine];
 #pragma unroll
-                        for (int j = 0; j < 4; j++) {
-                            if (OB) y[8 * i + 2 * j] += bf16_to_f32(w[j] & 0xffffu), y[8 * i + 2 * j + 1] += bf16_to_f32(w[j] >> 16);
-                            else y[4 * i + j] += __uint_as_float(w[j]);
-                        }
+        for (int c = 0; c < 2; c++)
+#pragma unroll
+            for (int i = 0; i < RX::kLoads; i++) xs[c][i] = (const char*)p.x + (int64_t)rows[min(32 * w + 16 * c + RX::row(i), u.n - 1)] * p.ldx * (XB ? 2 : 4);
+        // Load j of the wave: loads RA::kLoads a tile, tile by tile.
+        auto a_load = [&](int j) { return w * kMine + j; };
+#pragma unroll
+        for (int j = 0; j < kMine; j++) {
+            const int row = 64 / RA::kLanes * a_load(j) + lane / RA::kLanes;
+            as[j] = (const char*)p.A + (u.adapter * p.a_adapter + min(r0 + row, p.R - 1) * p.a_row) * (WB ? 2 : 4);
+        }
+        v4f acc[2][RT];
+#pragma unroll
+        for (int c = 0; c < 2; c++)
+#pragma unroll
+            for (int r = 0; r < RT; r++) acc[c][r] = v4f{0, 0, 0, 0};
+        struct Step {
+            RX x[2];
+            any4 a[kMine];
+        };
+        auto load = [&](Step& t, int s) __attribute__((always_inline)) {
+            if (s >= min(s1, p.K / kStep)) return;
+            const int k = kStep * s;
+            if (mine) t.x[0].load(xs[0], k), t.x[1].load(xs[1], k);
+#pragma unroll
+            for (int j = 0; j < kMine; j++) t.a[j] = *(const any4*)(as[j] + (size_t)(uint32_t)(k + RA::k()) * (WB ? 2 : 4));
+        };
+        // The last of K, zeros past its end, one by one and straight to LDS.
+        auto rest = [&](uint8_t* lds_a) {
+            const int k0 = p.K / kStep * kStep;
+#pragma unroll 1
+            for (int i = lane; i < 32 * kStep; i += 64) {
+                const int r = i / kStep, k = i % kStep, at = min(k0 + k, p.K - 1);
+                const char* from = (const char*)p.x + (rows[min(32 * w + r, u.n - 1)] * p.ldx + at) * (XB ? 2 : 4);
+                uint8_t* to = lds_x + r / 16 * RX::kBytes + r % 16 * RX::kPitch + k * (XB ? 2 : 4);
+                if (XB) *(uint16_t*)to = k0 + k < p.K ? *(const uint16_t*)from : 0;
+                else *(uint32_t*)to = k0 + k < p.K ? *(const uint32_t*)from : 0;
+            }
+#pragma unroll 1
+            for (int i = 64 * w + lane; i < 16 * RT * kStep; i += 256) {
+                const int r = i / kStep, k = i % kStep, at = min(k0 + k, p.K - 1);
+                const char* from = (const char*)p.A + (u.adapter * p.a_adapter + min(r0 + r, p.R - 1) * p.a_row + at) * (WB ? 2 : 4);
+                uint8_t* to = lds_a + r / 16 * RA::kBytes + r % 16 * RA::kPitch + k * (WB ? 2 : 4);
+                if (WB) *(uint16_t*)to = k0 + k < p.K ? *(const uint16_t*)from : 0;
+                else *(uint32_t*)to = k0 + k < p.K ? *(const uint32_t*)from : 0;
+            }
+        };
+        auto turn = [&](Step& t, int n) __attribute__((always_inline)) {
+            const int s = s0 + n;
+            uint8_t* const lds_a = lds + (2 * half + (n & 1)) * kA;
+            if (s < s1 && s < p.K / kStep) {
+#pragma unroll
+                for (int j = 0; j < kMine; j++) {
+                    const int at = a_load(j);
+                    if (at < RT * RA::kLoads)
+                        *(uint4*)(lds_a + (64 / RA::kLanes * at + lane / RA::kLanes) * RA::kPitch + 16 * (lane % RA::kLanes)) = make_uint4(t.a[j][0], t.a[j][1], t.a[j][2], t.a[j][3]);
+                }
+                if (mine) t.x[0].to(lds_x), t.x[1].to(lds_x + RX::kBytes);
+            } else if (s < s1) {
+                rest(lds_a);
+            }
+            load(t, s + 2);
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+            __builtin_amdgcn_s_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+            if (s < s1 && mine) {
+#pragma unroll
+                for (int h = 0; h < H; h++) {
+                    const Eight<XB> x0 = RX::from(lds_x, h), x1 = RX::from(lds_x + RX::kBytes, h);
+#pragma unroll
+                    for (int r = 0; r < RT; r++) {
+                        const Eight<WB> a = RA::from(lds_a + r * RA::kBytes, h);
+                        acc[0][r] = product(a, x0, acc[0][r]);
+                        acc[1][r] = product(a, x1, acc[1][r]);
                     }
                 }
+            }
+        };
+        Step even, odd;
+        load(even, s0);
+        load(odd, s0 + 1);
+#pragma unroll 1
+        for (int n = 0; n < turns; n += 2) {
+            turn(even, n);
+            turn(odd, n + 1);
+        }
+        // The second half's sums onto the first's.
+        float(*join)[P] = (float(*)[P])lds;
+        __syncthreads();
 #pragma unroll
-                for (int i = 0; i < (OB ? 2 : 4); i++) {
-                    if (OB) *((uint4*)((uint16_t*)p.out + to) + i) = make_uint4(f32x2_to_bf16x2(y[8 * i], y[8 * i + 1]), f32x2_to_bf16x2(y[8 * i + 2], y[8 * i + 3]), f32x2_to_bf16x2(y[8 * i + 4], y[8 * i + 5]), f32x2_to_bf16x2(y[8 * i + 6], y[8 * i + 7]));
-                    else *(float4*)((float*)p.out + to + 4 * i) = make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+        for (int c = 0; c < 2; c++)
+#pragma unroll
+            for (int r = 0; r < RT; r++)
+                if (half) *(v4f*)&join[32 * w + 16 * c + col][16 * r + 4 * g] = acc[c][r];
+        __syncthreads();
+#pragma unroll
+        for (int c = 0; c < 2; c++)
+#pragma unroll
+            for (int r = 0; r < RT; r++) {
+                const int at = 32 * w + 16 * c + col, rank = r0 + 16 * r + 4 * g;
+                if (half || at >= u.n || rank >= p.rank_pitch) continue;
+                *(v4f*)(p.h + ((int64_t)split * p.rows + rows[at]) * p.rank_pitch + rank) = acc[c][r] + *(const v4f*)&join[at][16 * r + 4 * g];
+            }
+        __syncthreads();
+    }
+}
+
+// h as the second product takes it: the parts of K summed and scaled, against bf16 factors
+// as three bf16, [row][term][ranks], zeros behind R.
+template <bool WB>
+__device__ __forceinline__ v4f h_of(const LoraBatched& p, int64_t row, int r, float scale) {
+    const float* from = p.h + row * p.rank_pitch + r;
+    const int64_t step = (int64_t)p.rows * p.rank_pitch;
+    v4f sum = {0, 0, 0, 0};
+    if (r >= p.R) return sum;
+#pragma unroll 1
+    for (int s = 0; s < p.splits; s += 4) {
+        v4f x[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[e] = *(const v4f*)(from + min(s + e, p.splits - 1) * step);
+        sum += x[0];
+#pragma unroll
+        for (int e = 1; e < 4; e++)
+            if (s + e < p.splits) sum += x[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) sum[e] = r + e < p.R ? sum[e] * scale : 0.0f;
+    return sum;
+}
+template <bool WB>
+__device__ __forceinline__ void store_h(v4f sum, void* to, int term) {
+    if constexpr (WB) {
+#pragma unroll
+        for (int t = 0; t < 3; t++) {
+            const uint32_t lo = f32x2_to_bf16x2(sum[0], sum[1]), hi = f32x2_to_bf16x2(sum[2], sum[3]);
+            *(uint2*)((uint16_t*)to + t * term) = make_uint2(lo, hi);
+            // What an infinity leaves is 0, not NaN.
+            const float y[4] = {bf16_to_f32(lo & 0xffffu), bf16_to_f32(lo >> 16), bf16_to_f32(hi & 0xffffu), bf16_to_f32(hi >> 16)};
+#pragma unroll
+            for (int e = 0; e < 4; e++) sum[e] = __builtin_isfinite(y[e]) ? sum[e] - y[e] : 0.0f;
+        }
+    } else {
+        *(v4f*)to = sum;
+    }
+}
+
+// The same once for all, where many blocks want it (4352 rows on 64 ranks, six parts: each
+// block of the update took 14 us to sum them).
+template <bool WB>
+__global__ __launch_bounds__(256) void lora_batched_join_kernel(LoraBatched p, int ranks) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, row = i / (ranks / 4);
+    if (row >= p.rows) return;
+    const int a = p.adapter[row], r = 4 * (int)(i - row * (ranks / 4));
+    if (a < 0 || a >= p.adapters) return;
+    store_h<WB>(h_of<WB>(p, row, r, p.scale ? p.scale[a] : 1.0f), (char*)p.joined + (row * ranks * (WB ? 3 : 1) + r) * (WB ? 2 : 4), ranks);
+}
+
+// The update.  A wave has 64 columns n of out: lane l's are the four from 4 (l % 16) on, column
+// l % 16 of each of four tiles of the matrix instruction, in rows 4 (l / 16) + i, so that
+// 16 lanes write 64 columns of a row together.  A block has 256 `chunks` columns for all
+// rows of every `parts`-th class of its tile, `most` rows' h in LDS and 16 rows at a time, the
+// base of the four times 16 after them loading meanwhile.  B's first KS steps of 32 ranks stay in
+// registers, further ones are read again for each 16 rows.
+template <bool WB, bool OB, int KS, bool WIDE>
+__global__ __launch_bounds__(256, 2) void lora_batched_up_kernel(LoraBatched p, int tiles, int around, int parts, int chunks, int most) {
+    constexpr int T = WB ? 3 : 1;  // terms of h
+    constexpr int O = OB ? 2 : 4;  // bytes of an element
+    constexpr int A = !WIDE ? 1 : OB ? 4 : 2;  // bases ahead
+    typedef std::conditional_t<OB, any2, any4> Four;
+    __shared__ int rows[kLoraTile];
+    extern __shared__ __align__(16) uint8_t lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int tile = lora_tile(blockIdx.x % around, around, tiles), col = lane & 15, g = lane >> 4;
+    if (tile >= tiles) return;
+    const int ranks = (p.R + 31) / 32 * 32, pitch = ranks + (WB ? 8 : 4);
+    uint16_t* hb = (uint16_t*)lds;  // [row][term][pitch]
+    float* hf = (float*)lds;        // [row][pitch]
+    const int first = blockIdx.y * chunks * 256 + 64 * wave;
+    const int classes = p.counts[tile];
+#pragma unroll 1
+    for (int i = blockIdx.x / around; i < classes; i += parts) {
+        const LoraClass cls = p.classes[(int64_t)tile * kLoraTile + i];
+        const bool some = cls.adapter >= 0;
+        const int all = __popcll(cls.rows[0]) + __popcll(cls.rows[1]);
+        if (!some && p.out == p.base) continue;
+#pragma unroll 1
+        for (int skip = 0; skip < all; skip += most) {
+            const int n = min(all - skip, most), cols = (n + 15) / 16;
+            class_rows(cls.rows, tile, skip, most, rows);
+            __syncthreads();
+            // B's rows of a chunk, 32 ranks.
+            auto load_b = [&](int n0, int k0, Eight<WB> (&b)[4]) __attribute__((always_inline)) {
+                const int k = k0 + 8 * g;
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    const char* from = (const char*)p.B + (cls.adapter * p.b_adapter + min(n0 + 4 * col + t, p.N - 1) * p.b_row) * (WB ? 2 : 4);
+                    if (p.R % 8 == 0) b[t] = k < p.R ? load_eight<WB>(from, k) : Eight<WB>{};
+                    else b[t] = load_masked<WB>(from, k, p.R, p.b_end);
                 }
-            } else {
+            };
+            // The base of 16 rows' columns, those from the last on: of the next chunk.
+            Four base[A][4] = {};
+            auto load_base = [&](int n0, int c, Four (&base)[4]) __attribute__((always_inline)) {
+                if (c >= cols) c -= cols, n0 += 256;
+                if (!p.base || c >= cols || n0 + 64 > p.N || n0 >= first + 256 * chunks) return;
 #pragma unroll
-                for (int j = 0; j < 16; j++) {
-                    if (n + j >= p.N) break;
-                    if (p.base) y[j] += OB ? bf16_to_f32(((const uint16_t*)p.base)[from + j]) : ((const float*)p.base)[from + j];
-                    if (OB) ((uint16_t*)p.out)[to + j] = (uint16_t)f32_to_bf16(y[j]);
-                    else ((float*)p.out)[to + j] = y[j];
+                for (int i = 0; i < 4; i++)
+                    base[i] = *(const Four*)((const char*)p.base + (rows[min(16 * c + 4 * g + i, n - 1)] * p.ld_base + n0 + 4 * col) * O);
+            };
+#pragma unroll 1
+            for (int chunk = 0; chunk < chunks; chunk++) {
+                const int n0 = first + 256 * chunk;
+                Eight<WB> b[KS][4];
+                if (some && n0 < p.N) {
+#pragma unroll
+                    for (int k = 0; k < KS; k++) load_b(n0, 32 * k, b[k]);
+                }
+                if (chunk == 0) {
+                    if (first < p.N) {
+#pragma unroll
+                        for (int j = 0; j < A; j++)
+                            if (j < cols) load_base(first, j, base[j]);
+                    }
+                    if (some && WIDE) {  // also by a wave without columns
+                        const int pieces = ranks * T * (WB ? 2 : 4) / 16, each = ranks * (WB ? 2 : 4) / 16;
+#pragma unroll 4
+                        for (int j = threadIdx.x; j < n * pieces; j += 256) {
+                            const int c = j / pieces, e = j - c * pieces;
+                            const uint4 v = *(const uint4*)((const char*)p.joined + ((int64_t)rows[c] * pieces + e) * 16);
+                            *(uint4*)(lds + (c * T + e / each) * pitch * (WB ? 2 : 4) + e % each * 16) = v;
+                        }
+                        __syncthreads();
+                    } else if (some) {
+                        const float scale = p.scale ? p.scale[cls.adapter] : 1.0f;
+#pragma unroll 1
+                        for (int j = threadIdx.x; j < n * ranks / 4; j += 256) {
+                            const int c = j / (ranks / 4), r = 4 * (j - c * (ranks / 4));
+                            store_h<WB>(h_of<WB>(p, rows[c], r, scale), lds + (c * T * pitch + r) * (WB ? 2 : 4), pitch);
+                        }
+                        __syncthreads();
+                    }
+                }
+                if (n0 >= p.N) break;
+                auto turn = [&](int c, Four (&base)[4]) __attribute__((always_inline)) {
+                    v4f acc[4];
+#pragma unroll
+                    for (int t = 0; t < 4; t++) acc[t] = v4f{0, 0, 0, 0};
+                    auto multiply = [&](int k0, const Eight<WB> (&b)[4]) __attribute__((always_inline)) {
+#pragma unroll
+                        for (int term = T - 1; term >= 0; term--) {
+                            Eight<WB> h;
+                            // Rows behind the last hold whatever lies there; theirs are not stored.
+                            if constexpr (WB) {
+                                *(uint4*)h.w = *(const uint4*)(hb + (min(16 * c + col, n - 1) * T + term) * pitch + k0 + 8 * g);
+                            } else {
+                                *(v4f*)h.w = *(const v4f*)(hf + min(16 * c + col, n - 1) * pitch + k0 + 8 * g);
+                                *(v4f*)(h.w + 4) = *(const v4f*)(hf + min(16 * c + col, n - 1) * pitch + k0 + 8 * g + 4);
+                            }
+#pragma unroll
+                            for (int t = 0; t < 4; t++) acc[t] = product(h, b[t], acc[t]);
+                        }
+                    };
+                    if (some) {
+#pragma unroll
+                        for (int k = 0; k < KS; k++) multiply(32 * k, b[k]);
+#pragma unroll 1
+                        for (int k0 = 32 * KS; k0 < ranks; k0 += 32) {
+                            Eight<WB> rest[4];
+                            load_b(n0, k0, rest);
+                            multiply(k0, rest);
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        if (16 * c + 4 * g + i >= n) continue;
+                        const int64_t row = rows[16 * c + 4 * g + i];
+                        char* to = (char*)p.out + (row * p.ldo + n0 + 4 * col) * O;
+                        float y[4];
+                        if (n0 + 64 <= p.N) {
+#pragma unroll
+                            for (int t = 0; t < 4; t++) {
+                                const uint32_t w = base[i][OB ? t >> 1 : t];
+                                const float was = OB ? bf16_to_f32(t & 1 ? w >> 16 : w & 0xffffu) : __uint_as_float(w);
+                                y[t] = p.base ? acc[t][i] + was : acc[t][i];
+                            }
+                            Four w;
+#pragma unroll
+                            for (int t = 0; t < (OB ? 2 : 4); t++) w[t] = OB ? f32x2_to_bf16x2(y[2 * t % 4], y[(2 * t + 1) % 4]) : __float_as_uint(y[t]);
+                            *(Four*)to = w;
+                        } else {
+                            const char* from = (const char*)p.base + (row * p.ld_base + n0 + 4 * col) * O;
+#pragma unroll
+                            for (int t = 0; t < 4; t++) {
+                                if (n0 + 4 * col + t >= p.N) continue;
+                                y[t] = acc[t][i];
+                                if (p.base) y[t] += OB ? bf16_to_f32(((const uint16_t*)from)[t]) : ((const float*)from)[t];
+                                if (OB) ((uint16_t*)to)[t] = (uint16_t)f32_to_bf16(y[t]);
+                                else ((float*)to)[t] = y[t];
+                            }
+                        }
+                    }
+                };
+                // Bases in turn: c's in c % A where cols is a multiple of A, else begun anew a chunk.
+#pragma unroll 1
+                for (int c = 0; c < cols; c += A) {
+#pragma unroll
+                    for (int j = 0; j < A; j++) {
+                        if (c + j >= cols) continue;
+                        turn(c + j, base[j]);
+                        if (c + j + A < cols || cols % A == 0) load_base(n0, c + j + A, base[j]);
+                    }
+                }
+                if (cols % A) {
+#pragma unroll
+                    for (int j = 0; j < A; j++)
+                        if (j < cols) load_base(n0, cols + j, base[j]);
                 }
             }
+            __syncthreads();
         }
     }
 }
@@ -294,61 +714,98 @@ int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 int rank_pitch(int64_t R) { return (int)(16 * ceil_div(R, 16)); }
 
-// Parts of K: enough blocks where there are few rows, a part no shorter than 16 steps of 32.
+constexpr size_t kMaxLds = 159 << 10;  // a compute unit's 160 KB, less the rows' numbers
+
+// Rows from which on blocks take whole tiles' rows.
+constexpr int64_t kWideRows = 512;
+
+// Parts of K: enough blocks where there are few rows, a part no shorter than 512; of wide
+// blocks no more than fit the compute units at once, with room for tiles of two classes.
 int splits_of(int64_t rows, int64_t K) {
-    return (int)std::clamp<int64_t>(512 / ceil_div(rows, kCols), 1, std::min<int64_t>(kSplits, ceil_div(K, 512)));
+    const int64_t want = rows >= kWideRows ? 256 / (ceil_div(rows, kLoraTile) * 5 / 4) : 512 / ceil_div(rows, kFewCols);
+    return (int)std::clamp<int64_t>(want, 1, std::min<int64_t>(kSplits, ceil_div(K, 512)));
 }
 
-bool at16(const void* p, int64_t bytes1, int64_t bytes2 = 0) { return (uintptr_t)p % 16 == 0 && bytes1 % 16 == 0 && bytes2 % 16 == 0; }
+template <bool XB, bool WB, int RT>
+void down_ranks(hipStream_t stream, const LoraBatched& p, int tiles, int around, int classes, int groups) {
+    if (p.rows >= kWideRows) {
+        const int parts = (int)std::clamp<int64_t>(256 / ((int64_t)tiles * p.splits * groups), 1, classes);
+        hipLaunchKernelGGL((lora_batched_down_wide_kernel<XB, WB, RT>), dim3((unsigned)(around * parts), (unsigned)p.splits, (unsigned)groups), dim3(512), 0, stream,
+                           p, tiles, around, parts);
+        return;
+    }
+    // A tile's units are more than its classes by those of more than kFewCols rows.
+    const int units = std::min(classes + kLoraTile / kFewCols - 1, kLoraTile);
+    const int parts = (int)std::clamp<int64_t>(1024 / ((int64_t)tiles * p.splits * groups), 1, units);
+    hipLaunchKernelGGL((lora_batched_down_kernel<XB, WB, RT>), dim3((unsigned)(around * parts), (unsigned)p.splits, (unsigned)groups), dim3(256), 0, stream, p, tiles,
+                       around, parts);
+}
 
-template <bool XB, bool WB, bool VEC>
-void down(hipStream_t stream, const LoraBatched& p, int tiles, int units) {
+template <bool XB, bool WB>
+void down(hipStream_t stream, const LoraBatched& p, int tiles, int around, int classes) {
     const int rt = (p.R + 15) / 16;
-    const dim3 block(256);
-    auto grid = [&](int RT) { return dim3((unsigned)(tiles * units), (unsigned)p.splits, (unsigned)((rt + RT - 1) / RT)); };
-    if (rt == 1) hipLaunchKernelGGL((lora_batched_down_kernel<XB, WB, VEC, 1>), grid(1), block, 0, stream, p, tiles);
-    else if (rt == 2) hipLaunchKernelGGL((lora_batched_down_kernel<XB, WB, VEC, 2>), grid(2), block, 0, stream, p, tiles);
-    else hipLaunchKernelGGL((lora_batched_down_kernel<XB, WB, VEC, 4>), grid(4), block, 0, stream, p, tiles);
+    if (rt == 1) down_ranks<XB, WB, 1>(stream, p, tiles, around, classes, 1);
+    else if (rt == 2) down_ranks<XB, WB, 2>(stream, p, tiles, around, classes, 1);
+    else down_ranks<XB, WB, 4>(stream, p, tiles, around, classes, (rt + 3) / 4);
+}
+
+template <bool WB, bool OB, int KS, bool WIDE>
+hipError_t up_ranks(hipStream_t stream, const LoraBatched& p, int tiles, int around, int classes) {
+    const int ranks = (p.R + 31) / 32 * 32, all = (p.N + 255) / 256;
+    const size_t row = WB ? 3 * (ranks + 8) * 2 : (ranks + 4) * 4;
+    const int most = row * kLoraTile <= kMaxLds ? kLoraTile : kLoraTile / 2;
+    const size_t lds = row * std::min(most, (p.rows + 15) / 16 * 16);
+    if (lds > 65536) {
+        const hipError_t e = hipFuncSetAttribute((const void*)lora_batched_up_kernel<WB, OB, KS, WIDE>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (e != hipSuccess) return e;
+    }
+    // Two blocks a compute unit.
+    const int want = (int)std::max<int64_t>(1, 512 / tiles);
+    const int chunks = (all + std::min(want, all) - 1) / std::min(want, all), across = (all + chunks - 1) / chunks;
+    const int parts = (int)std::clamp<int64_t>((WIDE ? 512 : 1024) / ((int64_t)tiles * across), 1, classes);
+    const dim3 grid((unsigned)(around * parts), (unsigned)across), block(256);
+    if (WIDE) {
+        const int64_t pieces = (int64_t)p.rows * (ranks / 4);
+        hipLaunchKernelGGL(lora_batched_join_kernel<WB>, dim3((unsigned)ceil_div(pieces, 256)), block, 0, stream, p, ranks);
+    }
+    hipLaunchKernelGGL((lora_batched_up_kernel<WB, OB, KS, WIDE>), grid, block, lds, stream, p, tiles, around, parts, chunks, most);
+    return hipGetLastError();
 }
 
 template <bool WB, bool OB>
-void up(hipStream_t stream, const LoraBatched& p, int tiles, int units, bool vec_b, bool vec_o) {
-    const int ranks = (p.R + 31) / 32 * 32, all = (p.N + 255) / 256;
-    const size_t lds = WB ? 3 * kCols * (ranks + 8) * 2 : kCols * (ranks + 4) * 4;
-    const int want = (int)std::max<int64_t>(1, 2048 / ceil_div(p.rows, kCols));
-    const int chunks = (all + std::min(want, all) - 1) / std::min(want, all);
-    const dim3 grid((unsigned)(tiles * units), (unsigned)((all + chunks - 1) / chunks)), block(256);
-    if (vec_b && vec_o) hipLaunchKernelGGL((lora_batched_up_kernel<WB, OB, true, true>), grid, block, lds, stream, p, tiles, chunks);
-    else if (vec_b) hipLaunchKernelGGL((lora_batched_up_kernel<WB, OB, true, false>), grid, block, lds, stream, p, tiles, chunks);
-    else if (vec_o) hipLaunchKernelGGL((lora_batched_up_kernel<WB, OB, false, true>), grid, block, lds, stream, p, tiles, chunks);
-    else hipLaunchKernelGGL((lora_batched_up_kernel<WB, OB, false, false>), grid, block, lds, stream, p, tiles, chunks);
+hipError_t up(hipStream_t stream, const LoraBatched& p, int tiles, int around, int classes) {
+    if (p.joined) return p.R <= 32 ? up_ranks<WB, OB, 1, true>(stream, p, tiles, around, classes) : up_ranks<WB, OB, 2, true>(stream, p, tiles, around, classes);
+    return up_ranks<WB, OB, 1, false>(stream, p, tiles, around, classes);
 }
+
+// h, the tiles' classes and how many they are.
+size_t h_bytes(int64_t rows, int64_t K, int64_t R) { return (size_t)splits_of(rows, K) * rows * rank_pitch(R) * sizeof(float); }
 
 }  // namespace
 
 size_t lora_batched_workspace(int64_t rows, int64_t K, int64_t R) {
-    return (size_t)splits_of(rows, K) * rows * rank_pitch(R) * sizeof(float);
+    const size_t joined = rows >= kWideRows ? (size_t)rows * (32 * ceil_div(R, 32)) * 6 : 0;  // three bf16, or fp32
+    return h_bytes(rows, K, R) + (size_t)ceil_div(rows, kLoraTile) * (kLoraTile * sizeof(LoraClass) + 16) + joined;
 }
 
 hipError_t launch_lora_batched(hipStream_t stream, LoraBatched p) {
     p.splits = splits_of(p.rows, p.K);
     p.rank_pitch = rank_pitch(p.R);
-    const int tiles = (p.rows + 63) / 64;
-    // Units of a tile, at most: a class each, and one more where a class has more than kCols rows.
-    const int units = std::min(std::min(64, p.adapters + 1) + 1, 64);
-    const int xe = p.x_bf16 ? 2 : 4, we = p.w_bf16 ? 2 : 4, oe = p.out_bf16 ? 2 : 4;
-    const bool vec = p.K % 8 == 0 && at16(p.x, p.ldx * xe) && at16(p.A, p.a_row * we, p.a_adapter * we);
-    if (p.x_bf16 && p.w_bf16) vec ? down<true, true, true>(stream, p, tiles, units) : down<true, true, false>(stream, p, tiles, units);
-    else if (p.x_bf16) vec ? down<true, false, true>(stream, p, tiles, units) : down<true, false, false>(stream, p, tiles, units);
-    else if (p.w_bf16) vec ? down<false, true, true>(stream, p, tiles, units) : down<false, true, false>(stream, p, tiles, units);
-    else vec ? down<false, false, true>(stream, p, tiles, units) : down<false, false, false>(stream, p, tiles, units);
+    const int tiles = (p.rows + kLoraTile - 1) / kLoraTile, around = tiles >= kSpread ? (tiles + 7) / 8 * 8 : tiles;
+    auto end = [](const void* from, int64_t elements, bool b16) { return (const char*)from + elements * (b16 ? 2 : 4); };
+    p.x_end = end(p.x, (p.rows - 1) * p.ldx + p.K, p.x_bf16);
+    p.a_end = end(p.A, (p.adapters - 1) * p.a_adapter + (p.R - 1) * p.a_row + p.K, p.w_bf16);
+    p.b_end = end(p.B, (p.adapters - 1) * p.b_adapter + (p.N - 1) * p.b_row + p.R, p.w_bf16);
+    p.classes = (LoraClass*)((char*)p.h + h_bytes(p.rows, p.K, p.R));
+    p.counts = (int*)(p.classes + (int64_t)tiles * kLoraTile);
+    p.joined = p.rows >= kWideRows ? (void*)((char*)p.counts + (int64_t)tiles * 16) : nullptr;
+    const int classes = std::min({kLoraTile - 1, p.adapters, p.rows}) + 1;  // of a tile, at most
+    if (p.x_bf16) p.w_bf16 ? down<true, true>(stream, p, tiles, around, classes) : down<true, false>(stream, p, tiles, around, classes);
+    else p.w_bf16 ? down<false, true>(stream, p, tiles, around, classes) : down<false, false>(stream, p, tiles, around, classes);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    const bool vec_b = p.R % 8 == 0 && at16(p.B, p.b_row * we, p.b_adapter * we);
-    const bool vec_o = p.N % 16 == 0 && at16(p.out, p.ldo * oe) && (!p.base || at16(p.base, p.ld_base * oe));
-    if (p.w_bf16) p.out_bf16 ? up<true, true>(stream, p, tiles, units, vec_b, vec_o) : up<true, false>(stream, p, tiles, units, vec_b, vec_o);
-    else p.out_bf16 ? up<false, true>(stream, p, tiles, units, vec_b, vec_o) : up<false, false>(stream, p, tiles, units, vec_b, vec_o);
-    return hipGetLastError();
+    if (p.w_bf16) return p.out_bf16 ? up<true, true>(stream, p, tiles, around, classes) : up<true, false>(stream, p, tiles, around, classes);
+    return p.out_bf16 ? up<false, true>(stream, p, tiles, around, classes) : up<false, false>(stream, p, tiles, around, classes);
 }
 
 }  // namespace phi_dev

@@ -45,9 +45,13 @@ struct LoraBatched {
     const void* base;    // null: 0
     void* out;
     float* h;        // [splits][rows][rank_pitch]: parts of A x
+    struct LoraClass* classes;  // [tiles][64]
+    int* counts;                // [tiles]
+    void* joined;               // h as the second product takes it; null: from its parts
     int64_t ldx, a_adapter, a_row, b_adapter, b_row, ld_base, ldo;
     int rows, K, N, R, adapters, splits, rank_pitch;
     bool x_bf16, w_bf16, out_bf16;
+    const char *x_end, *a_end, *b_end;  // of the operands' memory
 };
 hipError_t launch_lora_batched(hipStream_t stream, LoraBatched p);
 size_t lora_batched_workspace(int64_t rows, int64_t K, int64_t R);

@@ -233,7 +233,7 @@ phi_status phi_hip_lora_batched(phi_stream_t stream, const void* x, int x_dtype,
     if (meet(ws, to) || meet(ws, from)) return fail(PHI_ERR_ARG, "%s: the workspace overlaps an operand", who);
     const bool same = base == out && (rows == 1 || ld_base == ldo);
     if (!same && meet(to, from)) return fail(PHI_ERR_ARG, "%s: out overlaps base", who);
-    const phi_dev::LoraBatched p{x, A, B, adapter, scale, base, out, (float*)workspace, ldx, a_adapter_stride, a_row_stride, b_adapter_stride,
+    const phi_dev::LoraBatched p{x, A, B, adapter, scale, base, out, (float*)workspace, nullptr, nullptr, nullptr, ldx, a_adapter_stride, a_row_stride, b_adapter_stride,
                                  b_row_stride, ld_base, ldo, (int)rows, (int)K, (int)N, (int)R, (int)adapters, 0, 0,
                                  x_dtype == PHI_BF16, w_dtype == PHI_BF16, out_dtype == PHI_BF16};
     return check_hip(phi_dev::launch_lora_batched((hipStream_t)stream, p), who);
