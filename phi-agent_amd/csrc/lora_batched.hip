@@ -32,7 +32,7 @@ namespace {
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 
 constexpr int kSplits = 8;
-constexpr int kSpread = 32;  // tiles, from which on each XCD has neighbours
+constexpr int kSpread = 128;  // places, from which on each XCD has neighbours
 
 // Up to `most` rows of one class, from the skip-th on.
 struct LoraUnit {
@@ -122,9 +122,10 @@ struct LoraClasses {
     }
 };
 
-// Tile number `id` of `around`: where these are 8 ceil(tiles / 8), neighbours, which often
-// have one adapter, on one XCD, whose L2 keeps its factors (blocks go round the eight).
-__device__ __forceinline__ int lora_tile(int id, int around, int tiles) { return around >= kSpread ? (id & 7) * (around >> 3) + (id >> 3) : id; }
+// Block number `id` of `around` as a place (tile x across): where these are 8 ceil(places /
+// 8), neighbours, which often have one adapter, on one XCD, whose L2 keeps its factors
+// (blocks go round the eight).
+__device__ __forceinline__ int lora_place(int id, int around) { return around >= kSpread ? (id & 7) * (around >> 3) + (id >> 3) : id; }
 
 // Rows of a class from the skip-th on, `most` of them, in LDS; every wave writes the same.
 __device__ __forceinline__ void class_rows(const uint64_t (&mask)[2], int tile, int skip, int most, int* rows) {
@@ -241,7 +242,7 @@ __global__ __launch_bounds__(256, 2) void lora_batched_down_kernel(LoraBatched p
     __shared__ LoraTable table;
     __shared__ LoraUnit found;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int tile = lora_tile(blockIdx.x % around, around, tiles), split = blockIdx.y, r0 = 16 * RT * blockIdx.z;
+    const int at = lora_place(blockIdx.x % around, around), tile = at / p.splits, split = at - tile * p.splits, r0 = 16 * RT * blockIdx.z;
     if (tile >= tiles) return;
     const int col = lane & 15, g = lane >> 4;
     const int steps = (p.K + 31) / 32, waves = 4 * p.splits, me = 4 * split + wave;
@@ -352,7 +353,7 @@ __global__ __launch_bounds__(512, 2) void lora_batched_down_wide_kernel(LoraBatc
     __shared__ LoraTable table;
     __shared__ LoraUnit found;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = wave >> 2, w = wave & 3;
-    const int tile = lora_tile(blockIdx.x % around, around, tiles), split = blockIdx.y, r0 = 16 * RT * blockIdx.z;
+    const int at = lora_place(blockIdx.x % around, around), tile = at / p.splits, split = at - tile * p.splits, r0 = 16 * RT * blockIdx.z;
     if (tile >= tiles) return;
     const int col = lane & 15, g = lane >> 4;
     const int steps = (p.K + kStep - 1) / kStep, ranges = 2 * p.splits, me = 2 * split + half;
@@ -405,10 +406,12 @@ __global__ __launch_bounds__(512, 2) void lora_batched_down_wide_kernel(LoraBatc
             RX x[2];
             any4 a[kMine];
         };
+        // Without a branch (what loads meet a branch is waited for with all that came after
+        // it): past the last whole step the last again, for rows behind the last the last's.
+        const int last = max(min(s1, p.K / kStep) - 1, 0);
         auto load = [&](Step& t, int s) __attribute__((always_inline)) {
-            if (s >= min(s1, p.K / kStep)) return;
-            const int k = kStep * s;
-            if (mine) t.x[0].load(xs[0], k), t.x[1].load(xs[1], k);
+            const int k = kStep * min(s, last);
+            t.x[0].load(xs[0], k), t.x[1].load(xs[1], k);
 #pragma unroll
             for (int j = 0; j < kMine; j++) t.a[j] = *(const any4*)(as[j] + (size_t)(uint32_t)(k + RA::k()) * (WB ? 2 : 4));
         };
@@ -542,27 +545,31 @@ __global__ __launch_bounds__(256) void lora_batched_join_kernel(LoraBatched p, i
     store_h<WB>(h_of<WB>(p, row, r, p.scale ? p.scale[a] : 1.0f), (char*)p.joined + (row * ranks * (WB ? 3 : 1) + r) * (WB ? 2 : 4), ranks);
 }
 
-// The update.  A wave has 64 columns n of out: lane l's are the four from 4 (l % 16) on, column
-// l % 16 of each of four tiles of the matrix instruction, in rows 4 (l / 16) + i, so that
-// 16 lanes write 64 columns of a row together.  A block has 256 `chunks` columns for all
+// The update.  A wave has 16 NT columns n of out: lane l's are the NT from NT (l % 16) on, column
+// l % 16 of each of NT tiles of the matrix instruction, in rows 4 (l / 16) + i, so that
+// 16 lanes read and write 128 bytes of a row together, 256 of many rows (44.6 MB of base: 20 us
+// in pieces of 128).  A block has 4 waves' columns `chunks` times for all
 // rows of every `parts`-th class of its tile, `most` rows' h in LDS and 16 rows at a time, the
 // base of the four times 16 after them loading meanwhile.  B's first KS steps of 32 ranks stay in
 // registers, further ones are read again for each 16 rows.
+template <bool OB, bool WIDE> constexpr int up_tiles = OB && WIDE ? 4 : 4;
+
 template <bool WB, bool OB, int KS, bool WIDE>
-__global__ __launch_bounds__(256, 2) void lora_batched_up_kernel(LoraBatched p, int tiles, int around, int parts, int chunks, int most) {
+__global__ __launch_bounds__(256, 2) void lora_batched_up_kernel(LoraBatched p, int tiles, int across, int around, int parts, int chunks, int most) {
     constexpr int T = WB ? 3 : 1;  // terms of h
     constexpr int O = OB ? 2 : 4;  // bytes of an element
     constexpr int A = !WIDE ? 1 : OB ? 4 : 2;  // bases ahead
-    typedef std::conditional_t<OB, any2, any4> Four;
+    constexpr int NT = up_tiles<OB, WIDE>, kWave = 16 * NT, kBlock = 4 * kWave;
+    typedef std::conditional_t<NT * O == 8, any2, any4> Run;
     __shared__ int rows[kLoraTile];
     extern __shared__ __align__(16) uint8_t lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int tile = lora_tile(blockIdx.x % around, around, tiles), col = lane & 15, g = lane >> 4;
+    const int at = lora_place(blockIdx.x % around, around), tile = at / across, col = lane & 15, g = lane >> 4;
     if (tile >= tiles) return;
     const int ranks = (p.R + 31) / 32 * 32, pitch = ranks + (WB ? 8 : 4);
     uint16_t* hb = (uint16_t*)lds;  // [row][term][pitch]
     float* hf = (float*)lds;        // [row][pitch]
-    const int first = blockIdx.y * chunks * 256 + 64 * wave;
+    const int first = (at - tile * across) * chunks * kBlock + kWave * wave;
     const int classes = p.counts[tile];
 #pragma unroll 1
     for (int i = blockIdx.x / around; i < classes; i += parts) {
@@ -576,37 +583,38 @@ __global__ __launch_bounds__(256, 2) void lora_batched_up_kernel(LoraBatched p, 
             class_rows(cls.rows, tile, skip, most, rows);
             __syncthreads();
             // B's rows of a chunk, 32 ranks.
-            auto load_b = [&](int n0, int k0, Eight<WB> (&b)[4]) __attribute__((always_inline)) {
+            auto load_b = [&](int n0, int k0, Eight<WB> (&b)[NT]) __attribute__((always_inline)) {
                 const int k = k0 + 8 * g;
 #pragma unroll
-                for (int t = 0; t < 4; t++) {
-                    const char* from = (const char*)p.B + (cls.adapter * p.b_adapter + min(n0 + 4 * col + t, p.N - 1) * p.b_row) * (WB ? 2 : 4);
+                for (int t = 0; t < NT; t++) {
+                    const char* from = (const char*)p.B + (cls.adapter * p.b_adapter + min(n0 + NT * col + t, p.N - 1) * p.b_row) * (WB ? 2 : 4);
                     if (p.R % 8 == 0) b[t] = k < p.R ? load_eight<WB>(from, k) : Eight<WB>{};
                     else b[t] = load_masked<WB>(from, k, p.R, p.b_end);
                 }
             };
-            // The base of 16 rows' columns, those from the last on: of the next chunk.
-            Four base[A][4] = {};
-            auto load_base = [&](int n0, int c, Four (&base)[4]) __attribute__((always_inline)) {
-                if (c >= cols) c -= cols, n0 += 256;
-                if (!p.base || c >= cols || n0 + 64 > p.N || n0 >= first + 256 * chunks) return;
+            // The base of 16 rows' columns (rows behind the last: the last again, and of no base
+            // whatever out holds, unused).  No branch: what loads meet a branch is waited for
+            // with all that came after it.
+            Run base[A][4] = {};
+            const char* const was = (const char*)(p.base ? p.base : p.out);
+            const int64_t ld_was = p.base ? p.ld_base : p.ldo;
+            auto load_base = [&](int n0, int c, Run (&base)[4]) __attribute__((always_inline)) {
 #pragma unroll
-                for (int i = 0; i < 4; i++)
-                    base[i] = *(const Four*)((const char*)p.base + (rows[min(16 * c + 4 * g + i, n - 1)] * p.ld_base + n0 + 4 * col) * O);
+                for (int i = 0; i < 4; i++) base[i] = *(const Run*)(was + (rows[min(16 * c + 4 * g + i, n - 1)] * ld_was + n0 + NT * col) * O);
             };
+            const int ahead = cols / A * A;  // tiles whose bases are loaded ahead
 #pragma unroll 1
             for (int chunk = 0; chunk < chunks; chunk++) {
-                const int n0 = first + 256 * chunk;
-                Eight<WB> b[KS][4];
+                const int n0 = first + kBlock * chunk;
+                Eight<WB> b[KS][NT];
                 if (some && n0 < p.N) {
 #pragma unroll
                     for (int k = 0; k < KS; k++) load_b(n0, 32 * k, b[k]);
                 }
                 if (chunk == 0) {
-                    if (first < p.N) {
+                    if (ahead && first + kWave <= p.N) {
 #pragma unroll
-                        for (int j = 0; j < A; j++)
-                            if (j < cols) load_base(first, j, base[j]);
+                        for (int j = 0; j < A; j++) load_base(first, j, base[j]);
                     }
                     if (some && WIDE) {  // also by a wave without columns
                         const int pieces = ranks * T * (WB ? 2 : 4) / 16, each = ranks * (WB ? 2 : 4) / 16;
@@ -628,11 +636,12 @@ __global__ __launch_bounds__(256, 2) void lora_batched_up_kernel(LoraBatched p, 
                     }
                 }
                 if (n0 >= p.N) break;
-                auto turn = [&](int c, Four (&base)[4]) __attribute__((always_inline)) {
-                    v4f acc[4];
+                const bool inside = n0 + kWave <= p.N;
+                auto turn = [&](int c, Run (&base)[4], bool inside) __attribute__((always_inline)) {
+                    v4f acc[NT];
 #pragma unroll
-                    for (int t = 0; t < 4; t++) acc[t] = v4f{0, 0, 0, 0};
-                    auto multiply = [&](int k0, const Eight<WB> (&b)[4]) __attribute__((always_inline)) {
+                    for (int t = 0; t < NT; t++) acc[t] = v4f{0, 0, 0, 0};
+                    auto multiply = [&](int k0, const Eight<WB> (&b)[NT]) __attribute__((always_inline)) {
 #pragma unroll
                         for (int term = T - 1; term >= 0; term--) {
                             Eight<WB> h;
@@ -644,7 +653,7 @@ __global__ __launch_bounds__(256, 2) void lora_batched_up_kernel(LoraBatched p, 
                                 *(v4f*)(h.w + 4) = *(const v4f*)(hf + min(16 * c + col, n - 1) * pitch + k0 + 8 * g + 4);
                             }
 #pragma unroll
-                            for (int t = 0; t < 4; t++) acc[t] = product(h, b[t], acc[t]);
+                            for (int t = 0; t < NT; t++) acc[t] = product(h, b[t], acc[t]);
                         }
                     };
                     if (some) {
@@ -652,55 +661,66 @@ __global__ __launch_bounds__(256, 2) void lora_batched_up_kernel(LoraBatched p, 
                         for (int k = 0; k < KS; k++) multiply(32 * k, b[k]);
 #pragma unroll 1
                         for (int k0 = 32 * KS; k0 < ranks; k0 += 32) {
-                            Eight<WB> rest[4];
+                            Eight<WB> rest[NT];
                             load_b(n0, k0, rest);
                             multiply(k0, rest);
                         }
                     }
+                    if (inside) {
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        if (16 * c + 4 * g + i >= n) continue;
-                        const int64_t row = rows[16 * c + 4 * g + i];
-                        char* to = (char*)p.out + (row * p.ldo + n0 + 4 * col) * O;
-                        float y[4];
-                        if (n0 + 64 <= p.N) {
+                        for (int i = 0; i < 4; i++) {
+                            // A row behind the last writes the last's values once more.
+                            char* to = (char*)p.out + (rows[min(16 * c + 4 * g + i, n - 1)] * p.ldo + n0 + NT * col) * O;
+                            float y[NT];
 #pragma unroll
-                            for (int t = 0; t < 4; t++) {
+                            for (int t = 0; t < NT; t++) {
                                 const uint32_t w = base[i][OB ? t >> 1 : t];
-                                const float was = OB ? bf16_to_f32(t & 1 ? w >> 16 : w & 0xffffu) : __uint_as_float(w);
-                                y[t] = p.base ? acc[t][i] + was : acc[t][i];
+                                const float before = OB ? bf16_to_f32(t & 1 ? w >> 16 : w & 0xffffu) : __uint_as_float(w);
+                                y[t] = p.base ? acc[t][i] + before : acc[t][i];
                             }
-                            Four w;
+                            Run w;
 #pragma unroll
-                            for (int t = 0; t < (OB ? 2 : 4); t++) w[t] = OB ? f32x2_to_bf16x2(y[2 * t % 4], y[(2 * t + 1) % 4]) : __float_as_uint(y[t]);
-                            *(Four*)to = w;
-                        } else {
-                            const char* from = (const char*)p.base + (row * p.ld_base + n0 + 4 * col) * O;
+                            for (int t = 0; t < NT * O / 4; t++) w[t] = OB ? f32x2_to_bf16x2(y[2 * t % NT], y[(2 * t + 1) % NT]) : __float_as_uint(y[t]);
+                            *(Run*)to = w;
+                        }
+                    } else {
 #pragma unroll
-                            for (int t = 0; t < 4; t++) {
-                                if (n0 + 4 * col + t >= p.N) continue;
-                                y[t] = acc[t][i];
-                                if (p.base) y[t] += OB ? bf16_to_f32(((const uint16_t*)from)[t]) : ((const float*)from)[t];
-                                if (OB) ((uint16_t*)to)[t] = (uint16_t)f32_to_bf16(y[t]);
-                                else ((float*)to)[t] = y[t];
+                        for (int i = 0; i < 4; i++) {
+                            if (16 * c + 4 * g + i >= n) continue;
+                            const int64_t row = rows[16 * c + 4 * g + i];
+#pragma unroll
+                            for (int t = 0; t < NT; t++) {
+                                const int at = n0 + NT * col + t;
+                                if (at >= p.N) continue;
+                                float y = acc[t][i];
+                                if (p.base) y += OB ? bf16_to_f32(((const uint16_t*)p.base)[row * p.ld_base + at]) : ((const float*)p.base)[row * p.ld_base + at];
+                                if (OB) ((uint16_t*)p.out)[row * p.ldo + at] = (uint16_t)f32_to_bf16(y);
+                                else ((float*)p.out)[row * p.ldo + at] = y;
                             }
                         }
                     }
                 };
-                // Bases in turn: c's in c % A where cols is a multiple of A, else begun anew a chunk.
+                if (inside) {
+                    // After its last tile a base is that of the next chunk's, if there is one.
+                    const int next = chunk + 1 < chunks && n0 + kBlock + kWave <= p.N ? n0 + kBlock : n0;
 #pragma unroll 1
-                for (int c = 0; c < cols; c += A) {
+                    for (int c = 0; c < ahead; c += A) {
+                        const bool end = c + A >= ahead;
 #pragma unroll
-                    for (int j = 0; j < A; j++) {
-                        if (c + j >= cols) continue;
-                        turn(c + j, base[j]);
-                        if (c + j + A < cols || cols % A == 0) load_base(n0, c + j + A, base[j]);
+                        for (int j = 0; j < A; j++) {
+                            turn(c + j, base[j], true);
+                            load_base(end ? next : n0, end ? j : c + j + A, base[j]);
+                        }
                     }
-                }
-                if (cols % A) {
-#pragma unroll
-                    for (int j = 0; j < A; j++)
-                        if (j < cols) load_base(n0, cols + j, base[j]);
+#pragma unroll 1
+                    for (int c = ahead; c < cols; c++) {
+                        Run one[4];
+                        load_base(n0, c, one);
+                        turn(c, one, true);
+                    }
+                } else {
+#pragma unroll 1
+                    for (int c = 0; c < cols; c++) turn(c, base[0], false);
                 }
             }
             __syncthreads();
@@ -716,42 +736,45 @@ int rank_pitch(int64_t R) { return (int)(16 * ceil_div(R, 16)); }
 
 constexpr size_t kMaxLds = 159 << 10;  // a compute unit's 160 KB, less the rows' numbers
 
-// Rows from which on blocks take whole tiles' rows.
-constexpr int64_t kWideRows = 512;
+// Whether blocks take whole tiles' rows (whose loads are whole steps of K).
+bool is_wide(int64_t rows, int64_t K) { return rows >= 512 && K >= 512; }
 
 // Parts of K: enough blocks where there are few rows, a part no shorter than 512; of wide
 // blocks no more than fit the compute units at once, with room for tiles of two classes.
 int splits_of(int64_t rows, int64_t K) {
-    const int64_t want = rows >= kWideRows ? 256 / (ceil_div(rows, kLoraTile) * 5 / 4) : 512 / ceil_div(rows, kFewCols);
+    const int64_t want = is_wide(rows, K) ? 256 / (ceil_div(rows, kLoraTile) * 5 / 4) : 512 / ceil_div(rows, kFewCols);
     return (int)std::clamp<int64_t>(want, 1, std::min<int64_t>(kSplits, ceil_div(K, 512)));
 }
 
+int places(int n) { return n >= kSpread ? (n + 7) / 8 * 8 : n; }
+
 template <bool XB, bool WB, int RT>
-void down_ranks(hipStream_t stream, const LoraBatched& p, int tiles, int around, int classes, int groups) {
-    if (p.rows >= kWideRows) {
+void down_ranks(hipStream_t stream, const LoraBatched& p, int tiles, int classes, int groups) {
+    const int around = places(tiles * p.splits);
+    if (is_wide(p.rows, p.K)) {
         const int parts = (int)std::clamp<int64_t>(256 / ((int64_t)tiles * p.splits * groups), 1, classes);
-        hipLaunchKernelGGL((lora_batched_down_wide_kernel<XB, WB, RT>), dim3((unsigned)(around * parts), (unsigned)p.splits, (unsigned)groups), dim3(512), 0, stream,
+        hipLaunchKernelGGL((lora_batched_down_wide_kernel<XB, WB, RT>), dim3((unsigned)(around * parts), 1, (unsigned)groups), dim3(512), 0, stream,
                            p, tiles, around, parts);
         return;
     }
     // A tile's units are more than its classes by those of more than kFewCols rows.
     const int units = std::min(classes + kLoraTile / kFewCols - 1, kLoraTile);
     const int parts = (int)std::clamp<int64_t>(1024 / ((int64_t)tiles * p.splits * groups), 1, units);
-    hipLaunchKernelGGL((lora_batched_down_kernel<XB, WB, RT>), dim3((unsigned)(around * parts), (unsigned)p.splits, (unsigned)groups), dim3(256), 0, stream, p, tiles,
+    hipLaunchKernelGGL((lora_batched_down_kernel<XB, WB, RT>), dim3((unsigned)(around * parts), 1, (unsigned)groups), dim3(256), 0, stream, p, tiles,
                        around, parts);
 }
 
 template <bool XB, bool WB>
-void down(hipStream_t stream, const LoraBatched& p, int tiles, int around, int classes) {
+void down(hipStream_t stream, const LoraBatched& p, int tiles, int classes) {
     const int rt = (p.R + 15) / 16;
-    if (rt == 1) down_ranks<XB, WB, 1>(stream, p, tiles, around, classes, 1);
-    else if (rt == 2) down_ranks<XB, WB, 2>(stream, p, tiles, around, classes, 1);
-    else down_ranks<XB, WB, 4>(stream, p, tiles, around, classes, (rt + 3) / 4);
+    if (rt == 1) down_ranks<XB, WB, 1>(stream, p, tiles, classes, 1);
+    else if (rt == 2) down_ranks<XB, WB, 2>(stream, p, tiles, classes, 1);
+    else down_ranks<XB, WB, 4>(stream, p, tiles, classes, (rt + 3) / 4);
 }
 
 template <bool WB, bool OB, int KS, bool WIDE>
-hipError_t up_ranks(hipStream_t stream, const LoraBatched& p, int tiles, int around, int classes) {
-    const int ranks = (p.R + 31) / 32 * 32, all = (p.N + 255) / 256;
+hipError_t up_ranks(hipStream_t stream, const LoraBatched& p, int tiles, int classes) {
+    const int ranks = (p.R + 31) / 32 * 32, block_n = 64 * up_tiles<OB, WIDE>, all = (p.N + block_n - 1) / block_n;
     const size_t row = WB ? 3 * (ranks + 8) * 2 : (ranks + 4) * 4;
     const int most = row * kLoraTile <= kMaxLds ? kLoraTile : kLoraTile / 2;
     const size_t lds = row * std::min(most, (p.rows + 15) / 16 * 16);
@@ -760,22 +783,23 @@ hipError_t up_ranks(hipStream_t stream, const LoraBatched& p, int tiles, int aro
         if (e != hipSuccess) return e;
     }
     // Two blocks a compute unit.
-    const int want = (int)std::max<int64_t>(1, 512 / tiles);
+    const int want = (int)std::max<int64_t>(1, 1024 / tiles);
     const int chunks = (all + std::min(want, all) - 1) / std::min(want, all), across = (all + chunks - 1) / chunks;
     const int parts = (int)std::clamp<int64_t>((WIDE ? 512 : 1024) / ((int64_t)tiles * across), 1, classes);
-    const dim3 grid((unsigned)(around * parts), (unsigned)across), block(256);
+    const int around = places(tiles * across);
+    const dim3 grid((unsigned)(around * parts)), block(256);
     if (WIDE) {
         const int64_t pieces = (int64_t)p.rows * (ranks / 4);
         hipLaunchKernelGGL(lora_batched_join_kernel<WB>, dim3((unsigned)ceil_div(pieces, 256)), block, 0, stream, p, ranks);
     }
-    hipLaunchKernelGGL((lora_batched_up_kernel<WB, OB, KS, WIDE>), grid, block, lds, stream, p, tiles, around, parts, chunks, most);
+    hipLaunchKernelGGL((lora_batched_up_kernel<WB, OB, KS, WIDE>), grid, block, lds, stream, p, tiles, across, around, parts, chunks, most);
     return hipGetLastError();
 }
 
 template <bool WB, bool OB>
-hipError_t up(hipStream_t stream, const LoraBatched& p, int tiles, int around, int classes) {
-    if (p.joined) return p.R <= 32 ? up_ranks<WB, OB, 1, true>(stream, p, tiles, around, classes) : up_ranks<WB, OB, 2, true>(stream, p, tiles, around, classes);
-    return up_ranks<WB, OB, 1, false>(stream, p, tiles, around, classes);
+hipError_t up(hipStream_t stream, const LoraBatched& p, int tiles, int classes) {
+    if (p.joined) return p.R <= 32 ? up_ranks<WB, OB, 1, true>(stream, p, tiles, classes) : up_ranks<WB, OB, 2, true>(stream, p, tiles, classes);
+    return up_ranks<WB, OB, 1, false>(stream, p, tiles, classes);
 }
 
 // h, the tiles' classes and how many they are.
@@ -784,28 +808,28 @@ size_t h_bytes(int64_t rows, int64_t K, int64_t R) { return (size_t)splits_of(ro
 }  // namespace
 
 size_t lora_batched_workspace(int64_t rows, int64_t K, int64_t R) {
-    const size_t joined = rows >= kWideRows ? (size_t)rows * (32 * ceil_div(R, 32)) * 6 : 0;  // three bf16, or fp32
+    const size_t joined = is_wide(rows, K) ? (size_t)rows * (32 * ceil_div(R, 32)) * 6 : 0;  // three bf16, or fp32
     return h_bytes(rows, K, R) + (size_t)ceil_div(rows, kLoraTile) * (kLoraTile * sizeof(LoraClass) + 16) + joined;
 }
 
 hipError_t launch_lora_batched(hipStream_t stream, LoraBatched p) {
     p.splits = splits_of(p.rows, p.K);
     p.rank_pitch = rank_pitch(p.R);
-    const int tiles = (p.rows + kLoraTile - 1) / kLoraTile, around = tiles >= kSpread ? (tiles + 7) / 8 * 8 : tiles;
+    const int tiles = (p.rows + kLoraTile - 1) / kLoraTile;
     auto end = [](const void* from, int64_t elements, bool b16) { return (const char*)from + elements * (b16 ? 2 : 4); };
     p.x_end = end(p.x, (p.rows - 1) * p.ldx + p.K, p.x_bf16);
     p.a_end = end(p.A, (p.adapters - 1) * p.a_adapter + (p.R - 1) * p.a_row + p.K, p.w_bf16);
     p.b_end = end(p.B, (p.adapters - 1) * p.b_adapter + (p.N - 1) * p.b_row + p.R, p.w_bf16);
     p.classes = (LoraClass*)((char*)p.h + h_bytes(p.rows, p.K, p.R));
     p.counts = (int*)(p.classes + (int64_t)tiles * kLoraTile);
-    p.joined = p.rows >= kWideRows ? (void*)((char*)p.counts + (int64_t)tiles * 16) : nullptr;
+    p.joined = is_wide(p.rows, p.K) ? (void*)((char*)p.counts + (int64_t)tiles * 16) : nullptr;
     const int classes = std::min({kLoraTile - 1, p.adapters, p.rows}) + 1;  // of a tile, at most
-    if (p.x_bf16) p.w_bf16 ? down<true, true>(stream, p, tiles, around, classes) : down<true, false>(stream, p, tiles, around, classes);
-    else p.w_bf16 ? down<false, true>(stream, p, tiles, around, classes) : down<false, false>(stream, p, tiles, around, classes);
+    if (p.x_bf16) p.w_bf16 ? down<true, true>(stream, p, tiles, classes) : down<true, false>(stream, p, tiles, classes);
+    else p.w_bf16 ? down<false, true>(stream, p, tiles, classes) : down<false, false>(stream, p, tiles, classes);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    if (p.w_bf16) return p.out_bf16 ? up<true, true>(stream, p, tiles, around, classes) : up<true, false>(stream, p, tiles, around, classes);
-    return p.out_bf16 ? up<false, true>(stream, p, tiles, around, classes) : up<false, false>(stream, p, tiles, around, classes);
+    if (p.w_bf16) return p.out_bf16 ? up<true, true>(stream, p, tiles, classes) : up<true, false>(stream, p, tiles, classes);
+    return p.out_bf16 ? up<false, true>(stream, p, tiles, classes) : up<false, false>(stream, p, tiles, classes);
 }
 
 }  // namespace phi_dev

@@ -62,6 +62,12 @@ SIZES = [  # rows, K, N, ranks, adapters, mixed
     (50, 96, 300, 256, 3, True),
     (40, 333, 160, 200, 70, True),
     (1000, 512, 1536, 64, 8, False),
+    (640, 777, 333, 16, 3, False),
+    (515, 1030, 100, 40, 90, True),
+    (900, 600, 1300, 7, 2, True),
+    (512, 544, 96, 256, 4, False),
+    (600, 511, 200, 16, 5, False),
+    (2100, 520, 60, 32, 1, False),
 ]
 
 
