@@ -114,95 +114,101 @@ struct RowPart {
     __device__ __forceinline__ int64_t row(int kh, int z) const { return ((int64_t)kh * s.slots + (z < n - 1 ? first + z : last)) * s.rows + in; }
 };
 
-// A prefix's and the own tokens' partial softmaxes of rows joined: 16 rows of q (token x
-// head) a block and a wave a row, or one row a block and a wave for every fourth split (W = 4).  As
-// attn_join_kernel, over the splits of both in a row.
-template <int W>
+// A prefix's and the own tokens' partial softmaxes of rows joined, a wave a row of q (token x
+// head), or a block a row and a wave every fourth split (W = 4).  As attn_join_kernel, over the
+// splits of both in a row, of which SUB parts of a wave, wide enough for dim each, take turns.
+template <int W, int SUB>
 __global__ __launch_bounds__(256) void shared_join_kernel(PagedAttn p, AttnPart few, AttnPart many, int D) {
-    constexpr int kRows = W == 1 ? 16 : 1;
+    constexpr int kAhead = 8;
     __shared__ float4 lx[W][64];
     __shared__ float2 lml[W];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave % W;
-    const int batch = p.batch - p.groups, d = 4 * lane < D ? 4 * lane : 0;
-    for (int in = wave / W; in < kRows; in += 4) {
-        const int64_t r = (int64_t)blockIdx.x * kRows + in;
-        const int token = (int)(r / p.q_heads), head = (int)(r - (int64_t)token * p.q_heads), kh = head / p.group;
-        if (token >= p.tokens) return;
-        const int64_t at = (int64_t)token * p.group + (head - kh * p.group);
-        RowPart part[2];  // prefix, own
-        bool mine = false;
+    const int sub = lane / (64 / SUB), dl = 4 * (lane % (64 / SUB)), batch = p.batch - p.groups, d = dl < D ? dl : 0;
+    const int64_t r = (int64_t)blockIdx.x * (4 / W) + wave / W;
+    const int token = (int)(r / p.q_heads), head = (int)(r - (int64_t)token * p.q_heads), kh = head / p.group;
+    if (token >= p.tokens) return;  // W = 4: never
+    const int64_t at = (int64_t)token * p.group + (head - kh * p.group);
+    RowPart part[2];  // prefix, own
+    bool mine = false;
 #pragma unroll
-        for (int k = 0; k < 2; k++) {
-            const AttnRow a = (k ? p.own_rows : p.prefix_rows)[at];
-            const bool is_many = a.where >> 31;
-            RowPart& x = part[k];
-            x.s = is_many ? many : few;
-            x.n = a.where & 0xffff, x.in = a.where >> 16 & 0x7fff, x.first = a.first, x.last = a.last;
-            // Left by this call only if the row is of that group or sequence.
-            int from = a.id, to = a.id + 1;
-            bool is = a.id >= 0 && a.id < (k ? batch : p.groups);
-            if (k == 0 && is) from = min(max(p.group_start[a.id], 0), batch), to = min(max(p.group_start[a.id + 1], 0), batch);
-            if (is) {
-                const int first = p.q_start[from];
-                is = token >= first && token < p.q_start[to] && (k == 0 || token - first < p.own_q);
-            }
-            is = is && x.in < x.s.rows && x.n > 0 && (x.n == 1 || (x.first >= 0 && x.first + x.n - 1 <= x.s.slots)) && x.last >= 0 && x.last < x.s.slots;
-            x.n = is ? x.n : 0;
-            mine = k ? is : mine;
+    for (int k = 0; k < 2; k++) {
+        const AttnRow a = (k ? p.own_rows : p.prefix_rows)[at];
+        const bool is_many = a.where >> 31;
+        RowPart& x = part[k];
+        x.s = is_many ? many : few;
+        x.n = a.where & 0xffff, x.in = a.where >> 16 & 0x7fff, x.first = a.first, x.last = a.last;
+        // Left by this call only if the row is of that group or sequence.
+        int from = a.id, to = a.id + 1;
+        bool is = a.id >= 0 && a.id < (k ? batch : p.groups);
+        if (k == 0 && is) from = min(max(p.group_start[a.id], 0), batch), to = min(max(p.group_start[a.id + 1], 0), batch);
+        if (is) {
+            const int first = p.q_start[from];
+            is = token >= first && token < p.q_start[to] && (k == 0 || token - first < p.own_q);
         }
-        if (!mine) continue;  // W = 4: the same in all waves
-        const int n0 = part[0].n, n = n0 + part[1].n;
-        auto ml_of = [&](int z) { const RowPart& x = part[z < n0 ? 0 : 1]; return x.s.ml + 2 * x.row(kh, z < n0 ? z : z - n0); };
-        auto o_of = [&](int z) { const RowPart& x = part[z < n0 ? 0 : 1]; return x.s.o + x.row(kh, z < n0 ? z : z - n0) * D; };
-        float m = kNoMax, l = 0.0f;
-        v4f x = {0, 0, 0, 0};
-        for (int k0 = w; k0 < n; k0 += 64 * W) {
-            v4f y[8];
-            auto load = [&](int k) {
-#pragma unroll
-                for (int u = 0; u < 8; u++) y[u] = k + W * u < n ? *(const v4f*)(o_of(k + W * u) + d) : v4f{0, 0, 0, 0};
-            };
-            load(k0);
-            const int z = k0 + W * lane;
-            const float2 ml = z < n ? *(const float2*)ml_of(z) : make_float2(kNoMax, 0.0f);
-            const float m2 = fmaxf(m, wave_max(ml.x)), keep = __builtin_amdgcn_exp2f(m - m2);
-            const float share = z < n ? __builtin_amdgcn_exp2f(ml.x - m2) : 0.0f;
-            float sum = ml.y * share;
-#pragma unroll
-            for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
-            l = l * keep + sum;
-            x *= keep;
-            m = m2;
-            for (int k = 0;;) {
-#pragma unroll
-                for (int u = 0; u < 8; u++) x += y[u] * __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(share), k + u));
-                k += 8;
-                if (k >= 64 || k0 + W * k >= n) break;
-                load(k0 + W * k);
-            }
-        }
-        if (W > 1) {
-            lx[w][lane] = make_float4(x[0], x[1], x[2], x[3]);
-            if (lane == 0) lml[w] = make_float2(m, l);
-            __syncthreads();
-            if (w) return;
-#pragma unroll
-            for (int k = 1; k < W; k++) m = fmaxf(m, lml[k].x);
-            x = v4f{0, 0, 0, 0}, l = 0.0f;
-#pragma unroll
-            for (int k = 0; k < W; k++) {
-                const float4 t = lx[k][lane];
-                const float share = __builtin_amdgcn_exp2f(lml[k].x - m);
-                x += v4f{t.x, t.y, t.z, t.w} * share;
-                l = fmaf(lml[k].y, share, l);
-            }
-        }
-        x *= l != 0.0f ? 1.0f / l : 0.0f;
-        if (4 * lane >= D) continue;
-        const int64_t to = (int64_t)token * p.out_token + head * p.out_head + d;
-        if (!p.bf16) *(v4f*)((float*)p.out + to) = x;
-        else *(uint2*)((uint16_t*)p.out + to) = make_uint2(f32x2_to_bf16x2(x[0], x[1]), f32x2_to_bf16x2(x[2], x[3]));
+        is = is && x.in < x.s.rows && x.n > 0 && (x.n == 1 || (x.first >= 0 && x.first + x.n - 1 <= x.s.slots)) && x.last >= 0 && x.last < x.s.slots;
+        x.n = is ? x.n : 0;
+        mine = k ? is : mine;
     }
+    if (!mine) return;  // W = 4: the same in all waves
+    const int n0 = part[0].n, n = n0 + part[1].n;
+    auto ml_of = [&](int z) { const RowPart& x = part[z < n0 ? 0 : 1]; return x.s.ml + 2 * x.row(kh, z < n0 ? z : z - n0); };
+    auto o_of = [&](int z) { const RowPart& x = part[z < n0 ? 0 : 1]; return x.s.o + x.row(kh, z < n0 ? z : z - n0) * D; };
+    float m = kNoMax, l = 0.0f;
+    v4f x = {0, 0, 0, 0};
+    // 64 of the wave's splits at a time: w + W i in lane i, the sub-th of every SUB a part's.
+    for (int k0 = w; k0 < n; k0 += 64 * W) {
+        v4f y[kAhead];
+        auto load = [&](int i) {
+#pragma unroll
+            for (int u = 0; u < kAhead; u++) {
+                const int z = k0 + W * (i + SUB * u + sub);
+                y[u] = z < n ? *(const v4f*)(o_of(z) + d) : v4f{0, 0, 0, 0};
+            }
+        };
+        load(0);
+        const int z = k0 + W * lane;
+        const float2 ml = z < n ? *(const float2*)ml_of(z) : make_float2(kNoMax, 0.0f);
+        const float m2 = fmaxf(m, wave_max(ml.x)), keep = __builtin_amdgcn_exp2f(m - m2);
+        const float share = z < n ? __builtin_amdgcn_exp2f(ml.x - m2) : 0.0f;
+        float sum = ml.y * share;
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
+        l = l * keep + sum;
+        x *= keep;
+        m = m2;
+        for (int i = 0;;) {
+#pragma unroll
+            for (int u = 0; u < kAhead; u++) x += y[u] * __shfl(share, i + SUB * u + sub, 64);
+            i += SUB * kAhead;
+            if (i >= 64 || k0 + W * i >= n) break;
+            load(i);
+        }
+    }
+#pragma unroll
+    for (int off = 64 / SUB; off < 64; off <<= 1)
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[e] += __shfl_xor(x[e], off, 64);
+    if (W > 1) {
+        lx[w][lane] = make_float4(x[0], x[1], x[2], x[3]);
+        if (lane == 0) lml[w] = make_float2(m, l);
+        __syncthreads();
+        if (w) return;
+#pragma unroll
+        for (int k = 1; k < W; k++) m = fmaxf(m, lml[k].x);
+        x = v4f{0, 0, 0, 0}, l = 0.0f;
+#pragma unroll
+        for (int k = 0; k < W; k++) {
+            const float4 t = lx[k][lane];
+            const float share = __builtin_amdgcn_exp2f(lml[k].x - m);
+            x += v4f{t.x, t.y, t.z, t.w} * share;
+            l = fmaf(lml[k].y, share, l);
+        }
+    }
+    x *= l != 0.0f ? 1.0f / l : 0.0f;
+    if (sub || dl >= D) return;
+    const int64_t to = (int64_t)token * p.out_token + head * p.out_head + d;
+    if (!p.bf16) *(v4f*)((float*)p.out + to) = x;
+    else *(uint2*)((uint16_t*)p.out + to) = make_uint2(f32x2_to_bf16x2(x[0], x[1]), f32x2_to_bf16x2(x[2], x[3]));
 }
 
 namespace {
@@ -261,6 +267,7 @@ Plan attn_plan(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t dim, i
         const bool few = s == &a.few;
         if (few ? rows > a.few_rows && batch == 1 : rows <= a.few_rows) continue;
         s->rows = few ? kDecodeRows : dim <= 128 ? kChunkRows : kChunkRowsWide;
+        s->seqs = (int)batch;
         s->step = 1 << 30;
         // Tiles, at most.
         const int64_t units = std::min(batch * ceil_div(few ? std::min<int64_t>(rows, a.few_rows) : rows, s->rows), ceil_div(tokens * group, s->rows) + batch);
@@ -289,7 +296,8 @@ Plan shared_plan(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t dim,
         // Tiles, at most, of the groups and of the sequences.
         const int64_t most = ceil_div(all, s->rows), cap = ceil_div(few ? a.few_rows : all, s->rows);
         int64_t units = std::min(groups * cap, most + groups);
-        if (few || own > a.few_rows) units += std::min(batch * ceil_div(few ? std::min<int64_t>(own, a.few_rows) : own, s->rows), most + batch);
+        s->seqs = (int)groups;
+        if (few || own > a.few_rows) s->seqs += (int)batch, units += std::min(batch * ceil_div(few ? std::min<int64_t>(own, a.few_rows) : own, s->rows), most + batch);
         split(*s, units, (few ? dim <= 128 ? kShares : kShares / 2 : kSharesChunks) / kv_heads, std::max<int64_t>(longest, 1));
         s->blocks = (int)std::min<int64_t>(s->slots, INT32_MAX / kv_heads);
     }
@@ -355,8 +363,12 @@ hipError_t launch_paged_attention_shared(hipStream_t stream, const KvCache& c, c
     if (e == hipSuccess) e = launch_paged_decode(stream, c, p, a.few);
     if (e != hipSuccess) return e;
     const int64_t rows = p.tokens * p.q_heads;
-    if (rows <= kJoinWide) hipLaunchKernelGGL(shared_join_kernel<4>, dim3((unsigned)rows), dim3(256), 0, stream, p, a.few, a.many, c.dim);
-    else hipLaunchKernelGGL(shared_join_kernel<1>, dim3((unsigned)ceil_div(rows, 16)), dim3(256), 0, stream, p, a.few, a.many, c.dim);
+    const bool wide = rows <= kJoinWide;
+    const dim3 grid((unsigned)(wide ? rows : ceil_div(rows, 4))), block(256);
+    auto join = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, stream, p, a.few, a.many, c.dim); };
+    if (c.dim <= 64) wide ? join(shared_join_kernel<4, 4>) : join(shared_join_kernel<1, 4>);
+    else if (c.dim <= 128) wide ? join(shared_join_kernel<4, 2>) : join(shared_join_kernel<1, 2>);
+    else wide ? join(shared_join_kernel<4, 1>) : join(shared_join_kernel<1, 1>);
     return hipGetLastError();
 }
 

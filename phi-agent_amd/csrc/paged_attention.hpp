@@ -84,6 +84,7 @@ struct AttnPart {
     int slots;    // a key/value head
     int rows;     // a tile
     int blocks;   // the grid, over kv_heads; 0: does not run
+    int seqs;     // sequences that may be of this part, from the first on
     float* o;
     float* ml;
 };
@@ -167,7 +168,7 @@ template <bool FEW> struct AttnScan {
     // On to the next 64; false: there are none.
     __device__ __forceinline__ bool next(const PagedAttn& p, const AttnPart& s, int page) {
         for (;;) {
-            const bool counted = b0 + 64 >= p.batch;
+            const bool counted = b0 + 64 >= s.seqs;
             if (counted) {
                 if (len) return false;
                 len = max(1, (total + s.shares - 1) / s.shares);
@@ -179,7 +180,7 @@ template <bool FEW> struct AttnScan {
                 const int at = b0 + (threadIdx.x & 63);
                 q = SeqInfo{}, tiles = 0;
                 first = 0, n = 1;
-                if (at < p.batch) {
+                if (at < s.seqs) {
                     q = seq_info(p, page, at);
                     const int rows = min(q.n, p.max_q) * p.group;
                     if ((rows <= p.few_rows) == FEW) tiles = (rows + s.rows - 1) / s.rows;

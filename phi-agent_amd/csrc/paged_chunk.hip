@@ -543,6 +543,8 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel
     //   it over that of n - 2, which the softmax read until 2n - 2;
     // a barrier ends every turn.  Four waves have one turn a tile.  Tiles staged
     // past the last are never read.
+    // A wave behind the last row only stages (320 rows' second block: SKIPFIG).
+    const bool idle = w0 >= rows;
     auto walk = [&](auto with_v, auto with_k) __attribute__((always_inline)) {
         constexpr bool V = decltype(with_v)::value, K = decltype(with_k)::value;
         if (V) {
@@ -560,6 +562,19 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel
         }
         lds_barrier();
         if (NW == 8 && K) lds_barrier();
+        if constexpr (NW == 8) {
+            if (idle) {
+                lds_barrier();
+                for (int n = 0; n + 1 < count; n++) {
+                    lds_barrier();
+                    if (V) each<kVPieces>([&](auto i) __attribute__((always_inline)) { v_piece(i, n + 1, start(n + 2)); });
+                    if (K) each<kKPieces>([&](auto i) __attribute__((always_inline)) { k_piece(i, n + 2, start(n + 3)); });
+                    lds_barrier();
+                }
+                if (V) lds_barrier();
+                return;
+            }
+        }
         products(int_c<kNV>{}, int_c<kNV + kNS>{}, tile[0], tile[0], nothing);
         read_meta(0);
         lds_barrier();
