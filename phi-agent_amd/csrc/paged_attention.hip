@@ -17,7 +17,7 @@ struct TileSplits {
 
 template <bool FEW>
 __device__ __forceinline__ TileSplits tile_splits(const PagedAttn& p, const AttnPart& s, int page, int kh, int unit) {
-    AttnScan<FEW> f(s);
+    AttnScan<FEW, false> f(s);
     int tiles = 0;
     while (f.next(p, s, page)) {
         const int off = unit - tiles;
@@ -267,7 +267,6 @@ Plan attn_plan(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t dim, i
         const bool few = s == &a.few;
         if (few ? rows > a.few_rows && batch == 1 : rows <= a.few_rows) continue;
         s->rows = few ? kDecodeRows : dim <= 128 ? kChunkRows : kChunkRowsWide;
-        s->seqs = (int)batch;
         s->step = 1 << 30;
         // Tiles, at most.
         const int64_t units = std::min(batch * ceil_div(few ? std::min<int64_t>(rows, a.few_rows) : rows, s->rows), ceil_div(tokens * group, s->rows) + batch);

@@ -40,8 +40,18 @@ struct SeqInfo {
 
 // With shared prefixes a group's prefix is a sequence too, the groups' before the
 // batch's own: its rows are those of all its sequences, each past all of its tokens.
+template <bool SHARED>
 __device__ __forceinline__ SeqInfo seq_info(const PagedAttn& p, int page, int b) {
     SeqInfo s;
+    if constexpr (!SHARED) {
+        const int64_t a = p.q_start[b], e = p.q_start[b + 1], T = p.tokens;
+        s.first = (int)(a < 0 ? 0 : a > T ? T : a);
+        s.n = max(0, (int)(e < 0 ? 0 : e > T ? T : e) - s.first);
+        const int kv = max(0, p.kv_len[b]);
+        s.kv = (int)min((int64_t)min(kv, p.max_kv), (int64_t)p.table_width * page);
+        s.pos0 = kv - s.n;
+        return s;
+    }
     const bool prefix = b < p.groups;
     int from = b - p.groups, to = from + 1;
     if (prefix) {
@@ -54,12 +64,14 @@ __device__ __forceinline__ SeqInfo seq_info(const PagedAttn& p, int page, int b)
     const int kv = max(0, prefix ? p.prefix_len[b] : p.kv_len[from]);
     s.kv = (int)min((int64_t)min(kv, prefix ? p.max_prefix : p.max_kv), (int64_t)(prefix ? p.prefix_width : p.table_width) * page);
     s.pos0 = prefix ? s.kv : kv - s.n;
-    if (p.groups && !prefix) s.n = min(s.n, p.own_q);
+    if (!prefix) s.n = min(s.n, p.own_q);
     return s;
 }
 
 // A sequence's row of the block table; prefixes' lie prefix_at further on.
-__device__ __forceinline__ const int32_t* table_row(const PagedAttn& p, const int32_t* table, int b) {
+template <bool SHARED>
+__device__ __forceinline__ const int32_t* table_row(const PagedAttn& p, const int32_t* __restrict__ table, int b) {
+    if constexpr (!SHARED) return table + (int64_t)b * p.table_stride;
     const int64_t at = b < p.groups ? p.prefix_at + b * p.prefix_stride : (b - p.groups) * p.table_stride;
     return table + at;
 }
@@ -84,7 +96,7 @@ struct AttnPart {
     int slots;    // a key/value head
     int rows;     // a tile
     int blocks;   // the grid, over kv_heads; 0: does not run
-    int seqs;     // sequences that may be of this part, from the first on
+    int seqs;     // with shared prefixes, the sequences that may be of this part, from the first on
     float* o;
     float* ml;
 };
@@ -154,7 +166,7 @@ __device__ __forceinline__ int lanes_sum(int v) {
 // length, are at most `shares`.  These come first among the 64 sequences' blocks,
 // then the last ones, longer before shorter by quarters of that length, so that the
 // work evens out whatever the lengths.
-template <bool FEW> struct AttnScan {
+template <bool FEW, bool SHARED> struct AttnScan {
     int b0 = -64, base = 0;  // the first lane's sequence, blocks before its
     int len, total = 0;      // steps a split, 0: being counted; steps in all
     SeqInfo q;
@@ -168,7 +180,8 @@ template <bool FEW> struct AttnScan {
     // On to the next 64; false: there are none.
     __device__ __forceinline__ bool next(const PagedAttn& p, const AttnPart& s, int page) {
         for (;;) {
-            const bool counted = b0 + 64 >= s.seqs;
+            const int seqs = SHARED ? s.seqs : p.batch;
+            const bool counted = b0 + 64 >= seqs;
             if (counted) {
                 if (len) return false;
                 len = max(1, (total + s.shares - 1) / s.shares);
@@ -180,8 +193,8 @@ template <bool FEW> struct AttnScan {
                 const int at = b0 + (threadIdx.x & 63);
                 q = SeqInfo{}, tiles = 0;
                 first = 0, n = 1;
-                if (at < s.seqs) {
-                    q = seq_info(p, page, at);
+                if (at < seqs) {
+                    q = seq_info<SHARED>(p, page, at);
                     const int rows = min(q.n, p.max_q) * p.group;
                     if ((rows <= p.few_rows) == FEW) tiles = (rows + s.rows - 1) / s.rows;
                     // The steps that hold what some row sees.
@@ -209,9 +222,9 @@ template <bool FEW> struct AttnScan {
     }
 };
 
-template <bool FEW>
+template <bool FEW, bool SHARED>
 __device__ __forceinline__ AttnUnit attn_unit(const PagedAttn& p, const AttnPart& s, int page, int unit) {
-    AttnScan<FEW> f(s);
+    AttnScan<FEW, SHARED> f(s);
     while (f.next(p, s, page)) {
         const int local = unit - f.base;
         if (local >= f.blocks()) continue;
@@ -223,7 +236,7 @@ __device__ __forceinline__ AttnUnit attn_unit(const PagedAttn& p, const AttnPart
         const int tile = full ? in / (k - 1) : in, z = full ? in - tile * (k - 1) : k - 1;
         const int z0 = (__builtin_amdgcn_readlane(f.first, at) + z * f.len) * s.step;
         // Late tiles first: they see most tokens.
-        return {f.b0 + at, __builtin_amdgcn_readlane(f.tiles, at) - 1 - tile, k > 1 || p.groups ? unit : -1, z0, full ? z0 + f.len * s.step : INT_MAX, seq_of_lane(f.q, at),
+        return {f.b0 + at, __builtin_amdgcn_readlane(f.tiles, at) - 1 - tile, k > 1 || SHARED ? unit : -1, z0, full ? z0 + f.len * s.step : INT_MAX, seq_of_lane(f.q, at),
                 f.base + __builtin_amdgcn_readlane(full_begin, at) + tile * (k - 1), k, !full};
     }
     return {-1, 0, 0, 0, 0, {}, 0, 0, false};

@@ -131,7 +131,7 @@ __device__ __forceinline__ int k_slot(int t, int n) {
 
 // DP: dim rounded up to 64, 128 or 256; NW waves, 32 rows each; PAGE16 as in
 // paged_decode.hip.
-template <int DP, int NW, bool PAGE16>
+template <int DP, int NW, bool PAGE16, bool SHARED>
 __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel(KvCache c, PagedAttn p, AttnPart sp,
                                                                               const int32_t* __restrict__ table) {
     constexpr int KS = DP / 16, OT = DP / 32;
@@ -143,7 +143,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel
     const int col = lane & 31, h = lane >> 5;
     const int heads = c.heads, D = c.dim;
     const int kh = blockIdx.x % heads;
-    const AttnUnit unit_of = attn_unit<false>(p, sp, c.page, blockIdx.x / heads);
+    const AttnUnit unit_of = attn_unit<false, SHARED>(p, sp, c.page, blockIdx.x / heads);
     if (unit_of.b < 0) return;
     const int b = unit_of.b, z0 = unit_of.z0;
     const SeqInfo s = unit_of.s;
@@ -206,7 +206,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel
     const int begin = lo & ~(kTile - 1), count = begin < hi ? (hi - begin + kTile - 1) / kTile : 0;
     auto start = [&](int n) { return begin + n * kTile; };
     const int group = wave & 3, n16 = lane & 15;
-    const int32_t* trow = table_row(p, table, b);
+    const int32_t* trow = table_row<SHARED>(p, table, b);
     const int last_page = page_of(c, max(hi - 1, 0));
     struct Raw {
         uint32_t w[8 * NVI > 4 * NKI ? 8 * NVI : 4 * NKI];  // V's items' 8 words, K's items' 4
@@ -543,8 +543,6 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel
     //   it over that of n - 2, which the softmax read until 2n - 2;
     // a barrier ends every turn.  Four waves have one turn a tile.  Tiles staged
     // past the last are never read.
-    // A wave behind the last row only stages (320 rows' second block: SKIPFIG).
-    const bool idle = w0 >= rows;
     auto walk = [&](auto with_v, auto with_k) __attribute__((always_inline)) {
         constexpr bool V = decltype(with_v)::value, K = decltype(with_k)::value;
         if (V) {
@@ -562,8 +560,9 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel
         }
         lds_barrier();
         if (NW == 8 && K) lds_barrier();
-        if constexpr (NW == 8) {
-            if (idle) {
+        if constexpr (SHARED && NW == 8) {
+            if (w0 >= rows) {
+                // A wave behind the last row only stages, in the others' turns.
                 lds_barrier();
                 for (int n = 0; n + 1 < count; n++) {
                     lds_barrier();
@@ -614,7 +613,7 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel
     const int64_t at = ((int64_t)kh * sp.slots + unit_of.slot) * (32 * NW) + 32 * wave + col;
     // O holds sum p v in units of 2^(kP + kM - 9 - vexp), l of 2^kP.
     const float unit = pow2(vexp + 9 - kM), share = split ? 1.0f / (1 << kP) : l != 0.0f ? 1.0f / l : 0.0f;
-    if (p.groups && unit_of.last && kh == 0 && h == 0) leave_row(p, unit_of, w0 + col, 32 * wave + col, true);
+    if (SHARED && unit_of.last && kh == 0 && h == 0) leave_row(p, unit_of, w0 + col, 32 * wave + col, true);
     if (split && h == 0) sp.ml[2 * at] = m, sp.ml[2 * at + 1] = l * (1.0f / (1 << kP));
     // Value n, j is of slot 32 n + 8 (j / 4) + 4 h + j % 4, so d = 4 (slot % (DP/4))
     // + slot / (DP/4): the four d of a slot % (DP/4) together.
@@ -640,19 +639,24 @@ __global__ __launch_bounds__(64 * NW, DP <= 128 ? 2 : 1) void paged_chunk_kernel
     }
 }
 
-template <int DP, int NW>
-static hipError_t launch_dp(hipStream_t stream, const KvCache& c, const PagedAttn& p, const AttnPart& s) {
+template <int DP, int NW, bool SHARED>
+static hipError_t launch_shared(hipStream_t stream, const KvCache& c, const PagedAttn& p, const AttnPart& s) {
     const dim3 grid((unsigned)s.blocks * (unsigned)c.heads), block(64 * NW);
     const bool page16 = tiles_of_16(c);
-    const void* f = page16 ? (const void*)paged_chunk_kernel<DP, NW, true> : (const void*)paged_chunk_kernel<DP, NW, false>;
+    const void* f = page16 ? (const void*)paged_chunk_kernel<DP, NW, true, SHARED> : (const void*)paged_chunk_kernel<DP, NW, false, SHARED>;
     const size_t lds = sizeof(ChunkLds<DP>);
     if (lds > 65536) {
         const hipError_t e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (e != hipSuccess) return e;
     }
-    if (page16) hipLaunchKernelGGL((paged_chunk_kernel<DP, NW, true>), grid, block, lds, stream, c, p, s, p.table);
-    else hipLaunchKernelGGL((paged_chunk_kernel<DP, NW, false>), grid, block, lds, stream, c, p, s, p.table);
+    if (page16) hipLaunchKernelGGL((paged_chunk_kernel<DP, NW, true, SHARED>), grid, block, lds, stream, c, p, s, p.table);
+    else hipLaunchKernelGGL((paged_chunk_kernel<DP, NW, false, SHARED>), grid, block, lds, stream, c, p, s, p.table);
     return hipGetLastError();
+}
+
+template <int DP, int NW>
+static hipError_t launch_dp(hipStream_t stream, const KvCache& c, const PagedAttn& p, const AttnPart& s) {
+    return p.groups ? launch_shared<DP, NW, true>(stream, c, p, s) : launch_shared<DP, NW, false>(stream, c, p, s);
 }
 
 hipError_t launch_paged_chunk(hipStream_t stream, const KvCache& c, const PagedAttn& p, const AttnPart& s) {

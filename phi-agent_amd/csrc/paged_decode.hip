@@ -53,7 +53,7 @@ __device__ __forceinline__ float byte_f32(uint32_t w, int n) { return (float)((i
 // DP: dim rounded up to 64, 128 or 256.  F32: fp32 q and out, else bf16.
 // PAGE16: tiles_of_16, so that a tile of 16 tokens has one block and its loads
 // one scalar base; otherwise every token finds its own.
-template <int DP, bool F32, bool PAGE16>
+template <int DP, bool F32, bool PAGE16, bool SHARED>
 __global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void paged_decode_kernel(KvCache c, PagedAttn p, AttnPart sp,
                                                                   const int32_t* __restrict__ table) {
     constexpr int KS = DP / 64, EB = DP / 16, NT = q_terms<F32>, NP = F32 ? 3 : 2;
@@ -62,7 +62,7 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void paged_decode_k
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
     const int kh = blockIdx.x % c.heads;
-    const AttnUnit unit = attn_unit<true>(p, sp, c.page, blockIdx.x / c.heads);
+    const AttnUnit unit = attn_unit<true, SHARED>(p, sp, c.page, blockIdx.x / c.heads);
     if (unit.b < 0) return;
     const int b = unit.b, slot = unit.slot, z0 = unit.z0;
     const SeqInfo s = unit.s;
@@ -86,7 +86,7 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void paged_decode_k
     int kd[KS];
 #pragma unroll
     for (int ks = 0; ks < KS; ks++) kd[ks] = 64 * ks + 16 * g < D ? 64 * ks + 16 * g : 0;
-    const int32_t* trow = table_row(p, table, b);
+    const int32_t* trow = table_row<SHARED>(p, table, b);
     const int last_page = page_of(c, max(hi - 1, 0));
 
     // The table's entries of a step's tiles (a lane's token's), fetched a step
@@ -316,7 +316,7 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void paged_decode_k
     const int64_t at = ((int64_t)kh * sp.slots + slot) * kDecodeRows + row;
     const float div = slot >= 0 ? 1.0f : rl != 0.0f ? 1.0f / rl : 0.0f;
     if (slot >= 0 && part == 0) sp.ml[2 * at] = rm, sp.ml[2 * at + 1] = rl;
-    if (p.groups && unit.last && kh == 0 && part == 0) leave_row(p, unit, r0 + row, row, false);
+    if (SHARED && unit.last && kh == 0 && part == 0) leave_row(p, unit, r0 + row, row, false);
 #pragma unroll
     for (int q4 = 0; q4 < DP / 64; q4++) {
         const int d = 4 * (part + 16 * q4);
@@ -335,12 +335,17 @@ __global__ __launch_bounds__(64 * kWaves, DP <= 128 ? 2 : 1) void paged_decode_k
     }
 }
 
+template <int DP, bool F32, bool SHARED>
+static hipError_t launch_shared(hipStream_t stream, const KvCache& c, const PagedAttn& p, const AttnPart& s) {
+    const dim3 grid((unsigned)s.blocks * (unsigned)c.heads), block(64 * kWaves);
+    if (tiles_of_16(c)) hipLaunchKernelGGL((paged_decode_kernel<DP, F32, true, SHARED>), grid, block, 0, stream, c, p, s, p.table);
+    else hipLaunchKernelGGL((paged_decode_kernel<DP, F32, false, SHARED>), grid, block, 0, stream, c, p, s, p.table);
+    return hipGetLastError();
+}
+
 template <int DP, bool F32>
 static hipError_t launch_dp(hipStream_t stream, const KvCache& c, const PagedAttn& p, const AttnPart& s) {
-    const dim3 grid((unsigned)s.blocks * (unsigned)c.heads), block(64 * kWaves);
-    if (tiles_of_16(c)) hipLaunchKernelGGL((paged_decode_kernel<DP, F32, true>), grid, block, 0, stream, c, p, s, p.table);
-    else hipLaunchKernelGGL((paged_decode_kernel<DP, F32, false>), grid, block, 0, stream, c, p, s, p.table);
-    return hipGetLastError();
+    return p.groups ? launch_shared<DP, F32, true>(stream, c, p, s) : launch_shared<DP, F32, false>(stream, c, p, s);
 }
 
 hipError_t launch_paged_decode(hipStream_t stream, const KvCache& c, const PagedAttn& p, const AttnPart& s) {
