@@ -107,6 +107,8 @@ constexpr int kChunkRows = 256, kChunkRowsWide = 128;  // dim to 128, above
 
 hipError_t launch_paged_decode(hipStream_t stream, const KvCache& c, const PagedAttn& p, const AttnPart& s);
 hipError_t launch_paged_chunk(hipStream_t stream, const KvCache& c, const PagedAttn& p, const AttnPart& s);
+// Both in one launch (bf16, dim to 128).
+hipError_t launch_paged_shared(hipStream_t stream, const KvCache& c, const PagedAttn& p, const AttnPart& many, const AttnPart& few);
 
 // Whether 16 tokens from a multiple of 16 lie in one block, their scales in a
 // row at 16-byte alignment, with offsets in the block and strides of blocks
