@@ -304,10 +304,10 @@ Plan shared_plan(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t dim,
         if (!few && dim <= 128) {
             // In one launch with the own tokens' part a prefix's splits take as many compute
             // units as are its share of the work, so that both end together: microseconds a
-            // unit, of a block's tile of 64 tokens 2.3 beside 9, of 256 own tokens 2.8 beside 5.
-            // (64 sequences behind 8192 tokens: 50 us with 13 splits a head, 54 with 10, 59 with
-            // 24; 96 behind three documents to 32760: 230 with 22, 267 with 18, 244 with 28.)
-            const double prefix = 2.3 * most * ceil_div(max_prefix, 64), rest = batch * (5 + max_kv * 0.011), all_units = std::max<double>(1, 256.0 / kv_heads);
+            // unit, of a block's tile of 64 tokens 2.3 beside 9, of 256 own tokens 2 beside 5.
+            // (64 sequences behind 8192 tokens: 49 us with 12 splits a head, 53 with 10, 58 with
+            // 24; 96 behind three documents to 32760: 230 with 24, 268 with 18, 241 with 28.)
+            const double prefix = 2.3 * most * ceil_div(max_prefix, 64), rest = batch * (5 + max_kv * 0.008), all_units = std::max<double>(1, 256.0 / kv_heads);
             const double each = std::max((prefix + rest) / all_units - 9, 7.0);
             shares = (int64_t)std::min(prefix / each, all_units) + 1;
         }
