@@ -585,11 +585,19 @@ __global__ __launch_bounds__(256, 2) void lora_batched_up_kernel(LoraBatched p, 
             // B's rows of a chunk, 32 ranks.
             auto load_b = [&](int n0, int k0, Eight<WB> (&b)[NT]) __attribute__((always_inline)) {
                 const int k = k0 + 8 * g;
+                const char* from[NT];
 #pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    const char* from = (const char*)p.B + (cls.adapter * p.b_adapter + min(n0 + NT * col + t, p.N - 1) * p.b_row) * (WB ? 2 : 4);
-                    if (p.R % 8 == 0) b[t] = k < p.R ? load_eight<WB>(from, k) : Eight<WB>{};
-                    else b[t] = load_masked<WB>(from, k, p.R, p.b_end);
+                for (int t = 0; t < NT; t++) from[t] = (const char*)p.B + (cls.adapter * p.b_adapter + min(n0 + NT * col + t, p.N - 1) * p.b_row) * (WB ? 2 : 4);
+                if (p.R % 8 == 0) {
+#pragma unroll
+                    for (int t = 0; t < NT; t++) b[t] = load_eight<WB>(from[t], k < p.R ? k : 0);
+#pragma unroll
+                    for (int t = 0; t < NT; t++)
+#pragma unroll
+                        for (int i = 0; i < (WB ? 4 : 8); i++) b[t].w[i] = k < p.R ? b[t].w[i] : 0;
+                } else {
+#pragma unroll
+                    for (int t = 0; t < NT; t++) b[t] = load_masked<WB>(from[t], k, p.R, p.b_end);
                 }
             };
             // The base of 16 rows' columns (rows behind the last: the last again, and of no base
@@ -618,11 +626,19 @@ __global__ __launch_bounds__(256, 2) void lora_batched_up_kernel(LoraBatched p, 
                     }
                     if (some && WIDE) {  // also by a wave without columns
                         const int pieces = ranks * T * (WB ? 2 : 4) / 16, each = ranks * (WB ? 2 : 4) / 16;
-#pragma unroll 4
-                        for (int j = threadIdx.x; j < n * pieces; j += 256) {
-                            const int c = j / pieces, e = j - c * pieces;
-                            const uint4 v = *(const uint4*)((const char*)p.joined + ((int64_t)rows[c] * pieces + e) * 16);
-                            *(uint4*)(lds + (c * T + e / each) * pitch * (WB ? 2 : 4) + e % each * 16) = v;
+                        constexpr int kMore = 6;
+#pragma unroll 1
+                        for (int j = threadIdx.x; j < n * pieces; j += 256 * kMore) {
+                            uint4 v[kMore];
+                            int c[kMore], e[kMore];
+#pragma unroll
+                            for (int i = 0; i < kMore; i++) {  // past the last: the last again
+                                const int at = min(j + 256 * i, n * pieces - 1);
+                                c[i] = at / pieces, e[i] = at - c[i] * pieces;
+                                v[i] = *(const uint4*)((const char*)p.joined + ((int64_t)rows[c[i]] * pieces + e[i]) * 16);
+                            }
+#pragma unroll
+                            for (int i = 0; i < kMore; i++) *(uint4*)(lds + (c[i] * T + e[i] / each) * pitch * (WB ? 2 : 4) + e[i] % each * 16) = v[i];
                         }
                         __syncthreads();
                     } else if (some) {
