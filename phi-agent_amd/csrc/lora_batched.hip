@@ -33,6 +33,7 @@ typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 
 constexpr int kSplits = 8;
 constexpr int kSpread = 128;  // places, from which on each XCD has neighbours
+constexpr int kUpTiles = 4;   // of 16 columns a wave
 
 // Up to `most` rows of one class, from the skip-th on.
 struct LoraUnit {
@@ -547,19 +548,17 @@ __global__ __launch_bounds__(256) void lora_batched_join_kernel(LoraBatched p, i
 
 // The update.  A wave has 16 NT columns n of out: lane l's are the NT from NT (l % 16) on, column
 // l % 16 of each of NT tiles of the matrix instruction, in rows 4 (l / 16) + i, so that
-// 16 lanes read and write 128 bytes of a row together, 256 of many rows (44.6 MB of base: 20 us
-// in pieces of 128).  A block has 4 waves' columns `chunks` times for all
+// 16 lanes read and write 128 bytes of a row together, 256 in fp32.  A block has 4 waves'
+// columns `chunks` times for all
 // rows of every `parts`-th class of its tile, `most` rows' h in LDS and 16 rows at a time, the
 // base of the four times 16 after them loading meanwhile.  B's first KS steps of 32 ranks stay in
 // registers, further ones are read again for each 16 rows.
-template <bool OB, bool WIDE> constexpr int up_tiles = OB && WIDE ? 4 : 4;
-
 template <bool WB, bool OB, int KS, bool WIDE>
 __global__ __launch_bounds__(256, 2) void lora_batched_up_kernel(LoraBatched p, int tiles, int across, int around, int parts, int chunks, int most) {
     constexpr int T = WB ? 3 : 1;  // terms of h
     constexpr int O = OB ? 2 : 4;  // bytes of an element
     constexpr int A = !WIDE ? 1 : OB ? 4 : 2;  // bases ahead
-    constexpr int NT = up_tiles<OB, WIDE>, kWave = 16 * NT, kBlock = 4 * kWave;
+    constexpr int NT = kUpTiles, kWave = 16 * NT, kBlock = 4 * kWave;
     typedef std::conditional_t<NT * O == 8, any2, any4> Run;
     __shared__ int rows[kLoraTile];
     extern __shared__ __align__(16) uint8_t lds[];
@@ -608,7 +607,7 @@ __global__ __launch_bounds__(256, 2) void lora_batched_up_kernel(LoraBatched p, 
             const int64_t ld_was = p.base ? p.ld_base : p.ldo;
             auto load_base = [&](int n0, int c, Run (&base)[4]) __attribute__((always_inline)) {
 #pragma unroll
-                for (int i = 0; i < 4; i++) base[i] = *(const Run*)(was + (rows[min(16 * c + 4 * g + i, n - 1)] * ld_was + n0 + NT * col) * O);
+                for (int i = 0; i < 4; i++) base[i] = __builtin_nontemporal_load((const Run*)(was + (rows[min(16 * c + 4 * g + i, n - 1)] * ld_was + n0 + NT * col) * O));
             };
             const int ahead = cols / A * A;  // tiles whose bases are loaded ahead
 #pragma unroll 1
@@ -790,7 +789,7 @@ void down(hipStream_t stream, const LoraBatched& p, int tiles, int classes) {
 
 template <bool WB, bool OB, int KS, bool WIDE>
 hipError_t up_ranks(hipStream_t stream, const LoraBatched& p, int tiles, int classes) {
-    const int ranks = (p.R + 31) / 32 * 32, block_n = 64 * up_tiles<OB, WIDE>, all = (p.N + block_n - 1) / block_n;
+    const int ranks = (p.R + 31) / 32 * 32, block_n = 64 * kUpTiles, all = (p.N + block_n - 1) / block_n;
     const size_t row = WB ? 3 * (ranks + 8) * 2 : (ranks + 4) * 4;
     const int most = row * kLoraTile <= kMaxLds ? kLoraTile : kLoraTile / 2;
     const size_t lds = row * std::min(most, (p.rows + 15) / 16 * 16);
@@ -798,10 +797,13 @@ hipError_t up_ranks(hipStream_t stream, const LoraBatched& p, int tiles, int cla
         const hipError_t e = hipFuncSetAttribute((const void*)lora_batched_up_kernel<WB, OB, KS, WIDE>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (e != hipSuccess) return e;
     }
-    // Two blocks a compute unit.
-    const int want = (int)std::max<int64_t>(1, 1024 / tiles);
+    // A block's first loads take 10 us whatever it has to do with them.  Two fit a compute unit:
+    // of many rows no more than run at once, a fifth of them for tiles of two classes
+    // (4352 rows of 5120 columns in 34 tiles of 10 blocks: 31 us; in 34 of 20, the last of which
+    // begin when the first have ended, 42; of 5, 44).
+    const int want = (int)std::max<int64_t>(1, (WIDE ? 410 : 1024) / tiles);
     const int chunks = (all + std::min(want, all) - 1) / std::min(want, all), across = (all + chunks - 1) / chunks;
-    const int parts = (int)std::clamp<int64_t>((WIDE ? 512 : 1024) / ((int64_t)tiles * across), 1, classes);
+    const int parts = (int)std::clamp<int64_t>(1024 / ((int64_t)tiles * across), 1, classes);
     const int around = places(tiles * across);
     const dim3 grid((unsigned)(around * parts)), block(256);
     if (WIDE) {
