@@ -699,18 +699,31 @@ __global__ __launch_bounds__(256, 2) void lora_batched_up_kernel(LoraBatched p, 
                             *(Run*)to = w;
                         }
                     } else {
+                        // Element by element: all are loaded (behind the last: the last again)
+                        // before one is used.
+                        float was[4][NT] = {};
+                        if (p.base) {
+#pragma unroll
+                            for (int i = 0; i < 4; i++) {
+                                const int64_t from = rows[min(16 * c + 4 * g + i, n - 1)] * p.ld_base;
+#pragma unroll
+                                for (int t = 0; t < NT; t++) {
+                                    const int64_t at = from + min(n0 + NT * col + t, p.N - 1);
+                                    was[i][t] = OB ? bf16_to_f32(((const uint16_t*)p.base)[at]) : ((const float*)p.base)[at];
+                                }
+                            }
+                        }
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
                             if (16 * c + 4 * g + i >= n) continue;
-                            const int64_t row = rows[16 * c + 4 * g + i];
+                            const int64_t to = rows[16 * c + 4 * g + i] * p.ldo;
 #pragma unroll
                             for (int t = 0; t < NT; t++) {
                                 const int at = n0 + NT * col + t;
                                 if (at >= p.N) continue;
-                                float y = acc[t][i];
-                                if (p.base) y += OB ? bf16_to_f32(((const uint16_t*)p.base)[row * p.ld_base + at]) : ((const float*)p.base)[row * p.ld_base + at];
-                                if (OB) ((uint16_t*)p.out)[row * p.ldo + at] = (uint16_t)f32_to_bf16(y);
-                                else ((float*)p.out)[row * p.ldo + at] = y;
+                                const float y = p.base ? acc[t][i] + was[i][t] : acc[t][i];
+                                if (OB) ((uint16_t*)p.out)[to + at] = (uint16_t)f32_to_bf16(y);
+                                else ((float*)p.out)[to + at] = y;
                             }
                         }
                     }
