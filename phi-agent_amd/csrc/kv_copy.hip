@@ -3,6 +3,8 @@
 // Bound by memory.  A pair's codes of k, then of v, are pieces of 16 bytes in the order
 // in which they lie (tokens within heads, or heads within tokens), kPieces a thread, all
 // of a thread's loads before its stores; then both scales, a float each.
+#include <algorithm>
+
 #include "device_common.hpp"
 #include "serving.hpp"
 
@@ -93,11 +95,18 @@ hipError_t launch_kv_cache_copy(hipStream_t stream, const KvCopy& p) {
     const bool dense = inner == c.dim && outer == (token_inner ? c.page : c.heads) * inner && p.to.token_stride == c.token_stride && p.to.head_stride == c.head_stride;
     const int64_t vectors = (int64_t)c.heads * c.page, pieces = vectors * (c.dim / 16), each = 256 * kPieces;
     const int code_parts = (int)((pieces + each - 1) / each), scale_parts = (int)((vectors + each - 1) / each);
-    const int64_t grid = p.n * (2 * (int64_t)code_parts + scale_parts);
-    if (grid > INT32_MAX) return hipErrorInvalidConfiguration;
-    hipLaunchKernelGGL(kv_copy_kernel, dim3((unsigned)grid), dim3(256), 0, stream, p, div_by(c.dim / 16),
-                       div_by(token_inner ? c.page : c.heads), token_inner, dense, code_parts, scale_parts);
-    return hipGetLastError();
+    const int64_t per = 2 * (int64_t)code_parts + scale_parts, at_once = kMaxBlocks / per;
+    for (int64_t i = 0; i < p.n; i += at_once) {
+        KvCopy s = p;
+        s.n = std::min(p.n - i, at_once);
+        s.from_blocks += i, s.to_blocks += i;
+        if (s.tokens) s.tokens += i;
+        hipLaunchKernelGGL(kv_copy_kernel, dim3((unsigned)(s.n * per)), dim3(256), 0, stream, s, div_by(c.dim / 16),
+                           div_by(token_inner ? c.page : c.heads), token_inner, dense, code_parts, scale_parts);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace phi_dev

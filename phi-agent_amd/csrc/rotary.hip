@@ -261,14 +261,27 @@ static hipError_t launch(hipStream_t stream, const Rotary& p, const KvCache& c) 
     const int64_t want = (2048 + groups - 1) / groups;
     const int per_part = 4 * ((most + (int)(want < most ? want : most) - 1) / (int)(want < most ? want : most));
     const int parts = (heads + per_part - 1) / per_part;
-    if (groups * parts > INT32_MAX) return hipErrorInvalidConfiguration;
-    const dim3 grid((unsigned)(groups * parts)), block(256);
-    switch (rotary_width(p)) {
-        case 8: hipLaunchKernelGGL((rotary_kernel<BF16, INTER, WRITE, 8>), grid, block, 0, stream, p, c, lg, parts, per_part); break;
-        case 4: hipLaunchKernelGGL((rotary_kernel<BF16, INTER, WRITE, 4>), grid, block, 0, stream, p, c, lg, parts, per_part); break;
-        default: hipLaunchKernelGGL((rotary_kernel<BF16, INTER, WRITE, 1>), grid, block, 0, stream, p, c, lg, parts, per_part);
+    const int64_t at_once = kMaxBlocks / parts << (6 - lg);  // tokens
+    const int width = rotary_width(p);
+    for (int64_t t = 0; t < p.tokens; t += at_once) {
+        Rotary s = p;
+        s.tokens = p.tokens - t < at_once ? p.tokens - t : at_once;
+        for (RotaryHeads* h : {&s.q, &s.k, &s.v}) {
+            h->in = (const char*)h->in + t * h->in_token * (BF16 ? 2 : 4);
+            h->out = (char*)h->out + t * h->out_token * (BF16 ? 2 : 4);
+        }
+        s.positions += t;
+        if (WRITE) s.slots += t;
+        const dim3 grid((unsigned)((s.tokens + (64 >> lg) - 1 >> (6 - lg)) * parts)), block(256);
+        switch (width) {
+            case 8: hipLaunchKernelGGL((rotary_kernel<BF16, INTER, WRITE, 8>), grid, block, 0, stream, s, c, lg, parts, per_part); break;
+            case 4: hipLaunchKernelGGL((rotary_kernel<BF16, INTER, WRITE, 4>), grid, block, 0, stream, s, c, lg, parts, per_part); break;
+            default: hipLaunchKernelGGL((rotary_kernel<BF16, INTER, WRITE, 1>), grid, block, 0, stream, s, c, lg, parts, per_part);
+        }
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
     }
-    return hipGetLastError();
+    return hipSuccess;
 }
 
 hipError_t launch_rotary(hipStream_t stream, const Rotary& p, const KvCache& c) {

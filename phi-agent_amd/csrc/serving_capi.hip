@@ -9,8 +9,9 @@ using namespace phi_capi;
 namespace {
 
 constexpr int64_t kMaxRotaryDim = 1024;   // a wave has a vector
-constexpr int64_t kMaxRank = 256;              // of an adapter: h of 32 rows is held in LDS
+constexpr int64_t kMaxRank = 256;         // of an adapter: h of 32 rows is held in LDS
 constexpr int64_t kMaxLoraRows = 1 << 24, kMaxLoraK = 1 << 24;  // units and columns counted in 31 bits
+constexpr int64_t kMaxHeadRows = 1 << 26;     // of shared prefixes, a wave each: threads of a launch are counted in 32 bits
 constexpr int64_t kMaxPageVectors = 1 << 26;  // of at most 16 pieces: counted in 31 bits
 
 // [tokens, heads, dim] vectors that are written: one of the strides holds the other's
@@ -154,6 +155,7 @@ phi_status phi_hip_paged_attention_shared(phi_stream_t stream, const void* q, in
                     (long long)groups, (long long)batch, (long long)max_prefix, (long long)max_q, (long long)max_kv);
     if (tokens * (q_heads / c.heads) > kMaxRows)
         return fail(PHI_ERR_SHAPE, "%s: tokens=%lld at %lld query heads a key/value head is out of range", who, (long long)tokens, (long long)(q_heads / c.heads));
+    if (tokens * q_heads >= kMaxHeadRows) return fail(PHI_ERR_SHAPE, "%s: tokens=%lld of %lld heads is out of range", who, (long long)tokens, (long long)q_heads);
     if (groups == 0) return fail(PHI_ERR_SHAPE, "%s: no groups", who);
     if (max_kv > 0 && (table_width > INT32_MAX || max_kv > table_width * c.page))
         return fail(PHI_ERR_SHAPE, "%s: max_kv=%lld exceeds the block table's %lld x %d tokens", who, (long long)max_kv, (long long)table_width, c.page);
@@ -178,7 +180,8 @@ phi_status phi_hip_paged_attention_shared(phi_stream_t stream, const void* q, in
         return fail(PHI_ERR_WORKSPACE, "%s: needs %zu bytes of workspace, got %zu", who, need, workspace ? ws_bytes : (size_t)0);
     if (!aligned(workspace, 16)) return fail(PHI_ERR_ALIGN, "%s: the workspace must be 16-byte aligned", who);
     const Pieces ws{workspace, (int64_t)need};
-    if (meet(ws, qs) || meet(ws, os)) return fail(PHI_ERR_ARG, "%s: the workspace overlaps q or out", who);
+    if (meet(ws, qs) || meet(ws, os) || meets_cache(ws, c)) return fail(PHI_ERR_ARG, "%s: the workspace overlaps q, out or the cache", who);
+    if (meets_cache(os, c)) return fail(PHI_ERR_ARG, "%s: out overlaps the cache", who);
     phi_dev::PagedAttn p{q, out, block_table, q_start, kv_len, q_token_stride, q_head_stride, out_token_stride, out_head_stride, table_stride,
                          tokens, (int)q_heads, (int)(q_heads / c.heads), (int)batch, (int)max_q, (int)max_kv, (int)table_width, 0, 0, scale,
                          dtype == PHI_BF16, true, prefix_len, group_start, ((int64_t)(uintptr_t)prefix_table - (int64_t)(uintptr_t)block_table) / 4, prefix_stride, (int)groups,
@@ -191,7 +194,7 @@ size_t phi_hip_paged_attention_shared_workspace_bytes(int64_t tokens, int64_t q_
                                                       int64_t max_q, int64_t max_kv, int dtype) {
     if (tokens <= 0 || q_heads <= 0 || kv_heads <= 0 || dim <= 0 || groups <= 0 || batch <= 0 || max_q <= 0 || max_kv < 0 || max_prefix < 0) return 0;
     if (tokens > INT32_MAX || q_heads > 65535 || dim > 256 || groups > 65535 || batch > 65535 || max_q > tokens || max_kv > kMaxKv || max_prefix > kMaxKv) return 0;
-    if (q_heads % kv_heads != 0 || tokens * (q_heads / kv_heads) > kMaxRows) return 0;
+    if (q_heads % kv_heads != 0 || tokens * (q_heads / kv_heads) > kMaxRows || tokens * q_heads >= kMaxHeadRows) return 0;
     return phi_dev::paged_attention_shared_workspace(tokens, (int)q_heads, (int)kv_heads, (int)dim, (int)groups, (int)batch, (int)max_prefix, (int)max_q,
                                                      (int)max_kv, dtype == PHI_BF16);
 }

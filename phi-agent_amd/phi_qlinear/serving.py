@@ -152,7 +152,9 @@ class KvPages:
     (from, to, tokens), for `flush` to do before the next write or attention.
 
     A sequence's pages are append-only, so a forked one shares its parent's whole
-    pages and gets a copy of the last where that is not full."""
+    pages and gets a copy of the last where that is not full: the parent's tokens are
+    written before the flush that makes it.  Slots hold until pages move (`compact`);
+    those that were not written by then are not valid after it."""
 
     def __init__(self, blocks: int, page: int):
         self.page, self.of, self.length, self.copies = page, {}, {}, []

@@ -199,3 +199,72 @@ def test_on_a_stream_and_in_graphs(dev):
             g.replay()
         torch.cuda.synchronize()
         assert all(same_bits(a, b) for a, b in zip(outs, want))
+
+
+@pytest.mark.parametrize("M,K", [(130, 48), (600, 512)])
+def test_adapters_of_one_place_in_the_table(dev, M, K):
+    """Numbers that agree in their low bits, in every tile, few rows and many."""
+    n = 4200
+    x, A, B, _, scale, base = inputs(M, K, 40, 4, n, BF16, BF16, BF16)
+    i = torch.arange(M)
+    adapter = ((i * 7 % 5) * 1024 + i % 3 - 1).int()  # -1 to 4097
+    got = Q.lora_batched(*(t.to(dev) for t in (x, A, B, adapter)), scale=scale.to(dev), base=base.to(dev))
+    want, mag = R.adapted(x, A, B, adapter, scale, base)
+    fine, by = near(got, want, mag, base, K, 4)
+    assert fine, by
+
+
+@pytest.mark.parametrize("off", [1, 8])
+@pytest.mark.parametrize("wd,od,rank", [(BF16, BF16, 24), (F32, F32, 40), (BF16, F32, 256), (F32, BF16, 200)])
+def test_many_rows_in_place_and_strided(dev, off, wd, od, rank):
+    M, K, N, n = 700, 520, 333, 5
+    x, A, B, adapter, scale, base = (t.to(dev) for t in inputs(M, K, N, rank, n, BF16, wd, od))
+    want = Q.lora_batched(x, A, B, adapter, scale=scale, base=base)
+    exact, mag = R.adapted(*(t.cpu() for t in (x, A, B, adapter, scale, base)))
+    fine, by = near(want, exact, mag, base.cpu(), K, rank)
+    assert fine, by
+
+    def within(t):
+        wide = torch.full((*t.shape[:-1], t.shape[-1] + off + 3), 9.0, dtype=t.dtype, device=dev)
+        part = wide[..., off:off + t.shape[-1]]
+        part.copy_(t)
+        return wide, part
+
+    (_, xs), (_, As), (_, Bs), (wide, bs) = within(x), within(A), within(B), within(base)
+    assert Q.lora_batched(xs, As, Bs, adapter, scale=scale, base=bs, out=bs) is bs and same_bits(bs, want)
+    assert bool((wide[:, :off] == 9).all()) and bool((wide[:, off + N:] == 9).all())
+
+
+def test_many_rows_do_not_depend_on_their_neighbours(dev):
+    x, A, B, adapter, scale, base = (t.to(dev) for t in inputs(650, 576, 300, 16, 6, BF16, BF16, BF16))
+    adapter.clamp_(0, 5)
+    want = Q.lora_batched(x, A, B, adapter, scale=scale, base=base)
+    for a in range(6):
+        mine = adapter == a
+        got = Q.lora_batched(x, A, B, torch.where(mine, adapter, torch.full_like(adapter, 6)), scale=scale, base=base)
+        assert same_bits(got[mine], want[mine]) and same_bits(got[~mine], base[~mine])
+    x2, A2 = x.clone(), A.clone()
+    x2[7], A2[2] = math.nan, math.inf
+    keep = adapter != 2
+    keep[7] = False
+    assert same_bits(Q.lora_batched(x2, A2, B, adapter, scale=scale, base=base)[keep], want[keep])
+
+
+def test_many_rows_in_a_graph(dev):
+    """Captured in place, replayed on other adapters and activations, eager work between."""
+    M, K, N, rank, n = 640, 512, 384, 64, 3
+    x, A, B, adapter, scale, base = (t.to(dev) for t in inputs(M, K, N, rank, n, BF16, BF16, BF16))
+    ws, out = Q.lora_batched_workspace(M, K, rank, dev), base.clone()
+    call = lambda o: Q.lora_batched(x, A, B, adapter, scale=scale, base=o, out=o, workspace=ws)  # noqa: E731
+    call(out)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        call(out)
+    for k in range(3):
+        x.copy_(randn((M, K), 70 + k, BF16))
+        adapter.copy_(torch.randint(-1, n + 1, (M,), generator=torch.Generator().manual_seed(k)).int())
+        want = call(base.clone())
+        out.copy_(base)
+        g.replay()
+        torch.cuda.synchronize()
+        assert same_bits(out, want)

@@ -124,6 +124,18 @@ def test_rotary_of_no_tokens(dev):
     assert Q.rotary_cache_write(c, e, e[:, :2], e[:, 2:], z, f, z).shape == (0, 4, 64)
 
 
+def test_rotary_of_more_tokens_than_a_launch_has(dev):
+    """2^24 + 50 tokens, a block each: the last of the first launch, and the second's."""
+    T, D = (1 << 24) + 50, 513
+    row = randn((1, 1, D), 4, BF16)
+    pos, f = torch.arange(T, device=dev), Q.rotary_frequencies(512, device=dev)
+    out = torch.full((T, 1, D), 7, dtype=BF16, device=dev)
+    Q.rotary(row.to(dev).expand(T, 1, D), pos, f, out=out)
+    for a, b in ((0, 3), ((1 << 24) - 30, T)):
+        want = Q.rotary(row.to(dev).expand(b - a, 1, D).contiguous(), pos[a:b], f)
+        assert same_bits(out[a:b], want)
+
+
 def test_rotary_python_refusals(dev):
     x = torch.zeros((4, 2, 64), device=dev)
     pos, f = torch.arange(4, device=dev), Q.rotary_frequencies(64, device=dev)
@@ -250,6 +262,17 @@ def test_copy_between_caches(dev, H, page, D, n, majors, part):
         Q.kv_cache_copy(a, target, frm.to(dev), to.to(dev), tokens=None if tokens is None else tokens.to(dev))
         for x, y in zip(target, want):
             assert same_bits(x, y)
+
+
+def test_copy_of_more_pages_than_a_launch_has(dev):
+    n = 5_700_000  # three blocks a page
+    a, b = (Q.kv_cache_empty(n, 1, 1, 16, dev) for _ in range(2))
+    for x in a:
+        x.copy_(torch.arange(x.numel(), device=dev).view(x.shape) % 127)
+    to = torch.arange(n, device=dev, dtype=torch.int32)
+    Q.kv_cache_copy(a, b, to.flip(0), to, tokens=(to % 7 > 0).int())
+    for x, y in zip(a, b):
+        assert bool((x.flip(0) == y)[to % 7 > 0].all())
 
 
 def test_copy_of_a_part_of_a_wider_cache(dev):

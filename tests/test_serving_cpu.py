@@ -240,6 +240,7 @@ def shared(lib, c, q=A, dtype=Q.BF16, qt=256, qh=64, tokens=8, heads=4, ptable=B
     (2, "out of range", dict(groups=70000)),
     (2, "out of range", dict(max_prefix=(1 << 30) + 1)),
     (2, "out of range", dict(tokens=(1 << 29) + 1)),
+    (2, "out of range", dict(tokens=1 << 24)),
     (2, "no groups", dict(groups=0)),
     (2, "block table", dict(max_kv=65)),
     (2, "prefix table", dict(max_prefix=97)),
@@ -264,6 +265,8 @@ def shared(lib, c, q=A, dtype=Q.BF16, qt=256, qh=64, tokens=8, heads=4, ptable=B
     (3, "workspace", dict(ws=ctypes.c_void_p((8 << 28) + 8))),
     (1, "workspace overlaps", dict(ws=A)),
     (1, "workspace overlaps", dict(ws=G)),
+    (1, "workspace overlaps", dict(ws=ctypes.c_void_p(K2))),
+    (1, "out overlaps the cache", dict(out=ctypes.c_void_p(K2))),
 ])
 def test_shared_attention_refuses(lib, rc, text, kw):
     assert shared(lib, far(), **kw) == rc and text in Q.last_error() and "paged_attention_shared" in Q.last_error()
