@@ -240,3 +240,24 @@ def test_nothing_to_do_and_refusals(dev):
                      (dict(scale=math.inf), "scale"), (dict(out=args["q"]), "overlap"), (dict(workspace=torch.empty(64, dtype=torch.uint8, device=dev)), "workspace")):
         with pytest.raises(Q.QLinearError, match=text):
             Q.paged_attention_shared(**{**args, **kw})
+
+
+def test_past_32_bits_of_cache(dev):
+    """Blocks behind 2^32 bytes: written, copied to the first ones and seen, to the same bits."""
+    H, page, D, n = 2, 64, 256, 3
+    blocks = (1 << 32) // (H * page * D) + 4
+    c = Q.kv_cache_empty(blocks, page, H, D, dev)
+    T = n * page
+    k, v = (torch.randn((T, H, D), generator=torch.Generator().manual_seed(i)).to(dev, BF16) for i in (1, 2))
+    pos, freq = torch.arange(T, device=dev), Q.rotary_frequencies(D, device=dev)
+    high = torch.arange(blocks - n, blocks, dtype=torch.int32, device=dev)
+    low = torch.arange(n, dtype=torch.int32, device=dev)
+    Q.rotary_cache_write(c, None, k, v, pos, freq, (high.long()[:, None] * page + torch.arange(page, device=dev)).flatten())
+    Q.kv_cache_copy(c, c, high, low)
+    for x in c:
+        assert torch.equal(x[low.long()].view(torch.uint8), x[high.long()].view(torch.uint8))
+    q = torch.randn((40, 4, D), generator=torch.Generator().manual_seed(3)).to(dev, BF16)
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    got = [Q.paged_attention_shared(q, c, t[None, :2], i32(2 * page), i32(0, 2), t[None, 2:].expand(2, -1).contiguous(), i32(0, 20, 40), i32(page, 33),
+                                    max_prefix=2 * page, max_q=20, max_kv=page) for t in (low, high)]
+    assert same_bits(*got) and bool(got[0].any())
