@@ -1,8 +1,9 @@
 // Blocks of the paged cache copied: forked sequences' last pages, compaction.
 //
 // Bound by memory.  A pair's codes of k, then of v, are pieces of 16 bytes in the order
-// in which they lie (tokens within heads, or heads within tokens), kPieces a thread, all
-// of a thread's loads before its stores; then both scales, a float each.
+// in which they lie (tokens within heads, or heads within tokens), one a thread; then both
+// scales, a float each.  (Four pieces a thread, loaded before they are stored: 115 us, 113 so,
+// for 3/4 of 1536 pages of 64 tokens, 8 heads of 128.)
 #include <algorithm>
 
 #include "device_common.hpp"
@@ -11,8 +12,6 @@
 namespace phi_dev {
 
 namespace {
-
-constexpr int kPieces = 4;
 
 // n / d as (n * mul) >> shift for 0 <= n < 2^31.
 struct Div {
@@ -40,52 +39,35 @@ __global__ __launch_bounds__(256, 8) void kv_copy_kernel(KvCopy p, Div vector, D
     const uint32_t vectors = (uint32_t)p.from.heads * (uint32_t)p.from.page;
     const bool scales = part >= 2 * code_parts;
     const bool v = !scales && part >= code_parts;
-    const uint32_t first = (uint32_t)(scales ? part - 2 * code_parts : v ? part - code_parts : part) * (256 * kPieces) + threadIdx.x;
+    const uint32_t first = (uint32_t)(scales ? part - 2 * code_parts : v ? part - code_parts : part) * 256 + threadIdx.x;
     // Vector n's head and token.
     auto place = [&](uint32_t n, uint32_t& head, uint32_t& token) {
         const uint32_t o = quotient(inner, n), in = n - o * inner.d;
         head = token_inner ? o : in, token = token_inner ? in : o;
     };
     if (scales) {
-        for (int j = 0; j < kPieces; j++) {
-            const uint32_t n = first + 256 * j;
-            uint32_t head, token;
-            if (n >= vectors) return;
-            place(n, head, token);
-            if (token >= take) continue;
-            const int64_t a = from * p.from.s_block_stride + head * p.from.s_head_stride + token * p.from.s_token_stride;
-            const int64_t b = to * p.to.s_block_stride + head * p.to.s_head_stride + token * p.to.s_token_stride;
-            p.to.ks[b] = p.from.ks[a];
-            p.to.vs[b] = p.from.vs[a];
-        }
+        uint32_t head, token;
+        if (first >= vectors) return;
+        place(first, head, token);
+        if (token >= take) return;
+        const int64_t a = from * p.from.s_block_stride + head * p.from.s_head_stride + token * p.from.s_token_stride;
+        const int64_t b = to * p.to.s_block_stride + head * p.to.s_head_stride + token * p.to.s_token_stride;
+        p.to.ks[b] = p.from.ks[a];
+        p.to.vs[b] = p.from.vs[a];
         return;
     }
     const int8_t* src = (v ? p.from.v : p.from.k) + from * p.from.block_stride;
     int8_t* dst = (v ? p.to.v : p.to.k) + to * p.to.block_stride;
-    const uint32_t pieces = vectors * vector.d;
-    v4i x[kPieces];
+    if (first >= vectors * vector.d) return;
     if (dense && take == (uint32_t)p.from.page) {
-#pragma unroll
-        for (int j = 0; j < kPieces; j++) x[j] = first + 256 * j < pieces ? *(const v4i*)(src + 16 * (uint64_t)(first + 256 * j)) : v4i{0, 0, 0, 0};
-#pragma unroll
-        for (int j = 0; j < kPieces; j++)
-            if (first + 256 * j < pieces) *(v4i*)(dst + 16 * (uint64_t)(first + 256 * j)) = x[j];
+        *(v4i*)(dst + 16 * (uint64_t)first) = *(const v4i*)(src + 16 * (uint64_t)first);
         return;
     }
-    int64_t at[kPieces];
-#pragma unroll
-    for (int j = 0; j < kPieces; j++) {
-        const uint32_t n = first + 256 * j, vec = quotient(vector, n);
-        uint32_t head, token;
-        place(vec, head, token);
-        const bool has = vec < vectors && token < take;
-        const uint32_t in = 16 * (n - vec * vector.d);
-        at[j] = has ? head * p.to.head_stride + token * p.to.token_stride + in : -1;
-        if (has) x[j] = *(const v4i*)(src + head * p.from.head_stride + token * p.from.token_stride + in);
-    }
-#pragma unroll
-    for (int j = 0; j < kPieces; j++)
-        if (at[j] >= 0) *(v4i*)(dst + at[j]) = x[j];
+    const uint32_t vec = quotient(vector, first), in = 16 * (first - vec * vector.d);
+    uint32_t head, token;
+    place(vec, head, token);
+    if (token < take)
+        *(v4i*)(dst + head * p.to.head_stride + token * p.to.token_stride + in) = *(const v4i*)(src + head * p.from.head_stride + token * p.from.token_stride + in);
 }
 
 hipError_t launch_kv_cache_copy(hipStream_t stream, const KvCopy& p) {
@@ -93,7 +75,7 @@ hipError_t launch_kv_cache_copy(hipStream_t stream, const KvCopy& p) {
     const bool token_inner = c.token_stride <= c.head_stride;
     const int64_t inner = token_inner ? c.token_stride : c.head_stride, outer = token_inner ? c.head_stride : c.token_stride;
     const bool dense = inner == c.dim && outer == (token_inner ? c.page : c.heads) * inner && p.to.token_stride == c.token_stride && p.to.head_stride == c.head_stride;
-    const int64_t vectors = (int64_t)c.heads * c.page, pieces = vectors * (c.dim / 16), each = 256 * kPieces;
+    const int64_t vectors = (int64_t)c.heads * c.page, pieces = vectors * (c.dim / 16), each = 256;
     const int code_parts = (int)((pieces + each - 1) / each), scale_parts = (int)((vectors + each - 1) / each);
     const int64_t per = 2 * (int64_t)code_parts + scale_parts, at_once = kMaxBlocks / per;
     for (int64_t i = 0; i < p.n; i += at_once) {
