@@ -3,7 +3,7 @@
 // Bound by memory.  A pair's codes of k, then of v, are pieces of 16 bytes in the order
 // in which they lie (tokens within heads, or heads within tokens), one a thread; then both
 // scales, a float each.  (Four pieces a thread, loaded before they are stored: 115 us, 113 so,
-// for 3/4 of 1536 pages of 64 tokens, 8 heads of 128.)
+// for 2048 pages of 64 tokens, 8 heads of 128, 4.8 TB/s.)
 #include <algorithm>
 
 #include "device_common.hpp"

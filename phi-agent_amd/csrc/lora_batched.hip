@@ -11,6 +11,10 @@
 // in the e-th, g = l / 16, on both sides).
 // h is fp32 throughout: against bf16 factors it enters the second product as three
 // bf16, all of its 24 bits.
+// Bound by memory: x once, base and out once, each tile's factors from L2.  64 rows of
+// 4096 on 16 ranks to 6144, 32 adapters at random: 6 + 8 us, latency (counts, classes, rows and
+// factors are loads that wait for each other); eight prompts of 4352 rows of 5120 on 64 ranks
+// to 5120: 20 + 5 + 33 us, x at 2.3 TB/s, base and out at 2.7.
 #include <algorithm>
 #include <type_traits>
 
@@ -32,7 +36,7 @@ namespace {
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 
 constexpr int kSplits = 8;
-constexpr int kSpread = 128;  // places, from which on each XCD has neighbours
+constexpr int kSpread = 128;  // places, from which on each XCD has neighbours (4352 rows on 64 ranks: 56 us, 60 never)
 constexpr int kUpTiles = 4;   // of 16 columns a wave
 
 // Up to `most` rows of one class, from the skip-th on.
@@ -341,14 +345,13 @@ __global__ __launch_bounds__(256, 2) void lora_batched_down_kernel(LoraBatched p
 // Waves 0-3 have 32 rows each of the first half of the block's stretch of K, waves 4-7 of the
 // second; a half's four waves share A's step of H 32 k in LDS, two steps' in turn, and
 // load two steps ahead.
-template <bool XB, bool WB, int RT>
+template <bool XB, bool WB>
 __global__ __launch_bounds__(512, 2) void lora_batched_down_wide_kernel(LoraBatched p, int tiles, int around, int parts) {
-    constexpr int H = XB && WB ? 2 : 1, kStep = 32 * H, P = 16 * RT + 4;
+    constexpr int RT = 4, H = XB && WB ? 2 : 1, kStep = 32 * H, P = 16 * RT + 4;
     typedef Rows<XB, H> RX;
     typedef Rows<WB, H> RA;
     constexpr int kA = RT * RA::kBytes, kX = 2 * RX::kBytes, kStage = 2 * 2 * kA + 8 * kX, kJoin = kLoraTile * P * 4;
-    // A's rows to load: RT tiles by four waves.
-    constexpr int kMine = RT * RA::kLoads / 4 > 0 ? RT * RA::kLoads / 4 : 1;
+    constexpr int kMine = RA::kLoads;  // of A's: a tile a wave
     __shared__ int rows[kLoraTile];
     __shared__ __align__(16) uint8_t lds[kStage > kJoin ? kStage : kJoin];
     __shared__ LoraTable table;
@@ -391,7 +394,6 @@ __global__ __launch_bounds__(512, 2) void lora_batched_down_wide_kernel(LoraBatc
         for (int c = 0; c < 2; c++)
 #pragma unroll
             for (int i = 0; i < RX::kLoads; i++) xs[c][i] = (const char*)p.x + (int64_t)rows[min(32 * w + 16 * c + RX::row(i), u.n - 1)] * p.ldx * (XB ? 2 : 4);
-        // Load j of the wave: loads RA::kLoads a tile, tile by tile.
         auto a_load = [&](int j) { return w * kMine + j; };
 #pragma unroll
         for (int j = 0; j < kMine; j++) {
@@ -443,8 +445,7 @@ __global__ __launch_bounds__(512, 2) void lora_batched_down_wide_kernel(LoraBatc
 #pragma unroll
                 for (int j = 0; j < kMine; j++) {
                     const int at = a_load(j);
-                    if (at < RT * RA::kLoads)
-                        *(uint4*)(lds_a + (64 / RA::kLanes * at + lane / RA::kLanes) * RA::kPitch + 16 * (lane % RA::kLanes)) = make_uint4(t.a[j][0], t.a[j][1], t.a[j][2], t.a[j][3]);
+                    *(uint4*)(lds_a + (64 / RA::kLanes * at + lane / RA::kLanes) * RA::kPitch + 16 * (lane % RA::kLanes)) = make_uint4(t.a[j][0], t.a[j][1], t.a[j][2], t.a[j][3]);
                 }
                 if (mine) t.x[0].to(lds_x), t.x[1].to(lds_x + RX::kBytes);
             } else if (s < s1) {
@@ -764,13 +765,18 @@ int rank_pitch(int64_t R) { return (int)(16 * ceil_div(R, 16)); }
 
 constexpr size_t kMaxLds = 159 << 10;  // a compute unit's 160 KB, less the rows' numbers
 
-// Whether blocks take whole tiles' rows (whose loads are whole steps of K).
-bool is_wide(int64_t rows, int64_t K) { return rows >= 512 && K >= 512; }
+// Whether blocks take whole tiles' rows (whose loads are whole steps of K): what that saves
+// are readings of A, so it is for many ranks.  Microseconds for eight adapters of 4096 x 4096,
+// a run of rows each and at random: 4352 rows on 64 ranks 53 and 104, not wide 75 and 127;
+// 1024 rows 32 and 41, 39 and 36; 512 rows 24 and 29, 26 and 25; 4352 rows on 16 ranks 42 and
+// 87, 41 and 69.
+bool is_wide(int64_t rows, int64_t K, int64_t R) { return rows >= 1024 && K >= 512 && R > 32; }
 
 // Parts of K: enough blocks where there are few rows, a part no shorter than 512; of wide
 // blocks no more than fit the compute units at once, with room for tiles of two classes.
-int splits_of(int64_t rows, int64_t K) {
-    const int64_t want = is_wide(rows, K) ? 256 / (ceil_div(rows, kLoraTile) * 5 / 4) : 512 / ceil_div(rows, kFewCols);
+// (64 rows of 4096: 15.9 us with eight at most, 16.9 with four, 16.3 with 16.)
+int splits_of(int64_t rows, int64_t K, int64_t R) {
+    const int64_t want = is_wide(rows, K, R) ? 256 / (ceil_div(rows, kLoraTile) * 5 / 4) : 512 / ceil_div(rows, kFewCols);
     return (int)std::clamp<int64_t>(want, 1, std::min<int64_t>(kSplits, ceil_div(K, 512)));
 }
 
@@ -779,9 +785,9 @@ int places(int n) { return n >= kSpread ? (n + 7) / 8 * 8 : n; }
 template <bool XB, bool WB, int RT>
 void down_ranks(hipStream_t stream, const LoraBatched& p, int tiles, int classes, int groups) {
     const int around = places(tiles * p.splits);
-    if (is_wide(p.rows, p.K)) {
+    if (RT == 4 && p.joined) {
         const int parts = (int)std::clamp<int64_t>(256 / ((int64_t)tiles * p.splits * groups), 1, classes);
-        hipLaunchKernelGGL((lora_batched_down_wide_kernel<XB, WB, RT>), dim3((unsigned)(around * parts), 1, (unsigned)groups), dim3(512), 0, stream,
+        hipLaunchKernelGGL((lora_batched_down_wide_kernel<XB, WB>), dim3((unsigned)(around * parts), 1, (unsigned)groups), dim3(512), 0, stream,
                            p, tiles, around, parts);
         return;
     }
@@ -816,7 +822,9 @@ hipError_t up_ranks(hipStream_t stream, const LoraBatched& p, int tiles, int cla
     // begin when the first have ended, 42; of 5, 44).
     const int want = (int)std::max<int64_t>(1, (WIDE ? 410 : 1024) / tiles);
     const int chunks = (all + std::min(want, all) - 1) / std::min(want, all), across = (all + chunks - 1) / chunks;
-    const int parts = (int)std::clamp<int64_t>(1024 / ((int64_t)tiles * across), 1, classes);
+    // Of mixed rows a block has several classes, of others most blocks end at once: so more of
+    // wide ones (4352 rows of eight adapters at random: 104 us, 110 with 1024).
+    const int parts = (int)std::clamp<int64_t>((WIDE ? 4096 : 1024) / ((int64_t)tiles * across), 1, classes);
     const int around = places(tiles * across);
     const dim3 grid((unsigned)(around * parts)), block(256);
     if (WIDE) {
@@ -829,22 +837,21 @@ hipError_t up_ranks(hipStream_t stream, const LoraBatched& p, int tiles, int cla
 
 template <bool WB, bool OB>
 hipError_t up(hipStream_t stream, const LoraBatched& p, int tiles, int classes) {
-    if (p.joined) return p.R <= 32 ? up_ranks<WB, OB, 1, true>(stream, p, tiles, classes) : up_ranks<WB, OB, 2, true>(stream, p, tiles, classes);
-    return up_ranks<WB, OB, 1, false>(stream, p, tiles, classes);
+    return p.joined ? up_ranks<WB, OB, 2, true>(stream, p, tiles, classes) : up_ranks<WB, OB, 1, false>(stream, p, tiles, classes);
 }
 
 // h, the tiles' classes and how many they are.
-size_t h_bytes(int64_t rows, int64_t K, int64_t R) { return (size_t)splits_of(rows, K) * rows * rank_pitch(R) * sizeof(float); }
+size_t h_bytes(int64_t rows, int64_t K, int64_t R) { return (size_t)splits_of(rows, K, R) * rows * rank_pitch(R) * sizeof(float); }
 
 }  // namespace
 
 size_t lora_batched_workspace(int64_t rows, int64_t K, int64_t R) {
-    const size_t joined = is_wide(rows, K) ? (size_t)rows * (32 * ceil_div(R, 32)) * 6 : 0;  // three bf16, or fp32
+    const size_t joined = is_wide(rows, K, R) ? (size_t)rows * (32 * ceil_div(R, 32)) * 6 : 0;  // three bf16, or fp32
     return h_bytes(rows, K, R) + (size_t)ceil_div(rows, kLoraTile) * (kLoraTile * sizeof(LoraClass) + 16) + joined;
 }
 
 hipError_t launch_lora_batched(hipStream_t stream, LoraBatched p) {
-    p.splits = splits_of(p.rows, p.K);
+    p.splits = splits_of(p.rows, p.K, p.R);
     p.rank_pitch = rank_pitch(p.R);
     const int tiles = (p.rows + kLoraTile - 1) / kLoraTile;
     auto end = [](const void* from, int64_t elements, bool b16) { return (const char*)from + elements * (b16 ? 2 : 4); };
@@ -853,7 +860,7 @@ hipError_t launch_lora_batched(hipStream_t stream, LoraBatched p) {
     p.b_end = end(p.B, (p.adapters - 1) * p.b_adapter + (p.N - 1) * p.b_row + p.R, p.w_bf16);
     p.classes = (LoraClass*)((char*)p.h + h_bytes(p.rows, p.K, p.R));
     p.counts = (int*)(p.classes + (int64_t)tiles * kLoraTile);
-    p.joined = is_wide(p.rows, p.K) ? (void*)((char*)p.counts + (int64_t)tiles * 16) : nullptr;
+    p.joined = is_wide(p.rows, p.K, p.R) ? (void*)((char*)p.counts + (int64_t)tiles * 16) : nullptr;
     const int classes = std::min({kLoraTile - 1, p.adapters, p.rows}) + 1;  // of a tile, at most
     if (p.x_bf16) p.w_bf16 ? down<true, true>(stream, p, tiles, classes) : down<true, false>(stream, p, tiles, classes);
     else p.w_bf16 ? down<false, true>(stream, p, tiles, classes) : down<false, false>(stream, p, tiles, classes);

@@ -299,7 +299,7 @@ Plan shared_plan(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t dim,
         if (few || own > a.few_rows) s->seqs += (int)batch, units += std::min(batch * ceil_div(few ? std::min<int64_t>(own, a.few_rows) : own, s->rows), most + batch);
         int64_t shares = (few ? dim <= 128 ? kShares : kShares / 2 : kSharesChunks) / kv_heads;
         // Where the sequences fill the compute units, splits only even out their lengths: a
-        // unit costs 10 us beside its tokens.
+        // unit costs 10 us beside its tokens (64 sequences behind 8192: 47.9 us, 50.1 without).
         if (few && batch * kv_heads >= kShares) shares = (shares + 1) / 2;
         if (!few && dim <= 128) {
             // In one launch with the own tokens' part a prefix's splits take as many compute

@@ -52,14 +52,14 @@ __device__ __forceinline__ float byte_f32(uint32_t w, int n) { return (float)((i
 
 }  // namespace
 
-// DP: dim rounded up to 64, 128 or 256.  F32: fp32 q and out, else bf16.
-// PAGE16: tiles_of_16, so that a tile of 16 tokens has one block and its loads
-// one scalar base; otherwise every token finds its own.
 template <int DP> struct DecodeLds {
     float o[kWaves][kDecodeRows][DP];
     float m[kWaves][kDecodeRows], l[kWaves][kDecodeRows];
 };
 
+// DP: dim rounded up to 64, 128 or 256.  F32: fp32 q and out, else bf16.
+// PAGE16: tiles_of_16, so that a tile of 16 tokens has one block and its loads
+// one scalar base; otherwise every token finds its own.
 // Of block number `block`, in threads `tid` of 256.  PAIRED: two of them are one
 // block, which has the same barriers whatever they do.
 template <int DP, bool F32, bool PAGE16, bool SHARED, bool PAIRED>

@@ -68,6 +68,11 @@ SIZES = [  # rows, K, N, ranks, adapters, mixed
     (512, 544, 96, 256, 4, False),
     (600, 511, 200, 16, 5, False),
     (2100, 520, 60, 32, 1, False),
+    (1100, 520, 333, 40, 5, True),
+    (1030, 777, 200, 256, 3, False),
+    (1025, 512, 96, 200, 90, True),
+    (1500, 1030, 700, 33, 6, False),
+    (1024, 512, 64, 64, 1, False),
 ]
 
 
@@ -201,23 +206,23 @@ def test_on_a_stream_and_in_graphs(dev):
         assert all(same_bits(a, b) for a, b in zip(outs, want))
 
 
-@pytest.mark.parametrize("M,K", [(130, 48), (600, 512)])
-def test_adapters_of_one_place_in_the_table(dev, M, K):
+@pytest.mark.parametrize("M,K,rank", [(130, 48, 4), (600, 512, 4), (1100, 512, 40)])
+def test_adapters_of_one_place_in_the_table(dev, M, K, rank):
     """Numbers that agree in their low bits, in every tile, few rows and many."""
     n = 4200
-    x, A, B, _, scale, base = inputs(M, K, 40, 4, n, BF16, BF16, BF16)
+    x, A, B, _, scale, base = inputs(M, K, 40, rank, n, BF16, BF16, BF16)
     i = torch.arange(M)
     adapter = ((i * 7 % 5) * 1024 + i % 3 - 1).int()  # -1 to 4097
     got = Q.lora_batched(*(t.to(dev) for t in (x, A, B, adapter)), scale=scale.to(dev), base=base.to(dev))
     want, mag = R.adapted(x, A, B, adapter, scale, base)
-    fine, by = near(got, want, mag, base, K, 4)
+    fine, by = near(got, want, mag, base, K, rank)
     assert fine, by
 
 
 @pytest.mark.parametrize("off", [1, 8])
-@pytest.mark.parametrize("wd,od,rank", [(BF16, BF16, 24), (F32, F32, 40), (BF16, F32, 256), (F32, BF16, 200)])
+@pytest.mark.parametrize("wd,od,rank", [(BF16, BF16, 24), (BF16, BF16, 72), (F32, F32, 40), (BF16, F32, 256), (F32, BF16, 200)])
 def test_many_rows_in_place_and_strided(dev, off, wd, od, rank):
-    M, K, N, n = 700, 520, 333, 5
+    M, K, N, n = 1100, 520, 333, 5
     x, A, B, adapter, scale, base = (t.to(dev) for t in inputs(M, K, N, rank, n, BF16, wd, od))
     want = Q.lora_batched(x, A, B, adapter, scale=scale, base=base)
     exact, mag = R.adapted(*(t.cpu() for t in (x, A, B, adapter, scale, base)))
@@ -236,7 +241,7 @@ def test_many_rows_in_place_and_strided(dev, off, wd, od, rank):
 
 
 def test_many_rows_do_not_depend_on_their_neighbours(dev):
-    x, A, B, adapter, scale, base = (t.to(dev) for t in inputs(650, 576, 300, 16, 6, BF16, BF16, BF16))
+    x, A, B, adapter, scale, base = (t.to(dev) for t in inputs(1050, 576, 300, 48, 6, BF16, BF16, BF16))
     adapter.clamp_(0, 5)
     want = Q.lora_batched(x, A, B, adapter, scale=scale, base=base)
     for a in range(6):
@@ -252,7 +257,7 @@ def test_many_rows_do_not_depend_on_their_neighbours(dev):
 
 def test_many_rows_in_a_graph(dev):
     """Captured in place, replayed on other adapters and activations, eager work between."""
-    M, K, N, rank, n = 640, 512, 384, 64, 3
+    M, K, N, rank, n = 1040, 512, 384, 64, 3
     x, A, B, adapter, scale, base = (t.to(dev) for t in inputs(M, K, N, rank, n, BF16, BF16, BF16))
     ws, out = Q.lora_batched_workspace(M, K, rank, dev), base.clone()
     call = lambda o: Q.lora_batched(x, A, B, adapter, scale=scale, base=o, out=o, workspace=ws)  # noqa: E731
