@@ -765,11 +765,18 @@ int rank_pitch(int64_t R) { return (int)(16 * ceil_div(R, 16)); }
 
 constexpr size_t kMaxLds = 159 << 10;  // a compute unit's 160 KB, less the rows' numbers
 
+// Blocks that share a tile's classes are so many that there are about kParts: where rows are
+// mixed each has few classes, elsewhere most end at once (4352 rows of eight adapters at random, on
+// 16 ranks 60 us, on 64 104; with a fourth of the blocks 69 and 110; runs of rows 37 and 53, 41 and
+// 53; but 2048 rows in runs on 32 ranks 29, 27).  Not the wide ones of the first pass, of which
+// one fills a compute unit (at random on 64 ranks 112 us, 110 with 256).
+constexpr int64_t kParts = 4096;
+
 // Whether blocks take whole tiles' rows (whose loads are whole steps of K): what that saves
 // are readings of A, so it is for many ranks.  Microseconds for eight adapters of 4096 x 4096,
 // a run of rows each and at random: 4352 rows on 64 ranks 53 and 104, not wide 75 and 127;
 // 1024 rows 32 and 41, 39 and 36; 512 rows 24 and 29, 26 and 25; 4352 rows on 16 ranks 42 and
-// 87, 41 and 69.
+// 82, 37 and 60.
 bool is_wide(int64_t rows, int64_t K, int64_t R) { return rows >= 1024 && K >= 512 && R > 32; }
 
 // Parts of K: enough blocks where there are few rows, a part no shorter than 512; of wide
@@ -793,7 +800,7 @@ void down_ranks(hipStream_t stream, const LoraBatched& p, int tiles, int classes
     }
     // A tile's units are more than its classes by those of more than kFewCols rows.
     const int units = std::min(classes + kLoraTile / kFewCols - 1, kLoraTile);
-    const int parts = (int)std::clamp<int64_t>(1024 / ((int64_t)tiles * p.splits * groups), 1, units);
+    const int parts = (int)std::clamp<int64_t>(kParts / ((int64_t)tiles * p.splits * groups), 1, units);
     hipLaunchKernelGGL((lora_batched_down_kernel<XB, WB, RT>), dim3((unsigned)(around * parts), 1, (unsigned)groups), dim3(256), 0, stream, p, tiles,
                        around, parts);
 }
@@ -822,9 +829,7 @@ hipError_t up_ranks(hipStream_t stream, const LoraBatched& p, int tiles, int cla
     // begin when the first have ended, 42; of 5, 44).
     const int want = (int)std::max<int64_t>(1, (WIDE ? 410 : 1024) / tiles);
     const int chunks = (all + std::min(want, all) - 1) / std::min(want, all), across = (all + chunks - 1) / chunks;
-    // Of mixed rows a block has several classes, of others most blocks end at once: so more of
-    // wide ones (4352 rows of eight adapters at random: 104 us, 110 with 1024).
-    const int parts = (int)std::clamp<int64_t>((WIDE ? 4096 : 1024) / ((int64_t)tiles * across), 1, classes);
+    const int parts = (int)std::clamp<int64_t>(kParts / ((int64_t)tiles * across), 1, classes);
     const int around = places(tiles * across);
     const dim3 grid((unsigned)(around * parts)), block(256);
     if (WIDE) {
