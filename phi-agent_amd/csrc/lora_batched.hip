@@ -774,7 +774,7 @@ constexpr int64_t kParts = 4096;
 
 // Whether blocks take whole tiles' rows (whose loads are whole steps of K): what that saves
 // are readings of A, so it is for many ranks.  Microseconds for eight adapters of 4096 x 4096,
-// a run of rows each and at random: 4352 rows on 64 ranks 53 and 104, not wide 75 and 127;
+// a run of rows each and at random: 4352 rows on 64 ranks 53 and 104, not wide 70 and 100;
 // 1024 rows 32 and 41, 39 and 36; 512 rows 24 and 29, 26 and 25; 4352 rows on 16 ranks 42 and
 // 82, 37 and 60.
 bool is_wide(int64_t rows, int64_t K, int64_t R) { return rows >= 1024 && K >= 512 && R > 32; }
