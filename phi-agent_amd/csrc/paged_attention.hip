@@ -133,10 +133,9 @@ __global__ __launch_bounds__(256) void shared_join_kernel(PagedAttn p, AttnPart 
 #pragma unroll
     for (int k = 0; k < 2; k++) {
         const AttnRow a = (k ? p.own_rows : p.prefix_rows)[at];
-        const bool is_many = a.where >> 31;
         RowPart& x = part[k];
-        x.s = is_many ? many : few;
-        x.n = a.where & 0xffff, x.in = a.where >> 16 & 0x7fff, x.first = a.first, x.last = a.last;
+        x.s = a.many() ? many : few;
+        x.in = a.in(), x.first = a.first, x.last = a.last;
         // Left by this call only if the row is of that group or sequence.
         int from = a.id, to = a.id + 1;
         bool is = a.id >= 0 && a.id < (k ? batch : p.groups);
@@ -145,8 +144,8 @@ __global__ __launch_bounds__(256) void shared_join_kernel(PagedAttn p, AttnPart 
             const int first = p.q_start[from];
             is = token >= first && token < p.q_start[to] && (k == 0 || token - first < p.own_q);
         }
-        is = is && x.in < x.s.rows && x.n > 0 && (x.n == 1 || (x.first >= 0 && x.first + x.n - 1 <= x.s.slots)) && x.last >= 0 && x.last < x.s.slots;
-        x.n = is ? x.n : 0;
+        is = is && a.inside(x.s.slots, x.s.rows);
+        x.n = is ? a.splits() : 0;
         mine = k ? is : mine;
     }
     if (!mine) return;  // W = 4: the same in all waves

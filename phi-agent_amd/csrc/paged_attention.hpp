@@ -19,6 +19,7 @@
 
 #include <climits>
 
+#include "attn_row.hpp"
 #include "decoder.hpp"
 #include "device_common.hpp"
 
@@ -131,14 +132,6 @@ struct AttnUnit {
     bool last;
 };
 
-// Where a row's partial results are: for shared prefixes the last split of a tile
-// leaves this for each of its rows, [tokens][group], a prefix's apart from an own
-// one's.  `id` (of the group or sequence) tells a row that nothing was left for.
-struct AttnRow {
-    int first, last;  // slots: from first on, splits - 1 of them, and last
-    uint32_t where;   // splits | row of the tile << 16 | chunk kernel's << 31
-    int id;
-};
 __device__ __forceinline__ void leave_row(const PagedAttn& p, const AttnUnit& u, int r, int in, bool many) {
     const bool prefix = u.b < p.groups;
     const int i = r / p.group;
