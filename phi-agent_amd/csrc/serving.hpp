@@ -5,10 +5,10 @@
 
 namespace phi_dev {
 
-// [tokens, heads, dim] vectors, strides in elements.
 // A launch's threads are counted in 32 bits: blocks of 256, at most.
 constexpr int64_t kMaxBlocks = (1 << 24) - 1;
 
+// [tokens, heads, dim] vectors, strides in elements.
 struct RotaryHeads {
     const void* in;
     void* out;

@@ -11,7 +11,7 @@ namespace {
 constexpr int64_t kMaxRotaryDim = 1024;   // a wave has a vector
 constexpr int64_t kMaxRank = 256;         // of an adapter: h of 32 rows is held in LDS
 constexpr int64_t kMaxLoraRows = 1 << 24, kMaxLoraK = 1 << 24;  // units and columns counted in 31 bits
-constexpr int64_t kMaxHeadRows = 1 << 26;     // of shared prefixes, a wave each: threads of a launch are counted in 32 bits
+constexpr int64_t kMaxHeadRows = 4 * phi_dev::kMaxBlocks;  // of shared prefixes, four a block of their join
 constexpr int64_t kMaxPageVectors = 1 << 26;  // of at most 16 pieces: counted in 31 bits
 
 // [tokens, heads, dim] vectors that are written: one of the strides holds the other's
@@ -155,7 +155,7 @@ phi_status phi_hip_paged_attention_shared(phi_stream_t stream, const void* q, in
                     (long long)groups, (long long)batch, (long long)max_prefix, (long long)max_q, (long long)max_kv);
     if (tokens * (q_heads / c.heads) > kMaxRows)
         return fail(PHI_ERR_SHAPE, "%s: tokens=%lld at %lld query heads a key/value head is out of range", who, (long long)tokens, (long long)(q_heads / c.heads));
-    if (tokens * q_heads >= kMaxHeadRows) return fail(PHI_ERR_SHAPE, "%s: tokens=%lld of %lld heads is out of range", who, (long long)tokens, (long long)q_heads);
+    if (tokens * q_heads > kMaxHeadRows) return fail(PHI_ERR_SHAPE, "%s: tokens=%lld of %lld heads is out of range", who, (long long)tokens, (long long)q_heads);
     if (groups == 0) return fail(PHI_ERR_SHAPE, "%s: no groups", who);
     if (max_kv > 0 && (table_width > INT32_MAX || max_kv > table_width * c.page))
         return fail(PHI_ERR_SHAPE, "%s: max_kv=%lld exceeds the block table's %lld x %d tokens", who, (long long)max_kv, (long long)table_width, c.page);
@@ -194,7 +194,7 @@ size_t phi_hip_paged_attention_shared_workspace_bytes(int64_t tokens, int64_t q_
                                                       int64_t max_q, int64_t max_kv, int dtype) {
     if (tokens <= 0 || q_heads <= 0 || kv_heads <= 0 || dim <= 0 || groups <= 0 || batch <= 0 || max_q <= 0 || max_kv < 0 || max_prefix < 0) return 0;
     if (tokens > INT32_MAX || q_heads > 65535 || dim > 256 || groups > 65535 || batch > 65535 || max_q > tokens || max_kv > kMaxKv || max_prefix > kMaxKv) return 0;
-    if (q_heads % kv_heads != 0 || tokens * (q_heads / kv_heads) > kMaxRows || tokens * q_heads >= kMaxHeadRows) return 0;
+    if (q_heads % kv_heads != 0 || tokens * (q_heads / kv_heads) > kMaxRows || tokens * q_heads > kMaxHeadRows) return 0;
     return phi_dev::paged_attention_shared_workspace(tokens, (int)q_heads, (int)kv_heads, (int)dim, (int)groups, (int)batch, (int)max_prefix, (int)max_q,
                                                      (int)max_kv, dtype == PHI_BF16);
 }

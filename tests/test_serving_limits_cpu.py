@@ -1,7 +1,26 @@
 """CPU checks of the serving operators at the ends of what they take: records that hold
 anything, the largest launches, copies that fail."""
+import ctypes
 import os
 import subprocess
+
+import pytest
+
+import phi_qlinear as Q
+
+A, B, C, D, E, F, G = (ctypes.c_void_p(x << 40) for x in range(1, 8))  # well aligned and far apart, never dereferenced
+
+
+def attend(lib, *, tokens=8, heads=4, kv_heads=1, groups=1, batch=1, dim=16, dtype=Q.BF16, max_prefix=64, max_q=1, max_kv=64, ws=1 << 40):
+    """paged_attention_shared over a cache and tables that no call reads here."""
+    cache = Q.KvCacheDesc(k=8 << 40, v=9 << 40, k_scale=10 << 40, v_scale=11 << 40, blocks=10, heads=kv_heads, page=16, dim=dim,
+                          block_stride=16 * dim * kv_heads, head_stride=16 * dim, token_stride=dim, s_block_stride=16 * kv_heads,
+                          s_head_stride=16, s_token_stride=1)
+    w = 1 << 20
+    rc = lib.phi_hip_paged_attention_shared(None, A, dtype, heads * dim, dim, tokens, heads, ctypes.byref(cache), B, w, w, C, C, groups, max_prefix,
+                                            B, w, w, D, D, batch, max_q, max_kv, 0.25, E, heads * dim, dim, F, ws)
+    return rc, Q.last_error()
+
 
 
 def test_records_of_rows_stay_in_their_slots():
@@ -10,3 +29,13 @@ def test_records_of_rows_stay_in_their_slots():
     subprocess.run(["make", "-C", cdir, "attn_row"], check=True, capture_output=True)
     out = subprocess.run([os.path.join(cdir, "attn_row")], capture_output=True, text=True, timeout=60)
     assert out.returncode == 0 and "wrong 0" in out.stdout, out.stdout
+
+
+@pytest.mark.parametrize("tokens,heads", [((1 << 26) - 1, 1), ((1 << 26) - 3, 1), (((1 << 26) - 2) // 2, 2)])
+def test_more_rows_than_the_join_has_waves_are_refused(lib, tokens, heads):
+    """Four rows a block of 256 threads, and a launch's threads are counted in 32 bits."""
+    rc, text = attend(lib, tokens=tokens, heads=heads)
+    assert rc == 2 and "out of range" in text
+    size = lib.phi_hip_paged_attention_shared_workspace_bytes
+    assert size(tokens, heads, 1, 16, 1, 1, 64, 1, 64, Q.BF16) == 0
+    assert size((1 << 26) // heads - 4, heads, 1, 16, 1, 1, 64, 1, 64, Q.BF16) > 0
