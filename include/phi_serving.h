@@ -94,7 +94,9 @@ phi_status phi_hip_kv_cache_copy(phi_stream_t stream, const phi_kv_cache* from, 
  *   prefix_table [groups, prefix_stride] int32, `prefix_width` entries a row, as block_table
  *   prefix_len   [groups] int32; max_prefix at least the longest, at most
  *                prefix_width * page and 2^30: tokens past it are not seen
- *   tokens       at most 2^30 times key/value heads over query heads; times q_heads at most 2^26 - 4
+ *   tokens       at most 2^30 times key/value heads over query heads; times q_heads at most 2^26 - 4.
+ *                groups + batch times key/value heads past some 2^22 is more than a launch
+ *                has blocks for: refused
  *   workspace    phi_hip_paged_attention_shared_workspace_bytes() bytes, 16-byte aligned
  * All else as phi_hip_paged_attention, its arithmetic too, a group's rows over their
  * prefix being one sequence of it; the parts are joined in fp32.  Lengths, starts and

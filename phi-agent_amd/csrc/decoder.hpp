@@ -85,6 +85,7 @@ size_t paged_attention_workspace(int64_t tokens, int q_heads, int kv_heads, int 
                                  bool bf16);
 // p as a caller has it: batch, max_q of the sequences.
 hipError_t launch_paged_attention_shared(hipStream_t stream, const KvCache& c, const PagedAttn& p, void* workspace);
+// 0: no launch has that many blocks.
 size_t paged_attention_shared_workspace(int64_t tokens, int q_heads, int kv_heads, int dim, int groups, int batch, int max_prefix,
                                         int max_q, int max_kv, bool bf16);
 

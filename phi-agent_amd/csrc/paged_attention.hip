@@ -316,6 +316,13 @@ Plan shared_plan(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t dim,
     return a;
 }
 
+// Whether a launch can have the plan's blocks: its threads are counted in 32 bits.
+bool shared_fits(const Plan& a, int64_t kv_heads, int64_t dim) {
+    const int64_t most = (int64_t)1 << 32, many = a.many.blocks * kv_heads, few = a.few.blocks * kv_heads;
+    if (many && dim <= 128) return (many + (few + 1) / 2) * 512 < most;  // in one
+    return many * 256 < most && few * 256 < most;
+}
+
 }  // namespace
 
 size_t paged_attention_workspace(int64_t tokens, int q_heads, int kv_heads, int dim, int batch, int max_q, int max_kv, bool bf16) {
@@ -352,6 +359,7 @@ hipError_t launch_paged_attention(hipStream_t stream, const KvCache& c, const Pa
 size_t paged_attention_shared_workspace(int64_t tokens, int q_heads, int kv_heads, int dim, int groups, int batch, int max_prefix, int max_q,
                                         int max_kv, bool bf16) {
     const Plan a = shared_plan(tokens, q_heads, kv_heads, dim, groups, batch, max_prefix, max_q, max_kv, bf16);
+    if (!shared_fits(a, kv_heads, dim)) return 0;
     return (size_t)((part_rows(a.many, kv_heads) + part_rows(a.few, kv_heads)) * (dim + 2)) * sizeof(float) +
            (size_t)tokens * (q_heads / kv_heads) * 2 * sizeof(AttnRow);
 }

@@ -26,7 +26,6 @@ __global__ __launch_bounds__(512, 2) void paged_shared_kernel(KvCache c, PagedAt
 template <int DP>
 static hipError_t launch_dp(hipStream_t stream, const KvCache& c, const PagedAttn& p, const AttnPart& many, const AttnPart& few) {
     const int64_t blocks = (int64_t)many.blocks * c.heads + ((int64_t)few.blocks * c.heads + 1) / 2;
-    if (blocks > INT32_MAX) return hipErrorInvalidConfiguration;
     const bool page16 = tiles_of_16(c);
     const size_t lds = sizeof(ChunkLds<DP>) > 2 * sizeof(DecodeLds<DP>) ? sizeof(ChunkLds<DP>) : 2 * sizeof(DecodeLds<DP>);
     const void* f = page16 ? (const void*)paged_shared_kernel<DP, true> : (const void*)paged_shared_kernel<DP, false>;

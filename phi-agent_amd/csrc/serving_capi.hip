@@ -176,6 +176,7 @@ phi_status phi_hip_paged_attention_shared(phi_stream_t stream, const void* q, in
     const Pieces os = vectors_of(out, tokens, out_token_stride, q_heads, out_head_stride, c.dim, elem(dtype));
     if (meet(qs, os)) return fail(PHI_ERR_ARG, "%s: out overlaps q", who);
     const size_t need = phi_hip_paged_attention_shared_workspace_bytes(tokens, q_heads, c.heads, c.dim, groups, batch, max_prefix, max_q, max_kv, dtype);
+    if (need == 0) return fail(PHI_ERR_SHAPE, "%s: groups=%lld and batch=%lld are too many for a launch at %d key/value heads", who, (long long)groups, (long long)batch, c.heads);
     if (!workspace || ws_bytes < need)
         return fail(PHI_ERR_WORKSPACE, "%s: needs %zu bytes of workspace, got %zu", who, need, workspace ? ws_bytes : (size_t)0);
     if (!aligned(workspace, 16)) return fail(PHI_ERR_ALIGN, "%s: the workspace must be 16-byte aligned", who);

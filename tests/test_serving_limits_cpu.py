@@ -39,3 +39,13 @@ def test_more_rows_than_the_join_has_waves_are_refused(lib, tokens, heads):
     size = lib.phi_hip_paged_attention_shared_workspace_bytes
     assert size(tokens, heads, 1, 16, 1, 1, 64, 1, 64, Q.BF16) == 0
     assert size((1 << 26) // heads - 4, heads, 1, 16, 1, 1, 64, 1, 64, Q.BF16) > 0
+
+
+@pytest.mark.parametrize("dtype,dim,kv_heads", [(Q.BF16, 64, 256), (Q.BF16, 256, 512), (Q.F32, 64, 512)])
+def test_more_sequences_than_a_launch_has_blocks_for_are_refused(lib, dtype, dim, kv_heads):
+    sizes = dict(tokens=65535, heads=kv_heads, kv_heads=kv_heads, groups=65535, batch=65535, dim=dim, dtype=dtype)
+    rc, text = attend(lib, **sizes)
+    assert rc == 2 and "groups" in text and "too many" in text
+    size = lib.phi_hip_paged_attention_shared_workspace_bytes
+    assert size(65535, kv_heads, kv_heads, dim, 65535, 65535, 64, 1, 64, dtype) == 0
+    assert size(65535, 16, 16, dim, 65535, 65535, 64, 1, 64, dtype) > 0
