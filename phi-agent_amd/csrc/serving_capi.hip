@@ -220,7 +220,7 @@ phi_status phi_hip_lora_batched(phi_stream_t stream, const void* x, int x_dtype,
     if (ldx > kMaxPitch || ldo > kMaxPitch || (base && ld_base > kMaxPitch) || a_row_stride > kMaxPitch || b_row_stride > kMaxPitch)
         return fail(PHI_ERR_SHAPE, "%s: leading dimension too large", who);
     for (int64_t s : {a_adapter_stride, b_adapter_stride})
-        if (s < 0 || s > kMaxStride / 2) return fail(PHI_ERR_SHAPE, "%s: bad adapter stride %lld", who, (long long)s);
+        if (s < 0 || s > kMaxStride / 2 || (adapters > 1 && s > kMaxSpan / (adapters - 1))) return fail(PHI_ERR_SHAPE, "%s: bad adapter stride %lld", who, (long long)s);
     const int64_t xe = elem(x_dtype), we = elem(w_dtype), oe = elem(out_dtype);
     if (!aligned(x, xe) || !aligned(A, we) || !aligned(B, we) || !aligned(adapter, 4) || !aligned(scale, 4) || !aligned(out, oe) || !aligned(base, oe))
         return fail(PHI_ERR_ALIGN, "%s: a pointer is not aligned to its type", who);

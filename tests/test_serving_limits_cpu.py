@@ -49,3 +49,11 @@ def test_more_sequences_than_a_launch_has_blocks_for_are_refused(lib, dtype, dim
     size = lib.phi_hip_paged_attention_shared_workspace_bytes
     assert size(65535, kv_heads, kv_heads, dim, 65535, 65535, 64, 1, 64, dtype) == 0
     assert size(65535, 16, 16, dim, 65535, 65535, 64, 1, 64, dtype) > 0
+
+
+@pytest.mark.parametrize("a,b", [((1 << 39), 64), (64, (1 << 39)), (1 << 36, 1 << 36)])
+def test_factors_that_span_more_than_any_memory_are_refused(lib, a, b):
+    """The end of the last adapter's, in bytes, is counted in 63 bits."""
+    rc = lib.phi_hip_lora_batched(None, A, Q.BF16, 16, 4, 16, B, a, 16, C, b, 4, Q.BF16, (1 << 31) - 1, 4, 16, D, None, None, 0, E, Q.BF16,
+                                  16, F, 1 << 30)
+    assert rc == 2 and "adapter stride" in Q.last_error()
