@@ -223,20 +223,20 @@ class KvPages:
 
     def flush(self, cache: KvCache, stream=None) -> None:
         """Have the device do the copies, in as few calls as leave no block in one that
-        is written there and read, or written twice."""
+        is written there and read, or written twice.  Those of a call that raises, and
+        all after it, are kept."""
         if stream is not None:
             with torch.cuda.stream(stream):
                 return self.flush(cache)
-        left, self.copies = self.copies, []
-        while left:
+        while self.copies:
             read, written, now, later = set(), set(), [], []
-            for c in left:
+            for c in self.copies:
                 meets = c[0] in written or c[1] in written or c[1] in read
                 (later if later or meets else now).append(c)
                 read.add(c[0]), written.add(c[1])
             part = torch.tensor(now, dtype=torch.int32).t().contiguous().to(cache.k.device)
             kv_cache_copy(cache, cache, part[0], part[1], tokens=part[2])
-            left = later
+            self.copies = later
 
 
 def paged_attention_shared_workspace(tokens: int, q_heads: int, kv_heads: int, dim: int, groups: int, batch: int, max_prefix: int,

@@ -5,6 +5,7 @@ import os
 import subprocess
 
 import pytest
+import torch
 
 import phi_qlinear as Q
 
@@ -57,3 +58,28 @@ def test_factors_that_span_more_than_any_memory_are_refused(lib, a, b):
     rc = lib.phi_hip_lora_batched(None, A, Q.BF16, 16, 4, 16, B, a, 16, C, b, 4, Q.BF16, (1 << 31) - 1, 4, 16, D, None, None, 0, E, Q.BF16,
                                   16, F, 1 << 30)
     assert rc == 2 and "adapter stride" in Q.last_error()
+
+
+def test_copies_that_fail_are_kept(monkeypatch):
+    """What a flush could not do is left for the next one, what it did is not."""
+    calls, fails = [], [False, True]
+
+    def copy(a, b, frm, to, tokens):
+        if fails and fails.pop(0):
+            raise ValueError("tensors of another device")
+        calls.append(list(zip(frm.tolist(), to.tolist(), tokens.tolist())))
+
+    monkeypatch.setattr(Q.serving, "kv_cache_copy", copy)
+
+    class Host:
+        k = torch.zeros(1)
+
+    pages = Q.KvPages(8, 4)
+    pages.copies = [(0, 1, 4), (2, 3, 2), (3, 4, 2), (1, 5, 4), (5, 6, 1)]  # in three calls
+    with pytest.raises(ValueError):
+        pages.flush(Host)
+    assert calls == [[(0, 1, 4), (2, 3, 2)]] and pages.copies == [(3, 4, 2), (1, 5, 4), (5, 6, 1)]
+    pages.flush(Host)
+    assert calls[1:] == [[(3, 4, 2), (1, 5, 4)], [(5, 6, 1)]] and pages.copies == []
+    pages.flush(Host)
+    assert len(calls) == 3
