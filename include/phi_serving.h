@@ -38,9 +38,9 @@ extern "C" {
  *   freq       [rot / 2] fp64, finite, radians a position: contexts stretched by
  *              any rule are other frequencies (and a scale)
  *   dim        from 1 to 1024; rot even, from 2 to dim
- * The angle is kept as a 64-bit fraction of a turn, position * freq modulo 1 to
- * 2^-53 of the angle (as fp64 has it) and 2^-64 a position; its cosine and sine are
- * fp32 to 2^-22, products and sums fp32, rounded once.
+ * The angle is kept as a 64-bit fraction of a turn: freq / 2 pi modulo 1 to 2^-64 (freq
+ * to 2^40), its product with the position exactly; its cosine and sine are fp32 to 2^-22,
+ * products and sums fp32, rounded once.
  */
 phi_status phi_hip_rotary(phi_stream_t stream, const void* x, int dtype, int64_t x_token_stride, int64_t x_head_stride,
                           int64_t tokens, int64_t heads, int64_t dim, const int64_t* positions, const double* freq,

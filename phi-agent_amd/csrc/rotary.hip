@@ -9,7 +9,7 @@
 // the cache 27 us, 4 TB/s; 64 tokens 5 us, of which most is the launch and two loads in turn.
 //
 // The angle position * freq is wanted modulo a turn, to fp32 at any position.  With
-// step = freq / 2 pi as a 64-bit fraction of a turn, position * step in 64-bit
+// step = freq / 2 pi as a 64-bit fraction of a turn, to its nearest, position * step in 64-bit
 // integers drops whole turns by itself and is exact for the step as it is; its top 32
 // bits, taken about the nearest quarter turn, are an angle within pi/4, for which
 // Taylor's series to x^9 and x^10 are within 2^-29.
@@ -20,12 +20,19 @@ namespace phi_dev {
 
 namespace {
 
+// freq / 2 pi modulo 1 as a 64-bit fraction, to the nearest: the product in two doubles, of
+// which the first's whole turns are dropped and then 32 bits taken, all exactly.  (A product of
+// one double has its last bit at 2^-53 of the step, and what is cut off goes one way.)
+__device__ __forceinline__ uint64_t step_of(double freq) {
+    constexpr double k1 = 0x1.45f306dc9c883p-3, k0 = -0x1.6b01ec5417056p-57;  // 1 / 2 pi
+    const double hi = freq * k1, lo = fma(freq, k0, fma(freq, k1, -hi)), part = hi - rint(hi);
+    const double top = rint((part + lo) * 0x1p32), rest = fma(part, 0x1p32, -top) + lo * 0x1p32;
+    return ((uint64_t)(int64_t)top << 32) + (uint64_t)(int64_t)rint(rest * 0x1p32);
+}
+
 // Cosine and sine of position * freq.
 __device__ __forceinline__ float2 turn_of(int64_t position, double freq) {
-    const double turns = freq * 0.15915494309189533577;
-    // To 2^-63 of a turn, within half a turn either way.
-    const uint64_t step = (uint64_t)(int64_t)((turns - rint(turns)) * 0x1p63) << 1;
-    const uint32_t at = (uint32_t)((step * (uint64_t)position) >> 32) + 0x20000000u;
+    const uint32_t at = (uint32_t)((step_of(freq) * (uint64_t)position) >> 32) + 0x20000000u;
     const float x = (float)((int32_t)(at & 0x3fffffffu) - 0x20000000) * 1.4629180792671596e-9f;  // 2 pi / 2^32
     const float y = x * x;
     float s = fmaf(y, fmaf(y, fmaf(y, fmaf(y, 1.0f / 362880, -1.0f / 5040), 1.0f / 120), -1.0f / 6), 1.0f);
