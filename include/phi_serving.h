@@ -39,8 +39,8 @@ extern "C" {
  *              any rule are other frequencies (and a scale)
  *   dim        from 1 to 1024; rot even, from 2 to dim
  * The angle is kept as a 64-bit fraction of a turn: freq / 2 pi modulo 1 to 2^-64 (freq
- * to 2^40), its product with the position exactly; its cosine and sine are fp32 to 2^-22,
- * products and sums fp32, rounded once.
+ * to 2^40), its product with the position exactly; scale times its cosine and sine are
+ * the nearest fp32 (2^-24 of them and 2^-30), products and sums fp32, rounded once.
  */
 phi_status phi_hip_rotary(phi_stream_t stream, const void* x, int dtype, int64_t x_token_stride, int64_t x_head_stride,
                           int64_t tokens, int64_t heads, int64_t dim, const int64_t* positions, const double* freq,

@@ -64,3 +64,18 @@ def test_steps_are_held_to_the_nearest(dev, freq, lg):
     for got, want in zip(turned(dev, pos, freq), exact(pos, freq)):
         err = (got - want).abs() - 2.0 ** -22
         assert bool((err <= away).all()), float((err / away).max())
+
+
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("freq", FREQS)
+@pytest.mark.parametrize("lg,scale", [(4, 1.0), (20, 1.0), (24, 0.75)])
+def test_cosines_and_sines_are_the_nearest(dev, freq, lg, scale, inter):
+    """Scaled in 64 bits and rounded once."""
+    g = torch.Generator().manual_seed(lg)
+    pos = torch.randint(-(1 << lg), 1 << lg, (60,), generator=g)
+    pos[0] = 0
+    away = pos.double().abs()[:, None] * 2 * math.pi * 2.0 ** -64
+    for got, want in zip(turned(dev, pos, freq, inter, scale), exact(pos, freq)):
+        bound = 2.0 ** -24 * (scale * want).abs() + 2.0 ** -30 * abs(scale) + away
+        err = (got - scale * want).abs()
+        assert bool((err <= bound).all()), float((err / bound).max())
