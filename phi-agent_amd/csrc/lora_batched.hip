@@ -221,6 +221,16 @@ __device__ __forceinline__ float value(const Eight<B16>& e, int i) {
     return __uint_as_float(B16 ? i & 1 ? e.w[i >> 1] & 0xffff0000u : e.w[i >> 1] << 16 : e.w[i]);
 }
 
+// Eight bf16 with zeros for those that are not finite.
+__device__ __forceinline__ Eight<true> finite_of(Eight<true> e) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t f = ((e.w[i] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+        e.w[i] &= ~(f | (f - (f >> 15)));
+    }
+    return e;
+}
+
 template <bool AB, bool BB>
 __device__ __forceinline__ v4f product(const Eight<AB>& a, const Eight<BB>& b, v4f c) {
     if constexpr (AB && BB) {
@@ -657,17 +667,21 @@ __global__ __launch_bounds__(256, 2) void lora_batched_up_kernel(LoraBatched p, 
                     v4f acc[NT];
 #pragma unroll
                     for (int t = 0; t < NT; t++) acc[t] = v4f{0, 0, 0, 0};
+                    // (Rows behind the last are the last again.)
+                    auto load_h = [&](int c, int k0, int term) __attribute__((always_inline)) {
+                        Eight<WB> h;
+                        if constexpr (WB) {
+                            *(uint4*)h.w = *(const uint4*)(hb + (min(16 * c + col, n - 1) * T + term) * pitch + k0 + 8 * g);
+                        } else {
+                            *(v4f*)h.w = *(const v4f*)(hf + min(16 * c + col, n - 1) * pitch + k0 + 8 * g);
+                            *(v4f*)(h.w + 4) = *(const v4f*)(hf + min(16 * c + col, n - 1) * pitch + k0 + 8 * g + 4);
+                        }
+                        return h;
+                    };
                     auto multiply = [&](int k0, const Eight<WB> (&b)[NT]) __attribute__((always_inline)) {
 #pragma unroll
                         for (int term = T - 1; term >= 0; term--) {
-                            Eight<WB> h;
-                            // Rows behind the last hold whatever lies there; theirs are not stored.
-                            if constexpr (WB) {
-                                *(uint4*)h.w = *(const uint4*)(hb + (min(16 * c + col, n - 1) * T + term) * pitch + k0 + 8 * g);
-                            } else {
-                                *(v4f*)h.w = *(const v4f*)(hf + min(16 * c + col, n - 1) * pitch + k0 + 8 * g);
-                                *(v4f*)(h.w + 4) = *(const v4f*)(hf + min(16 * c + col, n - 1) * pitch + k0 + 8 * g + 4);
-                            }
+                            const Eight<WB> h = load_h(c, k0, term);
 #pragma unroll
                             for (int t = 0; t < NT; t++) acc[t] = product(h, b[t], acc[t]);
                         }
@@ -680,6 +694,31 @@ __global__ __launch_bounds__(256, 2) void lora_batched_up_kernel(LoraBatched p, 
                             Eight<WB> rest[NT];
                             load_b(n0, k0, rest);
                             multiply(k0, rest);
+                        }
+                        if constexpr (WB) {
+                            // h's lower terms may be 0 or of another sign, which an infinite factor
+                            // makes NaN of: where something is not finite, once more, such factors
+                            // with the first term only.
+                            float bad = 0.0f;
+#pragma unroll
+                            for (int t = 0; t < NT; t++)
+#pragma unroll
+                                for (int i = 0; i < 4; i++) bad = fmaf(acc[t][i], 0.0f, bad);
+                            if (__builtin_expect(__any(bad != 0.0f), 0)) {
+#pragma unroll
+                                for (int t = 0; t < NT; t++) acc[t] = v4f{0, 0, 0, 0};
+#pragma unroll 1
+                                for (int k0 = 0; k0 < ranks; k0 += 32) {
+                                    Eight<WB> all[NT];
+                                    load_b(n0, k0, all);
+#pragma unroll 1
+                                    for (int term = T - 1; term >= 0; term--) {
+                                        const Eight<WB> h = load_h(c, k0, term);
+#pragma unroll
+                                        for (int t = 0; t < NT; t++) acc[t] = product(h, term ? finite_of(all[t]) : all[t], acc[t]);
+                                    }
+                                }
+                            }
                         }
                     }
                     if (inside) {

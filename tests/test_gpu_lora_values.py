@@ -1,0 +1,59 @@
+"""GPU: what the adapters' second product makes of h's bits and of values that are not finite.
+
+A has one element a rank, so that h is x's elements themselves (times 1), exactly; B has few
+elements that are not 0, so that the result is known to its last bits."""
+import math
+
+import pytest
+import torch
+
+import phi_qlinear as Q
+
+pytestmark = pytest.mark.gpu
+
+BF16, F32 = torch.bfloat16, torch.float32
+# rows, K, ranks: few rows and many, ranks within the registers' steps and past them.
+SIZES = [(5, 64, 8), (40, 300, 40), (200, 512, 100), (1100, 512, 40), (1030, 520, 72), (1024, 1030, 256)]
+
+
+def bits(t):
+    return t.cpu().contiguous().view({2: torch.int16, 4: torch.int32}[t.element_size()])
+
+
+def same_bits(a, b):
+    return a.dtype == b.dtype and torch.equal(bits(a), bits(b))
+
+
+def passing(M, K, R, n, dtype):
+    """x of zeros and A [n, R, K] of which rank r passes x's element r on."""
+    A = torch.zeros((n, R, K), dtype=dtype)
+    A[:, torch.arange(R), torch.arange(R)] = 1.0
+    return torch.zeros((M, K)), A
+
+
+@pytest.mark.parametrize("wd,od", [(BF16, BF16), (BF16, F32), (F32, F32), (F32, BF16)])
+@pytest.mark.parametrize("M,K,R", SIZES)
+def test_infinite_factors(dev, M, K, R, wd, od):
+    """h times an infinity is one of h's sign whatever bits h has, NaN where h is 0; the columns
+    and adapters beside it keep their bits."""
+    n, N = 3, 200
+    g = torch.Generator().manual_seed(M)
+    x, A = passing(M, K, R, n, wd)
+    x[:, :R] = torch.randn((M, R), generator=g)  # of 24 bits, or 8, or none
+    x[1::3, :R] = x[1::3, :R].bfloat16().float()
+    x[2::7, R - 1] = 0.0
+    B = torch.randn((n, N, R), generator=g).to(wd)
+    adapter = (torch.arange(M) % (n + 1) - 1).int()
+    to = lambda t: t.to(dev)  # noqa: E731
+    plain = Q.lora_batched(to(x), to(A), to(B), to(adapter), out_dtype=od).cpu()
+    B[1, 7, R - 1], B[1, 70, R - 1], B[1, 130, R // 2], B[1, 199, 0], B[1, 131, R - 1] = math.inf, -math.inf, math.inf, -math.inf, math.nan
+    got = Q.lora_batched(to(x), to(A), to(B), to(adapter), out_dtype=od).cpu()
+    mine, cols = adapter == 1, [7, 70, 130, 131, 199]
+    want = plain.clone()
+    for c, r, s in ((7, R - 1, math.inf), (70, R - 1, -math.inf), (130, R // 2, math.inf), (199, 0, -math.inf), (131, R - 1, math.nan)):
+        want[mine, c] = (x[mine, r] * s).to(od)
+    assert torch.equal(got.isnan(), want.isnan())
+    assert torch.equal(got[:, cols].nan_to_num(0.0, 9.0, -9.0), want[:, cols].nan_to_num(0.0, 9.0, -9.0))
+    rest = torch.ones(N, dtype=torch.bool)
+    rest[cols] = False
+    assert same_bits(got[:, rest], plain[:, rest]) and same_bits(got[~mine], plain[~mine])
