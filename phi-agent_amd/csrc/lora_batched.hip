@@ -534,7 +534,12 @@ __device__ __forceinline__ void store_h(v4f sum, void* to, int term) {
     if constexpr (WB) {
 #pragma unroll
         for (int t = 0; t < 3; t++) {
-            const uint32_t lo = f32x2_to_bf16x2(sum[0], sum[1]), hi = f32x2_to_bf16x2(sum[2], sum[3]);
+            // What bf16 would round to infinity has its largest value first.
+            constexpr float kTop = 0x1.fep127f;
+            float x[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[e] = t == 0 && __builtin_isfinite(sum[e]) ? fminf(fmaxf(sum[e], -kTop), kTop) : sum[e];
+            const uint32_t lo = f32x2_to_bf16x2(x[0], x[1]), hi = f32x2_to_bf16x2(x[2], x[3]);
             *(uint2*)((uint16_t*)to + t * term) = make_uint2(lo, hi);
             // What an infinity leaves is 0, not NaN.
             const float y[4] = {bf16_to_f32(lo & 0xffffu), bf16_to_f32(lo >> 16), bf16_to_f32(hi & 0xffffu), bf16_to_f32(hi >> 16)};

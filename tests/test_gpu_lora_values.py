@@ -57,3 +57,19 @@ def test_infinite_factors(dev, M, K, R, wd, od):
     rest = torch.ones(N, dtype=torch.bool)
     rest[cols] = False
     assert same_bits(got[:, rest], plain[:, rest]) and same_bits(got[~mine], plain[~mine])
+
+
+@pytest.mark.parametrize("wd", [BF16, F32])
+@pytest.mark.parametrize("M,K,R", SIZES)
+def test_h_past_the_largest_bf16(dev, M, K, R, wd):
+    """fp32 values that bf16 would round to infinity: one product of 24 by 8 bits, exact before
+    the sum of its three parts, each rounded to 24 bits."""
+    x, A = passing(M, K, R, 1, wd)
+    top = torch.finfo(F32).max
+    x[:, 0] = top * (1 - torch.arange(M) * 2.0 ** -24 / M)
+    x[1::2, 0] *= -1
+    B = torch.zeros((1, 96, R), dtype=wd)
+    B[0, :, 0] = torch.arange(1, 97) / 128
+    got = Q.lora_batched(x.to(dev), A.to(dev), B.to(dev), torch.zeros(M, dtype=torch.int32, device=dev), out_dtype=F32).cpu().double()
+    want = x[:, :1].double() * B[0, :, 0].double()
+    assert bool(((got - want).abs() <= 3 * 2.0 ** -23 * want.abs()).all())
