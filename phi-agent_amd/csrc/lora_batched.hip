@@ -669,9 +669,11 @@ __global__ __launch_bounds__(256, 2) void lora_batched_up_kernel(LoraBatched p, 
                 if (n0 >= p.N) break;
                 const bool inside = n0 + kWave <= p.N;
                 auto turn = [&](int c, Run (&base)[4], bool inside) __attribute__((always_inline)) {
+                    // Without an adapter -0, which leaves the base's own zeros their signs.
+                    const float none = some || !p.base ? 0.0f : -0.0f;
                     v4f acc[NT];
 #pragma unroll
-                    for (int t = 0; t < NT; t++) acc[t] = v4f{0, 0, 0, 0};
+                    for (int t = 0; t < NT; t++) acc[t] = v4f{none, none, none, none};
                     // (Rows behind the last are the last again.)
                     auto load_h = [&](int c, int k0, int term) __attribute__((always_inline)) {
                         Eight<WB> h;

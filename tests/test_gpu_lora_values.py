@@ -73,3 +73,26 @@ def test_h_past_the_largest_bf16(dev, M, K, R, wd):
     got = Q.lora_batched(x.to(dev), A.to(dev), B.to(dev), torch.zeros(M, dtype=torch.int32, device=dev), out_dtype=F32).cpu().double()
     want = x[:, :1].double() * B[0, :, 0].double()
     assert bool(((got - want).abs() <= 3 * 2.0 ** -23 * want.abs()).all())
+
+
+@pytest.mark.parametrize("od", [BF16, F32])
+@pytest.mark.parametrize("wd", [BF16, F32])
+@pytest.mark.parametrize("M,K,R", SIZES)
+def test_rows_without_an_adapter_are_copied(dev, M, K, R, wd, od):
+    """Zeros of either sign and infinities among them, inside whole columns and at the ragged end,
+    into another tensor and in place."""
+    n, N = 2, 333
+    g = torch.Generator().manual_seed(M)
+    x, A = passing(M, K, R, n, wd)
+    base = torch.randn((M, N), generator=g).to(od)
+    base[:, ::3], base[:, 1::5], base[:, 2::7] = -0.0, 0.0, -math.inf
+    adapter = (torch.arange(M) % 4 - 1).int()  # -1 to 2
+    none = (adapter < 0) | (adapter >= n)
+    B = torch.randn((n, N, R), generator=g).to(wd)
+    out = base.to(dev)
+    to = [t.to(dev) for t in (x, A, B, adapter)]
+    got = Q.lora_batched(*to, base=out)
+    assert same_bits(got[none.to(dev)], base[none])
+    assert same_bits(Q.lora_batched(*to, base=out, out=out)[none.to(dev)], base[none])
+    zero = Q.lora_batched(*to, out_dtype=od)[none.to(dev)]
+    assert same_bits(zero, torch.zeros_like(zero))
