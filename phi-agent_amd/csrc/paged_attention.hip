@@ -306,9 +306,14 @@ Plan shared_plan(int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t dim,
             // unit, of a block's tile of 64 tokens 2.3 beside 9, of 256 own tokens 2 beside 5.
             // (64 sequences behind 8192 tokens: 49 us with 12 splits a head, 53 with 10, 58 with
             // 24; 96 behind three documents to 32760: 230 with 24, 268 with 18, 241 with 28.)
-            const double prefix = 2.3 * most * ceil_div(max_prefix, 64), rest = batch * (5 + max_kv * 0.008), all_units = std::max<double>(1, 256.0 / kv_heads);
-            const double each = std::max((prefix + rest) / all_units - 9, 7.0);
-            shares = (int64_t)std::min(prefix / each, all_units) + 1;
+            // Sequences of chunks, as many as `tokens` holds, have their own tokens here too (64 of
+            // 64 query heads over 4096, behind 64: 56 us, 154 unsplit; 1024 of 32 over 8192 behind
+            // nothing: 198, 316; paged_attention 44 and 182).
+            const int64_t chunks = own > a.few_rows ? std::min(batch, tokens / max_q) : 0;
+            const double tiles = most * ceil_div(max_prefix, 64) + chunks * ceil_div(own, s->rows) * ceil_div(max_kv, 64);
+            const double here = 2.3 * tiles, rest = (batch - chunks) * (5 + max_kv * 0.008), all_units = std::max<double>(1, 256.0 / kv_heads);
+            const double each = std::max((here + rest) / all_units - 9, 7.0);
+            shares = (int64_t)std::min(here / each, all_units) + 1;
         }
         split(*s, units, shares, std::max<int64_t>(longest, 1));
         s->blocks = (int)std::min<int64_t>(s->slots, INT32_MAX / kv_heads);

@@ -83,3 +83,14 @@ def test_copies_that_fail_are_kept(monkeypatch):
     assert calls[1:] == [[(3, 4, 2), (1, 5, 4)], [(5, 6, 1)]] and pages.copies == []
     pages.flush(Host)
     assert len(calls) == 3
+
+
+@pytest.mark.parametrize("tokens,heads,batch,max_prefix", [(64, 64, 1, 64), (64, 64, 1, 0), (1024, 32, 1, 0), (130, 64, 3, 16)])
+def test_long_own_contexts_of_chunks_are_split(lib, tokens, heads, batch, max_prefix):
+    """Sequences of more than 128 rows, whose own tokens the chunk kernel takes: as much of a
+    short prefix' call as of a long one's work is shared out (256 / 8 units a head, a split
+    of 3 tiles of 64 tokens or more)."""
+    slot = 8 * 256 * (128 + 2) * 4  # of all key/value heads
+    size = lambda kv: lib.phi_hip_paged_attention_shared_workspace_bytes(  # noqa: E731
+        tokens, heads, 8, 128, 1, batch, max_prefix, 64 if tokens < 1024 else tokens, kv, Q.BF16)
+    assert (size(8192) - size(64)) // slot >= 24
