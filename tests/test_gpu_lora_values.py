@@ -96,3 +96,23 @@ def test_rows_without_an_adapter_are_copied(dev, M, K, R, wd, od):
     assert same_bits(Q.lora_batched(*to, base=out, out=out)[none.to(dev)], base[none])
     zero = Q.lora_batched(*to, out_dtype=od)[none.to(dev)]
     assert same_bits(zero, torch.zeros_like(zero))
+
+
+@pytest.mark.parametrize("wd", [BF16, F32])
+@pytest.mark.parametrize("M,K,R", SIZES)
+def test_h_has_all_of_its_bits(dev, M, K, R, wd):
+    """One rank a column: h of 24 bits times 8, in up to three exact parts whose sum loses at
+    most a step, 2^-23, of the largest at each of two additions (two terms instead of three lose
+    2^-17, one 2^-9)."""
+    n, N = 3, 150
+    g = torch.Generator().manual_seed(K)
+    x, A = passing(M, K, R, n, wd)
+    x[:, :R] = torch.randn((M, R), generator=g)
+    rank = torch.randint(0, R, (n, N), generator=g)
+    B = torch.zeros((n, N, R), dtype=wd).scatter_(2, rank[..., None], (torch.randint(64, 128, (n, N, 1), generator=g) / 64).to(wd))
+    adapter = torch.randint(0, n, (M,), generator=g).int()
+    got = Q.lora_batched(*(t.to(dev) for t in (x, A, B, adapter)), out_dtype=F32).cpu().double()
+    for a in range(n):
+        mine = adapter == a
+        want = x[mine].double()[:, rank[a]] * B[a].double().gather(1, rank[a][:, None])[:, 0]
+        assert bool(((got[mine] - want).abs() <= 2 * 2.0 ** -23 * want.abs()).all())
