@@ -78,15 +78,19 @@ phi_status phi_hip_kv_cache_copy(phi_stream_t stream, const phi_kv_cache* from, 
                                  int64_t n);
 
 /*
- * phi_hip_paged_attention (causal) for a batch whose sequences share prefixes, each
- * prefix read once for all rows that see it.  Group g's prefix, prefix_len[g] tokens in the blocks
+ * phi_hip_paged_attention (causal) for a batch whose sequences share prefixes.  A prefix is
+ * read for all rows of its group together: once for every 16 (a row: one query head of a
+ * key/value head of one new token), but for every 256 (dim above 128: 128) where the group has
+ * more than 128 and q is PHI_BF16.  Group g's prefix, prefix_len[g] tokens in the blocks
  * prefix_table[g][0..], comes before the own tokens of the sequences
  * group_start[g] .. group_start[g+1] - 1: all of their rows see all of it.  A
  * sequence's own tokens, kv_len[b] with the new ones last, lie in the blocks
  * block_table[b][0..], from the first block's first place on; of these its row i sees
  * t <= kv_len[b] - n + i.  With n = q_start[b+1] - q_start[b],
  *   out = sum softmax(scale * q . k) v   over both, one softmax.
- * A row that sees nothing gives zeros.
+ * A row that sees nothing gives zeros.  For single tokens and a few at a time: chunks of many
+ * new tokens take less time in phi_hip_paged_attention, with the prefix' blocks first in each
+ * sequence's table, and so does a batch that shares nothing.
  *
  *   groups       from 1 to 65535; group_start [groups + 1] int32, ascending from 0 on
  *                to at most batch: sequences before the first group's or past the last's
@@ -99,9 +103,10 @@ phi_status phi_hip_kv_cache_copy(phi_stream_t stream, const phi_kv_cache* from, 
  *                has blocks for: refused
  *   workspace    phi_hip_paged_attention_shared_workspace_bytes() bytes, 16-byte aligned
  * All else as phi_hip_paged_attention, its arithmetic too, a group's rows over their
- * prefix being one sequence of it; the parts are joined in fp32.  Lengths, starts and
- * tables are read on the device, so a captured graph serves growing sequences and
- * other groups.
+ * prefix being one sequence of it: behind a prefix whose group has more than 128 rows,
+ * PHI_BF16's p has 11 bits as there, and a row's last bits depend on how many rows its
+ * group has.  The parts are joined in fp32.  Lengths, starts and tables are read on the
+ * device, so a captured graph serves growing sequences and other groups.
  */
 phi_status phi_hip_paged_attention_shared(phi_stream_t stream, const void* q, int dtype, int64_t q_token_stride,
                                           int64_t q_head_stride, int64_t tokens, int64_t q_heads,

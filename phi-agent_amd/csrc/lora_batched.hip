@@ -3,14 +3,15 @@
 //
 // Two passes, h = A[a] x[m] and the update.  A tile of 128 rows has its rows sorted
 // into classes, those of one adapter; a block takes rows of one class as the
-// columns of its products, so that an adapter's factors are read once for all of a
-// class's rows however they are mixed, and a row's values meet no other adapter's.  The
+// columns of its products, so that an adapter's factors are read for a tile's rows of it
+// together however these are mixed (A once for 32 of them, or 128; B's first 32 ranks, or 64,
+// once, further ones for every 16), and a row's values meet no other adapter's.  The
 // first pass leaves the classes for the second.
 // An operand of a matrix instruction is 16 rows of 32 k, 8 consecutive k of row l % 16 in
 // lane l: one v_mfma_f32_16x16x32_bf16 or, in fp32, eight v_mfma_f32_16x16x4_f32 (k 8 g + e
 // in the e-th, g = l / 16, on both sides).
 // h is fp32 throughout: against bf16 factors it enters the second product as three
-// bf16, all of its 24 bits.
+// bf16, all of its 24 bits; of a result that is not finite, infinite factors meet the first only.
 // Bound by memory: x once, base and out once, each tile's factors from L2.  64 rows of
 // 4096 on 16 ranks to 6144, 32 adapters at random: 6 + 8 us, latency (counts, classes, rows and
 // factors are loads that wait for each other); eight prompts of 4352 rows of 5120 on 64 ranks

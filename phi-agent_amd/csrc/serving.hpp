@@ -48,7 +48,7 @@ struct LoraBatched {
     const void* base;    // null: 0
     void* out;
     float* h;        // [splits][rows][rank_pitch]: parts of A x
-    struct LoraClass* classes;  // [tiles][64]
+    struct LoraClass* classes;  // [tiles][128]
     int* counts;                // [tiles]
     void* joined;               // h as the second product takes it; null: from its parts
     int64_t ldx, a_adapter, a_row, b_adapter, b_row, ld_base, ldo;

@@ -9,7 +9,7 @@ using namespace phi_capi;
 namespace {
 
 constexpr int64_t kMaxRotaryDim = 1024;   // a wave has a vector
-constexpr int64_t kMaxRank = 256;         // of an adapter: h of 32 rows is held in LDS
+constexpr int64_t kMaxRank = 256;         // of an adapter: h of 64 rows, as three bf16, is held in LDS
 constexpr int64_t kMaxLoraRows = 1 << 24, kMaxLoraK = 1 << 24;  // units and columns counted in 31 bits
 constexpr int64_t kMaxHeadRows = 4 * phi_dev::kMaxBlocks;  // of shared prefixes, four a block of their join
 constexpr int64_t kMaxPageVectors = 1 << 26;  // of at most 16 pieces: counted in 31 bits

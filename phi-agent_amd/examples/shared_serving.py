@@ -5,7 +5,7 @@
 on the int8 linears and the int8 paged cache, as decoder_attention.py, with what a server of
 many requests has beside it: positions, each request's own low-rank adapter on both
 linears, and requests that begin as forks of a document, whose pages they share and attention
-reads once for all of them.
+reads for many of them at a time.
 
     python phi-agent_amd/examples/shared_serving.py [--document 8192] [--requests 64] [--new 64] [--chunk 1024]
 """

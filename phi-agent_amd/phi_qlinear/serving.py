@@ -261,7 +261,7 @@ def paged_attention_shared(q: torch.Tensor, cache: KvCache, prefix_table: torch.
                            out: torch.Tensor | None = None, workspace: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     """Causal attention of new tokens q [tokens, q_heads, dim] (bf16/f32) over
     prefixes that sequences share and their own tokens
-    (phi_hip_paged_attention_shared).  Sequences group_start[g] ..
+    (phi_hip_paged_attention_shared; for a few new tokens each).  Sequences group_start[g] ..
     group_start[g + 1] - 1 see prefix_len[g] tokens in blocks prefix_table[g],
     then their own as by `paged_attention`: kv_len[b] in blocks block_table[b],
     the last of them rows q_start[b] .. q_start[b + 1] - 1 of q.  All int32;
